@@ -106,6 +106,95 @@ UD_API int ud_paged_kv_append(int32_t kv_dtype, const void* k_new, const void* v
                               const int32_t* block_table, int32_t max_blocks, const int32_t* positions_dev, int32_t n,
                               int32_t kv_heads, int32_t head_dim, int32_t block_size, void* hip_stream);
 
+/* ---------------------------------------------------------------- windows, sinks, prompts, 4-bit pages
+ * The calls below take the same pages and block tables, and besides bf16 and half pages (kv_format UD_BF16 / UD_F16)
+ * pages of 4 bits:
+ *   UD_MXFP4   per page and kv head block_size rows of head_dim / 2 bytes, channel 2b in the low nibble of byte b, then
+ *              block_size rows of head_dim / 32 bytes: the exponent + 127 of each block of 32 channels.  A nibble is a
+ *              sign bit and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (codes 0 .. 7), times 2^exponent: 4.25 bits a value.
+ *              Exponent byte 255: the block held a NaN or an infinity and reads as NaN.
+ * k_pages / v_pages are ud_kv_page_bytes(..) bytes a page, 16-byte aligned, num_blocks pages each.  A block-table entry
+ * outside [0, num_blocks) is a page that is not held: nothing of it is read or written, and its keys are not there.
+ * They have no counterpart in the reference beyond the ones named; limits: head_dim 64 or 128, block_size 16. */
+#define UD_MXFP4 16
+
+/* Bytes of one page of keys (or of values); 0 for a format or size that is not supported. */
+UD_API size_t ud_kv_page_bytes(int32_t kv_format, int32_t kv_heads, int32_t head_dim, int32_t block_size);
+
+/* The heads of one attention layer's projected rows, made ready in one pass (Step.rope and the K/V writes of
+ * VoxtralSession.decode, Voxtral.swift:364-376, with the per-head norm that decoders put before the rotation):
+ *   y = x / sqrt(mean_c x_c^2 + eps) * weight     per head of q and k, where its weight is given
+ *   (y_i, y_{i+d/2}) -> (y_i cos a - y_{i+d/2} sin a, y_{i+d/2} cos a + y_i sin a),  a = position * inv_freq[i]
+ * Row t belongs to sequence seqs_dev[t] (null: t) at position positions_dev[t].  q goes to q_out, k and v (as it is) to
+ * the pages.
+ *   q, k, v      dtype (UD_F32, UD_BF16, UD_F16), rows q_ld / k_ld / v_ld elements apart (pieces of one fused row, or
+ *                buffers of their own); q_heads 0: no q.  dtype is fp32 or the pages' own; any for UD_MXFP4
+ *   q_out        dtype, rows q_out_ld apart; may be q
+ *   q_weight, k_weight   fp32 [head_dim] or null (no norm);  inv_freq fp32 [head_dim / 2] or null (no rotation)
+ * A row whose sequence is outside [0, n), whose position is negative or not below max_blocks * block_size, or whose page
+ * is not held, is padding: nothing is written for it, q_out included.  Rows of one call name different keys.
+ * Precision: angles in 64 bits, the rest in fp32 and one rounding at the end (half saturates); k for UD_MXFP4 pages
+ * in 64 bits up to its codes.  MXFP4: a block's exponent is the smallest with max |x| <= 7 * 2^exponent (but
+ * -100 .. 125), values go to the nearest code, ties to the even one, beyond the largest to that. */
+UD_API int ud_qk_norm_rope_append(int32_t dtype, int32_t kv_format, const void* q_dev, int32_t q_ld, const void* k_dev,
+                                  int32_t k_ld, const void* v_dev, int32_t v_ld, void* q_out_dev, int32_t q_out_ld,
+                                  const float* q_weight_dev, const float* k_weight_dev, float eps, const float* inv_freq_dev,
+                                  const int32_t* positions_dev, const int32_t* seqs_dev, void* k_pages, void* v_pages,
+                                  int32_t num_blocks, const int32_t* block_table, int32_t n, int32_t max_blocks,
+                                  int32_t rows, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t block_size,
+                                  void* hip_stream);
+
+/* Rows of the cache read back: row t is the key / value of position positions_dev[t] of sequence seqs_dev[t] (null: t),
+ * [rows, kv_heads * head_dim] of dtype UD_F32, the pages' own type, or UD_BF16 from UD_MXFP4 pages (exact).  A row that
+ * ud_qk_norm_rope_append would take as padding is 0. */
+UD_API int ud_paged_kv_read(int32_t kv_format, int32_t dtype, const void* k_pages, const void* v_pages, int32_t num_blocks,
+                            const int32_t* block_table, int32_t n, int32_t max_blocks, const int32_t* positions_dev,
+                            const int32_t* seqs_dev, void* k_out, void* v_out, int32_t rows, int32_t kv_heads,
+                            int32_t head_dim, int32_t block_size, void* hip_stream);
+
+/* ud_gqa_attention_paged_mq with sinks, for any group of heads and page format, at a cost that follows the window:
+ *   out[i, m, h] = sum_j softmax_j(q[i, m, h] . k[i, j, h / (Hq/Hkv)] / sqrt(head_dim)) v[i, j, kvh]
+ *   over keys j in [lo, hi) = ranges[i][m] and the sinks j in [0, min(n_sinks, lo)); 0 where lo >= hi (then without the
+ *   sinks too).  Ranges are cut to [0, max_blocks * block_size).
+ *   q_dev, out_dev  [n, n_queries, q_heads * head_dim] of dtype UD_F32, or the pages' own type, or any 16-bit type on
+ *                   UD_MXFP4 pages
+ *   max_span        upper bound of a sequence's keys from its lowest lo to its highest hi (sizes the grid; a longer
+ *                   sequence is slower, not wrong)
+ *   workspace       ud_gqa_window_workspace_bytes(..) bytes (0: may be null); its contents need not be kept
+ * Only entries of the block table whose pages hold a sink or a key of the window are read: the pages between may have
+ * been given back.  n_queries 1 .. 8, n_queries * q_heads / kv_heads <= 64.
+ * Precision: fp32 queries and outputs are as good as fp32 arithmetic; 16-bit ones: exact products, sums in fp32, the
+ * probabilities rounded once to the pages' type (bf16 for UD_MXFP4, twice that for half queries).  A NaN or infinity in
+ * a key or value reaches only the rows that see it. */
+UD_API size_t ud_gqa_window_workspace_bytes(int32_t n, int32_t n_queries, int32_t q_heads, int32_t kv_heads,
+                                            int32_t head_dim, int32_t n_sinks, int32_t max_span);
+UD_API int ud_gqa_window_attention_paged(int32_t kv_format, int32_t dtype, const void* q_dev, const void* k_pages,
+                                         const void* v_pages, int32_t num_blocks, const int32_t* block_table,
+                                         int32_t max_blocks, const int32_t* ranges_dev, int32_t n_sinks, void* out_dev,
+                                         int32_t n, int32_t n_queries, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                                         int32_t block_size, int32_t max_span, void* workspace, size_t workspace_bytes,
+                                         void* hip_stream);
+
+/* The same attention for prompts and pieces of prompts: any number of query rows per sequence (Step.attention with the
+ * whole prompt's rows, Ops.swift:136-169; VoxtralSession's first decode, Voxtral.swift:425-465).
+ *   q_dev, out_dev  [rows, q_heads * head_dim] of dtype UD_BF16 or UD_F16 (the pages' own, or either on UD_MXFP4 pages)
+ *   q_start_dev     int32 [n + 1], ascending: rows q_start[i] .. q_start[i + 1] - 1 belong to sequence i, at most
+ *                   max_rows each; out rows of no sequence are left as they were
+ *   ranges_dev      int32 [rows, 2]: row r sees [lo, hi) and the sinks below lo, as above (a causal prompt: hi = its
+ *                   position + 1).  The keys are read from the pages: append before the call
+ *   max_span        upper bound of a sequence's keys from its lowest lo to its highest hi (a plan, as above)
+ *   workspace       ud_gqa_prefill_workspace_bytes(..) bytes (0: may be null)
+ * Precision: exact products, sums and softmax in fp32, probabilities rounded once to dtype, one rounding at the end.
+ * UD_MXFP4 pages under half queries: cached values past half's range saturate. */
+UD_API size_t ud_gqa_prefill_workspace_bytes(int32_t n, int32_t rows, int32_t max_rows, int32_t q_heads, int32_t kv_heads,
+                                             int32_t head_dim, int32_t n_sinks, int32_t max_span);
+UD_API int ud_gqa_prefill_paged(int32_t kv_format, int32_t dtype, const void* q_dev, const void* k_pages,
+                                const void* v_pages, int32_t num_blocks, const int32_t* block_table, int32_t max_blocks,
+                                const int32_t* q_start_dev, const int32_t* ranges_dev, int32_t n_sinks, void* out_dev,
+                                int32_t n, int32_t rows, int32_t max_rows, int32_t q_heads, int32_t kv_heads,
+                                int32_t head_dim, int32_t block_size, int32_t max_span, void* workspace,
+                                size_t workspace_bytes, void* hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

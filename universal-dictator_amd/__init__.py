@@ -27,6 +27,10 @@ UD_F32, UD_BF16, UD_F16 = 0, 1, 2
 _DTYPES = {"f32": UD_F32, "fp32": UD_F32, "float32": UD_F32, "bf16": UD_BF16, "bfloat16": UD_BF16,
            "f16": UD_F16, "float16": UD_F16}
 
+# Page formats of the paged cache calls (UD_MXFP4 in ud_decode.h: 4-bit codes with a shared exponent per 32 channels).
+UD_MXFP4 = 16
+_PAGES = {"bf16": UD_BF16, "bfloat16": UD_BF16, "f16": UD_F16, "float16": UD_F16, "mxfp4": UD_MXFP4}
+
 STATUS = {0: "ok", -1: "invalid argument", -2: "shape", -3: "out of memory", -4: "HIP error", -5: "state",
           -6: "weight", -7: "capacity"}
 
@@ -107,6 +111,16 @@ def _sig(lib):
                                           ctypes.c_size_t, p]),
         "ud_rope_rotate_half": (i, [_i32, p, _i32, _i32, _i32, _i32, p, _i32, p, p]),
         "ud_paged_kv_append": (i, [_i32, p, p, p, p, p, _i32, p, _i32, _i32, _i32, _i32, p]),
+        "ud_kv_page_bytes": (ctypes.c_size_t, [_i32, _i32, _i32, _i32]),
+        "ud_qk_norm_rope_append": (i, [_i32, _i32, p, _i32, p, _i32, p, _i32, p, _i32, p, p, ctypes.c_float, p, p, p, p, p, _i32,
+                                       p, _i32, _i32, _i32, _i32, _i32, _i32, _i32, p]),
+        "ud_paged_kv_read": (i, [_i32, _i32, p, p, _i32, p, _i32, _i32, p, p, p, p, _i32, _i32, _i32, _i32, p]),
+        "ud_gqa_window_workspace_bytes": (ctypes.c_size_t, [_i32] * 7),
+        "ud_gqa_window_attention_paged": (i, [_i32, _i32, p, p, p, _i32, p, _i32, p, _i32, p, _i32, _i32, _i32, _i32, _i32, _i32,
+                                              _i32, p, ctypes.c_size_t, p]),
+        "ud_gqa_prefill_workspace_bytes": (ctypes.c_size_t, [_i32] * 8),
+        "ud_gqa_prefill_paged": (i, [_i32, _i32, p, p, p, _i32, p, _i32, p, p, _i32, p, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
+                                     _i32, p, ctypes.c_size_t, p]),
         "ud_encoder_get_config": (i, [p, ctypes.POINTER(_Config)]),
         "ud_safetensors_open": (i, [ctypes.c_char_p, ctypes.POINTER(_vp)]),
         "ud_safetensors_close": (v, [p]),
@@ -654,6 +668,71 @@ def paged_kv_append(k_new, v_new, k_pages, v_pages, block_table, max_blocks, pos
     _check(lib().ud_paged_kv_append(_DTYPES[kv_dtype], k_new.ptr, v_new.ptr, k_pages.ptr, v_pages.ptr, block_table.ptr,
                                     max_blocks, positions.ptr, n, kv_heads, head_dim, block_size,
                                     hip_stream.ptr if hip_stream else None))
+
+
+def kv_page_bytes(kv_heads, head_dim, kv_format="bf16", block_size=16):
+    """Bytes of one page of keys (or of values) of the paged cache."""
+    return int(load_library().ud_kv_page_bytes(_PAGES[kv_format], kv_heads, head_dim, block_size))
+
+
+def qk_norm_rope_append(q, k, v, q_out, k_pages, v_pages, num_blocks, block_table, n, max_blocks, positions, rows, q_heads,
+                        kv_heads, head_dim, seqs=None, q_weight=None, k_weight=None, eps=1e-6, inv_freq=None, dtype="bf16",
+                        kv_format="bf16", q_ld=None, k_ld=None, v_ld=None, q_out_ld=None, block_size=16, hip_stream=None):
+    """The heads of projected rows in one pass: RMS norm per head of q and k (where a weight is given), rotation (where
+    inv_freq is given), q to q_out, k and v into the paged cache (kv_format bf16, f16 or mxfp4).  Row t is position
+    positions[t] of sequence seqs[t] (None: t); padding rows (see ud_decode.h) leave everything as it was.  *_ld: elements
+    between rows (None: contiguous)."""
+    ptr = lambda b: b.ptr if b is not None else None  # noqa: E731
+    qw, kw = q_heads * head_dim, kv_heads * head_dim
+    _check(lib().ud_qk_norm_rope_append(_DTYPES[dtype], _PAGES[kv_format], ptr(q), qw if q_ld is None else q_ld, k.ptr,
+                                        kw if k_ld is None else k_ld, v.ptr, kw if v_ld is None else v_ld, ptr(q_out),
+                                        qw if q_out_ld is None else q_out_ld, ptr(q_weight), ptr(k_weight), eps,
+                                        ptr(inv_freq), positions.ptr, ptr(seqs), k_pages.ptr, v_pages.ptr, num_blocks,
+                                        block_table.ptr, n, max_blocks, rows, q_heads, kv_heads, head_dim, block_size,
+                                        hip_stream.ptr if hip_stream else None))
+
+
+def paged_kv_read(k_pages, v_pages, num_blocks, block_table, n, max_blocks, positions, k_out, v_out, rows, kv_heads,
+                  head_dim, seqs=None, dtype="f32", kv_format="bf16", block_size=16, hip_stream=None):
+    """Cache rows read back to k_out / v_out [rows, kv_heads*head_dim]: position positions[t] of sequence seqs[t]."""
+    _check(lib().ud_paged_kv_read(_PAGES[kv_format], _DTYPES[dtype], k_pages.ptr, v_pages.ptr, num_blocks, block_table.ptr,
+                                  n, max_blocks, positions.ptr, seqs.ptr if seqs is not None else None, k_out.ptr,
+                                  v_out.ptr, rows, kv_heads, head_dim, block_size, hip_stream.ptr if hip_stream else None))
+
+
+def gqa_window_workspace_bytes(n, n_queries, q_heads, kv_heads, head_dim, n_sinks, max_span):
+    return int(load_library().ud_gqa_window_workspace_bytes(n, n_queries, q_heads, kv_heads, head_dim, n_sinks, max_span))
+
+
+def gqa_window_attention_paged(q, k_pages, v_pages, num_blocks, block_table, max_blocks, ranges, n_sinks, out, n, n_queries,
+                               q_heads, kv_heads, head_dim, max_span, workspace, dtype="f32", kv_format="bf16",
+                               block_size=16, hip_stream=None):
+    """Attention of n_queries (1 .. 8) positions per sequence over each one's window [lo, hi) = ranges[i][m] and the first
+    n_sinks keys before it, on bf16, half or MXFP4 pages; q/out [n, n_queries, q_heads*head_dim] of dtype.  workspace:
+    gqa_window_workspace_bytes(..) bytes, or None where that is 0."""
+    _check(lib().ud_gqa_window_attention_paged(_PAGES[kv_format], _DTYPES[dtype], q.ptr, k_pages.ptr, v_pages.ptr, num_blocks,
+                                               block_table.ptr, max_blocks, ranges.ptr, n_sinks, out.ptr, n, n_queries,
+                                               q_heads, kv_heads, head_dim, block_size, max_span,
+                                               workspace.ptr if workspace is not None else None,
+                                               workspace.nbytes if workspace is not None else 0,
+                                               hip_stream.ptr if hip_stream else None))
+
+
+def gqa_prefill_workspace_bytes(n, rows, max_rows, q_heads, kv_heads, head_dim, n_sinks, max_span):
+    return int(load_library().ud_gqa_prefill_workspace_bytes(n, rows, max_rows, q_heads, kv_heads, head_dim, n_sinks, max_span))
+
+
+def gqa_prefill_paged(q, k_pages, v_pages, num_blocks, block_table, max_blocks, q_start, ranges, n_sinks, out, n, rows,
+                      max_rows, q_heads, kv_heads, head_dim, max_span, workspace, dtype="bf16", kv_format="bf16",
+                      block_size=16, hip_stream=None):
+    """Attention of a ragged batch of prompt rows: q/out [rows, q_heads*head_dim] (bf16 or f16), rows q_start[i] ..
+    q_start[i + 1] - 1 of sequence i, row r over [lo, hi) = ranges[r] and the first n_sinks keys before it."""
+    _check(lib().ud_gqa_prefill_paged(_PAGES[kv_format], _DTYPES[dtype], q.ptr, k_pages.ptr, v_pages.ptr, num_blocks,
+                                      block_table.ptr, max_blocks, q_start.ptr, ranges.ptr, n_sinks, out.ptr, n, rows, max_rows,
+                                      q_heads, kv_heads, head_dim, block_size, max_span,
+                                      workspace.ptr if workspace is not None else None,
+                                      workspace.nbytes if workspace is not None else 0,
+                                      hip_stream.ptr if hip_stream else None))
 
 
 # ---------------------------------------------------------------- synthetic weights

@@ -1,0 +1,137 @@
+// What the windowed attention kernels (window.hip, prefill.hip) share: LDS tiles of values, products of 16-bit operands
+// and their terms, the join of the splits of a query row.
+#pragma once
+#include <type_traits>
+
+#include "paged.hpp"
+
+namespace ud {
+
+typedef short v4i16_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ uint2 lds_tr16(const char* p) {
+    return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4i16_t*)p));
+}
+
+// Address of piece p (16 bytes) of row r in a tile of 2 D-byte rows.
+template <int D> __device__ __forceinline__ int v_at(int r, int p) {
+    const int f = D == 128 ? (((r & 3) << 1) | ((r >> 2) & 1) | (r & 8)) : (r & 6);
+    return r * (2 * D) + ((p ^ f) << 4);
+}
+
+template <bool H> __device__ __forceinline__ f32x4_t mfma16(uint4 a, uint4 b, f32x4_t c) {
+    if constexpr (H) return __builtin_amdgcn_mfma_f32_16x16x32_f16(as_f16x8(a), as_f16x8(b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
+}
+// Two floats as a packed pair of the products' type, and the pair's values.
+template <bool H> __device__ __forceinline__ uint32_t pack16(float x, float y) {
+    if constexpr (H) return __builtin_bit_cast(uint32_t, half2_t{(_Float16)x, (_Float16)y});
+    else return pack_bf16x2(x, y);
+}
+template <bool H> __device__ __forceinline__ void unpack2(uint32_t w, float& x, float& y) {
+    if constexpr (H) { x = half_lo(w); y = half_hi(w); }
+    else { x = __uint_as_float(w << 16); y = __uint_as_float(w & 0xffff0000u); }
+}
+// Eight floats as T operands whose sum they are.
+template <bool H, int T> __device__ __forceinline__ void split8(const float (&x)[8], uint4 (&t)[T]) {
+    float r[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) r[e] = x[e];
+#pragma unroll
+    for (int k = 0; k < T; k++) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            w[e] = pack16<H>(r[2 * e], r[2 * e + 1]);
+            if (k + 1 < T) {
+                float a, b;
+                unpack2<H>(w[e], a, b);
+                r[2 * e] -= a;
+                r[2 * e + 1] -= b;
+            }
+        }
+        t[k] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
+// The splits of one (query row, head) joined, a wave each: with split s's maximum m_s (of scores times log2(e)), sum l_s
+// and unnormalised output x_s,  out = sum_s 2^(m_s - m) x_s / sum_s 2^(m_s - m) l_s.  A split without a key has m = -inf,
+// l = 0 and its x is not looked at.
+// The rows: `count` of them, or (start) those of each sequence y, tokens start[y] .. start[y + 1] - 1 of `tokens`, at most
+// `count` rows each.
+struct JoinRows {
+    int64_t count;
+    int heads, tokens;
+    const int32_t* start;
+    int n;
+};
+template <typename E, int D>
+__global__ __launch_bounds__(256) void join_splits_kernel(const float* part, const float* stat, void* out, JoinRows rows, int splits) {
+    typedef typename E::S S;
+    constexpr int DL = D / 64, DEEP = 8;
+    const int lane = threadIdx.x & 63;
+    int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    if (row >= rows.count) return;
+    if (rows.start) {
+        const int s0 = min(max(rows.start[blockIdx.y], 0), rows.tokens), s1 = min(max(rows.start[blockIdx.y + 1], s0), rows.tokens);
+        if (row >= (int64_t)(s1 - s0) * rows.heads) return;
+        row += (int64_t)s0 * rows.heads;
+    }
+    const float* st = stat + row * splits * 2;
+    const float* pr = part + row * splits * D + lane * DL;
+    constexpr int CH = MAX_SPLITS / 64;
+    float m[CH], l[CH], top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < CH; k++) {
+        const int s = 64 * k + lane;
+        const float2 v = s < splits ? *reinterpret_cast<const float2*>(st + 2 * s) : make_float2(-INFINITY, 0.0f);
+        m[k] = v.x; l[k] = v.y;
+        top = fmaxf(top, v.x);
+    }
+    top = wave_max(top);
+    float sum = 0.0f, acc[DL];
+#pragma unroll
+    for (int e = 0; e < DL; e++) acc[e] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < CH; k++) {
+        if (64 * k >= splits) break;
+        const float w = m[k] == top ? 1.0f : __builtin_amdgcn_exp2f(m[k] - top);
+        sum += w * l[k];
+        const float wx = m[k] == -INFINITY ? 0.0f : w;
+        const int cnt = min(64, splits - 64 * k);
+        for (int s0 = 0; s0 < cnt; s0 += DEEP) {
+            float x[DEEP][DL];
+#pragma unroll
+            for (int s = 0; s < DEEP; s++) {
+                const float* p = pr + (int64_t)(64 * k + min(s0 + s, cnt - 1)) * D;
+                if constexpr (DL == 2) {
+                    const float2 v = *reinterpret_cast<const float2*>(p);
+                    x[s][0] = v.x; x[s][1] = v.y;
+                } else {
+                    x[s][0] = *p;
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < DEEP; s++) {
+                const float ws = s0 + s < cnt ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wx), s0 + s)) : 0.0f;
+#pragma unroll
+                for (int e = 0; e < DL; e++) acc[e] += ws == 0.0f ? 0.0f : ws * x[s][e];
+            }
+        }
+    }
+    sum = wave_sum(sum);
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    S* o = static_cast<S*>(out) + row * D + lane * DL;
+#pragma unroll
+    for (int e = 0; e < DL; e++) {
+        const float y = acc[e] * inv;
+        if constexpr (std::is_same<E, El32>::value) o[e] = y;
+        else if constexpr (std::is_same<E, ElBf>::value) o[e] = f2bf(y);
+        else o[e] = f2h(y);
+    }
+}
+template <typename E, int D>
+static void launch_join(const float* part, const float* stat, void* out, const JoinRows& rows, int splits, hipStream_t st) {
+    hipLaunchKernelGGL((join_splits_kernel<E, D>), dim3((unsigned)((rows.count + 3) / 4), rows.start ? rows.n : 1), dim3(256), 0, st, part, stat, out, rows, splits);
+}
+
+}  // namespace ud

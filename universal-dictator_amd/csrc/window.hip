@@ -1,0 +1,521 @@
+// Attention of 1 .. 8 query positions per sequence over the sinks and the sliding window of a paged cache, held in
+// bf16, half or MXFP4 (include/ud_decode.h).
+//
+//   out[r] = sum_j softmax_j(q[r] . k[j] / sqrt(D)) v[j]   over j in [0, min(sinks, lo_r)) and [lo_r, hi_r)
+//
+// Bound: HBM; every visible K and V byte is read once.  One workgroup = (kv head, split of the page list, sequence);
+// its rows are the M positions times the G query heads of the kv head (up to 64, in tiles of 16), so a page is read
+// once for all of them.  Each of the 4 waves takes chunks of its split's pages (2 pages of 16 bits, 4 of MXFP4) on its
+// own, with its own running maximum and sum, so the loop has no barrier; the waves join once at the end, the splits in
+// a second kernel.
+//  - S^T = K . Q^T on v_mfma_f32_16x16x32: lane (c, g) loads the channels that the A operand wants of key c straight
+//    into registers.  An MXFP4 lane's 16 bytes are one block of 32 channels, whose pieces serve the products over all
+//    blocks in turn (the channel order within a sum is free as long as q has the same).
+//  - lane (c, g) then holds row c's scores of keys 4g .. 4g + 3 of each tile, which is the B operand of
+//    O^T = V^T . P^T as it stands.  V goes through the wave's own LDS tile (rows permuted piecewise against bank
+//    conflicts) and comes back transposed by ds_read_b64_tr_b16.  MXFP4 is turned into bf16, which holds its values
+//    exactly, on the way.
+//  - 16-bit operands with fp32 accuracy: a factor is split into terms (x = x0 + x1 + .., each the nearest 16-bit value
+//    of what is left), one product each.  q: one term of its own type; half for bf16 products two; fp32 three of bf16 or
+//    two of half (scaled by a power of two per row, so that no term leaves half's range).  Probabilities: as many terms
+//    as the output's type can show.
+#include <type_traits>
+
+#include "paged_attention.hpp"
+
+namespace ud {
+
+struct WindowArgs {
+    const void* q;                 // [n][M][Hq][D]
+    const char* kp; const char* vp;
+    const int32_t* bt;
+    const int32_t* ranges;         // [n][M][2]
+    void* out;                     // [n][M][Hq][D]
+    float* part;                   // [n][M][Hq][splits][D], then (maximum, sum) [n][M][Hq][splits][2]
+    float* stat;
+    int M, G, Hq, Hkv;
+    int max_blocks, num_blocks;
+    int sinks, splits, pages;      // pages: of a split
+    float scale;                   // log2(e) / sqrt(D)
+};
+
+// Terms of q and of the probabilities.
+template <typename E, int FMT> struct Terms {
+    static constexpr bool H = FMT == FMT_F16;      // half products; else bf16
+    static constexpr int Q = std::is_same<E, El32>::value ? (H ? 2 : 3) : FMT == FMT_FP4 && std::is_same<E, ElH>::value ? 2 : 1;
+    static constexpr int P = std::is_same<E, El32>::value ? (H ? 2 : 3) : std::is_same<E, ElH>::value && !H ? 2 : 1;
+};
+
+template <typename E, int FMT, int D, int RT>
+__global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
+    typedef typename E::S S;
+    constexpr bool H = Terms<E, FMT>::H;
+    constexpr int QT = Terms<E, FMT>::Q, PT = Terms<E, FMT>::P;
+    constexpr int CP = FMT == FMT_FP4 ? 4 : 2;     // pages per chunk
+    constexpr int KS = D / 32;                     // products over the channels
+    constexpr int DT = D / 16;                     // channel tiles
+    constexpr int HEAD = Page<FMT, D>::BYTES;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int col = lane & 15, g = lane >> 4;
+    const int kvh = blockIdx.x, split = blockIdx.y, seq = blockIdx.z;
+    const int G = a.G, M = a.M, QR = M * G;
+    __shared__ __align__(16) char tile[4][32 * 2 * D];
+    __shared__ float wmax[4][16 * RT], wsum[4][16 * RT];
+
+    // ---- the sequence's page list, and this lane's rows (row 16 rt + col: position r / G, head r % G)
+    const int32_t* rg = a.ranges + (int64_t)2 * seq * M;
+    const int kmax = a.max_blocks * KPAGE;
+    int lo = kmax, hi = 0, lo_most = 0, hi_least = kmax;
+    for (int m = 0; m < M; m++) {
+        const int l = max(rg[2 * m], 0), h = min(rg[2 * m + 1], kmax);
+        if (l < h) {
+            lo = min(lo, l); hi = max(hi, h);
+            lo_most = max(lo_most, l); hi_least = min(hi_least, h);
+        }
+    }
+    const PageList list = page_list(lo, hi, a.sinks);
+    const int u0 = (int)min((int64_t)split * a.pages, (int64_t)list.count);
+    const int u1 = split == a.splits - 1 ? list.count : (int)min((int64_t)u0 + a.pages, (int64_t)list.count);
+    const int64_t row0 = (int64_t)seq * M * a.Hq + (int64_t)kvh * G;         // (position 0, head 0) of the group
+    auto out_row = [&](int r) { return row0 + (int64_t)(r / G) * a.Hq + r % G; };
+    if (u0 >= u1) {                                // no key here
+        if (a.splits > 1 && tid < QR)
+            *reinterpret_cast<float2*>(a.stat + (out_row(tid) * a.splits + split) * 2) = make_float2(-INFINITY, 0.0f);
+        if (a.splits == 1) {
+            const float z[4] = {0, 0, 0, 0};
+            for (int x = tid; x < QR * (D / 4); x += 256)
+                store4<E>(static_cast<S*>(a.out) + out_row(x / (D / 4)) * D + x % (D / 4) * 4, z);
+        }
+        return;
+    }
+    int rlo[RT], rhi[RT], rsk[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const int m = min(16 * rt + col, QR - 1) / G;
+        rlo[rt] = max(rg[2 * m], 0);
+        rhi[rt] = min(rg[2 * m + 1], kmax);
+        rsk[rt] = rlo[rt] < rhi[rt] ? min(a.sinks, rlo[rt]) : 0;
+    }
+
+    // ---- q: B operand, lane (c, g): row c's channels chan(s) .. + 7 for product s
+    uint4 qf[RT][KS][QT];
+    float qscale[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const int r = 16 * rt + col;
+        const S* q = static_cast<const S*>(a.q) + out_row(min(r, QR - 1)) * D;
+        float x[KS][8];
+        float most = 0.0f;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+            const int ch = FMT == FMT_FP4 ? g * (D / 4) + 8 * s : 32 * s + 8 * g;
+            float u[4], v[4];
+            load4<E>(q + ch, u);
+            load4<E>(q + ch + 4, v);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                x[s][e] = r < QR ? u[e] : 0.0f;
+                x[s][4 + e] = r < QR ? v[e] : 0.0f;
+                most = fmaxf(most, fmaxf(fabsf(x[s][e]), fabsf(x[s][4 + e])));
+            }
+        }
+        qscale[rt] = a.scale;
+        if constexpr (H && QT > 1) {               // the row's largest value to 2^10 .. 2^11
+            most = xmax32(xmax16(most));
+            const int ex = most > 0.0f && most < INFINITY ? 10 - min(max(ilogbf(most), -110), 110) : 0;
+            const float up = ldexpf(1.0f, ex);
+            qscale[rt] = a.scale * ldexpf(1.0f, -ex);
+#pragma unroll
+            for (int s = 0; s < KS; s++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) x[s][e] *= up;
+        }
+#pragma unroll
+        for (int s = 0; s < KS; s++) split8<H, QT>(x[s], qf[rt][s]);
+    }
+
+    f32x4_t o[DT][RT];
+    float rmax[RT], rsum[RT];                      // running maximum (all of the row), sum (this lane's keys)
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        rmax[rt] = -INFINITY;
+        rsum[rt] = 0.0f;
+#pragma unroll
+        for (int d = 0; d < DT; d++) o[d][rt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    // ---- the wave's chunks: pages u0 + CP wave, + 4 CP, ..
+    const int32_t* bt = a.bt + (int64_t)seq * a.max_blocks;
+    // 16-bit: kr[page][s], vr[page][i] rows 16 bytes a lane.  MXFP4: one piece and one exponent per page (D = 64: half).
+    constexpr int KR = FMT == FMT_FP4 ? 1 : KS, VR = FMT == FMT_FP4 ? 1 : D / 32;
+    uint4 kr[CP][KR], vr[CP][VR];
+    uint32_t ks[CP], vs[CP];
+    int blk[CP];                                   // logical page, or a page past every range
+    uint32_t held = 0;                             // bit t: the page is one of the pool's
+    char* vt = tile[wave];
+
+    auto load = [&](int u) {
+        held = 0;
+#pragma unroll
+        for (int t = 0; t < CP; t++) {
+            const bool in = u + t < u1;
+            blk[t] = page_at(list, in ? u + t : u0);
+            int page = bt[blk[t]];
+            const bool ok = in && page >= 0 && page < a.num_blocks;
+            page = ok ? page : 0;
+            held |= (uint32_t)ok << t;
+            const int64_t base = ((int64_t)page * a.Hkv + kvh) * HEAD;
+            const char* k = a.kp + base;
+            const char* v = a.vp + base;
+            if constexpr (FMT == FMT_FP4) {
+                if constexpr (D == 128) {
+                    kr[t][0] = ld16(k + col * 64 + g * 16);
+                    vr[t][0] = ld16(v + lane * 16);
+                    ks[t] = *reinterpret_cast<const uint8_t*>(k + Page<FMT, D>::CODES + col * 4 + g);
+                    vs[t] = *reinterpret_cast<const uint8_t*>(v + Page<FMT, D>::CODES + lane);
+                } else {
+                    const uint2 x = *reinterpret_cast<const uint2*>(k + col * 32 + g * 8), y = *reinterpret_cast<const uint2*>(v + lane * 8);
+                    kr[t][0] = make_uint4(x.x, x.y, 0, 0);
+                    vr[t][0] = make_uint4(y.x, y.y, 0, 0);
+                    ks[t] = *reinterpret_cast<const uint8_t*>(k + Page<FMT, D>::CODES + col * 2 + (g >> 1));
+                    vs[t] = *reinterpret_cast<const uint8_t*>(v + Page<FMT, D>::CODES + (lane >> 1));
+                }
+            } else {
+#pragma unroll
+                for (int s = 0; s < KS; s++) kr[t][s] = ld16(k + col * (2 * D) + 64 * s + 16 * g);
+#pragma unroll
+                for (int i = 0; i < VR; i++) vr[t][i] = ld16(v + i * 1024 + lane * 16);
+            }
+        }
+    };
+
+    int u = u0 + CP * wave;
+    if (u < u1) load(u);
+    for (; u < u1; u += 4 * CP) {
+        // ---- scores, row c's keys 16t + 4g + i, times log2(e) / sqrt(D)
+        float p[RT][CP][4];
+#pragma unroll
+        for (int t = 0; t < CP; t++) {
+            uint4 kf[KS];
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                if constexpr (FMT == FMT_FP4) {
+                    const uint32_t w = s == 0 ? kr[t][0].x : s == 1 ? kr[t][0].y : s == 2 ? kr[t][0].z : kr[t][0].w;
+                    kf[s] = fp4_to_bf16(w, fp4_scale(ks[t]));
+                } else {
+                    kf[s] = kr[t][s];
+                }
+            }
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int x = QT - 1; x >= 0; x--)  // small terms first
+#pragma unroll
+                    for (int s = 0; s < KS; s++) acc = mfma16<H>(kf[s], qf[rt][s][x], acc);
+#pragma unroll
+                for (int i = 0; i < 4; i++) p[rt][t][i] = acc[i] * qscale[rt];
+            }
+        }
+        // a page that some row does not see whole (a row that sees nothing does not count: it is dropped at the end)
+        bool some = false;
+        int b[CP];
+#pragma unroll
+        for (int t = 0; t < CP; t++) {
+            b[t] = blk[t];
+            const int j = b[t] * KPAGE;
+            const bool whole = (held >> t & 1) && j >= lo_most && j + KPAGE <= hi_least;
+            some = some || !whole;
+        }
+        const uint32_t in_pool = held;
+        uint4 vk[CP][VR];
+        uint32_t vks[CP];
+#pragma unroll
+        for (int t = 0; t < CP; t++) {
+            vks[t] = vs[t];
+#pragma unroll
+            for (int i = 0; i < VR; i++) vk[t][i] = vr[t][i];
+        }
+        if (u + 4 * CP < u1) load(u + 4 * CP);
+        auto seen = [&](int rt, int t, int key) {  // key: row of page t
+            const int j = b[t] * KPAGE + key;
+            return (in_pool >> t & 1) && ((j >= rlo[rt] && j < rhi[rt]) || j < rsk[rt]);
+        };
+        if (some) {
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                for (int t = 0; t < CP; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) p[rt][t][i] = seen(rt, t, 4 * g + i) ? p[rt][t][i] : -INFINITY;
+        }
+        // ---- running maximum and sum, probabilities
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            float m = rmax[rt];
+#pragma unroll
+            for (int t = 0; t < CP; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) m = fmaxf(m, p[rt][t][i]);
+            m = xmax32(xmax16(m));
+            const float base = m == -INFINITY ? 0.0f : m;
+            const float keep = __builtin_amdgcn_exp2f(rmax[rt] - base);
+            rmax[rt] = m;
+            float sum = 0.0f;
+#pragma unroll
+            for (int t = 0; t < CP; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    p[rt][t][i] = __builtin_amdgcn_exp2f(p[rt][t][i] - base);
+                    sum += p[rt][t][i];
+                }
+            rsum[rt] = rsum[rt] * keep + sum;
+            if (__any(keep != 1.0f)) {
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[d][rt][i] *= keep;
+            }
+        }
+        // ---- O^T += V^T . P^T, 32 keys at a time through the wave's tile
+#pragma unroll
+        for (int half = 0; half < CP / 2; half++) {
+            __builtin_amdgcn_wave_barrier();       // the reads of the last 32 keys come first
+#pragma unroll
+            for (int tt = 0; tt < 2; tt++) {
+                const int t = 2 * half + tt;
+                const int j0 = b[t] * KPAGE;
+                // rows that no query row sees are zeroed: 0 x NaN is NaN
+                auto dead = [&](int key) {
+                    const int j = j0 + key;
+                    return some && !((in_pool >> t & 1) && ((j >= lo && j < hi) || (j < a.sinks && j < lo_most)));
+                };
+                if constexpr (FMT == FMT_FP4) {
+                    constexpr int LPR = D / 32;    // D = 128: a block a lane; D = 64: half a block
+                    const int key = D == 128 ? lane / LPR : lane >> 2;
+                    const float sc = fp4_scale(vks[t]);
+                    const uint32_t w[4] = {vk[t][0].x, vk[t][0].y, vk[t][0].z, vk[t][0].w};
+                    const bool z = dead(key);
+#pragma unroll
+                    for (int e = 0; e < D / 32; e++) {
+                        uint4 x = fp4_to_bf16(w[e], sc);
+                        if (z) x = make_uint4(0, 0, 0, 0);
+                        *reinterpret_cast<uint4*>(vt + v_at<D>(16 * tt + key, (lane & 3) * (D / 32) + e)) = x;
+                    }
+                } else {
+                    constexpr int PPR = D / 8;     // pieces per row
+#pragma unroll
+                    for (int i = 0; i < VR; i++) {
+                        const int key = (64 * i + lane) / PPR;
+                        const uint4 x = dead(key) ? make_uint4(0, 0, 0, 0) : vk[t][i];
+                        *reinterpret_cast<uint4*>(vt + v_at<D>(16 * tt + key, lane % PPR)) = x;
+                    }
+                }
+            }
+            __builtin_amdgcn_wave_barrier();
+            uint4 pf[RT][PT];
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                float x[8];
+#pragma unroll
+                for (int i = 0; i < 4; i++) { x[i] = p[rt][2 * half][i]; x[4 + i] = p[rt][2 * half + 1][i]; }
+                if constexpr (H) {                 // a half's last bit at 1 is 2^-10; kept in range by 2^10
+#pragma unroll
+                    for (int i = 0; i < 8; i++) x[i] *= 1024.0f;
+                }
+                split8<H, PT>(x, pf[rt]);
+            }
+            const int k0 = 4 * g + (col >> 2);
+            uint32_t bad = 0;                      // a value that is no number, where rows differ in what they see
+            uint4 av[DT];
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                const int pc = 2 * d + ((col & 3) >> 1), hb = (col & 1) * 8;
+                const uint2 x = lds_tr16(vt + v_at<D>(k0, pc) + hb), y = lds_tr16(vt + v_at<D>(k0 + 16, pc) + hb);
+                av[d] = make_uint4(x.x, x.y, y.x, y.y);
+                if (some) {
+                    constexpr uint32_t EX = H ? 0x7c00u : 0x7f80u;
+                    const uint32_t w[4] = {x.x, x.y, y.x, y.y};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) bad |= (w[e] & EX) == EX || (w[e] >> 16 & EX) == EX;
+                }
+            }
+            if (__any(bad)) {
+                // row by row, the values that the row does not see taken out of its product
+                for (int r = 0; r < QR; r++) {
+                    const int m = r / G, l = max(rg[2 * m], 0), h = min(rg[2 * m + 1], kmax);
+                    const int sk = l < h ? min(a.sinks, l) : 0;
+                    uint32_t mask[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int t = 2 * half + (e >> 1);
+                        mask[e] = 0;
+#pragma unroll
+                        for (int f = 0; f < 2; f++) {
+                            const int j = b[t] * KPAGE + 4 * g + 2 * (e & 1) + f;
+                            if ((j >= l && j < h) || j < sk) mask[e] |= 0xffffu << (16 * f);
+                        }
+                    }
+#pragma unroll
+                    for (int d = 0; d < DT; d++) {
+                        const uint4 v = make_uint4(av[d].x & mask[0], av[d].y & mask[1], av[d].z & mask[2], av[d].w & mask[3]);
+#pragma unroll
+                        for (int rt = 0; rt < RT; rt++) {
+                            f32x4_t x = o[d][rt];
+#pragma unroll
+                            for (int k = PT - 1; k >= 0; k--) x = mfma16<H>(v, pf[rt][k], x);
+#pragma unroll
+                            for (int i = 0; i < 4; i++) o[d][rt][i] = 16 * rt + col == r ? x[i] : o[d][rt][i];
+                        }
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                        for (int k = PT - 1; k >= 0; k--) o[d][rt] = mfma16<H>(av[d], pf[rt][k], o[d][rt]);
+            }
+        }
+    }
+
+    // ---- the four waves joined, a row tile at a time through their LDS tiles
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const float l = xadd32(xadd16(rsum[rt]));
+        const bool empty = rlo[rt] >= rhi[rt];
+        if (empty) rmax[rt] = -INFINITY;
+        if (g == 0) { wmax[wave][16 * rt + col] = rmax[rt]; wsum[wave][16 * rt + col] = empty ? 0.0f : l; }
+    }
+    __syncthreads();
+    constexpr float PUP = H ? 1.0f / 1024.0f : 1.0f;
+    // a wave's share of a row with maximum m over the waves (1 where both are -inf: a sum of NaN scores stays NaN)
+    auto share = [](float mine, float m) { return mine == m ? 1.0f : __builtin_amdgcn_exp2f(mine - m); };
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const int rr = 16 * rt + col;
+        float m = wmax[0][rr];
+#pragma unroll
+        for (int w = 1; w < 4; w++) m = fmaxf(m, wmax[w][rr]);
+        // a wave without a key of the row adds nothing
+        const bool none = rmax[rt] == -INFINITY;
+        const float f = share(rmax[rt], m) * PUP;
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+            const float4 x = none ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
+                                  : make_float4(o[d][rt][0] * f, o[d][rt][1] * f, o[d][rt][2] * f, o[d][rt][3] * f);
+            *reinterpret_cast<float4*>(vt + col * (4 * D) + (((4 * d + g) ^ col) << 4)) = x;
+        }
+        __syncthreads();
+        for (int x = tid; x < 16 * (D / 4); x += 256) {
+            const int c = x / (D / 4), piece = x % (D / 4), r = 16 * rt + c;
+            if (r >= QR) continue;
+            float y[4] = {0, 0, 0, 0};
+            float mm = wmax[0][r], l = 0.0f;
+#pragma unroll
+            for (int w = 1; w < 4; w++) mm = fmaxf(mm, wmax[w][r]);
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const float4 v = *reinterpret_cast<const float4*>(tile[w] + c * (4 * D) + ((piece ^ c) << 4));
+                y[0] += v.x; y[1] += v.y; y[2] += v.z; y[3] += v.w;
+                l += wsum[w][r] * share(wmax[w][r], mm);
+            }
+            if (a.splits == 1) {
+                const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e] *= inv;
+                store4<E>(static_cast<S*>(a.out) + out_row(r) * D + 4 * piece, y);
+            } else {
+                const int64_t at = out_row(r) * a.splits + split;
+                *reinterpret_cast<float4*>(a.part + at * D + 4 * piece) = make_float4(y[0], y[1], y[2], y[3]);
+                if (piece == 0) *reinterpret_cast<float2*>(a.stat + at * 2) = make_float2(mm, l);
+            }
+        }
+        if (rt + 1 < RT) __syncthreads();
+    }
+}
+
+template <typename E, int FMT, int D, int RT>
+static void launch_rows(const WindowArgs& a, dim3 grid, hipStream_t st) {
+    hipLaunchKernelGGL((window_split_kernel<E, FMT, D, RT>), grid, dim3(256), 0, st, a);
+}
+template <typename E, int FMT, int D>
+static void launch_window_d(const WindowArgs& a, int n, hipStream_t st) {
+    const dim3 grid(a.Hkv, a.splits, n);
+    const int rows = a.M * a.G;
+    if (rows <= 16) launch_rows<E, FMT, D, 1>(a, grid, st);
+    else if (rows <= 32) launch_rows<E, FMT, D, 2>(a, grid, st);
+    else launch_rows<E, FMT, D, 4>(a, grid, st);
+    if (a.splits > 1) launch_join<E, D>(a.part, a.stat, a.out, JoinRows{(int64_t)n * a.M * a.Hq, 0, 0, nullptr, 1}, a.splits, st);
+}
+template <typename E, int FMT>
+static void launch_window(const WindowArgs& a, int n, int D, hipStream_t st) {
+    if (D == 128) launch_window_d<E, FMT, 128>(a, n, st);
+    else launch_window_d<E, FMT, 64>(a, n, st);
+}
+
+// Workgroups wanted: four per CU.  A workgroup's waves take 2 pages each at a time (MXFP4: 4).
+constexpr int64_t WINDOW_TARGET = 1024;
+static SplitPlan window_plan(int32_t n, int32_t kv_heads, int32_t n_sinks, int32_t max_span, int step) {
+    return split_plan((int64_t)n * kv_heads, max_pages(max_span, n_sinks), WINDOW_TARGET, step, step);
+}
+
+}  // namespace ud
+
+using namespace ud;
+
+extern "C" UD_API size_t ud_gqa_window_workspace_bytes(int32_t n, int32_t n_queries, int32_t q_heads, int32_t kv_heads,
+                                                       int32_t head_dim, int32_t n_sinks, int32_t max_span) {
+    if (n <= 0 || n_queries <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || n_sinks < 0 || max_span < 0) return 0;
+    const int s = window_plan(n, kv_heads, n_sinks, max_span, 8).splits;     // the finer of the two
+    return s == 1 ? 0 : (size_t)n * n_queries * q_heads * s * (head_dim + 2) * sizeof(float);
+}
+
+extern "C" UD_API int ud_gqa_window_attention_paged(int32_t kv_format, int32_t dtype, const void* q_dev, const void* k_pages,
+                                                    const void* v_pages, int32_t num_blocks, const int32_t* block_table,
+                                                    int32_t max_blocks, const int32_t* ranges_dev, int32_t n_sinks, void* out_dev,
+                                                    int32_t n, int32_t n_queries, int32_t q_heads, int32_t kv_heads,
+                                                    int32_t head_dim, int32_t block_size, int32_t max_span, void* workspace,
+                                                    size_t workspace_bytes, void* hip_stream) {
+    static const char* who = "ud_gqa_window_attention_paged";
+    int rc = paged_check(who, kv_format, k_pages, v_pages, num_blocks, block_table, n, max_blocks, kv_heads, head_dim, block_size);
+    if (rc != UD_OK) return rc;
+    if (!q_dev || !ranges_dev || !out_dev) return paged_fail(UD_ERR_INVALID, "%s: null pointer", who);
+    if (dtype != UD_F32 && dtype != UD_BF16 && dtype != UD_F16) return paged_fail(UD_ERR_INVALID, "%s: dtype %d", who, dtype);
+    if (kv_format != UD_MXFP4 && dtype != UD_F32 && dtype != kv_format)
+        return paged_fail(UD_ERR_INVALID, "%s: queries of dtype %d for pages of format %d (the same, or fp32, or MXFP4 pages)", who, dtype, kv_format);
+    if (n_queries < 1 || n_queries > 8) return paged_fail(UD_ERR_SHAPE, "%s: %d queries per sequence (1 .. 8)", who, n_queries);
+    if (q_heads < 1 || q_heads % kv_heads || (int64_t)q_heads / kv_heads * n_queries > 64)
+        return paged_fail(UD_ERR_SHAPE, "%s: heads %d/%d x %d queries (at most 64 rows per kv head)", who, q_heads, kv_heads, n_queries);
+    if ((int64_t)n * n_queries * q_heads > 1 << 25)
+        return paged_fail(UD_ERR_SHAPE, "%s: %d sequences x %d queries x %d heads (at most 2^25 rows)", who, n, n_queries, q_heads);
+    if (n_sinks < 0 || max_span < 0) return paged_fail(UD_ERR_SHAPE, "%s: %d sinks, span %d", who, n_sinks, max_span);
+    if (((uintptr_t)q_dev | (uintptr_t)out_dev) & 15) return paged_fail(UD_ERR_INVALID, "%s: buffers must be 16-byte aligned", who);
+    const size_t need = ud_gqa_window_workspace_bytes(n, n_queries, q_heads, kv_heads, head_dim, n_sinks, max_span);
+    if (need && !workspace) return paged_fail(UD_ERR_INVALID, "%s: null workspace", who);
+    if (workspace_bytes < need) return paged_fail(UD_ERR_SHAPE, "%s: workspace %zu < %zu bytes", who, workspace_bytes, need);
+    if ((uintptr_t)workspace & 15) return paged_fail(UD_ERR_INVALID, "%s: workspace must be 16-byte aligned", who);
+    const SplitPlan plan = window_plan(n, kv_heads, n_sinks, max_span, kv_format == UD_MXFP4 ? 16 : 8);
+    WindowArgs a{};
+    a.q = q_dev; a.kp = static_cast<const char*>(k_pages); a.vp = static_cast<const char*>(v_pages); a.bt = block_table;
+    a.ranges = ranges_dev; a.out = out_dev;
+    a.part = static_cast<float*>(workspace);
+    a.stat = a.part + (size_t)n * n_queries * q_heads * plan.splits * head_dim;
+    a.M = n_queries; a.G = q_heads / kv_heads; a.Hq = q_heads; a.Hkv = kv_heads;
+    a.max_blocks = max_blocks; a.num_blocks = num_blocks; a.sinks = n_sinks; a.splits = plan.splits; a.pages = plan.pages;
+    a.scale = (float)(1.4426950408889634 / sqrt((double)head_dim));
+    hipStream_t st = static_cast<hipStream_t>(hip_stream);
+    if (kv_format == UD_BF16) {
+        if (dtype == UD_F32) launch_window<El32, FMT_BF16>(a, n, head_dim, st);
+        else launch_window<ElBf, FMT_BF16>(a, n, head_dim, st);
+    } else if (kv_format == UD_F16) {
+        if (dtype == UD_F32) launch_window<El32, FMT_F16>(a, n, head_dim, st);
+        else launch_window<ElH, FMT_F16>(a, n, head_dim, st);
+    } else {
+        if (dtype == UD_F32) launch_window<El32, FMT_FP4>(a, n, head_dim, st);
+        else if (dtype == UD_BF16) launch_window<ElBf, FMT_FP4>(a, n, head_dim, st);
+        else launch_window<ElH, FMT_FP4>(a, n, head_dim, st);
+    }
+    return paged_launched(who);
+}
