@@ -96,7 +96,7 @@ __global__ __launch_bounds__(256) void join_splits_kernel(const float* part, con
         if (64 * k >= splits) break;
         const float w = m[k] == top ? 1.0f : __builtin_amdgcn_exp2f(m[k] - top);
         sum += w * l[k];
-        const float wx = m[k] == -INFINITY ? 0.0f : w;
+        const float wx = m[k] == -INFINITY ? -1.0f : w;   // -1: not looked at
         const int cnt = min(64, splits - 64 * k);
         for (int s0 = 0; s0 < cnt; s0 += DEEP) {
             float x[DEEP][DL];
@@ -112,9 +112,9 @@ __global__ __launch_bounds__(256) void join_splits_kernel(const float* part, con
             }
 #pragma unroll
             for (int s = 0; s < DEEP; s++) {
-                const float ws = s0 + s < cnt ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wx), s0 + s)) : 0.0f;
+                const float ws = s0 + s < cnt ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wx), s0 + s)) : -1.0f;
 #pragma unroll
-                for (int e = 0; e < DL; e++) acc[e] += ws == 0.0f ? 0.0f : ws * x[s][e];
+                for (int e = 0; e < DL; e++) acc[e] += ws < 0.0f ? 0.0f : ws * x[s][e];
             }
         }
     }

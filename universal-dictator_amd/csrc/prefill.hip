@@ -73,8 +73,10 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
     const int s0 = min(max(a.q_start[seq], 0), a.rows), s1 = min(min(max(a.q_start[seq + 1], s0), a.rows), s0 + a.max_rows);
     const int64_t total = (int64_t)(s1 - s0) * a.G;
     if ((int64_t)qb * 128 >= total) return;
-    __shared__ __align__(16) char kt[64 * 2 * D], vt[64 * 2 * D];
-    __shared__ int fold[4][3];
+    __shared__ __align__(16) char kt[2][64 * 2 * D], vt[2][64 * 2 * D];
+    __shared__ int fold[4][4];
+    __shared__ int page_of[2][4];                  // logical page, or -1 where there is none
+    __shared__ int odd;                            // a value that is no number has been left out
 
     // ---- this lane's row, and what the workgroup's rows see
     const int64_t rho = (int64_t)qb * 128 + 32 * wave + col;
@@ -90,14 +92,19 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
     const int wlo = wave_fold<32>(some_key ? rlo : kmax, least), whi = wave_fold<32>(some_key ? rhi : 0, most);
     const int wlo_most = __builtin_amdgcn_readfirstlane(wave_fold<32>(some_key ? rlo : 0, most));
     const int whi_least = __builtin_amdgcn_readfirstlane(wave_fold<32>(some_key ? rhi : kmax, least));
-    if (lane == 0) { fold[wave][0] = wlo; fold[wave][1] = whi; fold[wave][2] = wlo_most; }
+    if (lane == 0) { fold[wave][0] = wlo; fold[wave][1] = whi; fold[wave][2] = wlo_most; fold[wave][3] = whi_least; }
+    if (tid == 0) odd = 0;
     __syncthreads();
-    int lo = fold[0][0], hi = fold[0][1], lo_most = fold[0][2];
+    int lo = fold[0][0], hi = fold[0][1], lo_most = fold[0][2], hi_least = fold[0][3];
 #pragma unroll
-    for (int w = 1; w < 4; w++) { lo = min(lo, fold[w][0]); hi = max(hi, fold[w][1]); lo_most = max(lo_most, fold[w][2]); }
+    for (int w = 1; w < 4; w++) {
+        lo = min(lo, fold[w][0]); hi = max(hi, fold[w][1]);
+        lo_most = max(lo_most, fold[w][2]); hi_least = min(hi_least, fold[w][3]);
+    }
     lo = __builtin_amdgcn_readfirstlane(lo);
     hi = __builtin_amdgcn_readfirstlane(hi);
     lo_most = __builtin_amdgcn_readfirstlane(lo_most);
+    hi_least = __builtin_amdgcn_readfirstlane(hi_least);
     const PageList list = page_list(lo, hi, a.sinks);
     const int tiles = (list.count + 3) / 4;
     const int t0 = (int)((int64_t)tiles * split / a.splits), t1 = (int)((int64_t)tiles * (split + 1) / a.splits);
@@ -112,9 +119,12 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
     for (int c = 0; c < CT; c++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[c][i] = 0.0f;
-    float rmax = -INFINITY, rsum = 0.0f;
+    // probabilities are 2^(score - base): base follows the running maximum, but not before that is BASE_LAG ahead, so that
+    // the sums are hardly ever rescaled (a probability is then at most 2^BASE_LAG, far inside half's range)
+    constexpr float BASE_LAG = 8.0f;
+    float base = -INFINITY, rsum = 0.0f;
 
-    // ---- wave w brings page 4 tile + w
+    // ---- wave w brings page 4 tile + w: into registers two tiles ahead, into LDS one tile ahead
     const int32_t* bt = a.bt + (int64_t)seq * a.max_blocks;
     uint4 kr[VR], vr[VR];
     uint32_t ks = 0, vs = 0;
@@ -127,9 +137,9 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
         int page = bt[myblk];
         myheld = in && page >= 0 && page < a.num_blocks;
         page = myheld ? page : 0;
-        const int64_t base = ((int64_t)page * a.Hkv + kvh) * HEAD;
-        const char* k = a.kp + base;
-        const char* v = a.vp + base;
+        const int64_t at = ((int64_t)page * a.Hkv + kvh) * HEAD;
+        const char* k = a.kp + at;
+        const char* v = a.vp + at;
         if constexpr (FMT == FMT_FP4) {
             if constexpr (D == 128) {
                 kr[0] = ld16(k + lane * 16);
@@ -151,157 +161,161 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
             }
         }
     };
-    __shared__ int page_of[4];                     // logical page, or -1 where there is none
-    if (t0 < t1) load(t0);
-    for (int tile = t0; tile < t1; tile++) {
-        __syncthreads();                           // the last tile has been read
-        {
-            const int j0 = myblk * KPAGE;
-            // rows that no query row of the workgroup sees are zeroed: 0 x NaN is NaN
-            auto dead = [&](int key) {
-                const int j = j0 + key;
-                return !(myheld && ((j >= lo && j < hi) || (j < a.sinks && j < lo_most)));
-            };
-            if constexpr (FMT == FMT_FP4) {
-                const int key = lane >> 2;
-                const uint32_t kw[4] = {kr[0].x, kr[0].y, kr[0].z, kr[0].w}, vw[4] = {vr[0].x, vr[0].y, vr[0].z, vr[0].w};
-                const bool z = dead(key);
+    auto sees = [&](int l, int e, int sk, int j) { return (j >= l && j < e) || j < sk; };
+    // a page that some row of the workgroup does not see whole
+    auto partial = [&](int blk) { return blk * KPAGE < lo_most || blk * KPAGE + KPAGE > hi_least; };
+    auto store = [&](int buf) {
+        // In such a page the values of rows that no query row sees become 0, and so does every value that is no number
+        // (0 x NaN is NaN): the rows that do see it are given it at the end.
+        const bool part = !myheld || partial(myblk);
+        auto keep = [&](uint4 x, int key) {
+            if (!part) return x;
+            const int j = myblk * KPAGE + key;
+            if (!myheld || !((j >= lo && j < hi) || (j < a.sinks && j < lo_most))) return make_uint4(0, 0, 0, 0);
+            uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                for (int e = 0; e < D / 32; e++) {
-                    const int p = v_at<D>(16 * wave + key, (lane & 3) * (D / 32) + e);
-                    *reinterpret_cast<uint4*>(kt + p) = fp4_to_16<H>(kw[e], ks);
-                    uint4 x = fp4_to_16<H>(vw[e], vs);
-                    if (z) x = make_uint4(0, 0, 0, 0);
-                    *reinterpret_cast<uint4*>(vt + p) = x;
-                }
-            } else {
-                constexpr int PPR = D / 8;
-#pragma unroll
-                for (int i = 0; i < VR; i++) {
-                    const int key = (64 * i + lane) / PPR, p = v_at<D>(16 * wave + key, lane % PPR);
-                    *reinterpret_cast<uint4*>(kt + p) = kr[i];
-                    *reinterpret_cast<uint4*>(vt + p) = dead(key) ? make_uint4(0, 0, 0, 0) : vr[i];
-                }
+            for (int e = 0; e < 4; e++) {
+                constexpr uint32_t EX = H ? 0x7c00u : 0x7f80u;
+                if ((w[e] & EX) == EX) { w[e] &= 0xffff0000u; odd = 1; }
+                if ((w[e] >> 16 & EX) == EX) { w[e] &= 0xffffu; odd = 1; }
             }
-            if (lane == 0) page_of[wave] = myheld ? myblk : -1;
+            return make_uint4(w[0], w[1], w[2], w[3]);
+        };
+        if constexpr (FMT == FMT_FP4) {
+            const int key = lane >> 2;
+            const uint32_t kw[4] = {kr[0].x, kr[0].y, kr[0].z, kr[0].w}, vw[4] = {vr[0].x, vr[0].y, vr[0].z, vr[0].w};
+#pragma unroll
+            for (int e = 0; e < D / 32; e++) {
+                const int p = v_at<D>(16 * wave + key, (lane & 3) * (D / 32) + e);
+                *reinterpret_cast<uint4*>(kt[buf] + p) = fp4_to_16<H>(kw[e], ks);
+                *reinterpret_cast<uint4*>(vt[buf] + p) = keep(fp4_to_16<H>(vw[e], vs), key);
+            }
+        } else {
+            constexpr int PPR = D / 8;
+#pragma unroll
+            for (int i = 0; i < VR; i++) {
+                const int key = (64 * i + lane) / PPR, p = v_at<D>(16 * wave + key, lane % PPR);
+                *reinterpret_cast<uint4*>(kt[buf] + p) = kr[i];
+                *reinterpret_cast<uint4*>(vt[buf] + p) = keep(vr[i], key);
+            }
         }
+        if (lane == 0) page_of[buf][wave] = myheld ? myblk : -1;
+    };
+    if (t0 < t1) {
+        load(t0);
+        store(0);
+        if (t0 + 1 < t1) load(t0 + 1);
         __syncthreads();
+    }
+    for (int tile = t0; tile < t1; tile++) {
+        const int buf = (tile - t0) & 1;
+        if (tile + 1 < t1) {
+            store(buf ^ 1);                        // read by all before the last barrier
+            if (tile + 2 < t1) load(tile + 2);
+        }
         int b[4];
         bool some = false;
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-            b[t] = __builtin_amdgcn_readfirstlane(page_of[t]);
-            const int j = b[t] * KPAGE;
-            some = some || b[t] < 0 || j < wlo_most || j + KPAGE > whi_least;
+            b[t] = __builtin_amdgcn_readfirstlane(page_of[buf][t]);
+            some = some || b[t] < 0 || b[t] * KPAGE < wlo_most || b[t] * KPAGE + KPAGE > whi_least;
         }
-        if (tile + 1 < t1) load(tile + 1);
 
         // ---- scores, keys 32 c + 8 (i / 4) + 4 h + i % 4 of the tile
-        float p[2][16];
+        f32x16_t p[2];
 #pragma unroll
-        for (int c = 0; c < 2; c++) {
-            f32x16_t acc;
+        for (int c = 0; c < 2; c++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) acc[i] = 0.0f;
+            for (int i = 0; i < 16; i++) p[c][i] = 0.0f;
 #pragma unroll
-            for (int s = 0; s < KS; s++)
-                acc = mfma32<H>(*reinterpret_cast<const uint4*>(kt + v_at<D>(32 * c + col, 2 * s + h)), qf[s], acc);
+        for (int s = 0; s < KS; s++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) p[c][i] = acc[i] * a.scale;
-        }
+            for (int c = 0; c < 2; c++)
+                p[c] = mfma32<H>(*reinterpret_cast<const uint4*>(kt[buf] + v_at<D>(32 * c + col, 2 * s + h)), qf[s], p[c]);
         if (some) {
 #pragma unroll
             for (int c = 0; c < 2; c++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const int t = 2 * c + (i >> 3), j = b[t] * KPAGE + 8 * ((i >> 2) & 1) + 4 * h + (i & 3);
-                    const bool in = b[t] >= 0 && ((j >= rlo && j < rhi) || j < rsk);
-                    p[c][i] = in ? p[c][i] : -INFINITY;
+                    p[c][i] = b[t] >= 0 && sees(rlo, rhi, rsk, j) ? p[c][i] : -INFINITY;
                 }
         }
-        float m = rmax;
+        float m = p[0][0];
 #pragma unroll
         for (int c = 0; c < 2; c++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) m = fmaxf(m, p[c][i]);
-        m = xmax32(m);
-        const float base = m == -INFINITY ? 0.0f : m;
-        const float keep = __builtin_amdgcn_exp2f(rmax - base);
-        rmax = m;
+            for (int i = c == 0; i < 16; i++) m = fmaxf(m, p[c][i]);
+        m = xmax32(m) * a.scale;
+        if (__any(m > base + BASE_LAG)) {          // the row's first key too: base is -inf
+            const float to = fmaxf(base, m), keep = to == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(base - to);
+            rsum *= keep;
+#pragma unroll
+            for (int c = 0; c < CT; c++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[c][i] *= keep;
+            base = to;
+        }
+        const float off = base == -INFINITY ? 0.0f : base;
         float sum = 0.0f;
 #pragma unroll
         for (int c = 0; c < 2; c++)
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                p[c][i] = __builtin_amdgcn_exp2f(p[c][i] - base);
+                p[c][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[c][i], a.scale, -off));
                 sum += p[c][i];
             }
-        rsum = rsum * keep + sum;
-        if (__any(keep != 1.0f)) {
-#pragma unroll
-            for (int c = 0; c < CT; c++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) o[c][i] *= keep;
-        }
+        rsum += sum;
 
         // ---- O^T += V^T . P^T, 16 keys at a time: 16 kk + 4 h .. + 3 and 8 on
-        auto values = [&](int kk, int c) {
-            const int r = 16 * kk + 4 * h + ((lane & 15) >> 2);
-            const int pc = 4 * c + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), hb = (lane & 1) * 8;
-            const uint2 x = lds_tr16(vt + v_at<D>(r, pc) + hb), y = lds_tr16(vt + v_at<D>(r + 8, pc) + hb);
-            return make_uint4(x.x, x.y, y.x, y.y);
-        };
-        uint32_t bad = 0;                          // a value that is no number, where rows differ in what they see
-        if (some) {
-            constexpr uint32_t EX = H ? 0x7c00u : 0x7f80u;
-#pragma unroll
-            for (int kk = 0; kk < 4; kk++)
-#pragma unroll
-                for (int c = 0; c < CT; c++) {
-                    const uint4 v = values(kk, c);
-                    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int e = 0; e < 4; e++) bad |= (w[e] & EX) == EX || (w[e] >> 16 & EX) == EX;
-                }
-        }
-        const bool each = __any(bad);
 #pragma unroll
         for (int kk = 0; kk < 4; kk++) {
-            const float* x = p[kk >> 1] + 8 * (kk & 1);
-            const uint4 pf = make_uint4(pack16<H>(x[0], x[1]), pack16<H>(x[2], x[3]), pack16<H>(x[4], x[5]), pack16<H>(x[6], x[7]));
-            if (!each) {
+            const int x = 8 * (kk & 1);
+            const f32x16_t& pp = p[kk >> 1];
+            const uint4 pf = make_uint4(pack16<H>(pp[x], pp[x + 1]), pack16<H>(pp[x + 2], pp[x + 3]), pack16<H>(pp[x + 4], pp[x + 5]),
+                                        pack16<H>(pp[x + 6], pp[x + 7]));
+            const int r = 16 * kk + 4 * h + ((lane & 15) >> 2);
 #pragma unroll
-                for (int c = 0; c < CT; c++) o[c] = mfma32<H>(values(kk, c), pf, o[c]);
-            } else {
-                // row by row, the values that the row does not see taken out of its product
-                for (int r = 0; r < 32; r++) {
-                    const int l = __builtin_amdgcn_readlane(rlo, r), e = __builtin_amdgcn_readlane(rhi, r), sk = __builtin_amdgcn_readlane(rsk, r);
-                    uint32_t mask[4];
+            for (int c = 0; c < CT; c++) {
+                const int pc = 4 * c + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), hb = (lane & 1) * 8;
+                const uint2 y = lds_tr16(vt[buf] + v_at<D>(r, pc) + hb), z = lds_tr16(vt[buf] + v_at<D>(r + 8, pc) + hb);
+                o[c] = mfma32<H>(make_uint4(y.x, y.y, z.x, z.y), pf, o[c]);
+            }
+        }
+        __syncthreads();
+    }
+
+    if (odd) {
+        // values that are no numbers, in pages that the workgroup's rows see in part: to the rows that see them
+        for (int u = 4 * t0; u < min(4 * t1, list.count); u++) {
+            const int blk = page_at(list, u), page = bt[blk];
+            if (!partial(blk) || page < 0 || page >= a.num_blocks) continue;
+            const char* v = a.vp + ((int64_t)page * a.Hkv + kvh) * HEAD;
+            for (int key = 0; key < KPAGE; key++) {
+                const bool mine = sees(rlo, rhi, rsk, blk * KPAGE + key);
 #pragma unroll
-                    for (int w = 0; w < 4; w++) {
-                        mask[w] = 0;
+                for (int c = 0; c < CT; c++)
 #pragma unroll
-                        for (int f = 0; f < 2; f++) {
-                            const int j = b[kk] * KPAGE + 8 * (w >> 1) + 4 * h + 2 * (w & 1) + f;
-                            if ((j >= l && j < e) || j < sk) mask[w] |= 0xffffu << (16 * f);
+                    for (int i = 0; i < 16; i++) {
+                        const int ch = 32 * c + 8 * (i >> 2) + 4 * h + (i & 3);
+                        float x;
+                        if constexpr (FMT == FMT_FP4) {
+                            const uint8_t e = *reinterpret_cast<const uint8_t*>(v + Page<FMT, D>::CODES + key * (D / FP4_BLOCK) + ch / FP4_BLOCK);
+                            x = e == 255 ? NAN : 0.0f;
+                        } else {
+                            const uint16_t w = *reinterpret_cast<const uint16_t*>(v + (key * D + ch) * 2);
+                            x = H ? h2f(w) : bf2f(w);
                         }
+                        o[c][i] += mine && !__builtin_isfinite(x) ? x : 0.0f;
                     }
-#pragma unroll
-                    for (int c = 0; c < CT; c++) {
-                        const uint4 v = values(kk, c);
-                        const f32x16_t y = mfma32<H>(make_uint4(v.x & mask[0], v.y & mask[1], v.z & mask[2], v.w & mask[3]), pf, o[c]);
-#pragma unroll
-                        for (int i = 0; i < 16; i++) o[c][i] = col == r ? y[i] : o[c][i];
-                    }
-                }
             }
         }
     }
 
     if (!real) return;
     const float l = some_key ? xadd32(rsum) : 0.0f;
-    const float f = l == 0.0f || rmax == -INFINITY ? 0.0f : 1.0f;
-    const float inv = a.splits > 1 ? f : l == 0.0f ? 0.0f : f == 0.0f ? l : 1.0f / l;
+    // a row without a key: 0.  l is NaN where a score is (base may still be -inf then).
+    const float inv = l == 0.0f ? 0.0f : a.splits > 1 ? 1.0f : 1.0f / l;
 #pragma unroll
     for (int c = 0; c < CT; c++)
 #pragma unroll
@@ -314,7 +328,7 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
             else store4<E>(static_cast<S*>(a.out) + at * D + ch, y);
         }
     if (a.splits > 1 && h == 0)
-        *reinterpret_cast<float2*>(a.stat + (at * a.splits + split) * 2) = make_float2(some_key ? rmax : -INFINITY, l);
+        *reinterpret_cast<float2*>(a.stat + (at * a.splits + split) * 2) = make_float2(some_key ? base : -INFINITY, l);
 }
 
 template <typename E, int FMT>
