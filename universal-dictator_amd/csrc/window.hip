@@ -4,8 +4,9 @@
 //   out[r] = sum_j softmax_j(q[r] . k[j] / sqrt(D)) v[j]   over j in [0, min(sinks, lo_r)) and [lo_r, hi_r)
 //
 // Bound: HBM; every visible K and V byte is read once.  One workgroup = (kv head, split of the page list, sequence);
-// its rows are the M positions times the G query heads of the kv head (up to 64, in tiles of 16), so a page is read
-// once for all of them.  Each of the 4 waves takes chunks of its split's pages (2 pages of 16 bits, 4 of MXFP4) on its
+// its rows are the M positions times the G query heads of the kv head, up to 32 (two tiles of 16), so a page is read
+// once for all of them; above 32 rows a second workgroup takes the rest, on the same XCD at 8 kv heads (the rows of 64
+// would not leave the registers room).  Each of the 4 waves takes chunks of its split's pages (2 pages of 16 bits, 4 of MXFP4) on its
 // own, with its own running maximum and sum, so the loop has no barrier; the waves join once at the end, the splits in
 // a second kernel.
 //  - S^T = K . Q^T on v_mfma_f32_16x16x32: lane (c, g) loads the channels that the A operand wants of key c straight
@@ -35,7 +36,7 @@ struct WindowArgs {
     float* stat;
     int M, G, Hq, Hkv;
     int max_blocks, num_blocks;
-    int sinks, splits, pages;      // pages: of a split
+    int sinks, splits, pages, groups;   // pages of a split, groups of 16 RT rows
     float scale;                   // log2(e) / sqrt(D)
 };
 
@@ -47,7 +48,7 @@ template <typename E, int FMT> struct Terms {
 };
 
 template <typename E, int FMT, int D, int RT>
-__global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
+__global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(WindowArgs a) {
     typedef typename E::S S;
     constexpr bool H = Terms<E, FMT>::H;
     constexpr int QT = Terms<E, FMT>::Q, PT = Terms<E, FMT>::P;
@@ -57,8 +58,9 @@ __global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
     constexpr int HEAD = Page<FMT, D>::BYTES;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
-    const int kvh = blockIdx.x, split = blockIdx.y, seq = blockIdx.z;
-    const int G = a.G, M = a.M, QR = M * G;
+    const int kvh = blockIdx.x, split = blockIdx.y / a.groups, seq = blockIdx.z;
+    const int r0 = blockIdx.y % a.groups * (16 * RT);   // first of this workgroup's rows
+    const int G = a.G, M = a.M, QR = min(M * G - r0, 16 * RT);
     __shared__ __align__(16) char tile[4][32 * 2 * D];
     __shared__ float wmax[4][16 * RT], wsum[4][16 * RT];
 
@@ -66,7 +68,7 @@ __global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
     const int32_t* rg = a.ranges + (int64_t)2 * seq * M;
     const int kmax = a.max_blocks * KPAGE;
     int lo = kmax, hi = 0, lo_most = 0, hi_least = kmax;
-    for (int m = 0; m < M; m++) {
+    for (int m = r0 / G; m <= (r0 + QR - 1) / G; m++) {
         const int l = max(rg[2 * m], 0), h = min(rg[2 * m + 1], kmax);
         if (l < h) {
             lo = min(lo, l); hi = max(hi, h);
@@ -77,7 +79,7 @@ __global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
     const int u0 = (int)min((int64_t)split * a.pages, (int64_t)list.count);
     const int u1 = split == a.splits - 1 ? list.count : (int)min((int64_t)u0 + a.pages, (int64_t)list.count);
     const int64_t row0 = (int64_t)seq * M * a.Hq + (int64_t)kvh * G;         // (position 0, head 0) of the group
-    auto out_row = [&](int r) { return row0 + (int64_t)(r / G) * a.Hq + r % G; };
+    auto out_row = [&](int r) { return row0 + (int64_t)((r0 + r) / G) * a.Hq + (r0 + r) % G; };
     if (u0 >= u1) {                                // no key here
         if (a.splits > 1 && tid < QR)
             *reinterpret_cast<float2*>(a.stat + (out_row(tid) * a.splits + split) * 2) = make_float2(-INFINITY, 0.0f);
@@ -91,7 +93,7 @@ __global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
     int rlo[RT], rhi[RT], rsk[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
-        const int m = min(16 * rt + col, QR - 1) / G;
+        const int m = (r0 + min(16 * rt + col, QR - 1)) / G;
         rlo[rt] = max(rg[2 * m], 0);
         rhi[rt] = min(rg[2 * m + 1], kmax);
         rsk[rt] = rlo[rt] < rhi[rt] ? min(a.sinks, rlo[rt]) : 0;
@@ -135,7 +137,10 @@ __global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
     }
 
     f32x4_t o[DT][RT];
-    float rmax[RT], rsum[RT];                      // running maximum (all of the row), sum (this lane's keys)
+    // probabilities are 2^(score - base): base follows the running maximum, but not before that is BASE_LAG ahead, so that
+    // the sums are hardly ever rescaled (a probability is then at most 2^BASE_LAG)
+    constexpr float BASE_LAG = 8.0f;
+    float rmax[RT], rsum[RT];                      // base (all of the row), sum (this lane's keys)
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         rmax[rt] = -INFINITY;
@@ -153,6 +158,7 @@ __global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
     int blk[CP];                                   // logical page, or a page past every range
     uint32_t held = 0;                             // bit t: the page is one of the pool's
     char* vt = tile[wave];
+    bool odd = false;                              // a value that is no number has been left out
 
     auto load = [&](int u) {
         held = 0;
@@ -217,25 +223,22 @@ __global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
                 for (int i = 0; i < 4; i++) p[rt][t][i] = acc[i] * qscale[rt];
             }
         }
-        // a page that some row does not see whole (a row that sees nothing does not count: it is dropped at the end)
-        bool some = false;
         int b[CP];
-#pragma unroll
-        for (int t = 0; t < CP; t++) {
-            b[t] = blk[t];
-            const int j = b[t] * KPAGE;
-            const bool whole = (held >> t & 1) && j >= lo_most && j + KPAGE <= hi_least;
-            some = some || !whole;
-        }
         const uint32_t in_pool = held;
         uint4 vk[CP][VR];
         uint32_t vks[CP];
 #pragma unroll
         for (int t = 0; t < CP; t++) {
+            b[t] = blk[t];
             vks[t] = vs[t];
 #pragma unroll
             for (int i = 0; i < VR; i++) vk[t][i] = vr[t][i];
         }
+        // a page that some row does not see whole (a row that sees nothing does not count: it is dropped at the end)
+        auto partial = [&](int t) { return !(in_pool >> t & 1) || b[t] * KPAGE < lo_most || b[t] * KPAGE + KPAGE > hi_least; };
+        bool some = false;
+#pragma unroll
+        for (int t = 0; t < CP; t++) some = some || partial(t);
         if (u + 4 * CP < u1) load(u + 4 * CP);
         auto seen = [&](int rt, int t, int key) {  // key: row of page t
             const int j = b[t] * KPAGE + key;
@@ -252,30 +255,31 @@ __global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
         // ---- running maximum and sum, probabilities
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
-            float m = rmax[rt];
+            float m = p[rt][0][0];
 #pragma unroll
             for (int t = 0; t < CP; t++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) m = fmaxf(m, p[rt][t][i]);
+                for (int i = t == 0; i < 4; i++) m = fmaxf(m, p[rt][t][i]);
             m = xmax32(xmax16(m));
-            const float base = m == -INFINITY ? 0.0f : m;
-            const float keep = __builtin_amdgcn_exp2f(rmax[rt] - base);
-            rmax[rt] = m;
+            if (__any(m > rmax[rt] + BASE_LAG)) {  // the row's first key too: base is -inf
+                const float to = fmaxf(rmax[rt], m), keep = to == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(rmax[rt] - to);
+                rsum[rt] *= keep;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) o[d][rt][i] *= keep;
+                rmax[rt] = to;
+            }
+            const float off = rmax[rt] == -INFINITY ? 0.0f : rmax[rt];
             float sum = 0.0f;
 #pragma unroll
             for (int t = 0; t < CP; t++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    p[rt][t][i] = __builtin_amdgcn_exp2f(p[rt][t][i] - base);
+                    p[rt][t][i] = __builtin_amdgcn_exp2f(p[rt][t][i] - off);
                     sum += p[rt][t][i];
                 }
-            rsum[rt] = rsum[rt] * keep + sum;
-            if (__any(keep != 1.0f)) {
-#pragma unroll
-                for (int d = 0; d < DT; d++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) o[d][rt][i] *= keep;
-            }
+            rsum[rt] += sum;
         }
         // ---- O^T += V^T . P^T, 32 keys at a time through the wave's tile
 #pragma unroll
@@ -284,31 +288,35 @@ __global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
 #pragma unroll
             for (int tt = 0; tt < 2; tt++) {
                 const int t = 2 * half + tt;
-                const int j0 = b[t] * KPAGE;
-                // rows that no query row sees are zeroed: 0 x NaN is NaN
-                auto dead = [&](int key) {
-                    const int j = j0 + key;
-                    return some && !((in_pool >> t & 1) && ((j >= lo && j < hi) || (j < a.sinks && j < lo_most)));
+                // In a page that rows see in part the values of keys that no row sees become 0, and so does every value
+                // that is no number (0 x NaN is NaN): the rows that do see it are given it at the end.
+                const bool part = some && partial(t);
+                auto keep = [&](uint4 x, int key) {
+                    if (!part) return x;
+                    const int j = b[t] * KPAGE + key;
+                    if (!(in_pool >> t & 1) || !((j >= lo && j < hi) || (j < a.sinks && j < lo_most))) return make_uint4(0, 0, 0, 0);
+                    uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        constexpr uint32_t EX = H ? 0x7c00u : 0x7f80u;
+                        if ((w[e] & EX) == EX) { w[e] &= 0xffff0000u; odd = true; }
+                        if ((w[e] >> 16 & EX) == EX) { w[e] &= 0xffffu; odd = true; }
+                    }
+                    return make_uint4(w[0], w[1], w[2], w[3]);
                 };
                 if constexpr (FMT == FMT_FP4) {
-                    constexpr int LPR = D / 32;    // D = 128: a block a lane; D = 64: half a block
-                    const int key = D == 128 ? lane / LPR : lane >> 2;
+                    const int key = lane >> 2;     // D = 128: a block a lane; D = 64: half a block
                     const float sc = fp4_scale(vks[t]);
                     const uint32_t w[4] = {vk[t][0].x, vk[t][0].y, vk[t][0].z, vk[t][0].w};
-                    const bool z = dead(key);
 #pragma unroll
-                    for (int e = 0; e < D / 32; e++) {
-                        uint4 x = fp4_to_bf16(w[e], sc);
-                        if (z) x = make_uint4(0, 0, 0, 0);
-                        *reinterpret_cast<uint4*>(vt + v_at<D>(16 * tt + key, (lane & 3) * (D / 32) + e)) = x;
-                    }
+                    for (int e = 0; e < D / 32; e++)
+                        *reinterpret_cast<uint4*>(vt + v_at<D>(16 * tt + key, (lane & 3) * (D / 32) + e)) = keep(fp4_to_bf16(w[e], sc), key);
                 } else {
                     constexpr int PPR = D / 8;     // pieces per row
 #pragma unroll
                     for (int i = 0; i < VR; i++) {
                         const int key = (64 * i + lane) / PPR;
-                        const uint4 x = dead(key) ? make_uint4(0, 0, 0, 0) : vk[t][i];
-                        *reinterpret_cast<uint4*>(vt + v_at<D>(16 * tt + key, lane % PPR)) = x;
+                        *reinterpret_cast<uint4*>(vt + v_at<D>(16 * tt + key, lane % PPR)) = keep(vk[t][i], key);
                     }
                 }
             }
@@ -319,63 +327,50 @@ __global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
                 float x[8];
 #pragma unroll
                 for (int i = 0; i < 4; i++) { x[i] = p[rt][2 * half][i]; x[4 + i] = p[rt][2 * half + 1][i]; }
-                if constexpr (H) {                 // a half's last bit at 1 is 2^-10; kept in range by 2^10
+                if constexpr (H) {                 // up to 2^15, so that small ones keep their bits
 #pragma unroll
-                    for (int i = 0; i < 8; i++) x[i] *= 1024.0f;
+                    for (int i = 0; i < 8; i++) x[i] *= 128.0f;
                 }
                 split8<H, PT>(x, pf[rt]);
             }
             const int k0 = 4 * g + (col >> 2);
-            uint32_t bad = 0;                      // a value that is no number, where rows differ in what they see
-            uint4 av[DT];
 #pragma unroll
             for (int d = 0; d < DT; d++) {
                 const int pc = 2 * d + ((col & 3) >> 1), hb = (col & 1) * 8;
                 const uint2 x = lds_tr16(vt + v_at<D>(k0, pc) + hb), y = lds_tr16(vt + v_at<D>(k0 + 16, pc) + hb);
-                av[d] = make_uint4(x.x, x.y, y.x, y.y);
-                if (some) {
-                    constexpr uint32_t EX = H ? 0x7c00u : 0x7f80u;
-                    const uint32_t w[4] = {x.x, x.y, y.x, y.y};
 #pragma unroll
-                    for (int e = 0; e < 4; e++) bad |= (w[e] & EX) == EX || (w[e] >> 16 & EX) == EX;
-                }
+                for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                    for (int k = PT - 1; k >= 0; k--) o[d][rt] = mfma16<H>(make_uint4(x.x, x.y, y.x, y.y), pf[rt][k], o[d][rt]);
             }
-            if (__any(bad)) {
-                // row by row, the values that the row does not see taken out of its product
-                for (int r = 0; r < QR; r++) {
-                    const int m = r / G, l = max(rg[2 * m], 0), h = min(rg[2 * m + 1], kmax);
-                    const int sk = l < h ? min(a.sinks, l) : 0;
-                    uint32_t mask[4];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int t = 2 * half + (e >> 1);
-                        mask[e] = 0;
-#pragma unroll
-                        for (int f = 0; f < 2; f++) {
-                            const int j = b[t] * KPAGE + 4 * g + 2 * (e & 1) + f;
-                            if ((j >= l && j < h) || j < sk) mask[e] |= 0xffffu << (16 * f);
-                        }
-                    }
-#pragma unroll
-                    for (int d = 0; d < DT; d++) {
-                        const uint4 v = make_uint4(av[d].x & mask[0], av[d].y & mask[1], av[d].z & mask[2], av[d].w & mask[3]);
-#pragma unroll
-                        for (int rt = 0; rt < RT; rt++) {
-                            f32x4_t x = o[d][rt];
-#pragma unroll
-                            for (int k = PT - 1; k >= 0; k--) x = mfma16<H>(v, pf[rt][k], x);
-#pragma unroll
-                            for (int i = 0; i < 4; i++) o[d][rt][i] = 16 * rt + col == r ? x[i] : o[d][rt][i];
-                        }
-                    }
-                }
-            } else {
+        }
+    }
+    if (__any(odd)) {
+        // values that are no numbers, in pages that rows see in part: to the rows that see them
+        for (int u = u0; u < u1; u++) {
+            if ((u - u0) / CP % 4 != wave) continue;
+            const int blk = page_at(list, u), page = bt[blk];
+            if (page < 0 || page >= a.num_blocks || (blk * KPAGE >= lo_most && blk * KPAGE + KPAGE <= hi_least)) continue;
+            const char* v = a.vp + ((int64_t)page * a.Hkv + kvh) * HEAD;
+            for (int key = 0; key < KPAGE; key++) {
+                const int j = blk * KPAGE + key;
 #pragma unroll
                 for (int d = 0; d < DT; d++)
 #pragma unroll
-                    for (int rt = 0; rt < RT; rt++)
+                    for (int i = 0; i < 4; i++) {
+                        const int ch = 16 * d + 4 * g + i;
+                        float x;
+                        if constexpr (FMT == FMT_FP4) {
+                            const uint8_t e = *reinterpret_cast<const uint8_t*>(v + Page<FMT, D>::CODES + key * (D / FP4_BLOCK) + ch / FP4_BLOCK);
+                            x = e == 255 ? NAN : 0.0f;
+                        } else {
+                            const uint16_t w = *reinterpret_cast<const uint16_t*>(v + (key * D + ch) * 2);
+                            x = H ? h2f(w) : bf2f(w);
+                        }
+                        x = __builtin_isfinite(x) ? 0.0f : x;
 #pragma unroll
-                        for (int k = PT - 1; k >= 0; k--) o[d][rt] = mfma16<H>(av[d], pf[rt][k], o[d][rt]);
+                        for (int rt = 0; rt < RT; rt++) o[d][rt][i] += (j >= rlo[rt] && j < rhi[rt]) || j < rsk[rt] ? x : 0.0f;
+                    }
             }
         }
     }
@@ -389,7 +384,7 @@ __global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
         if (g == 0) { wmax[wave][16 * rt + col] = rmax[rt]; wsum[wave][16 * rt + col] = empty ? 0.0f : l; }
     }
     __syncthreads();
-    constexpr float PUP = H ? 1.0f / 1024.0f : 1.0f;
+    constexpr float PUP = H ? 1.0f / 128.0f : 1.0f;
     // a wave's share of a row with maximum m over the waves (1 where both are -inf: a sum of NaN scores stays NaN)
     auto share = [](float mine, float m) { return mine == m ? 1.0f : __builtin_amdgcn_exp2f(mine - m); };
 #pragma unroll
@@ -436,17 +431,15 @@ __global__ __launch_bounds__(256) void window_split_kernel(WindowArgs a) {
     }
 }
 
-template <typename E, int FMT, int D, int RT>
-static void launch_rows(const WindowArgs& a, dim3 grid, hipStream_t st) {
-    hipLaunchKernelGGL((window_split_kernel<E, FMT, D, RT>), grid, dim3(256), 0, st, a);
-}
 template <typename E, int FMT, int D>
-static void launch_window_d(const WindowArgs& a, int n, hipStream_t st) {
-    const dim3 grid(a.Hkv, a.splits, n);
+static void launch_window_d(WindowArgs a, int n, hipStream_t st) {
     const int rows = a.M * a.G;
-    if (rows <= 16) launch_rows<E, FMT, D, 1>(a, grid, st);
-    else if (rows <= 32) launch_rows<E, FMT, D, 2>(a, grid, st);
-    else launch_rows<E, FMT, D, 4>(a, grid, st);
+    if (rows <= 16) {
+        hipLaunchKernelGGL((window_split_kernel<E, FMT, D, 1>), dim3(a.Hkv, a.splits, n), dim3(256), 0, st, a);
+    } else {
+        a.groups = (rows + 31) / 32;
+        hipLaunchKernelGGL((window_split_kernel<E, FMT, D, 2>), dim3(a.Hkv, a.splits * a.groups, n), dim3(256), 0, st, a);
+    }
     if (a.splits > 1) launch_join<E, D>(a.part, a.stat, a.out, JoinRows{(int64_t)n * a.M * a.Hq, 0, 0, nullptr, 1}, a.splits, st);
 }
 template <typename E, int FMT>
@@ -503,7 +496,7 @@ extern "C" UD_API int ud_gqa_window_attention_paged(int32_t kv_format, int32_t d
     a.part = static_cast<float*>(workspace);
     a.stat = a.part + (size_t)n * n_queries * q_heads * plan.splits * head_dim;
     a.M = n_queries; a.G = q_heads / kv_heads; a.Hq = q_heads; a.Hkv = kv_heads;
-    a.max_blocks = max_blocks; a.num_blocks = num_blocks; a.sinks = n_sinks; a.splits = plan.splits; a.pages = plan.pages;
+    a.max_blocks = max_blocks; a.num_blocks = num_blocks; a.sinks = n_sinks; a.splits = plan.splits; a.pages = plan.pages; a.groups = 1;
     a.scale = (float)(1.4426950408889634 / sqrt((double)head_dim));
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
     if (kv_format == UD_BF16) {
