@@ -68,13 +68,19 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
     const int32_t* rg = a.ranges + (int64_t)2 * seq * M;
     const int kmax = a.max_blocks * KPAGE;
     int lo = kmax, hi = 0, lo_most = 0, hi_least = kmax;
-    for (int m = r0 / G; m <= (r0 + QR - 1) / G; m++) {
+    const int m0 = r0 ? r0 / G : 0, m1 = a.groups == 1 ? M - 1 : (r0 + QR - 1) / G;
+    for (int m = m0; m <= m1; m++) {
         const int l = max(rg[2 * m], 0), h = min(rg[2 * m + 1], kmax);
         if (l < h) {
             lo = min(lo, l); hi = max(hi, h);
             lo_most = max(lo_most, l); hi_least = min(hi_least, h);
         }
     }
+    // (wave-uniform values in scalar registers: addresses of pages are then a scalar base and a lane's fixed offset)
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    hi = __builtin_amdgcn_readfirstlane(hi);
+    lo_most = __builtin_amdgcn_readfirstlane(lo_most);
+    hi_least = __builtin_amdgcn_readfirstlane(hi_least);
     const PageList list = page_list(lo, hi, a.sinks);
     const int u0 = (int)min((int64_t)split * a.pages, (int64_t)list.count);
     const int u1 = split == a.splits - 1 ? list.count : (int)min((int64_t)u0 + a.pages, (int64_t)list.count);
@@ -149,54 +155,61 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
         for (int d = 0; d < DT; d++) o[d][rt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    // ---- the wave's chunks: pages u0 + CP wave, + 4 CP, ..
+    // ---- the wave's chunks: pages u0 + CP wave, + 4 CP, ..  Lane l holds the pool's page (or -1) of the l-th of the next
+    // 64 pages of the wave, so that the table is read once for 64 / CP chunks, not before each.
     const int32_t* bt = a.bt + (int64_t)seq * a.max_blocks;
+    int pages = -1;
+    auto look_up = [&](int u) {
+        const int at = u + lane / CP * (4 * CP) + lane % CP;
+        pages = at < u1 ? bt[page_at(list, at)] : -1;
+        pages = pages < a.num_blocks ? pages : -1;
+    };
     // 16-bit: kr[page][s], vr[page][i] rows 16 bytes a lane.  MXFP4: one piece and one exponent per page (D = 64: half).
     constexpr int KR = FMT == FMT_FP4 ? 1 : KS, VR = FMT == FMT_FP4 ? 1 : D / 32;
     uint4 kr[CP][KR], vr[CP][VR];
     uint32_t ks[CP], vs[CP];
-    int blk[CP];                                   // logical page, or a page past every range
     uint32_t held = 0;                             // bit t: the page is one of the pool's
     char* vt = tile[wave];
     bool odd = false;                              // a value that is no number has been left out
+    const uint32_t k_off = FMT == FMT_FP4 ? col * (D / 2) + g * (D / 8) : col * (2 * D) + 16 * g;
+    const uint32_t ks_off = Page<FMT, D>::CODES + col * (D / 32) + (D == 128 ? g : g >> 1);
+    const uint32_t vs_off = Page<FMT, D>::CODES + (D == 128 ? lane : lane >> 1);
 
-    auto load = [&](int u) {
+    auto load = [&](int first) {                   // first: lane that holds the chunk's first page
         held = 0;
 #pragma unroll
         for (int t = 0; t < CP; t++) {
-            const bool in = u + t < u1;
-            blk[t] = page_at(list, in ? u + t : u0);
-            int page = bt[blk[t]];
-            const bool ok = in && page >= 0 && page < a.num_blocks;
-            page = ok ? page : 0;
-            held |= (uint32_t)ok << t;
-            const int64_t base = ((int64_t)page * a.Hkv + kvh) * HEAD;
+            const int page = __builtin_amdgcn_readlane(pages, first + t);
+            held |= (uint32_t)(page >= 0) << t;
+            const int64_t base = ((int64_t)max(page, 0) * a.Hkv + kvh) * HEAD;
             const char* k = a.kp + base;
             const char* v = a.vp + base;
             if constexpr (FMT == FMT_FP4) {
                 if constexpr (D == 128) {
-                    kr[t][0] = ld16(k + col * 64 + g * 16);
-                    vr[t][0] = ld16(v + lane * 16);
-                    ks[t] = *reinterpret_cast<const uint8_t*>(k + Page<FMT, D>::CODES + col * 4 + g);
-                    vs[t] = *reinterpret_cast<const uint8_t*>(v + Page<FMT, D>::CODES + lane);
+                    kr[t][0] = ld16(k + k_off);
+                    vr[t][0] = ld16(v + lane * 16u);
                 } else {
-                    const uint2 x = *reinterpret_cast<const uint2*>(k + col * 32 + g * 8), y = *reinterpret_cast<const uint2*>(v + lane * 8);
+                    const uint2 x = *reinterpret_cast<const uint2*>(k + k_off), y = *reinterpret_cast<const uint2*>(v + lane * 8u);
                     kr[t][0] = make_uint4(x.x, x.y, 0, 0);
                     vr[t][0] = make_uint4(y.x, y.y, 0, 0);
-                    ks[t] = *reinterpret_cast<const uint8_t*>(k + Page<FMT, D>::CODES + col * 2 + (g >> 1));
-                    vs[t] = *reinterpret_cast<const uint8_t*>(v + Page<FMT, D>::CODES + (lane >> 1));
                 }
+                ks[t] = *reinterpret_cast<const uint8_t*>(k + ks_off);
+                vs[t] = *reinterpret_cast<const uint8_t*>(v + vs_off);
             } else {
 #pragma unroll
-                for (int s = 0; s < KS; s++) kr[t][s] = ld16(k + col * (2 * D) + 64 * s + 16 * g);
+                for (int s = 0; s < KS; s++) kr[t][s] = ld16(k + (k_off + 64 * s));
 #pragma unroll
-                for (int i = 0; i < VR; i++) vr[t][i] = ld16(v + i * 1024 + lane * 16);
+                for (int i = 0; i < VR; i++) vr[t][i] = ld16(v + (lane * 16u + i * 1024));
             }
         }
     };
 
-    int u = u0 + CP * wave;
-    if (u < u1) load(u);
+    int u = u0 + CP * wave, next = 0;              // next: lane of the next chunk's first page
+    if (u < u1) {
+        look_up(u);
+        load(0);
+        next = CP;
+    }
     for (; u < u1; u += 4 * CP) {
         // ---- scores, row c's keys 16t + 4g + i, times log2(e) / sqrt(D)
         float p[RT][CP][4];
@@ -229,7 +242,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
         uint32_t vks[CP];
 #pragma unroll
         for (int t = 0; t < CP; t++) {
-            b[t] = blk[t];
+            b[t] = page_at(list, u + t);
             vks[t] = vs[t];
 #pragma unroll
             for (int i = 0; i < VR; i++) vk[t][i] = vr[t][i];
@@ -239,7 +252,11 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
         bool some = false;
 #pragma unroll
         for (int t = 0; t < CP; t++) some = some || partial(t);
-        if (u + 4 * CP < u1) load(u + 4 * CP);
+        if (u + 4 * CP < u1) {
+            if (next == 64) { look_up(u + 4 * CP); next = 0; }
+            load(next);
+            next += CP;
+        }
         auto seen = [&](int rt, int t, int key) {  // key: row of page t
             const int j = b[t] * KPAGE + key;
             return (in_pool >> t & 1) && ((j >= rlo[rt] && j < rhi[rt]) || j < rsk[rt]);
@@ -290,34 +307,39 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
                 const int t = 2 * half + tt;
                 // In a page that rows see in part the values of keys that no row sees become 0, and so does every value
                 // that is no number (0 x NaN is NaN): the rows that do see it are given it at the end.
-                const bool part = some && partial(t);
-                auto keep = [&](uint4 x, int key) {
-                    if (!part) return x;
-                    const int j = b[t] * KPAGE + key;
-                    if (!(in_pool >> t & 1) || !((j >= lo && j < hi) || (j < a.sinks && j < lo_most))) return make_uint4(0, 0, 0, 0);
-                    uint32_t w[4] = {x.x, x.y, x.z, x.w};
+                auto put = [&](auto keep) {
+                    if constexpr (FMT == FMT_FP4) {
+                        const int key = lane >> 2; // D = 128: a block a lane; D = 64: half a block
+                        const float sc = fp4_scale(vks[t]);
+                        const uint32_t w[4] = {vk[t][0].x, vk[t][0].y, vk[t][0].z, vk[t][0].w};
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        constexpr uint32_t EX = H ? 0x7c00u : 0x7f80u;
-                        if ((w[e] & EX) == EX) { w[e] &= 0xffff0000u; odd = true; }
-                        if ((w[e] >> 16 & EX) == EX) { w[e] &= 0xffffu; odd = true; }
+                        for (int e = 0; e < D / 32; e++)
+                            *reinterpret_cast<uint4*>(vt + v_at<D>(16 * tt + key, (lane & 3) * (D / 32) + e)) = keep(fp4_to_bf16(w[e], sc), key);
+                    } else {
+                        constexpr int PPR = D / 8; // pieces per row
+#pragma unroll
+                        for (int i = 0; i < VR; i++) {
+                            const int key = (64 * i + lane) / PPR;
+                            *reinterpret_cast<uint4*>(vt + v_at<D>(16 * tt + key, lane % PPR)) = keep(vk[t][i], key);
+                        }
                     }
-                    return make_uint4(w[0], w[1], w[2], w[3]);
                 };
-                if constexpr (FMT == FMT_FP4) {
-                    const int key = lane >> 2;     // D = 128: a block a lane; D = 64: half a block
-                    const float sc = fp4_scale(vks[t]);
-                    const uint32_t w[4] = {vk[t][0].x, vk[t][0].y, vk[t][0].z, vk[t][0].w};
+                if (some && partial(t)) {
+                    put([&](uint4 x, int key) {
+                        const int j = b[t] * KPAGE + key;
+                        if (!(in_pool >> t & 1) || !((j >= lo && j < hi) || (j < a.sinks && j < lo_most))) return make_uint4(0, 0, 0, 0);
+                        uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-                    for (int e = 0; e < D / 32; e++)
-                        *reinterpret_cast<uint4*>(vt + v_at<D>(16 * tt + key, (lane & 3) * (D / 32) + e)) = keep(fp4_to_bf16(w[e], sc), key);
+                        for (int e = 0; e < 4; e++) {
+                            constexpr uint32_t EX = H ? 0x7c00u : 0x7f80u;
+                            const bool low = (w[e] & EX) == EX, high = (w[e] >> 16 & EX) == EX;
+                            w[e] = (low ? 0u : w[e] & 0xffffu) | (high ? 0u : w[e] & 0xffff0000u);
+                            odd |= low | high;
+                        }
+                        return make_uint4(w[0], w[1], w[2], w[3]);
+                    });
                 } else {
-                    constexpr int PPR = D / 8;     // pieces per row
-#pragma unroll
-                    for (int i = 0; i < VR; i++) {
-                        const int key = (64 * i + lane) / PPR;
-                        *reinterpret_cast<uint4*>(vt + v_at<D>(16 * tt + key, lane % PPR)) = keep(vk[t][i], key);
-                    }
+                    put([](uint4 x, int) { return x; });
                 }
             }
             __builtin_amdgcn_wave_barrier();
