@@ -53,6 +53,15 @@ template <bool H> __device__ __forceinline__ uint4 fp4_to_16(uint32_t w, uint32_
     }
 }
 
+// x's two values added to acc.
+template <bool H> __device__ __forceinline__ float dot_ones(uint32_t x, float acc) {
+    if constexpr (H) return __builtin_amdgcn_fdot2(as_half2(x), as_half2(0x3c003c00u), acc, false);
+    else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, x), __builtin_bit_cast(bf16x2_t, 0x3f803f80u), acc, false);
+}
+
+// Keeps the instructions that make v where they are written.
+__device__ __forceinline__ void pin(float& v) { asm volatile("" : "+v"(v)); }
+
 template <int N, typename F> __device__ __forceinline__ int wave_fold(int v, F f) {
 #pragma unroll
     for (int d = N / 2; d > 0; d >>= 1) v = f(v, __shfl_xor(v, d));
@@ -75,14 +84,12 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
     if ((int64_t)qb * 128 >= total) return;
     __shared__ __align__(16) char kt[2][64 * 2 * D], vt[2][64 * 2 * D];
     __shared__ int fold[4][4];
-    __shared__ int page_of[2][4];                  // logical page, or -1 where there is none
     __shared__ int odd;                            // a value that is no number has been left out
 
     // ---- this lane's row, and what the workgroup's rows see
-    const int64_t rho = (int64_t)qb * 128 + 32 * wave + col;
+    const int64_t rho = (int64_t)qb * 128 + 32 * wave + col, rr = min(rho, total - 1);
     const bool real = rho < total;
-    const int64_t tok = s0 + (real ? rho : total - 1) / a.G;
-    const int64_t at = tok * a.Hq + (int64_t)kvh * a.G + (real ? rho : total - 1) % a.G;
+    const int64_t tok = s0 + rr / a.G, at = tok * a.Hq + (int64_t)kvh * a.G + rr % a.G;
     const int kmax = a.max_blocks * KPAGE;
     const int rlo = max(a.ranges[2 * tok], 0), rhi = min(a.ranges[2 * tok + 1], kmax);
     const bool some_key = real && rlo < rhi;
@@ -124,128 +131,114 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
     constexpr float BASE_LAG = 8.0f;
     float base = -INFINITY, rsum = 0.0f;
 
-    // ---- wave w brings page 4 tile + w: into registers two tiles ahead, into LDS one tile ahead
+    // ---- the pool's pages (or -1) of 16 tiles at a time, one a lane, and of the 16 after them: read long before their use,
+    // since a tile's page is needed to even ask for its rows
     const int32_t* bt = a.bt + (int64_t)seq * a.max_blocks;
-    uint4 kr[VR], vr[VR];
-    uint32_t ks = 0, vs = 0;
-    int myblk = 0;
-    bool myheld = false;
-    auto load = [&](int tile) {
-        const int u = 4 * tile + wave;
-        const bool in = u < list.count;
-        myblk = page_at(list, in ? u : 0);
-        int page = bt[myblk];
-        myheld = in && page >= 0 && page < a.num_blocks;
-        page = myheld ? page : 0;
-        const int64_t at = ((int64_t)page * a.Hkv + kvh) * HEAD;
-        const char* k = a.kp + at;
-        const char* v = a.vp + at;
+    auto look_up = [&](int tile) {
+        const int u = 4 * tile + lane, page = u < list.count ? bt[page_at(list, u)] : -1;
+        return page < a.num_blocks ? page : -1;
+    };
+    int now = look_up(t0), then = look_up(t0 + 16);
+    uint64_t gaps = __ballot(now < 0);
+    int group = 0;                                 // of 16 tiles, that `now` holds
+    auto page_of = [&](int tile) {                 // this wave's page of a tile of `now` or `then`
+        const int x = tile - t0;
+        return __builtin_amdgcn_readlane((x >> 4) == group ? now : then, (4 * x + wave) & 63);
+    };
+    // bit t: page t of a tile of `now` is one of the pool's
+    auto held_of = [&](int tile) { return (uint32_t)~(gaps >> (4 * ((tile - t0) & 15))) & 15u; };
+    struct Rows { uint4 r[VR]; uint32_t e; };
+    auto load = [&](const char* pool, int page) {
+        Rows y;
+        const char* m = pool + ((int64_t)max(page, 0) * a.Hkv + kvh) * HEAD;
         if constexpr (FMT == FMT_FP4) {
             if constexpr (D == 128) {
-                kr[0] = ld16(k + lane * 16);
-                vr[0] = ld16(v + lane * 16);
-                ks = *reinterpret_cast<const uint8_t*>(k + Page<FMT, D>::CODES + lane);
-                vs = *reinterpret_cast<const uint8_t*>(v + Page<FMT, D>::CODES + lane);
+                y.r[0] = ld16(m + lane * 16u);
+                y.e = *reinterpret_cast<const uint8_t*>(m + (Page<FMT, D>::CODES + lane));
             } else {
-                const uint2 x = *reinterpret_cast<const uint2*>(k + lane * 8), y = *reinterpret_cast<const uint2*>(v + lane * 8);
-                kr[0] = make_uint4(x.x, x.y, 0, 0);
-                vr[0] = make_uint4(y.x, y.y, 0, 0);
-                ks = *reinterpret_cast<const uint8_t*>(k + Page<FMT, D>::CODES + (lane >> 1));
-                vs = *reinterpret_cast<const uint8_t*>(v + Page<FMT, D>::CODES + (lane >> 1));
+                const uint2 v = *reinterpret_cast<const uint2*>(m + lane * 8u);
+                y.r[0] = make_uint4(v.x, v.y, 0, 0);
+                y.e = *reinterpret_cast<const uint8_t*>(m + (Page<FMT, D>::CODES + (lane >> 1)));
             }
         } else {
 #pragma unroll
-            for (int i = 0; i < VR; i++) {
-                kr[i] = ld16(k + i * 1024 + lane * 16);
-                vr[i] = ld16(v + i * 1024 + lane * 16);
-            }
+            for (int i = 0; i < VR; i++) y.r[i] = ld16(m + (i * 1024 + lane * 16u));
         }
+        return y;
     };
-    auto sees = [&](int l, int e, int sk, int j) { return (j >= l && j < e) || j < sk; };
+    auto sees = [&](int j) { return (j >= rlo && j < rhi) || j < rsk; };
     // a page that some row of the workgroup does not see whole
     auto partial = [&](int blk) { return blk * KPAGE < lo_most || blk * KPAGE + KPAGE > hi_least; };
-    auto store = [&](int buf) {
-        // In such a page the values of rows that no query row sees become 0, and so does every value that is no number
-        // (0 x NaN is NaN): the rows that do see it are given it at the end.
-        const bool part = !myheld || partial(myblk);
-        auto keep = [&](uint4 x, int key) {
-            if (!part) return x;
-            const int j = myblk * KPAGE + key;
-            if (!myheld || !((j >= lo && j < hi) || (j < a.sinks && j < lo_most))) return make_uint4(0, 0, 0, 0);
-            uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                constexpr uint32_t EX = H ? 0x7c00u : 0x7f80u;
-                if ((w[e] & EX) == EX) { w[e] &= 0xffff0000u; odd = 1; }
-                if ((w[e] >> 16 & EX) == EX) { w[e] &= 0xffffu; odd = 1; }
-            }
-            return make_uint4(w[0], w[1], w[2], w[3]);
-        };
+    auto put = [&](char* dst, const Rows& y, auto keep) {
         if constexpr (FMT == FMT_FP4) {
             const int key = lane >> 2;
-            const uint32_t kw[4] = {kr[0].x, kr[0].y, kr[0].z, kr[0].w}, vw[4] = {vr[0].x, vr[0].y, vr[0].z, vr[0].w};
+            const uint32_t w[4] = {y.r[0].x, y.r[0].y, y.r[0].z, y.r[0].w};
 #pragma unroll
-            for (int e = 0; e < D / 32; e++) {
-                const int p = v_at<D>(16 * wave + key, (lane & 3) * (D / 32) + e);
-                *reinterpret_cast<uint4*>(kt[buf] + p) = fp4_to_16<H>(kw[e], ks);
-                *reinterpret_cast<uint4*>(vt[buf] + p) = keep(fp4_to_16<H>(vw[e], vs), key);
-            }
+            for (int e = 0; e < D / 32; e++)
+                *reinterpret_cast<uint4*>(dst + v_at<D>(16 * wave + key, (lane & 3) * (D / 32) + e)) = keep(fp4_to_16<H>(w[e], y.e), key);
         } else {
             constexpr int PPR = D / 8;
 #pragma unroll
             for (int i = 0; i < VR; i++) {
-                const int key = (64 * i + lane) / PPR, p = v_at<D>(16 * wave + key, lane % PPR);
-                *reinterpret_cast<uint4*>(kt[buf] + p) = kr[i];
-                *reinterpret_cast<uint4*>(vt[buf] + p) = keep(vr[i], key);
+                const int key = (64 * i + lane) / PPR;
+                *reinterpret_cast<uint4*>(dst + v_at<D>(16 * wave + key, lane % PPR)) = keep(y.r[i], key);
             }
         }
-        if (lane == 0) page_of[buf][wave] = myheld ? myblk : -1;
     };
-    if (t0 < t1) {
-        load(t0);
-        store(0);
-        if (t0 + 1 < t1) load(t0 + 1);
-        __syncthreads();
-    }
-    for (int tile = t0; tile < t1; tile++) {
-        const int buf = (tile - t0) & 1;
-        if (tile + 1 < t1) {
-            store(buf ^ 1);                        // read by all before the last barrier
-            if (tile + 2 < t1) load(tile + 2);
-        }
-        int b[4];
-        bool some = false;
+    auto put_k = [&](int tile, const Rows& y) {
+        put(kt[(tile - t0) & 1], y, [](uint4 v, int) { return v; });
+    };
+    auto put_v = [&](int tile, const Rows& y, int page) {
+        char* dst = vt[(tile - t0) & 1];
+        const int u = 4 * tile + wave, blk = page_at(list, u < list.count ? u : 0);
+        if (page >= 0 && !partial(blk)) {
+            put(dst, y, [](uint4 v, int) { return v; });
+        } else {
+            // In a page that rows see in part the values of keys that no row sees become 0, and so does every value that is
+            // no number (0 x NaN is NaN): the rows that do see it are given it at the end.
+            put(dst, y, [&](uint4 v, int key) {
+                const int j = blk * KPAGE + key;
+                if (page < 0 || !((j >= lo && j < hi) || (j < a.sinks && j < lo_most))) return make_uint4(0, 0, 0, 0);
+                uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            b[t] = __builtin_amdgcn_readfirstlane(page_of[buf][t]);
-            some = some || b[t] < 0 || b[t] * KPAGE < wlo_most || b[t] * KPAGE + KPAGE > whi_least;
+                for (int e = 0; e < 4; e++) {
+                    constexpr uint32_t EX = H ? 0x7c00u : 0x7f80u;
+                    const bool low = (w[e] & EX) == EX, high = (w[e] >> 16 & EX) == EX;
+                    w[e] = (low ? 0u : w[e] & 0xffffu) | (high ? 0u : w[e] & 0xffff0000u);
+                    if (low || high) odd = 1;
+                }
+                return make_uint4(w[0], w[1], w[2], w[3]);
+            });
         }
+    };
 
-        // ---- scores, keys 32 c + 8 (i / 4) + 4 h + i % 4 of the tile
-        f32x16_t p[2];
+    f32x16_t p[2];                                 // scores: keys 32 c + 8 (i / 4) + 4 h + i % 4 of the tile
+    float m = -INFINITY;                           // the largest, times log2(e) / sqrt(D)
+    auto largest = [&]() {
+        m = p[0][0];
 #pragma unroll
         for (int c = 0; c < 2; c++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) p[c][i] = 0.0f;
+            for (int i = c == 0; i < 16; i++) m = fmaxf(m, p[c][i]);
+    };
+    auto key_frag = [&](const char* k, int c, int s) { return *reinterpret_cast<const uint4*>(k + v_at<D>(32 * c + col, 2 * s + h)); };
+    // Scores that a row does not see become -inf, in tiles that some row of the wave does not see whole; then the base.
+    auto finish = [&](int tile) {
+        const uint32_t held = held_of(tile);
+        const int first = 4 * tile - list.sink + list.first;      // its first page, behind the sinks
+        if (held != 15 || 4 * tile < list.sink || first * KPAGE < wlo_most || first * KPAGE + 64 > whi_least) {
+            int b[4];
 #pragma unroll
-        for (int s = 0; s < KS; s++)
-#pragma unroll
-            for (int c = 0; c < 2; c++)
-                p[c] = mfma32<H>(*reinterpret_cast<const uint4*>(kt[buf] + v_at<D>(32 * c + col, 2 * s + h)), qf[s], p[c]);
-        if (some) {
+            for (int t = 0; t < 4; t++) b[t] = page_at(list, 4 * tile + t);
 #pragma unroll
             for (int c = 0; c < 2; c++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const int t = 2 * c + (i >> 3), j = b[t] * KPAGE + 8 * ((i >> 2) & 1) + 4 * h + (i & 3);
-                    p[c][i] = b[t] >= 0 && sees(rlo, rhi, rsk, j) ? p[c][i] : -INFINITY;
+                    p[c][i] = (held >> t & 1) && sees(j) ? p[c][i] : -INFINITY;
                 }
+            largest();
         }
-        float m = p[0][0];
-#pragma unroll
-        for (int c = 0; c < 2; c++)
-#pragma unroll
-            for (int i = c == 0; i < 16; i++) m = fmaxf(m, p[c][i]);
         m = xmax32(m) * a.scale;
         if (__any(m > base + BASE_LAG)) {          // the row's first key too: base is -inf
             const float to = fmaxf(base, m), keep = to == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(base - to);
@@ -256,34 +249,121 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
                 for (int i = 0; i < 16; i++) o[c][i] *= keep;
             base = to;
         }
-        const float off = base == -INFINITY ? 0.0f : base;
-        float sum = 0.0f;
-#pragma unroll
-        for (int c = 0; c < 2; c++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) {
-                p[c][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[c][i], a.scale, -off));
-                sum += p[c][i];
-            }
-        rsum += sum;
+    };
 
-        // ---- O^T += V^T . P^T, 16 keys at a time: 16 kk + 4 h .. + 3 and 8 on
-#pragma unroll
-        for (int kk = 0; kk < 4; kk++) {
-            const int x = 8 * (kk & 1);
-            const f32x16_t& pp = p[kk >> 1];
-            const uint4 pf = make_uint4(pack16<H>(pp[x], pp[x + 1]), pack16<H>(pp[x + 2], pp[x + 3]), pack16<H>(pp[x + 4], pp[x + 5]),
-                                        pack16<H>(pp[x + 6], pp[x + 7]));
-            const int r = 16 * kk + 4 * h + ((lane & 15) >> 2);
-#pragma unroll
-            for (int c = 0; c < CT; c++) {
-                const int pc = 4 * c + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), hb = (lane & 1) * 8;
-                const uint2 y = lds_tr16(vt[buf] + v_at<D>(r, pc) + hb), z = lds_tr16(vt[buf] + v_at<D>(r + 8, pc) + hb);
-                o[c] = mfma32<H>(make_uint4(y.x, y.y, z.x, z.y), pf, o[c]);
-            }
-        }
+    if (t0 < t1) {
+        // A tile's life: its keys are asked for two iterations before their product and its values two before theirs; K is
+        // in LDS one iteration before Q . K^T, which runs one ahead of P . V, beside the exponentials of the tile before.
+        int pk = page_of(t0), p1 = page_of(t0 + 1), pn = page_of(t0 + 2);
+        Rows k = load(a.kp, pk), v = load(a.vp, pk), k1 = load(a.kp, p1);
+        put_k(t0, k);
+        put_v(t0, v, pk);
+        put_k(t0 + 1, k1);
+        pk = p1;
+        k = load(a.kp, pn);
+        v = load(a.vp, pk);
         __syncthreads();
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) p[c][i] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < KS; s++) p[c] = mfma32<H>(key_frag(kt[0], c, s), qf[s], p[c]);
+        }
+        largest();
+        finish(t0);
+        __syncthreads();
+        // state: kt holds tile + 1, vt tile; k is tile + 2 and v tile + 1 on their way, pn and pk their pages
+        auto turn = [&](int tile, auto more) {
+            constexpr bool MORE = decltype(more)::value;
+            if constexpr (MORE) {
+                put_k(tile + 2, k);
+                put_v(tile + 1, v, pk);
+                pk = pn;
+                pn = page_of(tile + 3);
+                k = load(a.kp, pn);
+                v = load(a.vp, pk);
+            }
+            // ---- the next tile's scores, two products at a time, and between them this tile's probabilities: packed pairs,
+            // eight of a lane's scores being the B operand of 16 keys.  The order is kept by the scheduling barriers.
+            const f32x16_t x[2] = {p[0], p[1]};
+            const float off = base == -INFINITY ? 0.0f : base;
+            uint32_t pw[16];
+            const char* kb = kt[(tile + 1 - t0) & 1];
+            const char* vb = vt[(tile - t0) & 1];
+            uint4 kf[2][2];
+            if constexpr (MORE) {
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    kf[0][c] = key_frag(kb, c, 0);
+#pragma unroll
+                    for (int i = 0; i < 16; i++) p[c][i] = 0.0f;
+                }
+            }
+#pragma unroll
+            for (int s = 0; s < KS; s++) {
+                if constexpr (MORE) {
+                    if (s + 1 < KS) {
+#pragma unroll
+                        for (int c = 0; c < 2; c++) kf[(s + 1) & 1][c] = key_frag(kb, c, s + 1);
+                    }
+#pragma unroll
+                    for (int c = 0; c < 2; c++) p[c] = mfma32<H>(kf[s & 1][c], qf[s], p[c]);
+                }
+#pragma unroll
+                for (int n = 0; n < 16 / KS; n++) {
+                    const int w = s * (16 / KS) + n, i = 2 * (w & 7);
+                    const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[w >> 3][i], a.scale, -off));
+                    const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[w >> 3][i + 1], a.scale, -off));
+                    pw[w] = pack16<H>(e0, e1);
+                    rsum = dot_ones<H>(pw[w], rsum);
+                }
+                if constexpr (MORE) {
+                    pin(rsum);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            // ---- O^T += V^T . P^T, 16 keys at a time (16 kk + 4 h .. + 3 and 8 on), and the next tile's largest score
+            auto value_frag = [&](int z) {
+                const int r = 16 * (z / CT) + 4 * h + ((lane & 15) >> 2);
+                const int pc = 4 * (z % CT) + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), hb = (lane & 1) * 8;
+                const uint2 y = lds_tr16(vb + v_at<D>(r, pc) + hb), z8 = lds_tr16(vb + v_at<D>(r + 8, pc) + hb);
+                return make_uint4(y.x, y.y, z8.x, z8.y);
+            };
+            constexpr int Z = 4 * CT, AHEAD = 2;
+            uint4 vf[AHEAD + 1];
+#pragma unroll
+            for (int z = 0; z < AHEAD; z++) vf[z] = value_frag(z);
+            if constexpr (MORE) m = p[0][0];
+#pragma unroll
+            for (int z = 0; z < Z; z++) {
+                if (z + AHEAD < Z) vf[(z + AHEAD) % (AHEAD + 1)] = value_frag(z + AHEAD);
+                const int kk = z / CT;
+                o[z % CT] = mfma32<H>(vf[z % (AHEAD + 1)], make_uint4(pw[4 * kk], pw[4 * kk + 1], pw[4 * kk + 2], pw[4 * kk + 3]), o[z % CT]);
+                if constexpr (MORE) {
+#pragma unroll
+                    for (int i = 0; i < 32 / Z; i++) { const int n = z * (32 / Z) + i; m = fmaxf(m, p[n >> 4][n & 15]); }
+                    pin(m);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            if constexpr (MORE) {
+                finish(tile + 1);
+                __syncthreads();
+            }
+        };
+        for (int tile = t0; tile + 1 < t1; tile++) {
+            if (((tile + 1 - t0) & 15) == 0) {     // the next tile is the first of `then`
+                group++;
+                now = then;
+                gaps = __ballot(now < 0);
+                then = look_up(t0 + 16 * (group + 1));
+            }
+            turn(tile, std::true_type{});
+        }
+        turn(t1 - 1, std::false_type{});
     }
+    __syncthreads();
 
     if (odd) {
         // values that are no numbers, in pages that the workgroup's rows see in part: to the rows that see them
@@ -292,7 +372,6 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
             if (!partial(blk) || page < 0 || page >= a.num_blocks) continue;
             const char* v = a.vp + ((int64_t)page * a.Hkv + kvh) * HEAD;
             for (int key = 0; key < KPAGE; key++) {
-                const bool mine = sees(rlo, rhi, rsk, blk * KPAGE + key);
 #pragma unroll
                 for (int c = 0; c < CT; c++)
 #pragma unroll
@@ -306,7 +385,7 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
                             const uint16_t w = *reinterpret_cast<const uint16_t*>(v + (key * D + ch) * 2);
                             x = H ? h2f(w) : bf2f(w);
                         }
-                        o[c][i] += mine && !__builtin_isfinite(x) ? x : 0.0f;
+                        o[c][i] += sees(blk * KPAGE + key) && !__builtin_isfinite(x) ? x : 0.0f;
                     }
             }
         }
