@@ -169,46 +169,41 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
     auto sees = [&](int j) { return (j >= rlo && j < rhi) || j < rsk; };
     // a page that some row of the workgroup does not see whole
     auto partial = [&](int blk) { return blk * KPAGE < lo_most || blk * KPAGE + KPAGE > hi_least; };
-    auto put = [&](char* dst, const Rows& y, auto keep) {
-        if constexpr (FMT == FMT_FP4) {
-            const int key = lane >> 2;
-            const uint32_t w[4] = {y.r[0].x, y.r[0].y, y.r[0].z, y.r[0].w};
-#pragma unroll
-            for (int e = 0; e < D / 32; e++)
-                *reinterpret_cast<uint4*>(dst + v_at<D>(16 * wave + key, (lane & 3) * (D / 32) + e)) = keep(fp4_to_16<H>(w[e], y.e), key);
-        } else {
-            constexpr int PPR = D / 8;
-#pragma unroll
-            for (int i = 0; i < VR; i++) {
-                const int key = (64 * i + lane) / PPR;
-                *reinterpret_cast<uint4*>(dst + v_at<D>(16 * wave + key, lane % PPR)) = keep(y.r[i], key);
-            }
-        }
+    // A page's rows go to LDS in PIECES writes a lane, which the products below are mixed with.
+    constexpr int PIECES = D / 32;
+    auto piece_at = [&](int e) {                   // (row of the page, piece of the row)
+        if constexpr (FMT == FMT_FP4) return make_int2(lane >> 2, (lane & 3) * (D / 32) + e);
+        else return make_int2((64 * e + lane) / (D / 8), lane % (D / 8));
     };
-    auto put_k = [&](int tile, const Rows& y) {
-        put(kt[(tile - t0) & 1], y, [](uint4 v, int) { return v; });
+    auto piece = [&](const Rows& y, int e) {
+        if constexpr (FMT == FMT_FP4) return fp4_to_16<H>(e == 0 ? y.r[0].x : e == 1 ? y.r[0].y : e == 2 ? y.r[0].z : y.r[0].w, y.e);
+        else return y.r[e];
     };
-    auto put_v = [&](int tile, const Rows& y, int page) {
-        char* dst = vt[(tile - t0) & 1];
+    auto put = [&](char* dst, const Rows& y, int e) {
+        const int2 at = piece_at(e);
+        *reinterpret_cast<uint4*>(dst + v_at<D>(16 * wave + at.x, at.y)) = piece(y, e);
+    };
+    // A page of values that rows see in part, put once more: the values of keys that no row sees as 0, and so every value that
+    // is no number (0 x NaN is NaN): the rows that do see it are given it at the end.
+    auto clean = [&](int tile, const Rows& y, int page) {
         const int u = 4 * tile + wave, blk = page_at(list, u < list.count ? u : 0);
-        if (page >= 0 && !partial(blk)) {
-            put(dst, y, [](uint4 v, int) { return v; });
-        } else {
-            // In a page that rows see in part the values of keys that no row sees become 0, and so does every value that is
-            // no number (0 x NaN is NaN): the rows that do see it are given it at the end.
-            put(dst, y, [&](uint4 v, int key) {
-                const int j = blk * KPAGE + key;
-                if (page < 0 || !((j >= lo && j < hi) || (j < a.sinks && j < lo_most))) return make_uint4(0, 0, 0, 0);
-                uint32_t w[4] = {v.x, v.y, v.z, v.w};
+        if (page >= 0 && !partial(blk)) return;
+        char* dst = vt[(tile - t0) & 1];
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    constexpr uint32_t EX = H ? 0x7c00u : 0x7f80u;
-                    const bool low = (w[e] & EX) == EX, high = (w[e] >> 16 & EX) == EX;
-                    w[e] = (low ? 0u : w[e] & 0xffffu) | (high ? 0u : w[e] & 0xffff0000u);
-                    if (low || high) odd = 1;
-                }
-                return make_uint4(w[0], w[1], w[2], w[3]);
-            });
+        for (int e = 0; e < PIECES; e++) {
+            const int2 at = piece_at(e);
+            const int j = blk * KPAGE + at.x;
+            const uint4 v = piece(y, e);
+            uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            const bool none = page < 0 || !((j >= lo && j < hi) || (j < a.sinks && j < lo_most));
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                constexpr uint32_t EX = H ? 0x7c00u : 0x7f80u;
+                const bool low = (w[i] & EX) == EX, high = (w[i] >> 16 & EX) == EX;
+                if (!none && (low || high)) odd = 1;
+                w[i] = none ? 0u : (low ? 0u : w[i] & 0xffffu) | (high ? 0u : w[i] & 0xffff0000u);
+            }
+            *reinterpret_cast<uint4*>(dst + v_at<D>(16 * wave + at.x, at.y)) = make_uint4(w[0], w[1], w[2], w[3]);
         }
     };
 
@@ -256,9 +251,9 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
         // in LDS one iteration before Q . K^T, which runs one ahead of P . V, beside the exponentials of the tile before.
         int pk = page_of(t0), p1 = page_of(t0 + 1), pn = page_of(t0 + 2);
         Rows k = load(a.kp, pk), v = load(a.vp, pk), k1 = load(a.kp, p1);
-        put_k(t0, k);
-        put_v(t0, v, pk);
-        put_k(t0 + 1, k1);
+#pragma unroll
+        for (int e = 0; e < PIECES; e++) { put(kt[0], k, e); put(vt[0], v, e); put(kt[1], k1, e); }
+        clean(t0, v, pk);
         pk = p1;
         k = load(a.kp, pn);
         v = load(a.vp, pk);
@@ -276,14 +271,6 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
         // state: kt holds tile + 1, vt tile; k is tile + 2 and v tile + 1 on their way, pn and pk their pages
         auto turn = [&](int tile, auto more) {
             constexpr bool MORE = decltype(more)::value;
-            if constexpr (MORE) {
-                put_k(tile + 2, k);
-                put_v(tile + 1, v, pk);
-                pk = pn;
-                pn = page_of(tile + 3);
-                k = load(a.kp, pn);
-                v = load(a.vp, pk);
-            }
             // ---- the next tile's scores, two products at a time, and between them this tile's probabilities: packed pairs,
             // eight of a lane's scores being the B operand of 16 keys.  The order is kept by the scheduling barriers.
             const f32x16_t x[2] = {p[0], p[1]};
@@ -320,8 +307,13 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
                 }
                 if constexpr (MORE) {
                     pin(rsum);
+                    if (KS - 1 - s < PIECES) put(kt[(tile - t0) & 1], k, KS - 1 - s);
                     __builtin_amdgcn_sched_barrier(0);
                 }
+            }
+            if constexpr (MORE) {
+                p1 = page_of(tile + 3);
+                k = load(a.kp, p1);
             }
             // ---- O^T += V^T . P^T, 16 keys at a time (16 kk + 4 h .. + 3 and 8 on), and the next tile's largest score
             auto value_frag = [&](int z) {
@@ -344,10 +336,15 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
 #pragma unroll
                     for (int i = 0; i < 32 / Z; i++) { const int n = z * (32 / Z) + i; m = fmaxf(m, p[n >> 4][n & 15]); }
                     pin(m);
+                    if (z >= 2 && z < 2 + PIECES) put(vt[(tile + 1 - t0) & 1], v, z - 2);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
             if constexpr (MORE) {
+                clean(tile + 1, v, pk);
+                v = load(a.vp, pn);
+                pk = pn;
+                pn = p1;
                 finish(tile + 1);
                 __syncthreads();
             }
