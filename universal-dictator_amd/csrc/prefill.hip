@@ -9,7 +9,9 @@
 //  - S^T = K . Q^T and O^T = V^T . P^T on v_mfma_f32_32x32x16, a wave's 32 rows in the lanes: a lane has 32 scores of its
 //    row (the other half of the wave has the row's other 32), so that the running maximum and sum are in-lane but for one
 //    swap of the halves, and its probabilities are the B operand of the second product as they stand.
-//  - K and V rows lie in LDS permuted piecewise against bank conflicts; V^T is read by ds_read_b64_tr_b16.
+//  - K and V rows lie in LDS at padded distances against bank conflicts; V^T is read by ds_read_b64_tr_b16.
+#include <algorithm>
+
 #include "paged_attention.hpp"
 
 namespace ud {
@@ -74,6 +76,10 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
     constexpr bool H = std::is_same<E, ElH>::value;
     constexpr int KS = D / 16, CT = D / 32;        // products over the channels; channel tiles
     constexpr int HEAD = Page<FMT, D>::BYTES;
+    // Bytes between rows in LDS.  A lane's products read at fixed distances from one address each for K and V: no address
+    // arithmetic between them (a permutation of the pieces would need some, and the loop is short of VALU slots).  K: 16
+    // rows' pieces on distinct banks; V: 4 rows' 64 bytes on distinct banks.
+    constexpr int KROW = 2 * D + 16, VROW = 2 * D + 64;
     constexpr int VR = FMT == FMT_FP4 ? 1 : D / 32;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, h = lane >> 5;
@@ -82,7 +88,7 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
     const int s0 = min(max(a.q_start[seq], 0), a.rows), s1 = min(min(max(a.q_start[seq + 1], s0), a.rows), s0 + a.max_rows);
     const int64_t total = (int64_t)(s1 - s0) * a.G;
     if ((int64_t)qb * 128 >= total) return;
-    __shared__ __align__(16) char kt[2][64 * 2 * D], vt[2][64 * 2 * D];
+    __shared__ __align__(16) char kt[2][64 * KROW], vt[2][64 * VROW];
     __shared__ int fold[4][4];
     __shared__ int odd;                            // a value that is no number has been left out
 
@@ -169,19 +175,33 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
     auto sees = [&](int j) { return (j >= rlo && j < rhi) || j < rsk; };
     // a page that some row of the workgroup does not see whole
     auto partial = [&](int blk) { return blk * KPAGE < lo_most || blk * KPAGE + KPAGE > hi_least; };
-    // A page's rows go to LDS in PIECES writes a lane, which the products below are mixed with.
+    // A page's rows go to LDS in PIECES writes a lane, which the products below are mixed with.  MXFP4: a lane's block is
+    // PIECES pieces of its row, which its neighbours take in turn against bank conflicts.
     constexpr int PIECES = D / 32;
+    const int turned = D == 128 ? lane & 3 : (lane >> 1) & 1;
     auto piece_at = [&](int e) {                   // (row of the page, piece of the row)
-        if constexpr (FMT == FMT_FP4) return make_int2(lane >> 2, (lane & 3) * (D / 32) + e);
+        if constexpr (FMT == FMT_FP4) return make_int2(lane >> 2, (lane & 3) * PIECES + ((e + turned) & (PIECES - 1)));
         else return make_int2((64 * e + lane) / (D / 8), lane % (D / 8));
     };
-    auto piece = [&](const Rows& y, int e) {
+    auto piece = [&](const Rows& y, int e) {       // MXFP4: of the turned words (load)
         if constexpr (FMT == FMT_FP4) return fp4_to_16<H>(e == 0 ? y.r[0].x : e == 1 ? y.r[0].y : e == 2 ? y.r[0].z : y.r[0].w, y.e);
         else return y.r[e];
     };
-    auto put = [&](char* dst, const Rows& y, int e) {
+    auto turn_words = [&](Rows& y) {
+        if constexpr (FMT == FMT_FP4) {
+            uint4 v = y.r[0];
+            if constexpr (PIECES == 4) {
+                v = turned & 1 ? make_uint4(v.y, v.z, v.w, v.x) : v;
+                v = turned & 2 ? make_uint4(v.z, v.w, v.x, v.y) : v;
+            } else {
+                v = turned ? make_uint4(v.y, v.x, 0, 0) : v;
+            }
+            y.r[0] = v;
+        }
+    };
+    auto put = [&](char* dst, int row, const Rows& y, int e) {
         const int2 at = piece_at(e);
-        *reinterpret_cast<uint4*>(dst + v_at<D>(16 * wave + at.x, at.y)) = piece(y, e);
+        *reinterpret_cast<uint4*>(dst + (16 * wave + at.x) * row + at.y * 16) = piece(y, e);
     };
     // A page of values that rows see in part, put once more: the values of keys that no row sees as 0, and so every value that
     // is no number (0 x NaN is NaN): the rows that do see it are given it at the end.
@@ -203,7 +223,7 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
                 if (!none && (low || high)) odd = 1;
                 w[i] = none ? 0u : (low ? 0u : w[i] & 0xffffu) | (high ? 0u : w[i] & 0xffff0000u);
             }
-            *reinterpret_cast<uint4*>(dst + v_at<D>(16 * wave + at.x, at.y)) = make_uint4(w[0], w[1], w[2], w[3]);
+            *reinterpret_cast<uint4*>(dst + (16 * wave + at.x) * VROW + at.y * 16) = make_uint4(w[0], w[1], w[2], w[3]);
         }
     };
 
@@ -216,7 +236,9 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
 #pragma unroll
             for (int i = c == 0; i < 16; i++) m = fmaxf(m, p[c][i]);
     };
-    auto key_frag = [&](const char* k, int c, int s) { return *reinterpret_cast<const uint4*>(k + v_at<D>(32 * c + col, 2 * s + h)); };
+    auto key_frag = [&](const char* k, int c, int s) { return *reinterpret_cast<const uint4*>(k + 32 * c * KROW + 32 * s); };
+    const int k_lane = col * KROW + 16 * h;
+    const int v_lane = (4 * h + ((lane & 15) >> 2)) * VROW + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
     // Scores that a row does not see become -inf, in tiles that some row of the wave does not see whole; then the base.
     auto finish = [&](int tile) {
         const uint32_t held = held_of(tile);
@@ -251,8 +273,11 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
         // in LDS one iteration before Q . K^T, which runs one ahead of P . V, beside the exponentials of the tile before.
         int pk = page_of(t0), p1 = page_of(t0 + 1), pn = page_of(t0 + 2);
         Rows k = load(a.kp, pk), v = load(a.vp, pk), k1 = load(a.kp, p1);
+        turn_words(k);
+        turn_words(v);
+        turn_words(k1);
 #pragma unroll
-        for (int e = 0; e < PIECES; e++) { put(kt[0], k, e); put(vt[0], v, e); put(kt[1], k1, e); }
+        for (int e = 0; e < PIECES; e++) { put(kt[0], KROW, k, e); put(vt[0], VROW, v, e); put(kt[1], KROW, k1, e); }
         clean(t0, v, pk);
         pk = p1;
         k = load(a.kp, pn);
@@ -263,7 +288,7 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
 #pragma unroll
             for (int i = 0; i < 16; i++) p[c][i] = 0.0f;
 #pragma unroll
-            for (int s = 0; s < KS; s++) p[c] = mfma32<H>(key_frag(kt[0], c, s), qf[s], p[c]);
+            for (int s = 0; s < KS; s++) p[c] = mfma32<H>(key_frag(kt[0] + k_lane, c, s), qf[s], p[c]);
         }
         largest();
         finish(t0);
@@ -276,8 +301,8 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
             const f32x16_t x[2] = {p[0], p[1]};
             const float off = base == -INFINITY ? 0.0f : base;
             uint32_t pw[16];
-            const char* kb = kt[(tile + 1 - t0) & 1];
-            const char* vb = vt[(tile - t0) & 1];
+            const char* kb = kt[(tile + 1 - t0) & 1] + k_lane;
+            const char* vb = vt[(tile - t0) & 1] + v_lane;
             uint4 kf[2][2];
             if constexpr (MORE) {
 #pragma unroll
@@ -307,7 +332,8 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
                 }
                 if constexpr (MORE) {
                     pin(rsum);
-                    if (KS - 1 - s < PIECES) put(kt[(tile - t0) & 1], k, KS - 1 - s);
+                    if (KS - s == PIECES) turn_words(k);
+                    if (KS - 1 - s < PIECES) put(kt[(tile - t0) & 1], KROW, k, KS - 1 - s);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
@@ -317,16 +343,18 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
             }
             // ---- O^T += V^T . P^T, 16 keys at a time (16 kk + 4 h .. + 3 and 8 on), and the next tile's largest score
             auto value_frag = [&](int z) {
-                const int r = 16 * (z / CT) + 4 * h + ((lane & 15) >> 2);
-                const int pc = 4 * (z % CT) + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1), hb = (lane & 1) * 8;
-                const uint2 y = lds_tr16(vb + v_at<D>(r, pc) + hb), z8 = lds_tr16(vb + v_at<D>(r + 8, pc) + hb);
+                const char* at = vb + 16 * (z / CT) * VROW + 64 * (z % CT);
+                const uint2 y = lds_tr16(at), z8 = lds_tr16(at + 8 * VROW);
                 return make_uint4(y.x, y.y, z8.x, z8.y);
             };
             constexpr int Z = 4 * CT, AHEAD = 2;
             uint4 vf[AHEAD + 1];
 #pragma unroll
             for (int z = 0; z < AHEAD; z++) vf[z] = value_frag(z);
-            if constexpr (MORE) m = p[0][0];
+            if constexpr (MORE) {
+                m = p[0][0];
+                turn_words(v);
+            }
 #pragma unroll
             for (int z = 0; z < Z; z++) {
                 if (z + AHEAD < Z) vf[(z + AHEAD) % (AHEAD + 1)] = value_frag(z + AHEAD);
@@ -336,7 +364,7 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
 #pragma unroll
                     for (int i = 0; i < 32 / Z; i++) { const int n = z * (32 / Z) + i; m = fmaxf(m, p[n >> 4][n & 15]); }
                     pin(m);
-                    if (z >= 2 && z < 2 + PIECES) put(vt[(tile + 1 - t0) & 1], v, z - 2);
+                    if (z >= 2 && z < 2 + PIECES) put(vt[(tile + 1 - t0) & 1], VROW, v, z - 2);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
@@ -420,12 +448,18 @@ static void launch_prefill(const PrefillArgs& a, int n, int D, hipStream_t st) {
     }
 }
 
-// Blocks of 128 query rows of the longest sequence, and splits of their keys: wanted where the blocks leave CUs idle, and
-// not below 8 tiles of 64 keys each.
-constexpr int64_t PREFILL_TARGET = 256;
+// Blocks of 128 query rows of the longest sequence, and splits of their keys.
+// - At most 256 workgroups (one per CU; two fit): split until there are 512, down to 8 tiles of 64 keys each.
+// - Above: split up to 2,048, so that the unequal workgroups of unequal sequences fill each other's gaps, but not below 64
+//   tiles, since every split of a row costs its fp32 partial, written and read (520 bytes at D = 128).
+// us, 32/8 heads of 128, bf16, one split -> this rule: 16 rows behind 16,000 keys 322 -> 28 (64 splits), 512 rows 335 -> 181
+// (4); 512 behind 2,000 61 -> 45; 6 x 37-563 rows behind 4,000-12,000 (MXFP4) 400 -> 326 (3); 8 x 64-500 behind 2,700-8,000
+// 302 -> 291 (2).  Where it keeps one split, two lose: a causal prompt of 2,000 rows 58 -> 85, of 4,000 169 -> 232.
 static int64_t prefill_blocks(int64_t max_rows, int64_t group) { return (max_rows * group + 127) / 128; }
 static int prefill_splits(int64_t n, int64_t kv_heads, int64_t blocks, int64_t n_sinks, int64_t max_span) {
-    return split_plan(n * kv_heads * blocks, (max_pages(max_span, n_sinks) + 3) / 4, PREFILL_TARGET, 1, 8).splits;
+    const int64_t units = n * kv_heads * blocks, tiles = (max_pages(max_span, n_sinks) + 3) / 4;
+    const int64_t want = ((units <= 256 ? 512 : 2048) + units - 1) / units, most = tiles / (units <= 256 ? 8 : 64);
+    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), MAX_SPLITS));
 }
 
 }  // namespace ud
