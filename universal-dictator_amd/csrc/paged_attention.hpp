@@ -1,5 +1,5 @@
-// What the windowed attention kernels (window.hip, prefill.hip) share: LDS tiles of values, products of 16-bit operands
-// and their terms, the join of the splits of a query row.
+// What the windowed attention kernels (window.hip, prefill.hip) share: products of 16-bit operands and their terms, the
+// join of the splits of a query row.
 #pragma once
 #include <type_traits>
 
@@ -12,10 +12,10 @@ __device__ __forceinline__ uint2 lds_tr16(const char* p) {
     return __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) v4i16_t*)p));
 }
 
-// Address of piece p (16 bytes) of row r in a tile of 2 D-byte rows.
-template <int D> __device__ __forceinline__ int v_at(int r, int p) {
-    const int f = D == 128 ? (((r & 3) << 1) | ((r >> 2) & 1) | (r & 8)) : (r & 6);
-    return r * (2 * D) + ((p ^ f) << 4);
+// x's two values added to acc.
+template <bool H> __device__ __forceinline__ float dot_ones(uint32_t x, float acc) {
+    if constexpr (H) return __builtin_amdgcn_fdot2(as_half2(x), as_half2(0x3c003c00u), acc, false);
+    else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, x), __builtin_bit_cast(bf16x2_t, 0x3f803f80u), acc, false);
 }
 
 template <bool H> __device__ __forceinline__ f32x4_t mfma16(uint4 a, uint4 b, f32x4_t c) {

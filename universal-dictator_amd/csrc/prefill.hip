@@ -55,12 +55,6 @@ template <bool H> __device__ __forceinline__ uint4 fp4_to_16(uint32_t w, uint32_
     }
 }
 
-// x's two values added to acc.
-template <bool H> __device__ __forceinline__ float dot_ones(uint32_t x, float acc) {
-    if constexpr (H) return __builtin_amdgcn_fdot2(as_half2(x), as_half2(0x3c003c00u), acc, false);
-    else return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2_t, x), __builtin_bit_cast(bf16x2_t, 0x3f803f80u), acc, false);
-}
-
 // Keeps the instructions that make v where they are written.
 __device__ __forceinline__ void pin(float& v) { asm volatile("" : "+v"(v)); }
 

@@ -13,9 +13,8 @@
 //    into registers.  An MXFP4 lane's 16 bytes are one block of 32 channels, whose pieces serve the products over all
 //    blocks in turn (the channel order within a sum is free as long as q has the same).
 //  - lane (c, g) then holds row c's scores of keys 4g .. 4g + 3 of each tile, which is the B operand of
-//    O^T = V^T . P^T as it stands.  V goes through the wave's own LDS tile (rows permuted piecewise against bank
-//    conflicts) and comes back transposed by ds_read_b64_tr_b16.  MXFP4 is turned into bf16, which holds its values
-//    exactly, on the way.
+//    O^T = V^T . P^T as it stands.  V goes through the wave's own LDS tile and comes back transposed by
+//    ds_read_b64_tr_b16.  MXFP4 is turned into bf16, which holds its values exactly, on the way.
 //  - 16-bit operands with fp32 accuracy: a factor is split into terms (x = x0 + x1 + .., each the nearest 16-bit value
 //    of what is left), one product each.  q: one term of its own type; half for bf16 products two; fp32 three of bf16 or
 //    two of half (scaled by a power of two per row, so that no term leaves half's range).  Probabilities: as many terms
@@ -56,12 +55,15 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
     constexpr int KS = D / 32;                     // products over the channels
     constexpr int DT = D / 16;                     // channel tiles
     constexpr int HEAD = Page<FMT, D>::BYTES;
+    // Bytes between the rows of V in LDS: 8 rows' 32 bytes, which a product reads at once, lie on distinct banks, and every
+    // product reads at a fixed distance from one address (no address arithmetic between them).
+    constexpr int VROW = 2 * D + 32;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
     const int kvh = blockIdx.x, split = blockIdx.y / a.groups, seq = blockIdx.z;
     const int r0 = blockIdx.y % a.groups * (16 * RT);   // first of this workgroup's rows
     const int G = a.G, M = a.M, QR = min(M * G - r0, 16 * RT);
-    __shared__ __align__(16) char tile[4][32 * 2 * D];
+    __shared__ __align__(16) char tile[4][32 * VROW];
     __shared__ float wmax[4][16 * RT], wsum[4][16 * RT];
 
     // ---- the sequence's page list, and this lane's rows (row 16 rt + col: position r / G, head r % G)
@@ -211,7 +213,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
         next = CP;
     }
     for (; u < u1; u += 4 * CP) {
-        // ---- scores, row c's keys 16t + 4g + i, times log2(e) / sqrt(D)
+        // ---- scores (of q as it was scaled), row c's keys 16t + 4g + i
         float p[RT][CP][4];
 #pragma unroll
         for (int t = 0; t < CP; t++) {
@@ -233,41 +235,39 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
 #pragma unroll
                     for (int s = 0; s < KS; s++) acc = mfma16<H>(kf[s], qf[rt][s][x], acc);
 #pragma unroll
-                for (int i = 0; i < 4; i++) p[rt][t][i] = acc[i] * qscale[rt];
+                for (int i = 0; i < 4; i++) p[rt][t][i] = acc[i];
             }
         }
-        int b[CP];
         const uint32_t in_pool = held;
         uint4 vk[CP][VR];
         uint32_t vks[CP];
 #pragma unroll
         for (int t = 0; t < CP; t++) {
-            b[t] = page_at(list, u + t);
             vks[t] = vs[t];
 #pragma unroll
             for (int i = 0; i < VR; i++) vk[t][i] = vr[t][i];
         }
-        // a page that some row does not see whole (a row that sees nothing does not count: it is dropped at the end)
-        auto partial = [&](int t) { return !(in_pool >> t & 1) || b[t] * KPAGE < lo_most || b[t] * KPAGE + KPAGE > hi_least; };
-        bool some = false;
-#pragma unroll
-        for (int t = 0; t < CP; t++) some = some || partial(t);
+        // a chunk that some row does not see whole (a row that sees nothing does not count: it is dropped at the end)
+        const int first = u - list.sink + list.first;
+        const bool some = in_pool != (1u << CP) - 1 || u < list.sink || first * KPAGE < lo_most || (first + CP) * KPAGE > hi_least;
         if (u + 4 * CP < u1) {
             if (next == 64) { look_up(u + 4 * CP); next = 0; }
             load(next);
             next += CP;
         }
-        auto seen = [&](int rt, int t, int key) {  // key: row of page t
-            const int j = b[t] * KPAGE + key;
-            return (in_pool >> t & 1) && ((j >= rlo[rt] && j < rhi[rt]) || j < rsk[rt]);
-        };
         if (some) {
 #pragma unroll
-            for (int rt = 0; rt < RT; rt++)
+            for (int t = 0; t < CP; t++) {
+                const int j0 = page_at(list, u + t) * KPAGE + 4 * g;
 #pragma unroll
-                for (int t = 0; t < CP; t++)
+                for (int rt = 0; rt < RT; rt++)
 #pragma unroll
-                    for (int i = 0; i < 4; i++) p[rt][t][i] = seen(rt, t, 4 * g + i) ? p[rt][t][i] : -INFINITY;
+                    for (int i = 0; i < 4; i++) {
+                        const int j = j0 + i;
+                        const bool in = (in_pool >> t & 1) && ((j >= rlo[rt] && j < rhi[rt]) || j < rsk[rt]);
+                        p[rt][t][i] = in ? p[rt][t][i] : -INFINITY;
+                    }
+            }
         }
         // ---- running maximum and sum, probabilities
 #pragma unroll
@@ -277,7 +277,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
             for (int t = 0; t < CP; t++)
 #pragma unroll
                 for (int i = t == 0; i < 4; i++) m = fmaxf(m, p[rt][t][i]);
-            m = xmax32(xmax16(m));
+            m = xmax32(xmax16(m)) * qscale[rt];
             if (__any(m > rmax[rt] + BASE_LAG)) {  // the row's first key too: base is -inf
                 const float to = fmaxf(rmax[rt], m), keep = to == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(rmax[rt] - to);
                 rsum[rt] *= keep;
@@ -287,61 +287,59 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
                     for (int i = 0; i < 4; i++) o[d][rt][i] *= keep;
                 rmax[rt] = to;
             }
-            const float off = rmax[rt] == -INFINITY ? 0.0f : rmax[rt];
+            // halves: 2^7 times the probabilities, up to 2^15, so that small ones keep their bits (the sum has it too)
+            const float off = (rmax[rt] == -INFINITY ? 0.0f : rmax[rt]) - (H ? 7.0f : 0.0f);
             float sum = 0.0f;
 #pragma unroll
             for (int t = 0; t < CP; t++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    p[rt][t][i] = __builtin_amdgcn_exp2f(p[rt][t][i] - off);
-                    sum += p[rt][t][i];
+                    p[rt][t][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(p[rt][t][i], qscale[rt], -off));
+                    if constexpr (PT > 1) sum += p[rt][t][i];
                 }
-            rsum[rt] += sum;
+            rsum[rt] += sum;                       // one term: summed below, as rounded
         }
         // ---- O^T += V^T . P^T, 32 keys at a time through the wave's tile
 #pragma unroll
         for (int half = 0; half < CP / 2; half++) {
             __builtin_amdgcn_wave_barrier();       // the reads of the last 32 keys come first
+            // Where rows see the chunk in part, values of keys that no row sees become 0, and so does every value that is no
+            // number (0 x NaN is NaN): the rows that do see it are given it at the end.
+            auto stage = [&](auto part) {
 #pragma unroll
-            for (int tt = 0; tt < 2; tt++) {
-                const int t = 2 * half + tt;
-                // In a page that rows see in part the values of keys that no row sees become 0, and so does every value
-                // that is no number (0 x NaN is NaN): the rows that do see it are given it at the end.
-                auto put = [&](auto keep) {
-                    if constexpr (FMT == FMT_FP4) {
-                        const int key = lane >> 2; // D = 128: a block a lane; D = 64: half a block
-                        const float sc = fp4_scale(vks[t]);
-                        const uint32_t w[4] = {vk[t][0].x, vk[t][0].y, vk[t][0].z, vk[t][0].w};
+                for (int tt = 0; tt < 2; tt++)
 #pragma unroll
-                        for (int e = 0; e < D / 32; e++)
-                            *reinterpret_cast<uint4*>(vt + v_at<D>(16 * tt + key, (lane & 3) * (D / 32) + e)) = keep(fp4_to_bf16(w[e], sc), key);
-                    } else {
-                        constexpr int PPR = D / 8; // pieces per row
-#pragma unroll
-                        for (int i = 0; i < VR; i++) {
-                            const int key = (64 * i + lane) / PPR;
-                            *reinterpret_cast<uint4*>(vt + v_at<D>(16 * tt + key, lane % PPR)) = keep(vk[t][i], key);
+                    for (int e = 0; e < D / 32; e++) {
+                        const int t = 2 * half + tt;
+                        // MXFP4: a lane's block (D = 64: half a block), its pieces in pairs turned against bank conflicts
+                        const int turned = FMT == FMT_FP4 ? (lane >> 3) & 1 : 0;
+                        const int row = FMT == FMT_FP4 ? lane >> 2 : (64 * e + lane) / (D / 8);
+                        const int piece = FMT == FMT_FP4 ? (lane & 3) * (D / 32) + (e ^ turned) : lane % (D / 8);
+                        uint4 x;
+                        if constexpr (FMT == FMT_FP4) {
+                            const uint32_t w[4] = {vk[t][0].x, vk[t][0].y, vk[t][0].z, vk[t][0].w};
+                            x = fp4_to_bf16(turned ? w[e ^ 1] : w[e], fp4_scale(vks[t]));
+                        } else {
+                            x = vk[t][e];
                         }
+                        if constexpr (decltype(part)::value) {
+                            const int j = page_at(list, u + t) * KPAGE + row;
+                            const bool none = !(in_pool >> t & 1) || !((j >= lo && j < hi) || (j < a.sinks && j < lo_most));
+                            uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                constexpr uint32_t EX = H ? 0x7c00u : 0x7f80u;
+                                const bool low = (w[i] & EX) == EX, high = (w[i] >> 16 & EX) == EX;
+                                w[i] = none ? 0u : (low ? 0u : w[i] & 0xffffu) | (high ? 0u : w[i] & 0xffff0000u);
+                                odd |= !none && (low || high);
+                            }
+                            x = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                        *reinterpret_cast<uint4*>(vt + (16 * tt + row) * VROW + piece * 16) = x;
                     }
-                };
-                if (some && partial(t)) {
-                    put([&](uint4 x, int key) {
-                        const int j = b[t] * KPAGE + key;
-                        if (!(in_pool >> t & 1) || !((j >= lo && j < hi) || (j < a.sinks && j < lo_most))) return make_uint4(0, 0, 0, 0);
-                        uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            constexpr uint32_t EX = H ? 0x7c00u : 0x7f80u;
-                            const bool low = (w[e] & EX) == EX, high = (w[e] >> 16 & EX) == EX;
-                            w[e] = (low ? 0u : w[e] & 0xffffu) | (high ? 0u : w[e] & 0xffff0000u);
-                            odd |= low | high;
-                        }
-                        return make_uint4(w[0], w[1], w[2], w[3]);
-                    });
-                } else {
-                    put([](uint4 x, int) { return x; });
-                }
-            }
+            };
+            if (some) stage(std::true_type{});
+            else stage(std::false_type{});
             __builtin_amdgcn_wave_barrier();
             uint4 pf[RT][PT];
 #pragma unroll
@@ -349,17 +347,16 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
                 float x[8];
 #pragma unroll
                 for (int i = 0; i < 4; i++) { x[i] = p[rt][2 * half][i]; x[4 + i] = p[rt][2 * half + 1][i]; }
-                if constexpr (H) {                 // up to 2^15, so that small ones keep their bits
-#pragma unroll
-                    for (int i = 0; i < 8; i++) x[i] *= 128.0f;
-                }
                 split8<H, PT>(x, pf[rt]);
+                if constexpr (PT == 1) {
+                    const uint4 y = pf[rt][0];
+                    rsum[rt] = dot_ones<H>(y.w, dot_ones<H>(y.z, dot_ones<H>(y.y, dot_ones<H>(y.x, rsum[rt]))));
+                }
             }
-            const int k0 = 4 * g + (col >> 2);
+            const char* v_lane = vt + (4 * g + (col >> 2)) * VROW + 8 * (col & 3);
 #pragma unroll
             for (int d = 0; d < DT; d++) {
-                const int pc = 2 * d + ((col & 3) >> 1), hb = (col & 1) * 8;
-                const uint2 x = lds_tr16(vt + v_at<D>(k0, pc) + hb), y = lds_tr16(vt + v_at<D>(k0 + 16, pc) + hb);
+                const uint2 x = lds_tr16(v_lane + 32 * d), y = lds_tr16(v_lane + 32 * d + 16 * VROW);
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++)
 #pragma unroll
@@ -368,11 +365,22 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
         }
     }
     if (__any(odd)) {
-        // values that are no numbers, in pages that rows see in part: to the rows that see them
+        // the chunk of page u was not seen whole (as above)
+        auto dropped = [&](int u) {
+            u -= (u - u0) % CP;
+            uint32_t in_pool = 0;
+            for (int t = 0; t < CP && u + t < u1; t++) {
+                const int page = bt[page_at(list, u + t)];
+                in_pool |= (uint32_t)(page >= 0 && page < a.num_blocks) << t;
+            }
+            const int first = u - list.sink + list.first;
+            return in_pool != (1u << CP) - 1 || u < list.sink || first * KPAGE < lo_most || (first + CP) * KPAGE > hi_least;
+        };
+        // values that are no numbers, in chunks that rows see in part: to the rows that see them
         for (int u = u0; u < u1; u++) {
             if ((u - u0) / CP % 4 != wave) continue;
             const int blk = page_at(list, u), page = bt[blk];
-            if (page < 0 || page >= a.num_blocks || (blk * KPAGE >= lo_most && blk * KPAGE + KPAGE <= hi_least)) continue;
+            if (page < 0 || page >= a.num_blocks || !dropped(u)) continue;
             const char* v = a.vp + ((int64_t)page * a.Hkv + kvh) * HEAD;
             for (int key = 0; key < KPAGE; key++) {
                 const int j = blk * KPAGE + key;
@@ -406,7 +414,6 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
         if (g == 0) { wmax[wave][16 * rt + col] = rmax[rt]; wsum[wave][16 * rt + col] = empty ? 0.0f : l; }
     }
     __syncthreads();
-    constexpr float PUP = H ? 1.0f / 128.0f : 1.0f;
     // a wave's share of a row with maximum m over the waves (1 where both are -inf: a sum of NaN scores stays NaN)
     auto share = [](float mine, float m) { return mine == m ? 1.0f : __builtin_amdgcn_exp2f(mine - m); };
 #pragma unroll
@@ -417,7 +424,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
         for (int w = 1; w < 4; w++) m = fmaxf(m, wmax[w][rr]);
         // a wave without a key of the row adds nothing
         const bool none = rmax[rt] == -INFINITY;
-        const float f = share(rmax[rt], m) * PUP;
+        const float f = share(rmax[rt], m);
 #pragma unroll
         for (int d = 0; d < DT; d++) {
             const float4 x = none ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
