@@ -53,7 +53,8 @@ template <bool H, int T> __device__ __forceinline__ void split8(const float (&x)
     }
 }
 
-// The splits of one (query row, head) joined, a wave each: with split s's maximum m_s (of scores times log2(e)), sum l_s
+// The splits of one (query row, head) joined, 16 a wave (one round trip to memory however many there are; at most 16
+// splits: four rows a workgroup): with split s's maximum m_s (of scores times log2(e)), sum l_s
 // and unnormalised output x_s,  out = sum_s 2^(m_s - m) x_s / sum_s 2^(m_s - m) l_s.  A split without a key has m = -inf,
 // l = 0 and its x is not looked at.
 // The rows: `count` of them, or (start) those of each sequence y, tokens start[y] .. start[y + 1] - 1 of `tokens`, at most
@@ -64,61 +65,75 @@ struct JoinRows {
     const int32_t* start;
     int n;
 };
+constexpr int JOIN_DEEP = 16;                      // splits per wave, all loads in flight at once
 template <typename E, int D>
-__global__ __launch_bounds__(256) void join_splits_kernel(const float* part, const float* stat, void* out, JoinRows rows, int splits) {
+__global__ __launch_bounds__(1024) void join_splits_kernel(const float* part, const float* stat, void* out, JoinRows rows, int splits) {
     typedef typename E::S S;
-    constexpr int DL = D / 64, DEEP = 8;
-    const int lane = threadIdx.x & 63;
-    int64_t row = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if (row >= rows.count) return;
+    constexpr int DL = D / 64, CH = MAX_SPLITS / 64;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int each = (splits + JOIN_DEEP - 1) / JOIN_DEEP;       // waves per row
+    const int per = each == 1 ? 4 : 1;                           // rows per workgroup
+    __shared__ float red[16][D];
+    int64_t row = (int64_t)blockIdx.x * per + (each == 1 ? wave : 0);
+    bool real = row < rows.count;
     if (rows.start) {
         const int s0 = min(max(rows.start[blockIdx.y], 0), rows.tokens), s1 = min(max(rows.start[blockIdx.y + 1], s0), rows.tokens);
-        if (row >= (int64_t)(s1 - s0) * rows.heads) return;
+        real = real && row < (int64_t)(s1 - s0) * rows.heads;
         row += (int64_t)s0 * rows.heads;
     }
+    if (!real) return;                                           // with it the whole row's waves
     const float* st = stat + row * splits * 2;
-    const float* pr = part + row * splits * D + lane * DL;
-    constexpr int CH = MAX_SPLITS / 64;
+    const int first = each == 1 ? 0 : JOIN_DEEP * wave;          // this wave's splits
+    const float* pr = part + (row * splits + first) * D + lane * DL;
+    float x[JOIN_DEEP][DL];
+#pragma unroll
+    for (int s = 0; s < JOIN_DEEP; s++) {
+        const float* p = pr + (int64_t)min(s, splits - 1 - first) * D;
+        if constexpr (DL == 2) {
+            const float2 v = *reinterpret_cast<const float2*>(p);
+            x[s][0] = v.x; x[s][1] = v.y;
+        } else {
+            x[s][0] = *p;
+        }
+    }
+    // every wave: the row's maximum and sum over all splits
     float m[CH], l[CH], top = -INFINITY;
 #pragma unroll
     for (int k = 0; k < CH; k++) {
-        const int s = 64 * k + lane;
-        const float2 v = s < splits ? *reinterpret_cast<const float2*>(st + 2 * s) : make_float2(-INFINITY, 0.0f);
-        m[k] = v.x; l[k] = v.y;
-        top = fmaxf(top, v.x);
+        m[k] = -INFINITY; l[k] = 0.0f;
+        if (64 * k + lane < splits) {
+            const float2 v = *reinterpret_cast<const float2*>(st + 2 * (64 * k + lane));
+            m[k] = v.x; l[k] = v.y;
+        }
+        top = fmaxf(top, m[k]);
     }
     top = wave_max(top);
-    float sum = 0.0f, acc[DL];
+    float sum = 0.0f, mine = -1.0f;                              // mine: the weights of the 64 splits that this wave's are among
+#pragma unroll
+    for (int k = 0; k < CH; k++) {
+        const float w = m[k] == top ? 1.0f : __builtin_amdgcn_exp2f(m[k] - top);
+        sum += w * l[k];
+        if (first >> 6 == k) mine = m[k] == -INFINITY ? -1.0f : w;   // -1: not looked at
+    }
+    sum = wave_sum(sum);
+    float acc[DL];
 #pragma unroll
     for (int e = 0; e < DL; e++) acc[e] = 0.0f;
 #pragma unroll
-    for (int k = 0; k < CH; k++) {
-        if (64 * k >= splits) break;
-        const float w = m[k] == top ? 1.0f : __builtin_amdgcn_exp2f(m[k] - top);
-        sum += w * l[k];
-        const float wx = m[k] == -INFINITY ? -1.0f : w;   // -1: not looked at
-        const int cnt = min(64, splits - 64 * k);
-        for (int s0 = 0; s0 < cnt; s0 += DEEP) {
-            float x[DEEP][DL];
+    for (int s = 0; s < JOIN_DEEP; s++) {
+        const float w = first + s < splits ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), (first & 63) + s)) : -1.0f;
 #pragma unroll
-            for (int s = 0; s < DEEP; s++) {
-                const float* p = pr + (int64_t)(64 * k + min(s0 + s, cnt - 1)) * D;
-                if constexpr (DL == 2) {
-                    const float2 v = *reinterpret_cast<const float2*>(p);
-                    x[s][0] = v.x; x[s][1] = v.y;
-                } else {
-                    x[s][0] = *p;
-                }
-            }
-#pragma unroll
-            for (int s = 0; s < DEEP; s++) {
-                const float ws = s0 + s < cnt ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wx), s0 + s)) : -1.0f;
-#pragma unroll
-                for (int e = 0; e < DL; e++) acc[e] += ws < 0.0f ? 0.0f : ws * x[s][e];
-            }
-        }
+        for (int e = 0; e < DL; e++) acc[e] += w < 0.0f ? 0.0f : w * x[s][e];
     }
-    sum = wave_sum(sum);
+    if (each > 1) {
+#pragma unroll
+        for (int e = 0; e < DL; e++) red[wave][lane * DL + e] = acc[e];
+        __syncthreads();
+        if (wave) return;
+#pragma unroll
+        for (int e = 0; e < DL; e++)
+            for (int w = 1; w < each; w++) acc[e] += red[w][lane * DL + e];
+    }
     const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
     S* o = static_cast<S*>(out) + row * D + lane * DL;
 #pragma unroll
@@ -131,7 +146,9 @@ __global__ __launch_bounds__(256) void join_splits_kernel(const float* part, con
 }
 template <typename E, int D>
 static void launch_join(const float* part, const float* stat, void* out, const JoinRows& rows, int splits, hipStream_t st) {
-    hipLaunchKernelGGL((join_splits_kernel<E, D>), dim3((unsigned)((rows.count + 3) / 4), rows.start ? rows.n : 1), dim3(256), 0, st, part, stat, out, rows, splits);
+    const int each = (splits + JOIN_DEEP - 1) / JOIN_DEEP, per = each == 1 ? 4 : 1;
+    hipLaunchKernelGGL((join_splits_kernel<E, D>), dim3((unsigned)((rows.count + per - 1) / per), rows.start ? rows.n : 1),
+                       dim3(64 * (each == 1 ? 4 : each)), 0, st, part, stat, out, rows, splits);
 }
 
 }  // namespace ud

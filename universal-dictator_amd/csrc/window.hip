@@ -65,6 +65,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
     const int G = a.G, M = a.M, QR = min(M * G - r0, 16 * RT);
     __shared__ __align__(16) char tile[4][32 * VROW];
     __shared__ float wmax[4][16 * RT], wsum[4][16 * RT];
+    __shared__ int odd_of[4];
 
     // ---- the sequence's page list, and this lane's rows (row 16 rt + col: position r / G, head r % G)
     const int32_t* rg = a.ranges + (int64_t)2 * seq * M;
@@ -113,35 +114,43 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         const int r = 16 * rt + col;
-        const S* q = static_cast<const S*>(a.q) + out_row(min(r, QR - 1)) * D;
-        float x[KS][8];
-        float most = 0.0f;
-#pragma unroll
-        for (int s = 0; s < KS; s++) {
-            const int ch = FMT == FMT_FP4 ? g * (D / 4) + 8 * s : 32 * s + 8 * g;
-            float u[4], v[4];
-            load4<E>(q + ch, u);
-            load4<E>(q + ch + 4, v);
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                x[s][e] = r < QR ? u[e] : 0.0f;
-                x[s][4 + e] = r < QR ? v[e] : 0.0f;
-                most = fmaxf(most, fmaxf(fabsf(x[s][e]), fabsf(x[s][4 + e])));
-            }
-        }
+        const S* q = static_cast<const S*>(a.q) + out_row(min(r, QR - 1)) * D + (FMT == FMT_FP4 ? g * (D / 4) : 8 * g);
+        constexpr int STEP = FMT == FMT_FP4 ? 8 : 32;
         qscale[rt] = a.scale;
-        if constexpr (H && QT > 1) {               // the row's largest value to 2^10 .. 2^11
-            most = xmax32(xmax16(most));
-            const int ex = most > 0.0f && most < INFINITY ? 10 - min(max(ilogbf(most), -110), 110) : 0;
-            const float up = ldexpf(1.0f, ex);
-            qscale[rt] = a.scale * ldexpf(1.0f, -ex);
+        if constexpr (QT == 1) {
 #pragma unroll
-            for (int s = 0; s < KS; s++)
+            for (int s = 0; s < KS; s++) {
+                const uint4 x = ld16(q + STEP * s);
+                qf[rt][s][0] = r < QR ? x : make_uint4(0, 0, 0, 0);
+            }
+        } else {
+            float x[KS][8];
+            float most = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 8; e++) x[s][e] *= up;
+            for (int s = 0; s < KS; s++) {
+                float u[4], v[4];
+                load4<E>(q + STEP * s, u);
+                load4<E>(q + STEP * s + 4, v);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    x[s][e] = r < QR ? u[e] : 0.0f;
+                    x[s][4 + e] = r < QR ? v[e] : 0.0f;
+                    most = fmaxf(most, fmaxf(fabsf(x[s][e]), fabsf(x[s][4 + e])));
+                }
+            }
+            if constexpr (H) {                     // the row's largest value to 2^10 .. 2^11
+                most = xmax32(xmax16(most));
+                const int ex = most > 0.0f && most < INFINITY ? 10 - min(max(ilogbf(most), -110), 110) : 0;
+                const float up = ldexpf(1.0f, ex);
+                qscale[rt] = a.scale * ldexpf(1.0f, -ex);
+#pragma unroll
+                for (int s = 0; s < KS; s++)
+#pragma unroll
+                    for (int e = 0; e < 8; e++) x[s][e] *= up;
+            }
+#pragma unroll
+            for (int s = 0; s < KS; s++) split8<H, QT>(x[s], qf[rt][s]);
         }
-#pragma unroll
-        for (int s = 0; s < KS; s++) split8<H, QT>(x[s], qf[rt][s]);
     }
 
     f32x4_t o[DT][RT];
@@ -161,7 +170,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
     // 64 pages of the wave, so that the table is read once for 64 / CP chunks, not before each.
     const int32_t* bt = a.bt + (int64_t)seq * a.max_blocks;
     int pages = -1;
-    auto look_up = [&](int u) {
+    auto look_up = [&](int u) __attribute__((always_inline)) {
         const int at = u + lane / CP * (4 * CP) + lane % CP;
         pages = at < u1 ? bt[page_at(list, at)] : -1;
         pages = pages < a.num_blocks ? pages : -1;
@@ -177,7 +186,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
     const uint32_t ks_off = Page<FMT, D>::CODES + col * (D / 32) + (D == 128 ? g : g >> 1);
     const uint32_t vs_off = Page<FMT, D>::CODES + (D == 128 ? lane : lane >> 1);
 
-    auto load = [&](int first) {                   // first: lane that holds the chunk's first page
+    auto load = [&](int first) __attribute__((always_inline)) {                   // first: lane that holds the chunk's first page
         held = 0;
 #pragma unroll
         for (int t = 0; t < CP; t++) {
@@ -239,17 +248,65 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
             }
         }
         const uint32_t in_pool = held;
-        uint4 vk[CP][VR];
-        uint32_t vks[CP];
-#pragma unroll
-        for (int t = 0; t < CP; t++) {
-            vks[t] = vs[t];
-#pragma unroll
-            for (int i = 0; i < VR; i++) vk[t][i] = vr[t][i];
-        }
         // a chunk that some row does not see whole (a row that sees nothing does not count: it is dropped at the end)
         const int first = u - list.sink + list.first;
         const bool some = in_pool != (1u << CP) - 1 || u < list.sink || first * KPAGE < lo_most || (first + CP) * KPAGE > hi_least;
+        uint4 vb[2][VR];
+        uint32_t vbs[2];
+        // Where rows see the chunk in part, values of keys that no row sees become 0, and so does every value that is no
+        // number (0 x NaN is NaN): the rows that do see it are given it at the end.
+        auto stage = [&](int half, auto part) __attribute__((always_inline)) {
+#pragma unroll
+            for (int tt = 0; tt < 2; tt++)
+#pragma unroll
+                for (int e = 0; e < D / 32; e++) {
+                    const int t = 2 * half + tt;
+                    // MXFP4: a lane's block (D = 64: half a block), its pieces in pairs turned against bank conflicts
+                    const int turned = FMT == FMT_FP4 ? (lane >> 3) & 1 : 0;
+                    const int row = FMT == FMT_FP4 ? lane >> 2 : (64 * e + lane) / (D / 8);
+                    const int piece = FMT == FMT_FP4 ? (lane & 3) * (D / 32) + (e ^ turned) : lane % (D / 8);
+                    uint4 x;
+                    if constexpr (FMT == FMT_FP4) {
+                        const uint32_t w[4] = {vb[tt][0].x, vb[tt][0].y, vb[tt][0].z, vb[tt][0].w};
+                        x = fp4_to_bf16(turned ? w[e ^ 1] : w[e], fp4_scale(vbs[tt]));
+                    } else {
+                        x = vb[tt][e];
+                    }
+                    if constexpr (decltype(part)::value) {
+                        const int j = page_at(list, u + t) * KPAGE + row;
+                        const bool none = !(in_pool >> t & 1) || !((j >= lo && j < hi) || (j < a.sinks && j < lo_most));
+                        uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            constexpr uint32_t EX = H ? 0x7c00u : 0x7f80u;
+                            const bool low = (w[i] & EX) == EX, high = (w[i] >> 16 & EX) == EX;
+                            w[i] = none ? 0u : (low ? 0u : w[i] & 0xffffu) | (high ? 0u : w[i] & 0xffff0000u);
+                            odd |= !none && (low || high);
+                        }
+                        x = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                    *reinterpret_cast<uint4*>(vt + (16 * tt + row) * VROW + piece * 16) = x;
+                    if constexpr (decltype(part)::value) __builtin_amdgcn_sched_barrier(0);   // one at a time: few registers
+                }
+        };
+        // The V rows of 32 keys into the wave's tile (the rows of a second 32 are kept in registers until then).
+        auto put_v = [&](int half) __attribute__((always_inline)) {
+            __builtin_amdgcn_wave_barrier();       // the reads of the last 32 keys come first
+            if (some) stage(half, std::true_type{});
+            else stage(half, std::false_type{});
+            __builtin_amdgcn_wave_barrier();
+        };
+        auto take = [&](int half) __attribute__((always_inline)) {
+#pragma unroll
+            for (int tt = 0; tt < 2; tt++) {
+                vbs[tt] = vs[2 * half + tt];
+#pragma unroll
+                for (int i = 0; i < VR; i++) vb[tt][i] = vr[2 * half + tt][i];
+            }
+        };
+        take(0);
+        put_v(0);
+        if constexpr (CP > 2) take(1);
         if (u + 4 * CP < u1) {
             if (next == 64) { look_up(u + 4 * CP); next = 0; }
             load(next);
@@ -302,45 +359,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
         // ---- O^T += V^T . P^T, 32 keys at a time through the wave's tile
 #pragma unroll
         for (int half = 0; half < CP / 2; half++) {
-            __builtin_amdgcn_wave_barrier();       // the reads of the last 32 keys come first
-            // Where rows see the chunk in part, values of keys that no row sees become 0, and so does every value that is no
-            // number (0 x NaN is NaN): the rows that do see it are given it at the end.
-            auto stage = [&](auto part) {
-#pragma unroll
-                for (int tt = 0; tt < 2; tt++)
-#pragma unroll
-                    for (int e = 0; e < D / 32; e++) {
-                        const int t = 2 * half + tt;
-                        // MXFP4: a lane's block (D = 64: half a block), its pieces in pairs turned against bank conflicts
-                        const int turned = FMT == FMT_FP4 ? (lane >> 3) & 1 : 0;
-                        const int row = FMT == FMT_FP4 ? lane >> 2 : (64 * e + lane) / (D / 8);
-                        const int piece = FMT == FMT_FP4 ? (lane & 3) * (D / 32) + (e ^ turned) : lane % (D / 8);
-                        uint4 x;
-                        if constexpr (FMT == FMT_FP4) {
-                            const uint32_t w[4] = {vk[t][0].x, vk[t][0].y, vk[t][0].z, vk[t][0].w};
-                            x = fp4_to_bf16(turned ? w[e ^ 1] : w[e], fp4_scale(vks[t]));
-                        } else {
-                            x = vk[t][e];
-                        }
-                        if constexpr (decltype(part)::value) {
-                            const int j = page_at(list, u + t) * KPAGE + row;
-                            const bool none = !(in_pool >> t & 1) || !((j >= lo && j < hi) || (j < a.sinks && j < lo_most));
-                            uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                            for (int i = 0; i < 4; i++) {
-                                constexpr uint32_t EX = H ? 0x7c00u : 0x7f80u;
-                                const bool low = (w[i] & EX) == EX, high = (w[i] >> 16 & EX) == EX;
-                                w[i] = none ? 0u : (low ? 0u : w[i] & 0xffffu) | (high ? 0u : w[i] & 0xffff0000u);
-                                odd |= !none && (low || high);
-                            }
-                            x = make_uint4(w[0], w[1], w[2], w[3]);
-                        }
-                        *reinterpret_cast<uint4*>(vt + (16 * tt + row) * VROW + piece * 16) = x;
-                    }
-            };
-            if (some) stage(std::true_type{});
-            else stage(std::false_type{});
-            __builtin_amdgcn_wave_barrier();
+            if (half) put_v(half);
             uint4 pf[RT][PT];
 #pragma unroll
             for (int rt = 0; rt < RT; rt++) {
@@ -364,48 +383,9 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
             }
         }
     }
-    if (__any(odd)) {
-        // the chunk of page u was not seen whole (as above)
-        auto dropped = [&](int u) {
-            u -= (u - u0) % CP;
-            uint32_t in_pool = 0;
-            for (int t = 0; t < CP && u + t < u1; t++) {
-                const int page = bt[page_at(list, u + t)];
-                in_pool |= (uint32_t)(page >= 0 && page < a.num_blocks) << t;
-            }
-            const int first = u - list.sink + list.first;
-            return in_pool != (1u << CP) - 1 || u < list.sink || first * KPAGE < lo_most || (first + CP) * KPAGE > hi_least;
-        };
-        // values that are no numbers, in chunks that rows see in part: to the rows that see them
-        for (int u = u0; u < u1; u++) {
-            if ((u - u0) / CP % 4 != wave) continue;
-            const int blk = page_at(list, u), page = bt[blk];
-            if (page < 0 || page >= a.num_blocks || !dropped(u)) continue;
-            const char* v = a.vp + ((int64_t)page * a.Hkv + kvh) * HEAD;
-            for (int key = 0; key < KPAGE; key++) {
-                const int j = blk * KPAGE + key;
-#pragma unroll
-                for (int d = 0; d < DT; d++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const int ch = 16 * d + 4 * g + i;
-                        float x;
-                        if constexpr (FMT == FMT_FP4) {
-                            const uint8_t e = *reinterpret_cast<const uint8_t*>(v + Page<FMT, D>::CODES + key * (D / FP4_BLOCK) + ch / FP4_BLOCK);
-                            x = e == 255 ? NAN : 0.0f;
-                        } else {
-                            const uint16_t w = *reinterpret_cast<const uint16_t*>(v + (key * D + ch) * 2);
-                            x = H ? h2f(w) : bf2f(w);
-                        }
-                        x = __builtin_isfinite(x) ? 0.0f : x;
-#pragma unroll
-                        for (int rt = 0; rt < RT; rt++) o[d][rt][i] += (j >= rlo[rt] && j < rhi[rt]) || j < rsk[rt] ? x : 0.0f;
-                    }
-            }
-        }
-    }
-
     // ---- the four waves joined, a row tile at a time through their LDS tiles
+    if (lane == 0) odd_of[wave] = 0;
+    if (odd) odd_of[wave] = 1;
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         const float l = xadd32(xadd16(rsum[rt]));
@@ -414,6 +394,40 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
         if (g == 0) { wmax[wave][16 * rt + col] = rmax[rt]; wsum[wave][16 * rt + col] = empty ? 0.0f : l; }
     }
     __syncthreads();
+    // To channels ch .. ch + 3 of row r: the values that are no numbers, of keys that it sees, in chunks where they were left
+    // out.
+    auto give_odd = [&](int r, int ch, float (&y)[4]) {
+        const int m = (r0 + r) / G, l = max(rg[2 * m], 0), e = min(rg[2 * m + 1], kmax), sk = l < e ? min(a.sinks, l) : 0;
+        for (int c = u0; c < u1; c += CP) {
+            const int n = min(CP, u1 - c), first = c - list.sink + list.first;
+            bool some = n < CP || c < list.sink || first * KPAGE < lo_most || (first + CP) * KPAGE > hi_least;
+            for (int t = 0; t < n; t++) {
+                const int page = bt[page_at(list, c + t)];
+                some = some || page < 0 || page >= a.num_blocks;
+            }
+            if (!some) continue;
+            for (int t = 0; t < n; t++) {
+                const int blk = page_at(list, c + t), page = bt[blk];
+                if (page < 0 || page >= a.num_blocks) continue;
+                const char* v = a.vp + ((int64_t)page * a.Hkv + kvh) * HEAD;
+                for (int key = 0; key < KPAGE; key++) {
+                    const int j = blk * KPAGE + key;
+                    if (!((j >= l && j < e) || j < sk)) continue;
+                    for (int i = 0; i < 4; i++) {
+                        float x;
+                        if constexpr (FMT == FMT_FP4) {
+                            const uint8_t b = *reinterpret_cast<const uint8_t*>(v + Page<FMT, D>::CODES + key * (D / FP4_BLOCK) + (ch + i) / FP4_BLOCK);
+                            x = b == 255 ? NAN : 0.0f;
+                        } else {
+                            const uint16_t w = *reinterpret_cast<const uint16_t*>(v + (key * D + ch + i) * 2);
+                            x = H ? h2f(w) : bf2f(w);
+                        }
+                        y[i] += __builtin_isfinite(x) ? 0.0f : x;
+                    }
+                }
+            }
+        }
+    };
     // a wave's share of a row with maximum m over the waves (1 where both are -inf: a sum of NaN scores stays NaN)
     auto share = [](float mine, float m) { return mine == m ? 1.0f : __builtin_amdgcn_exp2f(mine - m); };
 #pragma unroll
@@ -445,6 +459,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
                 y[0] += v.x; y[1] += v.y; y[2] += v.z; y[3] += v.w;
                 l += wsum[w][r] * share(wmax[w][r], mm);
             }
+            if (odd_of[0] | odd_of[1] | odd_of[2] | odd_of[3]) give_odd(r, 4 * piece, y);
             if (a.splits == 1) {
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -477,10 +492,17 @@ static void launch_window(const WindowArgs& a, int n, int D, hipStream_t st) {
     else launch_window_d<E, FMT, 64>(a, n, st);
 }
 
-// Workgroups wanted: four per CU.  A workgroup's waves take 2 pages each at a time (MXFP4: 4).
-constexpr int64_t WINDOW_TARGET = 1024;
+// Workgroups wanted: 512, one round of two per CU.  A workgroup's first rows arrive some 3 us after its start (its ranges,
+// its table entries, its pages) and its waves are joined at its end, so fewer, longer ones pay while the chip is full.
+// us at 512 / 1,024 / 2,048 wanted, 32/8 heads of 128: 1 x 60,000 keys bf16 50.6 / 52.4 / 57.4, MXFP4 21.9 / 24.9 / 30.0;
+// 64 x 4,096 bf16 184 / 191 / 194, MXFP4 57.6 / 64.6 / 66.2; 64 x 1,000 bf16 51.0 / 56.8 / 59.5.  More of them only helps
+// where contexts differ widely: 8 x 1,000-30,000 bf16 114 / 112 / 98.  A workgroup's waves take 2 pages each at a time
+// (MXFP4: 4).
+constexpr int64_t WINDOW_TARGET = 512;
 static SplitPlan window_plan(int32_t n, int32_t kv_heads, int32_t n_sinks, int32_t max_span, int step) {
-    return split_plan((int64_t)n * kv_heads, max_pages(max_span, n_sinks), WINDOW_TARGET, step, step);
+    // (a window that does not start with a page has one more: the last split takes it)
+    const int64_t pages = ((int64_t)max_span + KPAGE - 1) / KPAGE + ((int64_t)n_sinks + KPAGE - 1) / KPAGE;
+    return split_plan((int64_t)n * kv_heads, pages < 1 ? 1 : pages, WINDOW_TARGET, step, step);
 }
 
 }  // namespace ud
