@@ -17,8 +17,8 @@ using namespace ud;
 extern "C" void list_of(int lo, int hi, int sinks, int* out) { PageList p = page_list(lo, hi, sinks); out[0] = p.sink; out[1] = p.first; out[2] = p.count; }
 extern "C" int at(int lo, int hi, int sinks, int u) { return page_at(page_list(lo, hi, sinks), u); }
 extern "C" long long most(int span, int sinks) { return max_pages(span, sinks); }
-extern "C" void plan(long long units, long long pages, long long target, long long step, long long least, int* out) {
-    SplitPlan p = split_plan(units, pages, target, step, least); out[0] = p.splits; out[1] = p.pages; }
+extern "C" void plan(long long want, long long pages, long long step, int* out) {
+    SplitPlan p = split_plan(want, pages, step); out[0] = p.splits; out[1] = p.pages; }
 '''
 
 
@@ -31,7 +31,7 @@ def plan(tmp_path_factory):
                     str(d / "plan.cpp"), "-o", so], check=True)
     lib = ctypes.CDLL(so)
     lib.most.restype = ctypes.c_longlong
-    lib.plan.argtypes = [ctypes.c_longlong] * 5 + [ctypes.c_void_p]
+    lib.plan.argtypes = [ctypes.c_longlong] * 3 + [ctypes.c_void_p]
     return lib
 
 
@@ -61,12 +61,12 @@ def test_page_lists_hold_every_visible_key_once(plan):
 def test_split_plans_cover_the_list(plan):
     rng = np.random.default_rng(2)
     for _ in range(500):
-        units, pages = int(rng.integers(1, 5000)), int(rng.integers(1, 20000))
+        want, pages = int(rng.integers(0, 600)), int(rng.integers(1, 20000))
         step = int(rng.choice([1, 8, 16]))
         out = (ctypes.c_int * 2)()
-        plan.plan(units, pages, 1024, step, step, out)
+        plan.plan(want, pages, step, out)
         splits, each = out
-        assert 1 <= splits <= 256 and each % step == 0
+        assert 1 <= splits <= min(256, max(1, want)) and each % step == 0
         assert splits * each >= pages > (splits - 1) * each
 
 

@@ -187,13 +187,19 @@ def _check(rc):
         raise EngineError(rc, (_lib.ud_last_error() or b"").decode())
 
 
+_device_seen = False
+
+
 def lib():
-    """The library, after checking that a HIP device is present."""
+    """The library, after checking (once) that a HIP device is present."""
+    global _device_seen
     l = load_library()
-    n = _i32(0)
-    rc = l.ud_device_count(ctypes.byref(n))
-    if rc != 0 or n.value < 1:
-        raise EngineError(-4, "no HIP device visible: the encoder step runs only on the GPU")
+    if not _device_seen:
+        n = _i32(0)
+        rc = l.ud_device_count(ctypes.byref(n))
+        if rc != 0 or n.value < 1:
+            raise EngineError(-4, "no HIP device visible: the encoder step runs only on the GPU")
+        _device_seen = True
     return l
 
 

@@ -54,19 +54,12 @@ struct SplitPlan {
 
 constexpr int MAX_SPLITS = 256;
 
-// units: workgroups without a split; target: workgroups wanted; step: pages that a workgroup takes at a time.
-inline SplitPlan split_plan(int64_t units, int64_t pages, int64_t target, int64_t step, int64_t least) {
-    int64_t want = (target + units - 1) / units;
-    const int64_t most = (pages + least - 1) / least;
-    if (want > most) want = most;
+// want: splits wanted; step: pages that a workgroup takes at a time, which a split is a multiple of.
+inline SplitPlan split_plan(int64_t want, int64_t pages, int64_t step) {
     if (want > MAX_SPLITS) want = MAX_SPLITS;
     if (want < 1) want = 1;
-    int64_t each = ((pages + want - 1) / want + step - 1) / step * step;
-    SplitPlan p;
-    p.splits = (int)((pages + each - 1) / each);
-    if (p.splits < 1) p.splits = 1;
-    p.pages = (int)each;
-    return p;
+    const int64_t each = ((pages + want - 1) / want + step - 1) / step * step;
+    return SplitPlan{(int)((pages + each - 1) / each), (int)each};
 }
 
 }  // namespace ud

@@ -492,17 +492,23 @@ static void launch_window(const WindowArgs& a, int n, int D, hipStream_t st) {
     else launch_window_d<E, FMT, 64>(a, n, st);
 }
 
-// Workgroups wanted: 512, one round of two per CU.  A workgroup's first rows arrive some 3 us after its start (its ranges,
-// its table entries, its pages) and its waves are joined at its end, so fewer, longer ones pay while the chip is full.
+// Workgroups: one round of two per CU (512), not quite full rather than just beyond, but at least three quarters of it.
+// A workgroup's first rows arrive some 3 us after its start (its ranges, its table entries, its pages) and its waves are
+// joined at its end, so few, long ones pay while the chip is full.
 // us at 512 / 1,024 / 2,048 wanted, 32/8 heads of 128: 1 x 60,000 keys bf16 50.6 / 52.4 / 57.4, MXFP4 21.9 / 24.9 / 30.0;
 // 64 x 4,096 bf16 184 / 191 / 194, MXFP4 57.6 / 64.6 / 66.2; 64 x 1,000 bf16 51.0 / 56.8 / 59.5.  More of them only helps
-// where contexts differ widely: 8 x 1,000-30,000 bf16 114 / 112 / 98.  A workgroup's waves take 2 pages each at a time
-// (MXFP4: 4).
-constexpr int64_t WINDOW_TARGET = 512;
+// where contexts differ widely: 8 x 1,000-30,000 bf16 114 / 112 / 98.
+// Beyond or below a round, 4,000 keys: 12 sequences (96 units) 576 -> 480 workgroups bf16 47.8 -> 43.2 us; 50 (400) 800 ->
+// 400 162 -> 146, MXFP4 61.5 -> 51.9; but 33 (264) 528 -> 264 117 -> 132.
+// A workgroup's waves take 2 pages each at a time (MXFP4: 4): step.
+constexpr int64_t WINDOW_ROUND = 512;
 static SplitPlan window_plan(int32_t n, int32_t kv_heads, int32_t n_sinks, int32_t max_span, int step) {
     // (a window that does not start with a page has one more: the last split takes it)
     const int64_t pages = ((int64_t)max_span + KPAGE - 1) / KPAGE + ((int64_t)n_sinks + KPAGE - 1) / KPAGE;
-    return split_plan((int64_t)n * kv_heads, pages < 1 ? 1 : pages, WINDOW_TARGET, step, step);
+    const int64_t units = (int64_t)n * kv_heads;
+    int64_t want = WINDOW_ROUND / units;
+    if (want * units < WINDOW_ROUND * 3 / 4) want++;
+    return split_plan(want, pages < 1 ? 1 : pages, step);
 }
 
 }  // namespace ud
