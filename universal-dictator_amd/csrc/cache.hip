@@ -123,6 +123,24 @@ __global__ __launch_bounds__(256) void norm_rope_append_kernel(AppendArgs a) {
     const int p = a.pos[row], s = a.seqs ? a.seqs[row] : (int)min(row, (int64_t)INT32_MAX);
     const int page = row_page(s, p, a.bt, a.n, a.max_blocks, a.num_blocks);
     if (page < 0) return;                          // uniform in the workgroup
+    // Raw values of four passes over the heads at a time: the first four are on their way while the angles are made.
+    constexpr int DEEP = 4, HPP = 256 / LPH;       // heads per pass
+    const int i = tid % LPH, heads = a.Hq + 2 * a.Hkv;
+    typedef typename std::conditional<sizeof(S) == 4, uint4, uint2>::type Raw;
+    Raw raw[DEEP][2];
+    auto load = [&](int h0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int n = 0; n < DEEP; n++) {
+            const int h = h0 + HPP * n;
+            if (h >= heads) continue;
+            const S* src = h < a.Hq ? static_cast<const S*>(a.q) + row * a.q_ld + (int64_t)h * D
+                           : h < a.Hq + a.Hkv ? static_cast<const S*>(a.k) + row * a.k_ld + (int64_t)(h - a.Hq) * D
+                                              : static_cast<const S*>(a.v) + row * a.v_ld + (int64_t)(h - a.Hq - a.Hkv) * D;
+            raw[n][0] = *reinterpret_cast<const Raw*>(src + 4 * i);
+            raw[n][1] = *reinterpret_cast<const Raw*>(src + 4 * i + D / 2);
+        }
+    };
+    load(tid / LPH);
     if (a.inv_freq) {
         if (tid < D / 2) {
             double sn, cs;
@@ -132,71 +150,73 @@ __global__ __launch_bounds__(256) void norm_rope_append_kernel(AppendArgs a) {
         }
         __syncthreads();
     }
-    const int i = tid % LPH;
-    for (int h = tid / LPH; h < a.Hq + 2 * a.Hkv; h += 256 / LPH) {
-        const bool is_q = h < a.Hq, is_k = !is_q && h < a.Hq + a.Hkv;
-        const int kvh = is_q ? 0 : is_k ? h - a.Hq : h - a.Hq - a.Hkv;
-        const S* src = is_q ? static_cast<const S*>(a.q) + row * a.q_ld + (int64_t)h * D
-                            : is_k ? static_cast<const S*>(a.k) + row * a.k_ld + (int64_t)kvh * D
-                                   : static_cast<const S*>(a.v) + row * a.v_ld + (int64_t)kvh * D;
-        float lo[4], hi[4];
-        load4<E>(src + 4 * i, lo);
-        load4<E>(src + 4 * i + D / 2, hi);
-        if (is_q || (is_k && !WIDE)) {
-            const float* w = is_q ? a.qw : a.kw;
-            if (w) {
-                float ss = 0.0f;
+    for (int h0 = tid / LPH; h0 < heads; h0 += DEEP * HPP) {
+        if (h0 >= DEEP * HPP) load(h0);
 #pragma unroll
-                for (int e = 0; e < 4; e++) ss += lo[e] * lo[e] + hi[e] * hi[e];
-                const float r = 1.0f / sqrtf(group_sum<LPH>(ss) * (1.0f / D) + a.eps);
+        for (int n = 0; n < DEEP; n++) {
+            const int h = h0 + HPP * n;
+            if (h >= heads) break;
+            const bool is_q = h < a.Hq, is_k = !is_q && h < a.Hq + a.Hkv;
+            const int kvh = is_q ? 0 : is_k ? h - a.Hq : h - a.Hq - a.Hkv;
+            float lo[4], hi[4];
+            widen4<E>(raw[n][0], lo);
+            widen4<E>(raw[n][1], hi);
+            if (is_q || (is_k && !WIDE)) {
+                const float* w = is_q ? a.qw : a.kw;
+                if (w) {
+                    float ss = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    lo[e] *= r * w[4 * i + e];
-                    hi[e] *= r * w[4 * i + e + D / 2];
-                }
-            }
-            if (a.inv_freq) {
+                    for (int e = 0; e < 4; e++) ss += lo[e] * lo[e] + hi[e] * hi[e];
+                    const float r = 1.0f / sqrtf(group_sum<LPH>(ss) * (1.0f / D) + a.eps);
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const float2 t = turn[4 * i + e];
-                    const float x = lo[e], y = hi[e];
-                    lo[e] = x * t.x - y * t.y;
-                    hi[e] = y * t.x + x * t.y;
-                }
-            }
-            if (is_q) {
-                S* o = static_cast<S*>(a.q_out) + row * a.qo_ld + (int64_t)h * D + 4 * i;
-                store4<E>(o, lo);
-                store4<E>(o + D / 2, hi);
-                continue;
-            }
-        } else if (is_k) {
-            double r = 1.0;
-            if (a.kw) {
-                double ss = 0.0;
-#pragma unroll
-                for (int e = 0; e < 4; e++) ss += (double)lo[e] * lo[e] + (double)hi[e] * hi[e];
-                r = 1.0 / sqrt(group_sum_d<LPH>(ss) * (1.0 / D) + (double)a.eps);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                double x = lo[e], y = hi[e];
-                if (a.kw) {
-                    x *= r * (double)a.kw[4 * i + e];
-                    y *= r * (double)a.kw[4 * i + e + D / 2];
+                    for (int e = 0; e < 4; e++) {
+                        lo[e] *= r * w[4 * i + e];
+                        hi[e] *= r * w[4 * i + e + D / 2];
+                    }
                 }
                 if (a.inv_freq) {
-                    const double2 t = turn_d[WIDE ? 4 * i + e : 0];
-                    const double z = x * t.x - y * t.y;
-                    y = y * t.x + x * t.y;
-                    x = z;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float2 t = turn[4 * i + e];
+                        const float x = lo[e], y = hi[e];
+                        lo[e] = x * t.x - y * t.y;
+                        hi[e] = y * t.x + x * t.y;
+                    }
                 }
-                lo[e] = round_odd(x);
-                hi[e] = round_odd(y);
+                if (is_q) {
+                    S* o = static_cast<S*>(a.q_out) + row * a.qo_ld + (int64_t)h * D + 4 * i;
+                    store4<E>(o, lo);
+                    store4<E>(o + D / 2, hi);
+                    continue;
+                }
+            } else if (is_k) {
+                double r = 1.0;
+                if (a.kw) {
+                    double ss = 0.0;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) ss += (double)lo[e] * lo[e] + (double)hi[e] * hi[e];
+                    r = 1.0 / sqrt(group_sum_d<LPH>(ss) * (1.0 / D) + (double)a.eps);
+                }
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    double x = lo[e], y = hi[e];
+                    if (a.kw) {
+                        x *= r * (double)a.kw[4 * i + e];
+                        y *= r * (double)a.kw[4 * i + e + D / 2];
+                    }
+                    if (a.inv_freq) {
+                        const double2 t = turn_d[WIDE ? 4 * i + e : 0];
+                        const double z = x * t.x - y * t.y;
+                        y = y * t.x + x * t.y;
+                        x = z;
+                    }
+                    lo[e] = round_odd(x);
+                    hi[e] = round_odd(y);
+                }
             }
+            char* pool = is_k ? a.kp : a.vp;
+            store_row<FMT, D>(pool + ((int64_t)page * a.Hkv + kvh) * Page<FMT, D>::BYTES, p % KPAGE, i, lo, hi);
         }
-        char* pool = is_k ? a.kp : a.vp;
-        store_row<FMT, D>(pool + ((int64_t)page * a.Hkv + kvh) * Page<FMT, D>::BYTES, p % KPAGE, i, lo, hi);
     }
 }
 

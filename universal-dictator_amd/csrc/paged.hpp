@@ -32,22 +32,21 @@ struct El32 { typedef float S; };
 struct ElBf { typedef uint16_t S; };
 struct ElH { typedef uint16_t S; };
 
-typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
-
-// Four consecutive elements as floats, and four floats stored (16-bit: rounded to nearest even; half saturates).
-template <typename E> __device__ __forceinline__ void load4(const typename E::S* p, float (&f)[4]);
-template <> __device__ __forceinline__ void load4<El32>(const float* p, float (&f)[4]) {
-    const float4 v = *reinterpret_cast<const float4*>(p);
-    f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
-}
-template <> __device__ __forceinline__ void load4<ElBf>(const uint16_t* p, float (&f)[4]) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
+// Four elements as floats, and four floats stored (16-bit: rounded to nearest even; half saturates).
+template <typename E> __device__ __forceinline__ void widen4(uint2 v, float (&f)[4]);
+template <> __device__ __forceinline__ void widen4<ElBf>(uint2 v, float (&f)[4]) {
     f[0] = __uint_as_float(v.x << 16); f[1] = __uint_as_float(v.x & 0xffff0000u);
     f[2] = __uint_as_float(v.y << 16); f[3] = __uint_as_float(v.y & 0xffff0000u);
 }
-template <> __device__ __forceinline__ void load4<ElH>(const uint16_t* p, float (&f)[4]) {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
+template <> __device__ __forceinline__ void widen4<ElH>(uint2 v, float (&f)[4]) {
     f[0] = half_lo(v.x); f[1] = half_hi(v.x); f[2] = half_lo(v.y); f[3] = half_hi(v.y);
+}
+template <typename E> __device__ __forceinline__ void widen4(uint4 v, float (&f)[4]) {
+    f[0] = __uint_as_float(v.x); f[1] = __uint_as_float(v.y); f[2] = __uint_as_float(v.z); f[3] = __uint_as_float(v.w);
+}
+template <typename E> __device__ __forceinline__ void load4(const typename E::S* p, float (&f)[4]) {
+    if constexpr (sizeof(typename E::S) == 4) widen4<E>(*reinterpret_cast<const uint4*>(p), f);
+    else widen4<E>(*reinterpret_cast<const uint2*>(p), f);
 }
 template <typename E> __device__ __forceinline__ void store4(typename E::S* p, const float (&f)[4]);
 template <> __device__ __forceinline__ void store4<El32>(float* p, const float (&f)[4]) {
