@@ -58,10 +58,15 @@ template <bool H> __device__ __forceinline__ uint4 fp4_to_16(uint32_t w, uint32_
 // Keeps the instructions that make v where they are written.
 __device__ __forceinline__ void pin(float& v) { asm volatile("" : "+v"(v)); }
 
-template <int N, typename F> __device__ __forceinline__ int wave_fold(int v, F f) {
-#pragma unroll
-    for (int d = N / 2; d > 0; d >>= 1) v = f(v, __shfl_xor(v, d));
-    return v;
+// f over 32 lanes (each half of the wave has the same values), in every lane.
+template <int CTRL> __device__ __forceinline__ int dpp_int(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xF, 0xF, false); }
+template <typename F> __device__ __forceinline__ int fold32(int v, F f) {
+    v = f(v, dpp_int<DPP_QUAD_1032>(v));
+    v = f(v, dpp_int<DPP_QUAD_2301>(v));
+    v = f(v, dpp_int<DPP_ROW_HALF_MIRROR>(v));
+    v = f(v, dpp_int<DPP_ROW_MIRROR>(v));
+    const auto r = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+    return f((int)r[0], (int)r[1]);
 }
 
 template <typename E, int FMT, int D>
@@ -80,25 +85,25 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
     const int kvh = blockIdx.x, seq = blockIdx.z;
     const int split = blockIdx.y % a.splits, qb = a.q_blocks - 1 - (int)(blockIdx.y / a.splits);   // the longest first
     const int s0 = min(max(a.q_start[seq], 0), a.rows), s1 = min(min(max(a.q_start[seq + 1], s0), a.rows), s0 + a.max_rows);
-    const int64_t total = (int64_t)(s1 - s0) * a.G;
-    if ((int64_t)qb * 128 >= total) return;
+    const int total = (s1 - s0) * a.G;             // at most 65535 x 128, the grid's limit
+    if (qb * 128 >= total) return;
     __shared__ __align__(16) char kt[2][64 * KROW], vt[2][64 * VROW];
     __shared__ int fold[4][4];
     __shared__ int odd;                            // a value that is no number has been left out
 
     // ---- this lane's row, and what the workgroup's rows see
-    const int64_t rho = (int64_t)qb * 128 + 32 * wave + col, rr = min(rho, total - 1);
+    const int rho = qb * 128 + 32 * wave + col, rr = min(rho, total - 1), tk = rr / a.G;
     const bool real = rho < total;
-    const int64_t tok = s0 + rr / a.G, at = tok * a.Hq + (int64_t)kvh * a.G + rr % a.G;
+    const int64_t tok = s0 + tk, at = tok * a.Hq + (int64_t)kvh * a.G + (rr - tk * a.G);
     const int kmax = a.max_blocks * KPAGE;
     const int rlo = max(a.ranges[2 * tok], 0), rhi = min(a.ranges[2 * tok + 1], kmax);
     const bool some_key = real && rlo < rhi;
     const int rsk = some_key ? min(a.sinks, rlo) : 0;
     auto least = [](int x, int y) { return min(x, y); };
     auto most = [](int x, int y) { return max(x, y); };
-    const int wlo = wave_fold<32>(some_key ? rlo : kmax, least), whi = wave_fold<32>(some_key ? rhi : 0, most);
-    const int wlo_most = __builtin_amdgcn_readfirstlane(wave_fold<32>(some_key ? rlo : 0, most));
-    const int whi_least = __builtin_amdgcn_readfirstlane(wave_fold<32>(some_key ? rhi : kmax, least));
+    const int wlo = fold32(some_key ? rlo : kmax, least), whi = fold32(some_key ? rhi : 0, most);
+    const int wlo_most = __builtin_amdgcn_readfirstlane(fold32(some_key ? rlo : 0, most));
+    const int whi_least = __builtin_amdgcn_readfirstlane(fold32(some_key ? rhi : kmax, least));
     if (lane == 0) { fold[wave][0] = wlo; fold[wave][1] = whi; fold[wave][2] = wlo_most; fold[wave][3] = whi_least; }
     if (tid == 0) odd = 0;
     __syncthreads();
