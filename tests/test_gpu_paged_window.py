@@ -60,6 +60,12 @@ def close(got, want, c, d, dtype, p_step):
     out, mag, top, dot, count = want
     got = got.reshape(out.shape)
     tol = ref.attention_tolerance(out, mag, top, dot, count, d, dtype, p_step)
+    if dtype == "f16":
+        tol = tol + 2.0 ** -25                          # an output below half's normal range: half its smallest step
+    if dtype == "f16" or c.fmt == "f16":
+        # a probability below half's normal range is off by half the smallest step, 2^-25 of 2^7 times it; their sum is 1 or more
+        most = max([np.abs(x[np.isfinite(x)]).max(initial=0) for x in c.v])
+        tol = tol + (count * 2.0 ** -32 * most)[:, None, None]
     off = np.abs(got - out)
     assert np.all(off <= tol), "worst %.3g of its tolerance at %s" % (np.nanmax(off / tol), np.unravel_index(np.nanargmax(off / tol), off.shape))
     assert np.all(got[count == 0] == 0)
@@ -321,6 +327,76 @@ def test_half_queries_saturate_large_fp4(gpu):
     held = ref.held(v[0, 0], "mxfp4")
     assert held[0] == 65536 and got[0] == 65504 and got[1] == -65504
     np.testing.assert_array_equal(got[2:], held[2:])
+
+
+def _ramp(rng, lens, hkv, d, fmt):
+    """Keys whose scores with a query along e climb (sequence 0), fall (1) or jump about (2) by far more than a running
+    maximum is allowed to lag behind."""
+    e = rng.standard_normal(d)
+    e /= np.linalg.norm(e)
+    out = []
+    for i, L in enumerate(lens):
+        t = np.arange(L) / 16
+        a = (t, -t, 40 * rng.standard_normal(L))[i % 3]
+        out.append(ref.held(0.1 * rng.standard_normal((L, hkv, d)) + a[:, None, None] * e, fmt))
+    return e, out
+
+
+@pytest.mark.parametrize("fmt,dtype", TYPES)
+def test_window_steep_scores(gpu, fmt, dtype):
+    """Scores that climb by hundreds over the keys: the sums are rescaled again and again, most of the keys end at 0."""
+    ud, rng, hq, hkv, d = gpu, np.random.default_rng(61), 8, 2, 128
+    lens = [1500, 900, 1200]
+    e, k = _ramp(rng, lens, hkv, d, fmt)
+    c = Cache(ud, rng, fmt, lens, hkv, d, k=k)
+    q = ref.rounded(rng.standard_normal((3, 2, hq, d)) * 0.3 + 30 * e, dtype)
+    ranges = np.array([[[0, L], [L // 3, L - 7]] for L in lens])
+    got = window(ud, c, q, ranges, 3, dtype)
+    want = ref.attention(q.reshape(6, hq, d), c.k, c.v, np.repeat(np.arange(3), 2), ranges.reshape(-1, 2), 3, hkv, c.most * 16)
+    close(got, want, c, d, dtype, P_STEP[fmt, dtype])
+
+
+@pytest.mark.parametrize("fmt,dtype", PROMPTS)
+def test_prefill_steep_scores(gpu, fmt, dtype):
+    ud, rng, hq, hkv, d = gpu, np.random.default_rng(62), 4, 2, 64
+    lens = [400, 300, 350]
+    e, k = _ramp(rng, lens, hkv, d, fmt)
+    c = Cache(ud, rng, fmt, lens, hkv, d, k=k)
+    new, past = [150, 60, 130], [250, 240, 220]
+    q = ref.rounded(rng.standard_normal((340, hq, d)) * 0.3 + 30 * e, dtype)
+    ranges = causal(new, past, 0)
+    got = prefill(ud, c, q, [0, 150, 210, 340], ranges, 0, dtype)
+    want = ref.attention(q, c.k, c.v, np.repeat(np.arange(3), new), ranges, 0, hkv, c.most * 16)
+    close(got, want, c, d, dtype, PROMPT_STEP[dtype])
+
+
+@pytest.mark.parametrize("fmt,dtype", [("bf16", "bf16"), ("f16", "f32"), ("mxfp4", "f16"), ("mxfp4", "f32"), ("f16", "f16")])
+def test_queries_that_are_no_numbers(gpu, fmt, dtype):
+    """A NaN or an infinity in one query row makes that row NaN and no other, an empty range stays 0."""
+    ud, rng, hq, hkv, d = gpu, np.random.default_rng(63), 4, 2, 64
+    c = Cache(ud, rng, fmt, [700, 40], hkv, d)
+    q = ref.rounded(rng.standard_normal((2, 3, hq, d)), dtype)
+    ranges = np.array([[[0, 700], [5, 690], [9, 9]], [[0, 40], [0, 1], [0, 39]]])
+    clean = window(ud, c, q, ranges, 0, dtype)
+    bad = q.copy()
+    bad[0, 1, 2, 7], bad[1, 0, 0, :], bad[0, 2, 1, 3], bad[1, 1, 3, 5] = np.nan, np.nan, np.nan, np.inf
+    got = window(ud, c, bad, ranges, 0, dtype)
+    rows = np.zeros(got.shape[:3], bool)
+    rows[0, 1, 2] = rows[1, 0, 0] = rows[1, 1, 3] = True
+    assert np.all(np.isnan(got[rows]))
+    np.testing.assert_array_equal(got[~rows], clean[~rows])
+    assert np.all(got[0, 2] == 0)
+    if dtype == "f32":
+        return
+    new = causal([130], [0], 0)
+    q = ref.rounded(rng.standard_normal((130, hq, d)), dtype)
+    clean = prefill(ud, c, q, [0, 130], new, 0, dtype)
+    bad = q.copy()
+    bad[77, 1, 0] = np.nan
+    got = prefill(ud, c, bad, [0, 130], new, 0, dtype)
+    assert np.all(np.isnan(got[77, 1]))
+    got[77, 1] = clean[77, 1]
+    np.testing.assert_array_equal(got, clean)
 
 
 # ---------------------------------------------------------------- together
