@@ -181,6 +181,8 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
     uint32_t ks[CP], vs[CP];
     uint32_t held = 0;                             // bit t: the page is one of the pool's
     char* vt = tile[wave];
+    // a page that every row sees whole
+    auto whole = [&](int blk) { return blk * KPAGE >= lo_most && blk * KPAGE + KPAGE <= hi_least; };
     bool odd = false;                              // a value that is no number has been left out
     const uint32_t k_off = FMT == FMT_FP4 ? col * (D / 2) + g * (D / 8) : col * (2 * D) + 16 * g;
     const uint32_t ks_off = Page<FMT, D>::CODES + col * (D / 32) + (D == 128 ? g : g >> 1);
@@ -223,48 +225,55 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
     }
     for (; u < u1; u += 4 * CP) {
         // ---- scores (of q as it was scaled), row c's keys 16t + 4g + i
+        // (the tiles side by side: their products do not wait for each other)
         float p[RT][CP][4];
+        f32x4_t acc[RT][CP];
 #pragma unroll
-        for (int t = 0; t < CP; t++) {
-            uint4 kf[KS];
+        for (int rt = 0; rt < RT; rt++)
 #pragma unroll
-            for (int s = 0; s < KS; s++) {
+            for (int t = 0; t < CP; t++) acc[rt][t] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int s = 0; s < KS; s++)
+#pragma unroll
+            for (int t = 0; t < CP; t++) {
+                uint4 kf;
                 if constexpr (FMT == FMT_FP4) {
                     const uint32_t w = s == 0 ? kr[t][0].x : s == 1 ? kr[t][0].y : s == 2 ? kr[t][0].z : kr[t][0].w;
-                    kf[s] = fp4_to_bf16(w, fp4_scale(ks[t]));
+                    kf = fp4_to_bf16(w, fp4_scale(ks[t]));
                 } else {
-                    kf[s] = kr[t][s];
+                    kf = kr[t][s];
                 }
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++)
+#pragma unroll
+                    for (int x = QT - 1; x >= 0; x--) acc[rt][t] = mfma16<H>(kf, qf[rt][s][x], acc[rt][t]);
             }
 #pragma unroll
-            for (int rt = 0; rt < RT; rt++) {
-                f32x4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int rt = 0; rt < RT; rt++)
 #pragma unroll
-                for (int x = QT - 1; x >= 0; x--)  // small terms first
+            for (int t = 0; t < CP; t++)
 #pragma unroll
-                    for (int s = 0; s < KS; s++) acc = mfma16<H>(kf[s], qf[rt][s][x], acc);
-#pragma unroll
-                for (int i = 0; i < 4; i++) p[rt][t][i] = acc[i];
-            }
-        }
+                for (int i = 0; i < 4; i++) p[rt][t][i] = acc[rt][t][i];
         const uint32_t in_pool = held;
         // a chunk that some row does not see whole (a row that sees nothing does not count: it is dropped at the end)
         const int first = u - list.sink + list.first;
         const bool some = in_pool != (1u << CP) - 1 || u < list.sink || first * KPAGE < lo_most || (first + CP) * KPAGE > hi_least;
         uint4 vb[2][VR];
         uint32_t vbs[2];
-        // Where rows see the chunk in part, values of keys that no row sees become 0, and so does every value that is no
-        // number (0 x NaN is NaN): the rows that do see it are given it at the end.
-        auto stage = [&](int half, auto part) __attribute__((always_inline)) {
+        // The V rows of 32 keys into the wave's tile (the rows of a second 32 are kept in registers until then).  MXFP4: a
+        // lane's block (D = 64: half a block), its pieces in pairs turned against bank conflicts.
+        const int turned = FMT == FMT_FP4 ? (lane >> 3) & 1 : 0;
+        auto at = [&](int tt, int e) {
+            const int row = FMT == FMT_FP4 ? lane >> 2 : (64 * e + lane) / (D / 8);
+            const int piece = FMT == FMT_FP4 ? (lane & 3) * (D / 32) + (e ^ turned) : lane % (D / 8);
+            return make_int2(row, (16 * tt + row) * VROW + piece * 16);
+        };
+        auto put_v = [&](int half) __attribute__((always_inline)) {
+            __builtin_amdgcn_wave_barrier();       // the reads of the last 32 keys come first
 #pragma unroll
             for (int tt = 0; tt < 2; tt++)
 #pragma unroll
                 for (int e = 0; e < D / 32; e++) {
-                    const int t = 2 * half + tt;
-                    // MXFP4: a lane's block (D = 64: half a block), its pieces in pairs turned against bank conflicts
-                    const int turned = FMT == FMT_FP4 ? (lane >> 3) & 1 : 0;
-                    const int row = FMT == FMT_FP4 ? lane >> 2 : (64 * e + lane) / (D / 8);
-                    const int piece = FMT == FMT_FP4 ? (lane & 3) * (D / 32) + (e ^ turned) : lane % (D / 8);
                     uint4 x;
                     if constexpr (FMT == FMT_FP4) {
                         const uint32_t w[4] = {vb[tt][0].x, vb[tt][0].y, vb[tt][0].z, vb[tt][0].w};
@@ -272,28 +281,30 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
                     } else {
                         x = vb[tt][e];
                     }
-                    if constexpr (decltype(part)::value) {
-                        const int j = page_at(list, u + t) * KPAGE + row;
-                        const bool none = !(in_pool >> t & 1) || !((j >= lo && j < hi) || (j < a.sinks && j < lo_most));
-                        uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            constexpr uint32_t EX = H ? 0x7c00u : 0x7f80u;
-                            const bool low = (w[i] & EX) == EX, high = (w[i] >> 16 & EX) == EX;
-                            w[i] = none ? 0u : (low ? 0u : w[i] & 0xffffu) | (high ? 0u : w[i] & 0xffff0000u);
-                            odd |= !none && (low || high);
-                        }
-                        x = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
-                    *reinterpret_cast<uint4*>(vt + (16 * tt + row) * VROW + piece * 16) = x;
-                    if constexpr (decltype(part)::value) __builtin_amdgcn_sched_barrier(0);   // one at a time: few registers
+                    *reinterpret_cast<uint4*>(vt + at(tt, e).y) = x;
                 }
-        };
-        // The V rows of 32 keys into the wave's tile (the rows of a second 32 are kept in registers until then).
-        auto put_v = [&](int half) __attribute__((always_inline)) {
-            __builtin_amdgcn_wave_barrier();       // the reads of the last 32 keys come first
-            if (some) stage(half, std::true_type{});
-            else stage(half, std::false_type{});
+            if (__builtin_expect(some, 0)) {
+                // In pages that rows see in part, values of keys that no row sees become 0, and so does every value that is
+                // no number (0 x NaN is NaN): the rows that do see it are given it at the end.  (A loop over what this lane has
+                // just written: few instructions, seldom run.)
+#pragma unroll 1
+                for (int i = 0; i < D / 16; i++) {
+                    const int tt = i / (D / 32), t = 2 * half + tt, blk = page_at(list, u + t);
+                    if ((in_pool >> t & 1) && whole(blk)) continue;
+                    const int2 x = at(tt, i % (D / 32));
+                    const int j = blk * KPAGE + x.x;
+                    const bool none = !(in_pool >> t & 1) || !((j >= lo && j < hi) || (j < a.sinks && j < lo_most));
+                    uint32_t* w = reinterpret_cast<uint32_t*>(vt + x.y);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        constexpr uint32_t EX = H ? 0x7c00u : 0x7f80u;
+                        const uint32_t v = w[k];
+                        const bool low = (v & EX) == EX, high = (v >> 16 & EX) == EX;
+                        w[k] = none ? 0u : (low ? 0u : v & 0xffffu) | (high ? 0u : v & 0xffff0000u);
+                        odd |= !none && (low || high);
+                    }
+                }
+            }
             __builtin_amdgcn_wave_barrier();
         };
         auto take = [&](int half) __attribute__((always_inline)) {
@@ -312,7 +323,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
             load(next);
             next += CP;
         }
-        if (some) {
+        if (__builtin_expect(some, 0)) {
 #pragma unroll
             for (int t = 0; t < CP; t++) {
                 const int j0 = page_at(list, u + t) * KPAGE + 4 * g;
@@ -394,36 +405,27 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
         if (g == 0) { wmax[wave][16 * rt + col] = rmax[rt]; wsum[wave][16 * rt + col] = empty ? 0.0f : l; }
     }
     __syncthreads();
-    // To channels ch .. ch + 3 of row r: the values that are no numbers, of keys that it sees, in chunks where they were left
+    // To channels ch .. ch + 3 of row r: the values that are no numbers, of keys that it sees, in pages where they were left
     // out.
     auto give_odd = [&](int r, int ch, float (&y)[4]) {
         const int m = (r0 + r) / G, l = max(rg[2 * m], 0), e = min(rg[2 * m + 1], kmax), sk = l < e ? min(a.sinks, l) : 0;
-        for (int c = u0; c < u1; c += CP) {
-            const int n = min(CP, u1 - c), first = c - list.sink + list.first;
-            bool some = n < CP || c < list.sink || first * KPAGE < lo_most || (first + CP) * KPAGE > hi_least;
-            for (int t = 0; t < n; t++) {
-                const int page = bt[page_at(list, c + t)];
-                some = some || page < 0 || page >= a.num_blocks;
-            }
-            if (!some) continue;
-            for (int t = 0; t < n; t++) {
-                const int blk = page_at(list, c + t), page = bt[blk];
-                if (page < 0 || page >= a.num_blocks) continue;
-                const char* v = a.vp + ((int64_t)page * a.Hkv + kvh) * HEAD;
-                for (int key = 0; key < KPAGE; key++) {
-                    const int j = blk * KPAGE + key;
-                    if (!((j >= l && j < e) || j < sk)) continue;
-                    for (int i = 0; i < 4; i++) {
-                        float x;
-                        if constexpr (FMT == FMT_FP4) {
-                            const uint8_t b = *reinterpret_cast<const uint8_t*>(v + Page<FMT, D>::CODES + key * (D / FP4_BLOCK) + (ch + i) / FP4_BLOCK);
-                            x = b == 255 ? NAN : 0.0f;
-                        } else {
-                            const uint16_t w = *reinterpret_cast<const uint16_t*>(v + (key * D + ch + i) * 2);
-                            x = H ? h2f(w) : bf2f(w);
-                        }
-                        y[i] += __builtin_isfinite(x) ? 0.0f : x;
+        for (int c = u0; c < u1; c++) {
+            const int blk = page_at(list, c), page = bt[blk];
+            if (whole(blk) || page < 0 || page >= a.num_blocks) continue;
+            const char* v = a.vp + ((int64_t)page * a.Hkv + kvh) * HEAD;
+            for (int key = 0; key < KPAGE; key++) {
+                const int j = blk * KPAGE + key;
+                if (!((j >= l && j < e) || j < sk)) continue;
+                for (int i = 0; i < 4; i++) {
+                    float x;
+                    if constexpr (FMT == FMT_FP4) {
+                        const uint8_t b = *reinterpret_cast<const uint8_t*>(v + Page<FMT, D>::CODES + key * (D / FP4_BLOCK) + (ch + i) / FP4_BLOCK);
+                        x = b == 255 ? NAN : 0.0f;
+                    } else {
+                        const uint16_t w = *reinterpret_cast<const uint16_t*>(v + (key * D + ch + i) * 2);
+                        x = H ? h2f(w) : bf2f(w);
                     }
+                    y[i] += __builtin_isfinite(x) ? 0.0f : x;
                 }
             }
         }
