@@ -65,13 +65,13 @@ struct JoinRows {
     const int32_t* start;
     int n;
 };
-constexpr int JOIN_DEEP = 16;                      // splits per wave, all loads in flight at once
-template <typename E, int D>
+// DEEP: splits per wave, all loads in flight at once.
+template <typename E, int D, int DEEP>
 __global__ __launch_bounds__(1024) void join_splits_kernel(const float* part, const float* stat, void* out, JoinRows rows, int splits) {
     typedef typename E::S S;
     constexpr int DL = D / 64, CH = MAX_SPLITS / 64;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int each = (splits + JOIN_DEEP - 1) / JOIN_DEEP;       // waves per row
+    const int each = (splits + DEEP - 1) / DEEP;                 // waves per row
     const int per = each == 1 ? 4 : 1;                           // rows per workgroup
     __shared__ float red[16][D];
     int64_t row = (int64_t)blockIdx.x * per + (each == 1 ? wave : 0);
@@ -83,11 +83,11 @@ __global__ __launch_bounds__(1024) void join_splits_kernel(const float* part, co
     }
     if (!real) return;                                           // with it the whole row's waves
     const float* st = stat + row * splits * 2;
-    const int first = each == 1 ? 0 : JOIN_DEEP * wave;          // this wave's splits
+    const int first = each == 1 ? 0 : DEEP * wave;               // this wave's splits
     const float* pr = part + (row * splits + first) * D + lane * DL;
-    float x[JOIN_DEEP][DL];
+    float x[DEEP][DL];
 #pragma unroll
-    for (int s = 0; s < JOIN_DEEP; s++) {
+    for (int s = 0; s < DEEP; s++) {
         const float* p = pr + (int64_t)min(s, splits - 1 - first) * D;
         if constexpr (DL == 2) {
             const float2 v = *reinterpret_cast<const float2*>(p);
@@ -120,7 +120,7 @@ __global__ __launch_bounds__(1024) void join_splits_kernel(const float* part, co
 #pragma unroll
     for (int e = 0; e < DL; e++) acc[e] = 0.0f;
 #pragma unroll
-    for (int s = 0; s < JOIN_DEEP; s++) {
+    for (int s = 0; s < DEEP; s++) {
         const float w = first + s < splits ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), (first & 63) + s)) : -1.0f;
 #pragma unroll
         for (int e = 0; e < DL; e++) acc[e] += w < 0.0f ? 0.0f : w * x[s][e];
@@ -144,11 +144,13 @@ __global__ __launch_bounds__(1024) void join_splits_kernel(const float* part, co
         else o[e] = f2h(y);
     }
 }
+// Up to four splits (prompts) a wave asks for no more than those: 57,600 rows of 3 splits 37.2 -> 23.1 us
 template <typename E, int D>
 static void launch_join(const float* part, const float* stat, void* out, const JoinRows& rows, int splits, hipStream_t st) {
-    const int each = (splits + JOIN_DEEP - 1) / JOIN_DEEP, per = each == 1 ? 4 : 1;
-    hipLaunchKernelGGL((join_splits_kernel<E, D>), dim3((unsigned)((rows.count + per - 1) / per), rows.start ? rows.n : 1),
-                       dim3(64 * (each == 1 ? 4 : each)), 0, st, part, stat, out, rows, splits);
+    const int each = splits <= 4 ? 1 : (splits + 15) / 16, per = each == 1 ? 4 : 1;
+    const dim3 grid((unsigned)((rows.count + per - 1) / per), rows.start ? rows.n : 1), block(64 * (each == 1 ? 4 : each));
+    if (splits <= 4) hipLaunchKernelGGL((join_splits_kernel<E, D, 4>), grid, block, 0, st, part, stat, out, rows, splits);
+    else hipLaunchKernelGGL((join_splits_kernel<E, D, 16>), grid, block, 0, st, part, stat, out, rows, splits);
 }
 
 }  // namespace ud
