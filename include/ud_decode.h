@@ -161,8 +161,10 @@ UD_API int ud_paged_kv_read(int32_t kv_format, int32_t dtype, const void* k_page
  *   max_span        upper bound of a sequence's keys from its lowest lo to its highest hi (sizes the grid; a longer
  *                   sequence is slower, not wrong)
  *   workspace       ud_gqa_window_workspace_bytes(..) bytes (0: may be null); its contents need not be kept
- * Only entries of the block table whose pages hold a sink or a key of the window are read: the pages between may have
- * been given back.  n_queries 1 .. 8, n_queries * q_heads / kv_heads <= 64.
+ * Only entries of the block table whose pages hold a sink or a key between a sequence's lowest lo and highest hi are
+ * read: the pages between may have been given back.  n_queries 1 .. 8, n_queries * q_heads / kv_heads <= 64.
+ * A call repeated gives the same bits; the keys are split over workgroups by n and max_span, so that the last bits of a
+ * row may differ between calls that differ in these.
  * Precision: fp32 queries and outputs are as good as fp32 arithmetic; 16-bit ones: exact products, sums in fp32, the
  * probabilities rounded once to the pages' type (bf16 for UD_MXFP4, twice that for half queries).  A NaN or infinity in
  * a key or value reaches only the rows that see it. */
@@ -182,7 +184,8 @@ UD_API int ud_gqa_window_attention_paged(int32_t kv_format, int32_t dtype, const
  *                   max_rows each; out rows of no sequence are left as they were
  *   ranges_dev      int32 [rows, 2]: row r sees [lo, hi) and the sinks below lo, as above (a causal prompt: hi = its
  *                   position + 1).  The keys are read from the pages: append before the call
- *   max_span        upper bound of a sequence's keys from its lowest lo to its highest hi (a plan, as above)
+ *   max_span        upper bound of a sequence's keys from its lowest lo to its highest hi (a plan, as above; n and
+ *                   max_rows count in it too)
  *   workspace       ud_gqa_prefill_workspace_bytes(..) bytes (0: may be null)
  * Precision: exact products, sums and softmax in fp32, probabilities rounded once to dtype, one rounding at the end.
  * UD_MXFP4 pages under half queries: cached values past half's range saturate. */

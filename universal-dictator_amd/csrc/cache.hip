@@ -12,7 +12,10 @@
 // frequency near 1 is off by 0.004 rad.
 // Keys for MXFP4 pages are normalised and rotated in 64 bits: a key next to a border between two codes would
 // otherwise move by a whole step of its block with the order of a sum, and so would every key of a block whose
-// largest value is next to a power of two's border.  That is 8 of 48 heads at 32/8, and hidden behind the loads.
+// largest value is next to a power of two's border.  That is 8 of 48 heads at 32/8.
+// Measured, 32/8 heads of 128: 8,200 rows of bf16 to MXFP4 pages 46 us (253 MB, 5.5 TB/s; a large copy on the same card
+// 4.7 .. 5.0), 64 rows 5.7 us, one row of fp32 to half pages 3.2 us: an empty launch's and one round trip to memory for the
+// row's position, its page and its heads.  Read back: 17.6, 3.6 and 1.9 us.
 #include <type_traits>
 
 #include "paged.hpp"

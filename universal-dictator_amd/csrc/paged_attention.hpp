@@ -57,6 +57,8 @@ template <bool H, int T> __device__ __forceinline__ void split8(const float (&x)
 // splits: four rows a workgroup): with split s's maximum m_s (of scores times log2(e)), sum l_s
 // and unnormalised output x_s,  out = sum_s 2^(m_s - m) x_s / sum_s 2^(m_s - m) l_s.  A split without a key has m = -inf,
 // l = 0 and its x is not looked at.
+// Bound: memory; of few rows the round trip.  57,600 rows of 3 splits at D = 128 (90 MB of partials) 23 us, 32 rows of 64
+// splits 4 us.
 // The rows: `count` of them, or (start) those of each sequence y, tokens start[y] .. start[y + 1] - 1 of `tokens`, at most
 // `count` rows each.
 struct JoinRows {
