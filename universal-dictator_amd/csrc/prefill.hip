@@ -180,31 +180,28 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
     // a page that some row of the workgroup does not see whole
     auto partial = [&](int blk) { return blk * KPAGE < lo_most || blk * KPAGE + KPAGE > hi_least; };
     // A page's rows go to LDS in PIECES writes a lane, which the products below are mixed with.  MXFP4: a lane's block is
-    // PIECES pieces of its row, which its neighbours take in turn against bank conflicts.
+    // PIECES pieces of its row, which lanes take in an order (e ^ turn) by which eight of them (two rows, which a write stores
+    // at once) fill the 128 bytes that LDS takes.
     constexpr int PIECES = D / 32;
-    const int turned = D == 128 ? lane & 3 : (lane >> 1) & 1;
-    auto piece_at = [&](int e) {                   // (row of the page, piece of the row)
-        if constexpr (FMT == FMT_FP4) return make_int2(lane >> 2, (lane & 3) * PIECES + ((e + turned) & (PIECES - 1)));
+    const int k_turn = D == 128 ? lane & 2 : 0, v_turn = D == 128 ? lane & 3 : (lane >> 1) & 1;
+    auto piece_at = [&](int e, int turn) {         // (row of the page, piece of the row)
+        if constexpr (FMT == FMT_FP4) return make_int2(lane >> 2, (lane & 3) * PIECES + (e ^ turn));
         else return make_int2((64 * e + lane) / (D / 8), lane % (D / 8));
     };
     auto piece = [&](const Rows& y, int e) {       // MXFP4: of the turned words (load)
         if constexpr (FMT == FMT_FP4) return fp4_to_16<H>(e == 0 ? y.r[0].x : e == 1 ? y.r[0].y : e == 2 ? y.r[0].z : y.r[0].w, y.e);
         else return y.r[e];
     };
-    auto turn_words = [&](Rows& y) {
+    auto turn_words = [&](Rows& y, int turn) {
         if constexpr (FMT == FMT_FP4) {
             uint4 v = y.r[0];
-            if constexpr (PIECES == 4) {
-                v = turned & 1 ? make_uint4(v.y, v.z, v.w, v.x) : v;
-                v = turned & 2 ? make_uint4(v.z, v.w, v.x, v.y) : v;
-            } else {
-                v = turned ? make_uint4(v.y, v.x, 0, 0) : v;
-            }
+            v = turn & 1 ? make_uint4(v.y, v.x, v.w, v.z) : v;
+            if constexpr (PIECES == 4) v = turn & 2 ? make_uint4(v.z, v.w, v.x, v.y) : v;
             y.r[0] = v;
         }
     };
-    auto put = [&](char* dst, int row, const Rows& y, int e) {
-        const int2 at = piece_at(e);
+    auto put = [&](char* dst, int row, const Rows& y, int e, int turn) {
+        const int2 at = piece_at(e, turn);
         *reinterpret_cast<uint4*>(dst + (16 * wave + at.x) * row + at.y * 16) = piece(y, e);
     };
     // A page of values that rows see in part, put once more: the values of keys that no row sees as 0, and so every value that
@@ -215,7 +212,7 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
         char* dst = vt[(tile - t0) & 1];
 #pragma unroll
         for (int e = 0; e < PIECES; e++) {
-            const int2 at = piece_at(e);
+            const int2 at = piece_at(e, v_turn);
             const int j = blk * KPAGE + at.x;
             const uint4 v = piece(y, e);
             uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -277,11 +274,11 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
         // in LDS one iteration before Q . K^T, which runs one ahead of P . V, beside the exponentials of the tile before.
         int pk = page_of(t0), p1 = page_of(t0 + 1), pn = page_of(t0 + 2);
         Rows k = load(a.kp, pk), v = load(a.vp, pk), k1 = load(a.kp, p1);
-        turn_words(k);
-        turn_words(v);
-        turn_words(k1);
+        turn_words(k, k_turn);
+        turn_words(v, v_turn);
+        turn_words(k1, k_turn);
 #pragma unroll
-        for (int e = 0; e < PIECES; e++) { put(kt[0], KROW, k, e); put(vt[0], VROW, v, e); put(kt[1], KROW, k1, e); }
+        for (int e = 0; e < PIECES; e++) { put(kt[0], KROW, k, e, k_turn); put(vt[0], VROW, v, e, v_turn); put(kt[1], KROW, k1, e, k_turn); }
         clean(t0, v, pk);
         pk = p1;
         k = load(a.kp, pn);
@@ -337,8 +334,8 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
                 }
                 if constexpr (MORE) {
                     pin(rsum);
-                    if (KS - s == PIECES) turn_words(k);
-                    if (KS - 1 - s < PIECES) put(kt[(tile - t0) & 1], KROW, k, KS - 1 - s);
+                    if (KS - s == PIECES) turn_words(k, k_turn);
+                    if (KS - 1 - s < PIECES) put(kt[(tile - t0) & 1], KROW, k, KS - 1 - s, k_turn);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
@@ -358,7 +355,7 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
             for (int z = 0; z < AHEAD; z++) vf[z] = value_frag(z);
             if constexpr (MORE) {
                 m = p[0][0];
-                turn_words(v);
+                turn_words(v, v_turn);
             }
 #pragma unroll
             for (int z = 0; z < Z; z++) {
@@ -369,7 +366,7 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
 #pragma unroll
                     for (int i = 0; i < 32 / Z; i++) { const int n = z * (32 / Z) + i; m = fmaxf(m, p[n >> 4][n & 15]); }
                     pin(m);
-                    if (z >= 2 && z < 2 + PIECES) put(vt[(tile + 1 - t0) & 1], VROW, v, z - 2);
+                    if (z >= 2 && z < 2 + PIECES) put(vt[(tile + 1 - t0) & 1], VROW, v, z - 2, v_turn);
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }

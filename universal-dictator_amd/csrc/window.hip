@@ -265,8 +265,9 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
         uint4 vb[2][VR];
         uint32_t vbs[2];
         // The V rows of 32 keys into the wave's tile (the rows of a second 32 are kept in registers until then).  MXFP4: a
-        // lane's block (D = 64: half a block), its pieces in pairs turned against bank conflicts.
-        const int turned = FMT == FMT_FP4 ? (lane >> 3) & 1 : 0;
+        // lane's block (D = 64: half a block), its pieces in pairs turned so that eight lanes (two rows, which a write stores
+        // at once) fill the 128 bytes that LDS takes.
+        const int turned = FMT != FMT_FP4 ? 0 : D == 128 ? (lane >> 1) & 1 : (lane >> 2) & 1;
         auto at = [&](int tt, int e) {
             const int row = FMT == FMT_FP4 ? lane >> 2 : (64 * e + lane) / (D / 8);
             const int piece = FMT == FMT_FP4 ? (lane & 3) * (D / 32) + (e ^ turned) : lane % (D / 8);
