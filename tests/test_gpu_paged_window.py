@@ -152,6 +152,42 @@ def test_window_masked_values_are_not_seen(gpu, fmt):
         np.testing.assert_array_equal(got, clean)
 
 
+@pytest.mark.parametrize("fmt,dtype", TYPES)
+@pytest.mark.parametrize("d,hkv,lens", [(128, 16, [1, 16, 33] + list(range(40, 300, 17))), (64, 90, [2100, 64, 700])])
+def test_window_more_than_a_round_of_workgroups(gpu, fmt, dtype, d, hkv, lens):
+    """More sequences times kv heads than CUs: short ones (workgroups of four waves), and one long enough for eight."""
+    assert len(lens) * hkv > 256
+    rng = np.random.default_rng([71, d, len(fmt), len(dtype)])
+    check_window(gpu, rng, fmt, dtype, hkv, hkv, d, lens, 2, 0, 0, empty=[(1, 1)])
+    check_window(gpu, rng, fmt, dtype, hkv, hkv, d, lens, 1, 100, 5, give_back=True)
+
+
+@pytest.mark.parametrize("fmt,dtype", [("bf16", "bf16"), ("f16", "f32"), ("mxfp4", "bf16")])
+def test_window_masked_values_in_many_workgroups(gpu, fmt, dtype):
+    """NaN and infinities behind the range and between sinks and window, on more units than CUs: nothing changes; in a key and a
+    value that is seen: that head's rows alone are NaN."""
+    ud, rng, hkv, d = gpu, np.random.default_rng(72), 100, 64
+    lens = [150, 40, 97]
+    c0 = Cache(ud, np.random.default_rng(73), fmt, lens, hkv, d)
+    ranges = np.array([[[L - 31, L - 10]] for L in lens])
+    q = ref.rounded(rng.standard_normal((3, 1, hkv, d)), dtype)
+    clean = window(ud, c0, q, ranges, 4, dtype)
+    k, v = [x.copy() for x in c0.k], [x.copy() for x in c0.v]
+    for i, L in enumerate(lens):
+        for x in (k[i], v[i]):
+            x[L - 10:] = (np.nan, np.inf, -np.inf)[i]
+            x[4:L - 31] = (np.inf, np.nan, np.nan)[i]
+    c1 = Cache(ud, np.random.default_rng(73), fmt, lens, hkv, d, k=k, v=v)
+    np.testing.assert_array_equal(window(ud, c1, q, ranges, 4, dtype), clean)
+    v[2][80, 55] = np.nan
+    k[0][135, 7] = np.nan
+    c2 = Cache(ud, np.random.default_rng(73), fmt, lens, hkv, d, k=k, v=v)
+    got = window(ud, c2, q, ranges, 4, dtype)
+    assert np.all(np.isnan(got[2, 0, 55])) and np.all(np.isnan(got[0, 0, 7]))
+    got[2, 0, 55], got[0, 0, 7] = clean[2, 0, 55], clean[0, 0, 7]
+    np.testing.assert_array_equal(got, clean)
+
+
 def test_window_pages_that_are_not_held(gpu):
     """A block-table entry outside the pool inside the range: its keys are not there."""
     ud, rng, hq, hkv, d = gpu, np.random.default_rng(14), 4, 2, 128

@@ -6,7 +6,7 @@
 // Bound: HBM; every visible K and V byte is read once.  One workgroup = (kv head, split of the page list, sequence);
 // its rows are the M positions times the G query heads of the kv head, up to 32 (two tiles of 16), so a page is read
 // once for all of them; above 32 rows a second workgroup takes the rest, on the same XCD at 8 kv heads (the rows of 64
-// would not leave the registers room).  Each of the 4 waves takes chunks of its split's pages (2 pages of 16 bits, 4 of MXFP4) on its
+// would not leave the registers room).  Each of the 4 or 8 waves takes chunks of its split's pages (2 pages of 16 bits, 4 of MXFP4) on its
 // own, with its own running maximum and sum, so the loop has no barrier; the waves join once at the end, the splits in
 // a second kernel.
 //  - S^T = K . Q^T on v_mfma_f32_16x16x32: lane (c, g) loads the channels that the A operand wants of key c straight
@@ -23,6 +23,7 @@
 // the same kernel with its loads alone takes 99 % of that (181.5 and 183.9 us at 64 x 4,096 keys).  MXFP4 pages, 64 x 4,096 keys
 // 57.5 us, its loads alone 52.0; 64 x 512 .. 8,192 keys (304 MB) 81 us, 3.8 TB/s: the longest sequences' workgroups end last.
 // One sequence of 8,192 half keys is latency: 14 us in 64 splits, and 4 for the join.
+#include <algorithm>
 #include <type_traits>
 
 #include "paged_attention.hpp"
@@ -50,8 +51,8 @@ template <typename E, int FMT> struct Terms {
     static constexpr int P = std::is_same<E, El32>::value ? (H ? 2 : 3) : std::is_same<E, ElH>::value && !H ? 2 : 1;
 };
 
-template <typename E, int FMT, int D, int RT>
-__global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(WindowArgs a) {
+template <typename E, int FMT, int D, int RT, int NW>
+__global__ __launch_bounds__(64 * NW, RT == 1 ? 2 : 1) void window_split_kernel(WindowArgs a) {
     typedef typename E::S S;
     constexpr bool H = Terms<E, FMT>::H;
     constexpr int QT = Terms<E, FMT>::Q, PT = Terms<E, FMT>::P;
@@ -67,9 +68,9 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
     const int kvh = blockIdx.x, split = blockIdx.y / a.groups, seq = blockIdx.z;
     const int r0 = blockIdx.y % a.groups * (16 * RT);   // first of this workgroup's rows
     const int G = a.G, M = a.M, QR = min(M * G - r0, 16 * RT);
-    __shared__ __align__(16) char tile[4][32 * VROW];
-    __shared__ float wmax[4][16 * RT], wsum[4][16 * RT];
-    __shared__ int odd_of[4];
+    __shared__ __align__(16) char tile[NW][32 * VROW];
+    __shared__ float wmax[NW][16 * RT], wsum[NW][16 * RT];
+    __shared__ int odd_of[NW];
 
     // ---- the sequence's page list, and this lane's rows (row 16 rt + col: position r / G, head r % G)
     const int32_t* rg = a.ranges + (int64_t)2 * seq * M;
@@ -98,7 +99,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
             *reinterpret_cast<float2*>(a.stat + (out_row(tid) * a.splits + split) * 2) = make_float2(-INFINITY, 0.0f);
         if (a.splits == 1) {
             const float z[4] = {0, 0, 0, 0};
-            for (int x = tid; x < QR * (D / 4); x += 256)
+            for (int x = tid; x < QR * (D / 4); x += 64 * NW)
                 store4<E>(static_cast<S*>(a.out) + out_row(x / (D / 4)) * D + x % (D / 4) * 4, z);
         }
         return;
@@ -170,12 +171,12 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
         for (int d = 0; d < DT; d++) o[d][rt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    // ---- the wave's chunks: pages u0 + CP wave, + 4 CP, ..  Lane l holds the pool's page (or -1) of the l-th of the next
+    // ---- the wave's chunks: pages u0 + CP wave, + NW CP, ..  Lane l holds the pool's page (or -1) of the l-th of the next
     // 64 pages of the wave, so that the table is read once for 64 / CP chunks, not before each.
     const int32_t* bt = a.bt + (int64_t)seq * a.max_blocks;
     int pages = -1;
     auto look_up = [&](int u) __attribute__((always_inline)) {
-        const int at = u + lane / CP * (4 * CP) + lane % CP;
+        const int at = u + lane / CP * (NW * CP) + lane % CP;
         pages = at < u1 ? bt[page_at(list, at)] : -1;
         pages = pages < a.num_blocks ? pages : -1;
     };
@@ -227,7 +228,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
         load(0);
         next = CP;
     }
-    for (; u < u1; u += 4 * CP) {
+    for (; u < u1; u += NW * CP) {
         // ---- scores (of q as it was scaled), row c's keys 16t + 4g + i
         // (the tiles side by side: their products do not wait for each other)
         float p[RT][CP][4];
@@ -323,8 +324,8 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
         take(0);
         put_v(0);
         if constexpr (CP > 2) take(1);
-        if (u + 4 * CP < u1) {
-            if (next == 64) { look_up(u + 4 * CP); next = 0; }
+        if (u + NW * CP < u1) {
+            if (next == 64) { look_up(u + NW * CP); next = 0; }
             load(next);
             next += CP;
         }
@@ -399,7 +400,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
             }
         }
     }
-    // ---- the four waves joined, a row tile at a time through their LDS tiles
+    // ---- the waves joined, a row tile at a time through their LDS tiles
     if (lane == 0) odd_of[wave] = 0;
     if (odd) odd_of[wave] = 1;
 #pragma unroll
@@ -442,7 +443,7 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
         const int rr = 16 * rt + col;
         float m = wmax[0][rr];
 #pragma unroll
-        for (int w = 1; w < 4; w++) m = fmaxf(m, wmax[w][rr]);
+        for (int w = 1; w < NW; w++) m = fmaxf(m, wmax[w][rr]);
         // a wave without a key of the row adds nothing
         const bool none = rmax[rt] == -INFINITY;
         const float f = share(rmax[rt], m);
@@ -453,20 +454,22 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
             *reinterpret_cast<float4*>(vt + col * (4 * D) + (((4 * d + g) ^ col) << 4)) = x;
         }
         __syncthreads();
-        for (int x = tid; x < 16 * (D / 4); x += 256) {
+        for (int x = tid; x < 16 * (D / 4); x += 64 * NW) {
             const int c = x / (D / 4), piece = x % (D / 4), r = 16 * rt + c;
             if (r >= QR) continue;
             float y[4] = {0, 0, 0, 0};
             float mm = wmax[0][r], l = 0.0f;
+            int any_odd = 0;
 #pragma unroll
-            for (int w = 1; w < 4; w++) mm = fmaxf(mm, wmax[w][r]);
+            for (int w = 1; w < NW; w++) mm = fmaxf(mm, wmax[w][r]);
 #pragma unroll
-            for (int w = 0; w < 4; w++) {
+            for (int w = 0; w < NW; w++) {
                 const float4 v = *reinterpret_cast<const float4*>(tile[w] + c * (4 * D) + ((piece ^ c) << 4));
                 y[0] += v.x; y[1] += v.y; y[2] += v.z; y[3] += v.w;
                 l += wsum[w][r] * share(wmax[w][r], mm);
+                any_odd |= odd_of[w];
             }
-            if (odd_of[0] | odd_of[1] | odd_of[2] | odd_of[3]) give_odd(r, 4 * piece, y);
+            if (any_odd) give_odd(r, 4 * piece, y);
             if (a.splits == 1) {
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
@@ -483,39 +486,53 @@ __global__ __launch_bounds__(256, RT == 1 ? 2 : 1) void window_split_kernel(Wind
 }
 
 template <typename E, int FMT, int D>
-static void launch_window_d(WindowArgs a, int n, hipStream_t st) {
+static void launch_window_d(WindowArgs a, int n, int waves, hipStream_t st) {
     const int rows = a.M * a.G;
-    if (rows <= 16) {
-        hipLaunchKernelGGL((window_split_kernel<E, FMT, D, 1>), dim3(a.Hkv, a.splits, n), dim3(256), 0, st, a);
-    } else {
-        a.groups = (rows + 31) / 32;
-        hipLaunchKernelGGL((window_split_kernel<E, FMT, D, 2>), dim3(a.Hkv, a.splits * a.groups, n), dim3(256), 0, st, a);
+    auto go = [&](auto kernel, int groups, int nw) {
+        a.groups = groups;
+        hipLaunchKernelGGL(kernel, dim3(a.Hkv, a.splits * groups, n), dim3(64 * nw), 0, st, a);
+    };
+    if constexpr (FMT != FMT_FP4)
+        if (waves == 8) go(window_split_kernel<E, FMT, D, 1, 8>, 1, 8);
+    if (waves == 4) {
+        if (rows <= 16) go(window_split_kernel<E, FMT, D, 1, 4>, 1, 4);
+        else go(window_split_kernel<E, FMT, D, 2, 4>, (rows + 31) / 32, 4);
     }
     if (a.splits > 1) launch_join<E, D>(a.part, a.stat, a.out, JoinRows{(int64_t)n * a.M * a.Hq, 0, 0, nullptr, 1}, a.splits, st);
 }
 template <typename E, int FMT>
-static void launch_window(const WindowArgs& a, int n, int D, hipStream_t st) {
-    if (D == 128) launch_window_d<E, FMT, 128>(a, n, st);
-    else launch_window_d<E, FMT, 64>(a, n, st);
+static void launch_window(const WindowArgs& a, int n, int D, int waves, hipStream_t st) {
+    if (D == 128) launch_window_d<E, FMT, 128>(a, n, waves, st);
+    else launch_window_d<E, FMT, 64>(a, n, waves, st);
 }
 
-// Workgroups: one round of two per CU (512), not quite full rather than just beyond, but at least three quarters of it.
-// A workgroup's first rows arrive some 3 us after its start (its ranges, its table entries, its pages) and its waves are
-// joined at its end, so few, long ones pay while the chip is full.
-// us at 512 / 1,024 / 2,048 wanted, 32/8 heads of 128: 1 x 60,000 keys bf16 50.6 / 52.4 / 57.4, MXFP4 21.9 / 24.9 / 30.0;
-// 64 x 4,096 bf16 184 / 191 / 194, MXFP4 57.6 / 64.6 / 66.2; 64 x 1,000 bf16 51.0 / 56.8 / 59.5.  More of them only helps
-// where contexts differ widely: 8 x 1,000-30,000 bf16 114 / 112 / 98.
+// Waves of a workgroup, and workgroups: one round of eight waves per CU (512 workgroups of 4 waves, 256 of 8), not quite full
+// rather than just beyond, but at least three quarters of it.  A workgroup's first rows arrive some 3 us after its start (its
+// ranges, its table entries, its pages) and its waves are joined at its end, so few, long ones pay while the chip is full.
+// us at 512 / 1,024 / 2,048 of 4 waves wanted, 32/8 heads of 128: 1 x 60,000 keys bf16 50.6 / 52.4 / 57.4, MXFP4 21.9 / 24.9 /
+// 30.0; 64 x 4,096 bf16 184 / 191 / 194, MXFP4 57.6 / 64.6 / 66.2; 64 x 1,000 bf16 51.0 / 56.8 / 59.5.
 // Beyond or below a round, 4,000 keys: 12 sequences (96 units) 576 -> 480 workgroups bf16 47.8 -> 43.2 us; 50 (400) 800 ->
 // 400 162 -> 146, MXFP4 61.5 -> 51.9; but 33 (264) 528 -> 264 117 -> 132.
-// A workgroup's waves take 2 pages each at a time (MXFP4: 4): step.
-constexpr int64_t WINDOW_ROUND = 512;
-static SplitPlan window_plan(int32_t n, int32_t kv_heads, int32_t n_sinks, int32_t max_span, int step) {
+// 8 waves, 16-bit pages of up to 16 rows: the grid is one round, or a sequence has 2,048 keys and more.  They halve the longest
+// workgroup of unequal contexts, and half as many splits are joined; of short ones too many start and end with the CU to
+// themselves.  4 -> 8 waves, bf16, us: 24 x 1,000 25.3 -> 22.1, 24 x 4 queries of 500-8,000 114 -> 104, 8 x 1,000-30,000 111 ->
+// 104, 64 x 512-8,192 231 -> 224, 400 x 100-3,000 452 -> 436, 64 x 4,096 182.4 -> 181.9, but 12 x 4 of 300-8,192 57 -> 61;
+// where 4 stay: 40 x 2,000 67 -> 74, 64 x 1,000 51 -> 55, 200 x 500 80 -> 96.  MXFP4 (its waves are busy, and three
+// workgroups of 4 fit a CU): 64 x 4,096 56 -> 60, 200 x 300-2,000 65 -> 93.
+// A workgroup's waves take 2 pages each at a time (MXFP4: 4), of which a split is a multiple.
+struct WindowPlan {
+    SplitPlan split;
+    int waves;
+};
+static WindowPlan window_plan(bool fp4, int64_t rows, int32_t n, int32_t kv_heads, int32_t n_sinks, int32_t max_span) {
     // (a window that does not start with a page has one more: the last split takes it)
-    const int64_t pages = ((int64_t)max_span + KPAGE - 1) / KPAGE + ((int64_t)n_sinks + KPAGE - 1) / KPAGE;
+    const int64_t pages = std::max<int64_t>(1, ((int64_t)max_span + KPAGE - 1) / KPAGE + ((int64_t)n_sinks + KPAGE - 1) / KPAGE);
     const int64_t units = (int64_t)n * kv_heads;
-    int64_t want = WINDOW_ROUND / units;
-    if (want * units < WINDOW_ROUND * 3 / 4) want++;
-    return split_plan(want, pages < 1 ? 1 : pages, step);
+    const int waves = !fp4 && rows <= 16 && (units <= 256 || pages >= 128) ? 8 : 4;
+    const int64_t round = 2048 / waves;
+    int64_t want = round / units;
+    if (want * units < round * 3 / 4) want++;
+    return WindowPlan{split_plan(want, pages, waves * (fp4 ? 4 : 2)), waves};
 }
 
 }  // namespace ud
@@ -525,7 +542,7 @@ using namespace ud;
 extern "C" UD_API size_t ud_gqa_window_workspace_bytes(int32_t n, int32_t n_queries, int32_t q_heads, int32_t kv_heads,
                                                        int32_t head_dim, int32_t n_sinks, int32_t max_span) {
     if (n <= 0 || n_queries <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || n_sinks < 0 || max_span < 0) return 0;
-    const int s = window_plan(n, kv_heads, n_sinks, max_span, 8).splits;     // the finer of the two
+    const int s = window_plan(false, 64, n, kv_heads, n_sinks, max_span).split.splits;    // the finest of all
     return s == 1 ? 0 : (size_t)n * n_queries * q_heads * s * (head_dim + 2) * sizeof(float);
 }
 
@@ -553,26 +570,26 @@ extern "C" UD_API int ud_gqa_window_attention_paged(int32_t kv_format, int32_t d
     if (need && !workspace) return paged_fail(UD_ERR_INVALID, "%s: null workspace", who);
     if (workspace_bytes < need) return paged_fail(UD_ERR_SHAPE, "%s: workspace %zu < %zu bytes", who, workspace_bytes, need);
     if ((uintptr_t)workspace & 15) return paged_fail(UD_ERR_INVALID, "%s: workspace must be 16-byte aligned", who);
-    const SplitPlan plan = window_plan(n, kv_heads, n_sinks, max_span, kv_format == UD_MXFP4 ? 16 : 8);
+    const WindowPlan plan = window_plan(kv_format == UD_MXFP4, (int64_t)n_queries * (q_heads / kv_heads), n, kv_heads, n_sinks, max_span);
     WindowArgs a{};
     a.q = q_dev; a.kp = static_cast<const char*>(k_pages); a.vp = static_cast<const char*>(v_pages); a.bt = block_table;
     a.ranges = ranges_dev; a.out = out_dev;
     a.part = static_cast<float*>(workspace);
-    a.stat = a.part + (size_t)n * n_queries * q_heads * plan.splits * head_dim;
+    a.stat = a.part + (size_t)n * n_queries * q_heads * plan.split.splits * head_dim;
     a.M = n_queries; a.G = q_heads / kv_heads; a.Hq = q_heads; a.Hkv = kv_heads;
-    a.max_blocks = max_blocks; a.num_blocks = num_blocks; a.sinks = n_sinks; a.splits = plan.splits; a.pages = plan.pages; a.groups = 1;
+    a.max_blocks = max_blocks; a.num_blocks = num_blocks; a.sinks = n_sinks; a.splits = plan.split.splits; a.pages = plan.split.pages;
     a.scale = (float)(1.4426950408889634 / sqrt((double)head_dim));
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
     if (kv_format == UD_BF16) {
-        if (dtype == UD_F32) launch_window<El32, FMT_BF16>(a, n, head_dim, st);
-        else launch_window<ElBf, FMT_BF16>(a, n, head_dim, st);
+        if (dtype == UD_F32) launch_window<El32, FMT_BF16>(a, n, head_dim, plan.waves, st);
+        else launch_window<ElBf, FMT_BF16>(a, n, head_dim, plan.waves, st);
     } else if (kv_format == UD_F16) {
-        if (dtype == UD_F32) launch_window<El32, FMT_F16>(a, n, head_dim, st);
-        else launch_window<ElH, FMT_F16>(a, n, head_dim, st);
+        if (dtype == UD_F32) launch_window<El32, FMT_F16>(a, n, head_dim, plan.waves, st);
+        else launch_window<ElH, FMT_F16>(a, n, head_dim, plan.waves, st);
     } else {
-        if (dtype == UD_F32) launch_window<El32, FMT_FP4>(a, n, head_dim, st);
-        else if (dtype == UD_BF16) launch_window<ElBf, FMT_FP4>(a, n, head_dim, st);
-        else launch_window<ElH, FMT_FP4>(a, n, head_dim, st);
+        if (dtype == UD_F32) launch_window<El32, FMT_FP4>(a, n, head_dim, plan.waves, st);
+        else if (dtype == UD_BF16) launch_window<ElBf, FMT_FP4>(a, n, head_dim, plan.waves, st);
+        else launch_window<ElH, FMT_FP4>(a, n, head_dim, plan.waves, st);
     }
     return paged_launched(who);
 }
