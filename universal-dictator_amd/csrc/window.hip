@@ -61,8 +61,10 @@ __global__ __launch_bounds__(64 * NW, RT == 1 ? 2 : 1) void window_split_kernel(
     constexpr int DT = D / 16;                     // channel tiles
     constexpr int HEAD = Page<FMT, D>::BYTES;
     // Bytes between the rows of V in LDS: 8 rows' 32 bytes, which a product reads at once, lie on distinct banks, and every
-    // product reads at a fixed distance from one address (no address arithmetic between them).
-    constexpr int VROW = 2 * D + 32;
+    // product reads at a fixed distance from one address (no address arithmetic between them).  MXFP4 at D = 128: a row's
+    // even pieces of 16 bytes before its odd ones (HALVES), so that the writes, four pieces a lane, are without conflicts too.
+    constexpr bool HALVES = FMT == FMT_FP4 && D == 128;
+    constexpr int VROW = HALVES ? 2 * D + 16 : 2 * D + 32;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
     const int kvh = blockIdx.x, split = blockIdx.y / a.groups, seq = blockIdx.z;
@@ -171,14 +173,20 @@ __global__ __launch_bounds__(64 * NW, RT == 1 ? 2 : 1) void window_split_kernel(
         for (int d = 0; d < DT; d++) o[d][rt] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    // ---- the wave's chunks: pages u0 + CP wave, + NW CP, ..  Lane l holds the pool's page (or -1) of the l-th of the next
-    // 64 pages of the wave, so that the table is read once for 64 / CP chunks, not before each.
+    // ---- the wave's chunks: pages u0 + CP wave, + NW CP, ..  Lane l holds where the l-th of the next 64 pages of the wave
+    // lies in the pools (page 0 where it is none of theirs), so that the table is read once for 64 / CP chunks, not before
+    // each.
     const int32_t* bt = a.bt + (int64_t)seq * a.max_blocks;
-    int pages = -1;
+    uint32_t page_lo = 0, page_hi = 0;
+    uint64_t in_pools = 0;                         // bit l: of lane l's page
     auto look_up = [&](int u) __attribute__((always_inline)) {
         const int at = u + lane / CP * (NW * CP) + lane % CP;
-        pages = at < u1 ? bt[page_at(list, at)] : -1;
-        pages = pages < a.num_blocks ? pages : -1;
+        const int page = at < u1 ? bt[page_at(list, at)] : -1;
+        const bool ours = page >= 0 && page < a.num_blocks;
+        const uint64_t base = ((uint64_t)(ours ? page : 0) * a.Hkv + kvh) * HEAD;
+        page_lo = (uint32_t)base;
+        page_hi = (uint32_t)(base >> 32);
+        in_pools = __ballot(ours);
     };
     // 16-bit: kr[page][s], vr[page][i] rows 16 bytes a lane.  MXFP4: one piece and one exponent per page (D = 64: half).
     constexpr int KR = FMT == FMT_FP4 ? 1 : KS, VR = FMT == FMT_FP4 ? 1 : D / 32;
@@ -189,25 +197,23 @@ __global__ __launch_bounds__(64 * NW, RT == 1 ? 2 : 1) void window_split_kernel(
     // a page that every row sees whole
     auto whole = [&](int blk) { return blk * KPAGE >= lo_most && blk * KPAGE + KPAGE <= hi_least; };
     bool odd = false;                              // a value that is no number has been left out
-    const uint32_t k_off = FMT == FMT_FP4 ? col * (D / 2) + g * (D / 8) : col * (2 * D) + 16 * g;
-    const uint32_t ks_off = Page<FMT, D>::CODES + col * (D / 32) + (D == 128 ? g : g >> 1);
-    const uint32_t vs_off = Page<FMT, D>::CODES + (D == 128 ? lane : lane >> 1);
-
     auto load = [&](int first) __attribute__((always_inline)) {                   // first: lane that holds the chunk's first page
-        held = 0;
+        const uint32_t k_off = FMT == FMT_FP4 ? col * (D / 2) + g * (D / 8) : col * (2 * D) + 16 * g, v_off = lane * (FMT == FMT_FP4 ? D / 8 : 16);
+        const uint32_t ks_off = Page<FMT, D>::CODES + col * (D / 32) + (D == 128 ? g : g >> 1);
+        const uint32_t vs_off = Page<FMT, D>::CODES + (D == 128 ? lane : lane >> 1);
+        held = (uint32_t)(in_pools >> first) & ((1u << CP) - 1);
 #pragma unroll
         for (int t = 0; t < CP; t++) {
-            const int page = __builtin_amdgcn_readlane(pages, first + t);
-            held |= (uint32_t)(page >= 0) << t;
-            const int64_t base = ((int64_t)max(page, 0) * a.Hkv + kvh) * HEAD;
+            const uint32_t lo32 = __builtin_amdgcn_readlane(page_lo, first + t), hi32 = __builtin_amdgcn_readlane(page_hi, first + t);
+            const uint64_t base = (uint64_t)hi32 << 32 | lo32;
             const char* k = a.kp + base;
             const char* v = a.vp + base;
             if constexpr (FMT == FMT_FP4) {
                 if constexpr (D == 128) {
                     kr[t][0] = ld16(k + k_off);
-                    vr[t][0] = ld16(v + lane * 16u);
+                    vr[t][0] = ld16(v + v_off);
                 } else {
-                    const uint2 x = *reinterpret_cast<const uint2*>(k + k_off), y = *reinterpret_cast<const uint2*>(v + lane * 8u);
+                    const uint2 x = *reinterpret_cast<const uint2*>(k + k_off), y = *reinterpret_cast<const uint2*>(v + v_off);
                     kr[t][0] = make_uint4(x.x, x.y, 0, 0);
                     vr[t][0] = make_uint4(y.x, y.y, 0, 0);
                 }
@@ -217,7 +223,7 @@ __global__ __launch_bounds__(64 * NW, RT == 1 ? 2 : 1) void window_split_kernel(
 #pragma unroll
                 for (int s = 0; s < KS; s++) kr[t][s] = ld16(k + (k_off + 64 * s));
 #pragma unroll
-                for (int i = 0; i < VR; i++) vr[t][i] = ld16(v + (lane * 16u + i * 1024));
+                for (int i = 0; i < VR; i++) vr[t][i] = ld16(v + (v_off + i * 1024));
             }
         }
     };
@@ -266,13 +272,13 @@ __global__ __launch_bounds__(64 * NW, RT == 1 ? 2 : 1) void window_split_kernel(
         uint4 vb[2][VR];
         uint32_t vbs[2];
         // The V rows of 32 keys into the wave's tile (the rows of a second 32 are kept in registers until then).  MXFP4: a
-        // lane's block (D = 64: half a block), its pieces in pairs turned so that eight lanes (two rows, which a write stores
-        // at once) fill the 128 bytes that LDS takes.
-        const int turned = FMT != FMT_FP4 ? 0 : D == 128 ? (lane >> 1) & 1 : (lane >> 2) & 1;
+        // lane's block, or (D = 64) half a block, whose two pieces are turned so that eight lanes (two rows, which a write
+        // stores at once) fill the 128 bytes that LDS takes.
+        const int turned = FMT == FMT_FP4 && D == 64 ? (lane >> 2) & 1 : 0;
         auto at = [&](int tt, int e) {
             const int row = FMT == FMT_FP4 ? lane >> 2 : (64 * e + lane) / (D / 8);
             const int piece = FMT == FMT_FP4 ? (lane & 3) * (D / 32) + (e ^ turned) : lane % (D / 8);
-            return make_int2(row, (16 * tt + row) * VROW + piece * 16);
+            return make_int2(row, (16 * tt + row) * VROW + (HALVES ? (piece & 1) * D + (piece >> 1) * 16 : piece * 16));
         };
         auto put_v = [&](int half) __attribute__((always_inline)) {
             __builtin_amdgcn_wave_barrier();       // the reads of the last 32 keys come first
@@ -389,10 +395,11 @@ __global__ __launch_bounds__(64 * NW, RT == 1 ? 2 : 1) void window_split_kernel(
                     rsum[rt] = dot_ones<H>(y.w, dot_ones<H>(y.z, dot_ones<H>(y.y, dot_ones<H>(y.x, rsum[rt]))));
                 }
             }
-            const char* v_lane = vt + (4 * g + (col >> 2)) * VROW + 8 * (col & 3);
+            const char* v_lane = vt + (4 * g + (col >> 2)) * VROW + (HALVES ? 8 * (col & 1) + ((col >> 1) & 1) * D : 8 * (col & 3));
+            constexpr int VD = HALVES ? 16 : 32;   // bytes between the channel tiles
 #pragma unroll
             for (int d = 0; d < DT; d++) {
-                const uint2 x = lds_tr16(v_lane + 32 * d), y = lds_tr16(v_lane + 32 * d + 16 * VROW);
+                const uint2 x = lds_tr16(v_lane + VD * d), y = lds_tr16(v_lane + VD * d + 16 * VROW);
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++)
 #pragma unroll
