@@ -13,9 +13,9 @@
 // Keys for MXFP4 pages are normalised and rotated in 64 bits: a key next to a border between two codes would
 // otherwise move by a whole step of its block with the order of a sum, and so would every key of a block whose
 // largest value is next to a power of two's border.  That is 8 of 48 heads at 32/8.
-// Measured, 32/8 heads of 128: 8,200 rows of bf16 to MXFP4 pages 46 us (253 MB, 5.5 TB/s; a large copy on the same card
-// 4.7 .. 5.0), 64 rows 5.7 us, one row of fp32 to half pages 3.2 us: an empty launch's and one round trip to memory for the
-// row's position, its page and its heads.  Read back: 17.6, 3.6 and 1.9 us.
+// Measured, 32/8 heads of 128: 8,200 rows of bf16 to MXFP4 pages 46 us (177 MB, 3.8 TB/s; a large copy on the same card
+// 4.7 .. 5.0; vector units busy 68 % of the time), 64 rows 5.7 us, one row of fp32 to half pages 3.2 us:
+// little more than an empty launch.  Read back: 17.6 (76 MB, 4.3 TB/s), 3.6 and 1.9 us.
 #include <type_traits>
 
 #include "paged.hpp"
@@ -114,8 +114,9 @@ __device__ __forceinline__ void store_row(char* head, int r, int i, const float 
     }
 }
 
+// (64 registers from 16-bit rows, eight workgroups a CU: 8,200 rows, with the read-back, 65.8 -> 64.2 us)
 template <typename E, int FMT, int D>
-__global__ __launch_bounds__(256) void norm_rope_append_kernel(AppendArgs a) {
+__global__ __launch_bounds__(256, sizeof(typename E::S) == 4 ? 6 : 8) void norm_rope_append_kernel(AppendArgs a) {
     constexpr int LPH = D / 8;                     // lanes per head
     constexpr bool WIDE = FMT == FMT_FP4;          // keys in 64 bits
     typedef typename E::S S;
@@ -126,8 +127,9 @@ __global__ __launch_bounds__(256) void norm_rope_append_kernel(AppendArgs a) {
     const int p = a.pos[row], s = a.seqs ? a.seqs[row] : (int)min(row, (int64_t)INT32_MAX);
     const int page = row_page(s, p, a.bt, a.n, a.max_blocks, a.num_blocks);
     if (page < 0) return;                          // uniform in the workgroup
-    // Raw values of four passes over the heads at a time: the first four are on their way while the angles are made.
-    constexpr int DEEP = 4, HPP = 256 / LPH;       // heads per pass
+    // Raw values of three passes over the heads at a time (48 heads of 128): the first are on their way while the angles are
+    // made.
+    constexpr int DEEP = 3, HPP = 256 / LPH;       // heads per pass
     const int i = tid % LPH, heads = a.Hq + 2 * a.Hkv;
     typedef typename std::conditional<sizeof(S) == 4, uint4, uint2>::type Raw;
     Raw raw[DEEP][2];
