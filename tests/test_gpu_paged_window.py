@@ -162,6 +162,16 @@ def test_window_more_than_a_round_of_workgroups(gpu, fmt, dtype, d, hkv, lens):
     check_window(gpu, rng, fmt, dtype, hkv, hkv, d, lens, 1, 100, 5, give_back=True)
 
 
+@pytest.mark.parametrize("fmt,dtype", TYPES)
+@pytest.mark.parametrize("n,hkv,M", [(60, 5, 1), (64, 5, 3), (2, 200, 1), (33, 8, 2)])
+def test_window_batches_taken_by_length(gpu, fmt, dtype, n, hkv, M):
+    """Long ragged batches of up to 64 sequences, equal lengths and rows that see nothing among them."""
+    rng = np.random.default_rng([74, n, M, len(fmt), len(dtype)])
+    lens = [2100, 17] + [int(x) for x in rng.choice([5, 64, 64, 130, 300, 301], n - 2)]
+    empty = [(i, m) for i in range(0, n, 7) for m in range(M) if i] + [(1, M - 1)]
+    check_window(gpu, rng, fmt, dtype, 2 * hkv, hkv, 64, lens, M, 0, 0, empty=empty)
+
+
 @pytest.mark.parametrize("fmt,dtype", [("bf16", "bf16"), ("f16", "f32"), ("mxfp4", "bf16")])
 def test_window_masked_values_in_many_workgroups(gpu, fmt, dtype):
     """NaN and infinities behind the range and between sinks and window, on more units than CUs: nothing changes; in a key and a

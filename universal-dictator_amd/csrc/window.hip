@@ -41,6 +41,7 @@ struct WindowArgs {
     int M, G, Hq, Hkv;
     int max_blocks, num_blocks;
     int sinks, splits, pages, groups;   // pages of a split, groups of 16 RT rows
+    int n, layer;                  // sequences; > 0: taken longest first, and back from the layer-th on (sorted_sequence)
     float scale;                   // log2(e) / sqrt(D)
 };
 
@@ -50,6 +51,29 @@ template <typename E, int FMT> struct Terms {
     static constexpr int Q = std::is_same<E, El32>::value ? (H ? 2 : 3) : FMT == FMT_FP4 && std::is_same<E, ElH>::value ? 2 : 1;
     static constexpr int P = std::is_same<E, El32>::value ? (H ? 2 : 3) : std::is_same<E, ElH>::value && !H ? 2 : 1;
 };
+
+// The sequence of layer z of the workgroups where a batch of up to 64 is taken by length: rank z of the descending order up
+// to `layer`, then from the shortest back, so that workgroups that share a CU make up for each other.  Each wave ranks them by
+// itself: a lane's sequence has as many before it as have a larger key.  Also its range, from the first lo to the last hi.
+__device__ __forceinline__ int sorted_sequence(const WindowArgs& a, int z, int& lo, int& hi) {
+    const int lane = threadIdx.x & 63, kmax = a.max_blocks * KPAGE;
+    int key = -1, l = 0, h = 0;
+    if (lane < a.n) {
+        const int32_t* rg = a.ranges + (int64_t)2 * lane * a.M;
+        l = max(rg[0], 0);
+        h = min(max(rg[2 * a.M - 1], 0), kmax);
+        key = min(max(h - l, 0), (1 << 25) - 1) << 6 | lane;
+    }
+    int before = 0;
+    for (int j0 = 0; j0 < a.n; j0 += 8)
+#pragma unroll
+        for (int j = 0; j < 8; j++) before += __builtin_amdgcn_readlane(key, j0 + j) > key;
+    const int rank = z < a.layer ? z : a.n - 1 - (z - a.layer);
+    const int seq = __builtin_ctzll(__ballot(key >= 0 && before == rank));
+    lo = __builtin_amdgcn_readlane(l, seq);
+    hi = __builtin_amdgcn_readlane(h, seq);
+    return seq;
+}
 
 template <typename E, int FMT, int D, int RT, int NW>
 __global__ __launch_bounds__(64 * NW, RT == 1 ? 2 : 1) void window_split_kernel(WindowArgs a) {
@@ -67,7 +91,9 @@ __global__ __launch_bounds__(64 * NW, RT == 1 ? 2 : 1) void window_split_kernel(
     constexpr int VROW = HALVES ? 2 * D + 16 : 2 * D + 32;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
-    const int kvh = blockIdx.x, split = blockIdx.y / a.groups, seq = blockIdx.z;
+    const int kvh = blockIdx.x, split = blockIdx.y / a.groups;
+    int seq_lo = 0, seq_hi = 0;
+    const int seq = a.layer ? sorted_sequence(a, blockIdx.z, seq_lo, seq_hi) : (int)blockIdx.z;
     const int r0 = blockIdx.y % a.groups * (16 * RT);   // first of this workgroup's rows
     const int G = a.G, M = a.M, QR = min(M * G - r0, 16 * RT);
     __shared__ __align__(16) char tile[NW][32 * VROW];
@@ -80,7 +106,8 @@ __global__ __launch_bounds__(64 * NW, RT == 1 ? 2 : 1) void window_split_kernel(
     int lo = kmax, hi = 0, lo_most = 0, hi_least = kmax;
     const int m0 = r0 ? r0 / G : 0, m1 = a.groups == 1 ? M - 1 : (r0 + QR - 1) / G;
     for (int m = m0; m <= m1; m++) {
-        const int l = max(rg[2 * m], 0), h = min(rg[2 * m + 1], kmax);
+        const bool known = a.layer && M == 1;
+        const int l = known ? seq_lo : max(rg[2 * m], 0), h = known ? seq_hi : min(rg[2 * m + 1], kmax);
         if (l < h) {
             lo = min(lo, l); hi = max(hi, h);
             lo_most = max(lo_most, l); hi_least = min(hi_least, h);
@@ -493,10 +520,12 @@ __global__ __launch_bounds__(64 * NW, RT == 1 ? 2 : 1) void window_split_kernel(
 }
 
 template <typename E, int FMT, int D>
-static void launch_window_d(WindowArgs a, int n, int waves, hipStream_t st) {
+static void launch_window_d(WindowArgs a, int n, int waves, bool by_length, hipStream_t st) {
     const int rows = a.M * a.G;
     auto go = [&](auto kernel, int groups, int nw) {
         a.groups = groups;
+        a.n = n;
+        a.layer = !by_length ? 0 : FMT == FMT_FP4 ? std::max(1, 256 / (a.Hkv * groups)) : n;
         hipLaunchKernelGGL(kernel, dim3(a.Hkv, a.splits * groups, n), dim3(64 * nw), 0, st, a);
     };
     if constexpr (FMT != FMT_FP4)
@@ -508,9 +537,9 @@ static void launch_window_d(WindowArgs a, int n, int waves, hipStream_t st) {
     if (a.splits > 1) launch_join<E, D>(a.part, a.stat, a.out, JoinRows{(int64_t)n * a.M * a.Hq, 0, 0, nullptr, 1}, a.splits, st);
 }
 template <typename E, int FMT>
-static void launch_window(const WindowArgs& a, int n, int D, int waves, hipStream_t st) {
-    if (D == 128) launch_window_d<E, FMT, 128>(a, n, waves, st);
-    else launch_window_d<E, FMT, 64>(a, n, waves, st);
+static void launch_window(const WindowArgs& a, int n, int D, int waves, bool by_length, hipStream_t st) {
+    if (D == 128) launch_window_d<E, FMT, 128>(a, n, waves, by_length, st);
+    else launch_window_d<E, FMT, 64>(a, n, waves, by_length, st);
 }
 
 // Waves of a workgroup, and workgroups: one round of eight waves per CU (512 workgroups of 4 waves, 256 of 8), not quite full
@@ -526,10 +555,16 @@ static void launch_window(const WindowArgs& a, int n, int D, int waves, hipStrea
 // 104, 64 x 512-8,192 231 -> 224, 400 x 100-3,000 452 -> 436, 64 x 4,096 182.4 -> 181.9, but 12 x 4 of 300-8,192 57 -> 61;
 // where 4 stay: 40 x 2,000 67 -> 74, 64 x 1,000 51 -> 55, 200 x 500 80 -> 96.  MXFP4 (its waves are busy, and three
 // workgroups of 4 fit a CU): 64 x 4,096 56 -> 60, 200 x 300-2,000 65 -> 93.
+// By length (sorted_sequence), up to 64 sequences of 2,048 keys and more in more workgroups than CUs: 16-bit pages (a workgroup
+// of 8 waves to a CU) longest first, MXFP4 (two of 4 waves to a CU) the second 256 workgroups shortest first.  In the order given
+// -> by length, us: 64 x 512-8,192 bf16 224 -> 196, MXFP4 75.2 -> 66.8; 40 x 1,000-6,000 bf16 126 -> 110; 64 x 4 queries of
+// 500-8,000 MXFP4 77 -> 69; what it costs where all are alike: 64 x 4,096 bf16 181.4 -> 182.6, 40 x 3,000 107 -> 108.5; where the
+// order given stays: 64 x 1,000 bf16 50.8 -> 53.3, 12 x 4 of 300-8,192 MXFP4 (5 splits) 26 -> 30.
 // A workgroup's waves take 2 pages each at a time (MXFP4: 4), of which a split is a multiple.
 struct WindowPlan {
     SplitPlan split;
     int waves;
+    bool by_length;
 };
 static WindowPlan window_plan(bool fp4, int64_t rows, int32_t n, int32_t kv_heads, int32_t n_sinks, int32_t max_span) {
     // (a window that does not start with a page has one more: the last split takes it)
@@ -539,7 +574,8 @@ static WindowPlan window_plan(bool fp4, int64_t rows, int32_t n, int32_t kv_head
     const int64_t round = 2048 / waves;
     int64_t want = round / units;
     if (want * units < round * 3 / 4) want++;
-    return WindowPlan{split_plan(want, pages, waves * (fp4 ? 4 : 2)), waves};
+    const SplitPlan split = split_plan(want, pages, waves * (fp4 ? 4 : 2));
+    return WindowPlan{split, waves, n <= 64 && units > 256 && split.splits == 1 && pages >= 128};
 }
 
 }  // namespace ud
@@ -588,15 +624,15 @@ extern "C" UD_API int ud_gqa_window_attention_paged(int32_t kv_format, int32_t d
     a.scale = (float)(1.4426950408889634 / sqrt((double)head_dim));
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
     if (kv_format == UD_BF16) {
-        if (dtype == UD_F32) launch_window<El32, FMT_BF16>(a, n, head_dim, plan.waves, st);
-        else launch_window<ElBf, FMT_BF16>(a, n, head_dim, plan.waves, st);
+        if (dtype == UD_F32) launch_window<El32, FMT_BF16>(a, n, head_dim, plan.waves, plan.by_length, st);
+        else launch_window<ElBf, FMT_BF16>(a, n, head_dim, plan.waves, plan.by_length, st);
     } else if (kv_format == UD_F16) {
-        if (dtype == UD_F32) launch_window<El32, FMT_F16>(a, n, head_dim, plan.waves, st);
-        else launch_window<ElH, FMT_F16>(a, n, head_dim, plan.waves, st);
+        if (dtype == UD_F32) launch_window<El32, FMT_F16>(a, n, head_dim, plan.waves, plan.by_length, st);
+        else launch_window<ElH, FMT_F16>(a, n, head_dim, plan.waves, plan.by_length, st);
     } else {
-        if (dtype == UD_F32) launch_window<El32, FMT_FP4>(a, n, head_dim, plan.waves, st);
-        else if (dtype == UD_BF16) launch_window<ElBf, FMT_FP4>(a, n, head_dim, plan.waves, st);
-        else launch_window<ElH, FMT_FP4>(a, n, head_dim, plan.waves, st);
+        if (dtype == UD_F32) launch_window<El32, FMT_FP4>(a, n, head_dim, plan.waves, plan.by_length, st);
+        else if (dtype == UD_BF16) launch_window<ElBf, FMT_FP4>(a, n, head_dim, plan.waves, plan.by_length, st);
+        else launch_window<ElH, FMT_FP4>(a, n, head_dim, plan.waves, plan.by_length, st);
     }
     return paged_launched(who);
 }
