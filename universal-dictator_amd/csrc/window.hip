@@ -585,7 +585,9 @@ using namespace ud;
 extern "C" UD_API size_t ud_gqa_window_workspace_bytes(int32_t n, int32_t n_queries, int32_t q_heads, int32_t kv_heads,
                                                        int32_t head_dim, int32_t n_sinks, int32_t max_span) {
     if (n <= 0 || n_queries <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || n_sinks < 0 || max_span < 0) return 0;
-    const int s = window_plan(false, 64, n, kv_heads, n_sinks, max_span).split.splits;    // the finest of all
+    // 4 waves over 16-bit pages: the finest of all plans (8 waves want half a round, which is never more splits, of twice the step;
+    // MXFP4 the same round, of twice the step)
+    const int s = window_plan(false, 64, n, kv_heads, n_sinks, max_span).split.splits;
     return s == 1 ? 0 : (size_t)n * n_queries * q_heads * s * (head_dim + 2) * sizeof(float);
 }
 
