@@ -15,7 +15,6 @@
 // side between the two of a SIMD.  Without bank conflicts.  One row group more per wave (64 rows) is slower, 515 us for 482:
 // its registers leave one wave per SIMD.
 //  - K and V rows lie in LDS at padded distances against bank conflicts; V^T is read by ds_read_b64_tr_b16.
-#include <algorithm>
 
 #include "paged_attention.hpp"
 
@@ -448,20 +447,6 @@ static void launch_prefill(const PrefillArgs& a, int n, int D, hipStream_t st) {
         hipLaunchKernelGGL((prefill_kernel<E, FMT, 64>), grid, dim3(256), 0, st, a);
         if (a.splits > 1) launch_join<E, 64>(a.part, a.stat, a.out, rows, a.splits, st);
     }
-}
-
-// Blocks of 128 query rows of the longest sequence, and splits of their keys.
-// - At most 256 workgroups (one per CU; two fit): split until there are 512, down to 8 tiles of 64 keys each.
-// - Above: split up to 2,048, so that the unequal workgroups of unequal sequences fill each other's gaps, but not below 64
-//   tiles, since every split of a row costs its fp32 partial, written and read (520 bytes at D = 128).
-// us, 32/8 heads of 128, bf16, one split -> this rule: 16 rows behind 16,000 keys 322 -> 28 (64 splits), 512 rows 335 -> 181
-// (4); 512 behind 2,000 61 -> 45; 6 x 37-563 rows behind 4,000-12,000 (MXFP4) 400 -> 326 (3); 8 x 64-500 behind 2,700-8,000
-// 302 -> 291 (2).  Where it keeps one split, two lose: a causal prompt of 2,000 rows 58 -> 85, of 4,000 169 -> 232.
-static int64_t prefill_blocks(int64_t max_rows, int64_t group) { return (max_rows * group + 127) / 128; }
-static int prefill_splits(int64_t n, int64_t kv_heads, int64_t blocks, int64_t n_sinks, int64_t max_span) {
-    const int64_t units = n * kv_heads * blocks, tiles = (max_pages(max_span, n_sinks) + 3) / 4;
-    const int64_t want = ((units <= 256 ? 512 : 2048) + units - 1) / units, most = tiles / (units <= 256 ? 8 : 64);
-    return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), MAX_SPLITS));
 }
 
 }  // namespace ud

@@ -23,7 +23,6 @@
 // 64 x 4,096 keys 182 us, of which the loads alone take all but 2.  MXFP4 pages, 64 x 4,096 keys 55.5 us, the loads alone 52;
 // 64 x 512 .. 8,192 keys (304 MB) 66 us, 4.6 TB/s: conversions, products and softmax in turn in each wave.  One sequence of 8,192 half
 // keys is latency: 12.5 us in 32 splits, and 4 for the join.
-#include <algorithm>
 #include <type_traits>
 
 #include "paged_attention.hpp"
@@ -41,7 +40,7 @@ struct WindowArgs {
     int M, G, Hq, Hkv;
     int max_blocks, num_blocks;
     int sinks, splits, pages, groups;   // pages of a split, groups of 16 RT rows
-    int n, layer;                  // sequences; > 0: taken longest first, and back from the layer-th on (sorted_sequence)
+    int n, layer;                  // sequences; > 0: taken by length (rank_of_layer)
     float scale;                   // log2(e) / sqrt(D)
 };
 
@@ -52,9 +51,8 @@ template <typename E, int FMT> struct Terms {
     static constexpr int P = std::is_same<E, El32>::value ? (H ? 2 : 3) : std::is_same<E, ElH>::value && !H ? 2 : 1;
 };
 
-// The sequence of layer z of the workgroups where a batch of up to 64 is taken by length: rank z of the descending order up
-// to `layer`, then from the shortest back, so that workgroups that share a CU make up for each other.  Each wave ranks them by
-// itself: a lane's sequence has as many before it as have a larger key.  Also its range, from the first lo to the last hi.
+// The sequence of layer z of the workgroups where a batch is taken by length (rank_of_layer, length_key).  Each wave ranks them
+// by itself: a lane's sequence has as many before it as have a larger key.  Also its range, from the first lo to the last hi.
 __device__ __forceinline__ int sorted_sequence(const WindowArgs& a, int z, int& lo, int& hi) {
     const int lane = threadIdx.x & 63, kmax = a.max_blocks * KPAGE;
     int key = -1, l = 0, h = 0;
@@ -62,13 +60,13 @@ __device__ __forceinline__ int sorted_sequence(const WindowArgs& a, int z, int& 
         const int32_t* rg = a.ranges + (int64_t)2 * lane * a.M;
         l = max(rg[0], 0);
         h = min(max(rg[2 * a.M - 1], 0), kmax);
-        key = min(max(h - l, 0), (1 << 25) - 1) << 6 | lane;
+        key = length_key(h - l, lane);
     }
     int before = 0;
     for (int j0 = 0; j0 < a.n; j0 += 8)
 #pragma unroll
         for (int j = 0; j < 8; j++) before += __builtin_amdgcn_readlane(key, j0 + j) > key;
-    const int rank = z < a.layer ? z : a.n - 1 - (z - a.layer);
+    const int rank = rank_of_layer(z, a.layer, a.n);
     const int seq = __builtin_ctzll(__ballot(key >= 0 && before == rank));
     lo = __builtin_amdgcn_readlane(l, seq);
     hi = __builtin_amdgcn_readlane(h, seq);
@@ -520,62 +518,22 @@ __global__ __launch_bounds__(64 * NW, RT == 1 ? 2 : 1) void window_split_kernel(
 }
 
 template <typename E, int FMT, int D>
-static void launch_window_d(WindowArgs a, int n, int waves, bool by_length, hipStream_t st) {
-    const int rows = a.M * a.G;
-    auto go = [&](auto kernel, int groups, int nw) {
-        a.groups = groups;
-        a.n = n;
-        a.layer = !by_length ? 0 : FMT == FMT_FP4 ? std::max(1, 256 / (a.Hkv * groups)) : n;
-        hipLaunchKernelGGL(kernel, dim3(a.Hkv, a.splits * groups, n), dim3(64 * nw), 0, st, a);
+static void launch_window_d(const WindowArgs& a, const WindowPlan& plan, hipStream_t st) {
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(a.Hkv, a.splits * a.groups, a.n), dim3(64 * plan.waves), 0, st, a);
     };
     if constexpr (FMT != FMT_FP4)
-        if (waves == 8) go(window_split_kernel<E, FMT, D, 1, 8>, 1, 8);
-    if (waves == 4) {
-        if (rows <= 16) go(window_split_kernel<E, FMT, D, 1, 4>, 1, 4);
-        else go(window_split_kernel<E, FMT, D, 2, 4>, (rows + 31) / 32, 4);
+        if (plan.waves == 8) go(window_split_kernel<E, FMT, D, 1, 8>);
+    if (plan.waves == 4) {
+        if (plan.tiles == 1) go(window_split_kernel<E, FMT, D, 1, 4>);
+        else go(window_split_kernel<E, FMT, D, 2, 4>);
     }
-    if (a.splits > 1) launch_join<E, D>(a.part, a.stat, a.out, JoinRows{(int64_t)n * a.M * a.Hq, 0, 0, nullptr, 1}, a.splits, st);
+    if (a.splits > 1) launch_join<E, D>(a.part, a.stat, a.out, JoinRows{(int64_t)a.n * a.M * a.Hq, 0, 0, nullptr, 1}, a.splits, st);
 }
 template <typename E, int FMT>
-static void launch_window(const WindowArgs& a, int n, int D, int waves, bool by_length, hipStream_t st) {
-    if (D == 128) launch_window_d<E, FMT, 128>(a, n, waves, by_length, st);
-    else launch_window_d<E, FMT, 64>(a, n, waves, by_length, st);
-}
-
-// Waves of a workgroup, and workgroups: one round of eight waves per CU (512 workgroups of 4 waves, 256 of 8), not quite full
-// rather than just beyond, but at least three quarters of it.  A workgroup's first rows arrive some 3 us after its start (its
-// ranges, its table entries, its pages) and its waves are joined at its end, so few, long ones pay while the chip is full.
-// us at 512 / 1,024 / 2,048 of 4 waves wanted, 32/8 heads of 128: 1 x 60,000 keys bf16 50.6 / 52.4 / 57.4, MXFP4 21.9 / 24.9 /
-// 30.0; 64 x 4,096 bf16 184 / 191 / 194, MXFP4 57.6 / 64.6 / 66.2; 64 x 1,000 bf16 51.0 / 56.8 / 59.5.
-// Beyond or below a round, 4,000 keys: 12 sequences (96 units) 576 -> 480 workgroups bf16 47.8 -> 43.2 us; 50 (400) 800 ->
-// 400 162 -> 146, MXFP4 61.5 -> 51.9; but 33 (264) 528 -> 264 117 -> 132.
-// 8 waves, 16-bit pages of up to 16 rows: the grid is one round, or a sequence has 2,048 keys and more.  They halve the longest
-// workgroup of unequal contexts, and half as many splits are joined; of short ones too many start and end with the CU to
-// themselves.  4 -> 8 waves, bf16, us: 24 x 1,000 25.3 -> 22.1, 24 x 4 queries of 500-8,000 114 -> 104, 8 x 1,000-30,000 111 ->
-// 104, 64 x 512-8,192 231 -> 224, 400 x 100-3,000 452 -> 436, 64 x 4,096 182.4 -> 181.9, but 12 x 4 of 300-8,192 57 -> 61;
-// where 4 stay: 40 x 2,000 67 -> 74, 64 x 1,000 51 -> 55, 200 x 500 80 -> 96.  MXFP4 (its waves are busy, and three
-// workgroups of 4 fit a CU): 64 x 4,096 56 -> 60, 200 x 300-2,000 65 -> 93.
-// By length (sorted_sequence), up to 64 sequences of 2,048 keys and more in more workgroups than CUs: 16-bit pages (a workgroup
-// of 8 waves to a CU) longest first, MXFP4 (two of 4 waves to a CU) the second 256 workgroups shortest first.  In the order given
-// -> by length, us: 64 x 512-8,192 bf16 224 -> 196, MXFP4 75.2 -> 66.8; 40 x 1,000-6,000 bf16 126 -> 110; 64 x 4 queries of
-// 500-8,000 MXFP4 77 -> 69; what it costs where all are alike: 64 x 4,096 bf16 181.4 -> 182.6, 40 x 3,000 107 -> 108.5; where the
-// order given stays: 64 x 1,000 bf16 50.8 -> 53.3, 12 x 4 of 300-8,192 MXFP4 (5 splits) 26 -> 30.
-// A workgroup's waves take 2 pages each at a time (MXFP4: 4), of which a split is a multiple.
-struct WindowPlan {
-    SplitPlan split;
-    int waves;
-    bool by_length;
-};
-static WindowPlan window_plan(bool fp4, int64_t rows, int32_t n, int32_t kv_heads, int32_t n_sinks, int32_t max_span) {
-    // (a window that does not start with a page has one more: the last split takes it)
-    const int64_t pages = std::max<int64_t>(1, ((int64_t)max_span + KPAGE - 1) / KPAGE + ((int64_t)n_sinks + KPAGE - 1) / KPAGE);
-    const int64_t units = (int64_t)n * kv_heads;
-    const int waves = !fp4 && rows <= 16 && (units <= 256 || pages >= 128) ? 8 : 4;
-    const int64_t round = 2048 / waves;
-    int64_t want = round / units;
-    if (want * units < round * 3 / 4) want++;
-    const SplitPlan split = split_plan(want, pages, waves * (fp4 ? 4 : 2));
-    return WindowPlan{split, waves, n <= 64 && units > 256 && split.splits == 1 && pages >= 128};
+static void launch_window(const WindowArgs& a, int D, const WindowPlan& plan, hipStream_t st) {
+    if (D == 128) launch_window_d<E, FMT, 128>(a, plan, st);
+    else launch_window_d<E, FMT, 64>(a, plan, st);
 }
 
 }  // namespace ud
@@ -585,9 +543,7 @@ using namespace ud;
 extern "C" UD_API size_t ud_gqa_window_workspace_bytes(int32_t n, int32_t n_queries, int32_t q_heads, int32_t kv_heads,
                                                        int32_t head_dim, int32_t n_sinks, int32_t max_span) {
     if (n <= 0 || n_queries <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 || n_sinks < 0 || max_span < 0) return 0;
-    // 4 waves over 16-bit pages: the finest of all plans (8 waves want half a round, which is never more splits, of twice the step;
-    // MXFP4 the same round, of twice the step)
-    const int s = window_plan(false, 64, n, kv_heads, n_sinks, max_span).split.splits;
+    const int s = window_most_splits(n, kv_heads, n_sinks, max_span);
     return s == 1 ? 0 : (size_t)n * n_queries * q_heads * s * (head_dim + 2) * sizeof(float);
 }
 
@@ -623,18 +579,19 @@ extern "C" UD_API int ud_gqa_window_attention_paged(int32_t kv_format, int32_t d
     a.stat = a.part + (size_t)n * n_queries * q_heads * plan.split.splits * head_dim;
     a.M = n_queries; a.G = q_heads / kv_heads; a.Hq = q_heads; a.Hkv = kv_heads;
     a.max_blocks = max_blocks; a.num_blocks = num_blocks; a.sinks = n_sinks; a.splits = plan.split.splits; a.pages = plan.split.pages;
+    a.groups = plan.groups; a.n = n; a.layer = plan.layer;
     a.scale = (float)(1.4426950408889634 / sqrt((double)head_dim));
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
     if (kv_format == UD_BF16) {
-        if (dtype == UD_F32) launch_window<El32, FMT_BF16>(a, n, head_dim, plan.waves, plan.by_length, st);
-        else launch_window<ElBf, FMT_BF16>(a, n, head_dim, plan.waves, plan.by_length, st);
+        if (dtype == UD_F32) launch_window<El32, FMT_BF16>(a, head_dim, plan, st);
+        else launch_window<ElBf, FMT_BF16>(a, head_dim, plan, st);
     } else if (kv_format == UD_F16) {
-        if (dtype == UD_F32) launch_window<El32, FMT_F16>(a, n, head_dim, plan.waves, plan.by_length, st);
-        else launch_window<ElH, FMT_F16>(a, n, head_dim, plan.waves, plan.by_length, st);
+        if (dtype == UD_F32) launch_window<El32, FMT_F16>(a, head_dim, plan, st);
+        else launch_window<ElH, FMT_F16>(a, head_dim, plan, st);
     } else {
-        if (dtype == UD_F32) launch_window<El32, FMT_FP4>(a, n, head_dim, plan.waves, plan.by_length, st);
-        else if (dtype == UD_BF16) launch_window<ElBf, FMT_FP4>(a, n, head_dim, plan.waves, plan.by_length, st);
-        else launch_window<ElH, FMT_FP4>(a, n, head_dim, plan.waves, plan.by_length, st);
+        if (dtype == UD_F32) launch_window<El32, FMT_FP4>(a, head_dim, plan, st);
+        else if (dtype == UD_BF16) launch_window<ElBf, FMT_FP4>(a, head_dim, plan, st);
+        else launch_window<ElH, FMT_FP4>(a, head_dim, plan, st);
     }
     return paged_launched(who);
 }
