@@ -129,7 +129,7 @@ UD_API size_t ud_kv_page_bytes(int32_t kv_format, int32_t kv_heads, int32_t head
  * the pages.
  *   q, k, v      dtype (UD_F32, UD_BF16, UD_F16), rows q_ld / k_ld / v_ld elements apart (pieces of one fused row, or
  *                buffers of their own); q_heads 0: no q.  dtype is fp32 or the pages' own; any for UD_MXFP4
- *   q_out        dtype, rows q_out_ld apart; may be q
+ *   q_out        dtype, rows q_out_ld apart; may be q where q_out_ld is q_ld, and shares no memory with q, k and v otherwise
  *   q_weight, k_weight   fp32 [head_dim] or null (no norm);  inv_freq fp32 [head_dim / 2] or null (no rotation)
  * A row whose sequence is outside [0, n), whose position is negative or not below max_blocks * block_size, or whose page
  * is not held, is padding: nothing is written for it, q_out included.  Rows of one call name different keys.

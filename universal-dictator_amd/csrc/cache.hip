@@ -300,6 +300,18 @@ extern "C" UD_API size_t ud_kv_page_bytes(int32_t kv_format, int32_t kv_heads, i
     return (size_t)kv_heads * KPAGE * row;
 }
 
+// Whether `rows` rows of aw elements at a, lda elements apart, share memory with rows of bw at b, ldb apart (byte
+// addresses; different distances: whether the stretches from first to last row do).
+static bool rows_overlap(const void* a, int64_t lda, int64_t aw, const void* b, int64_t ldb, int64_t bw, int64_t rows, int64_t size) {
+    const int64_t d = (int64_t)((uintptr_t)b - (uintptr_t)a), la = aw * size, lb = bw * size;
+    if (rows == 1 || lda != ldb) return d < ((rows - 1) * lda) * size + la && -d < ((rows - 1) * ldb) * size + lb;
+    // row i of a meets row i + t of b where -lb < d + t lda size < la: t is one of the two around -d / (lda size)
+    const int64_t step = lda * size;
+    for (int64_t t = -d / step - 1; t <= -d / step + 1; t++)
+        if (t > -rows && t < rows && d + t * step < la && d + t * step > -lb) return true;
+    return false;
+}
+
 extern "C" UD_API int ud_qk_norm_rope_append(int32_t dtype, int32_t kv_format, const void* q_dev, int32_t q_ld, const void* k_dev,
                                              int32_t k_ld, const void* v_dev, int32_t v_ld, void* q_out_dev, int32_t q_out_ld,
                                              const float* q_weight_dev, const float* k_weight_dev, float eps,
@@ -328,6 +340,11 @@ extern "C" UD_API int ud_qk_norm_rope_append(int32_t dtype, int32_t kv_format, c
     int32_t lds = k_ld | v_ld;
     if (q_heads) { at |= (uintptr_t)q_dev | (uintptr_t)q_out_dev; lds |= q_ld | q_out_ld; }
     if ((at & piece) || (lds & 3)) return paged_fail(UD_ERR_INVALID, "%s: rows must be aligned to four elements", who);
+    // a row's heads are read by one part of a workgroup and written by another
+    const int64_t size = dtype == UD_F32 ? 4 : 2;
+    if (q_heads && ((!(q_out_dev == q_dev && (q_out_ld == q_ld || rows == 1)) && rows_overlap(q_out_dev, q_out_ld, qw, q_dev, q_ld, qw, rows, size)) ||
+                    rows_overlap(q_out_dev, q_out_ld, qw, k_dev, k_ld, kw, rows, size) || rows_overlap(q_out_dev, q_out_ld, qw, v_dev, v_ld, kw, rows, size)))
+        return paged_fail(UD_ERR_INVALID, "%s: q_out overlaps k, v or q (it may be q, at the same distance between rows)", who);
     AppendArgs a{};
     a.q = q_dev; a.k = k_dev; a.v = v_dev; a.q_out = q_out_dev;
     a.q_ld = q_ld; a.k_ld = k_ld; a.v_ld = v_ld; a.qo_ld = q_out_ld;
