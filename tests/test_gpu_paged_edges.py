@@ -57,3 +57,37 @@ def test_append_outputs_beside_inputs(gpu, rows, place):
     want_k = ref.norm_rope(x[:, k0:v0].reshape(rows, hkv, d), None, 0, pos, inv).reshape(rows, -1)
     got_k = ref.from_bits(kb.download((rows, kw), np.uint16), "bf16")
     assert np.all(np.abs(got_k - want_k) <= ref.HALF_STEP["bf16"] * np.abs(want_k) * 1.01 + 5 * 2.0 ** -24 * np.sqrt(2) * np.abs(x).max())
+
+
+@pytest.mark.parametrize("norm", [False, True])
+def test_fp4_keys_past_fp32_saturate(gpu, norm):
+    """Finite rows whose normalised and rotated keys pass fp32's range: the largest code and exponent, not a block of NaN; the
+    other blocks, and blocks of infinities and NaN, as ever."""
+    ud, rng, d = gpu, np.random.default_rng(92), 128
+    rows, big = 6, float(np.float32(3.3e38))
+    x = rng.standard_normal((rows, 2, d))
+    weight = None
+    pos, inv = np.arange(rows) * 7 + 1, ud.rope_inv_freq(d)
+    if norm:
+        weight = np.ones(d, np.float32)
+        weight[[3, 40, 67, 100]] = 3e38                  # times up to sqrt(d): past fp32
+        x[:, 0, 3], x[:, 0, 100] = 9, -7
+    else:
+        x[:, 0, 0], x[:, 0, 64] = big, -big              # rotated by pos: up to 1.41 times as long
+        x[1, 0, 70], x[1, 0, 6] = big, big
+        x[2, 0, 33], x[3, 0, 97] = np.inf, np.nan
+    x = ref.rounded(x, "f32")
+    table, num = ref.assign_pages(rng, [int(p) + 1 for p in pos])
+    kp, vp = (_dev(ud, ref.new_pool("mxfp4", num, 1, d)) for _ in range(2))
+    k, v, bt, pd, iv = (_dev(ud, a) for a in (x[:, 0].astype(np.float32), x[:, 1].astype(np.float32), table, pos.astype(np.int32), inv))
+    ud.qk_norm_rope_append(None, k, v, None, kp, vp, num, bt, rows, table.shape[1], pd, rows, 0, 1, d, inv_freq=iv, dtype="f32",
+                           kv_format="mxfp4", k_weight=None if weight is None else _dev(ud, weight))
+    kb, vb = ud.DeviceBuffer(rows * d * 4), ud.DeviceBuffer(rows * d * 4)
+    ud.paged_kv_read(kp, vp, num, bt, rows, table.shape[1], pd, kb, vb, rows, 1, d, kv_format="mxfp4")
+    ud.synchronize()
+    with np.errstate(invalid="ignore"):
+        want = ref.norm_rope(x[:, :1], weight, 1e-6, pos, inv)
+    finite = np.isfinite(want)
+    assert np.abs(want[finite]).max() > 3.41e38
+    np.testing.assert_array_equal(kb.download((rows, 1, d)), ref.held(want, "mxfp4"))
+    np.testing.assert_array_equal(vb.download((rows, 1, d)), ref.held(x[:, 1:], "mxfp4"))

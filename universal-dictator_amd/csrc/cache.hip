@@ -62,11 +62,12 @@ __device__ __forceinline__ uint32_t group_max8(uint32_t v) {
 }
 
 // x in fp32 by rounding to odd: not exact -> the last bit is set.  Such a value is on the same side of every
-// border of fewer bits as x, so that a second rounding to nearest gives what one rounding of x would.
+// border of fewer bits as x, so that a second rounding to nearest gives what one rounding of x would.  A finite x past
+// fp32's range becomes its largest value, which is odd.
 __device__ __forceinline__ float round_odd(double x) {
     const float f = (float)x;
     const double b = (double)f;
-    if (b == x || !__builtin_isfinite(f)) return f;
+    if (b == x || x != x) return f;
     uint32_t u = __float_as_uint(f);
     if (fabs(b) > fabs(x)) u -= 1;                 // towards zero
     return __uint_as_float(u | 1);
