@@ -166,8 +166,10 @@ UD_API int ud_paged_kv_read(int32_t kv_format, int32_t dtype, const void* k_page
  * A call repeated gives the same bits; the keys are split over workgroups by n and max_span, so that the last bits of a
  * row may differ between calls that differ in these.
  * Precision: fp32 queries and outputs are as good as fp32 arithmetic; 16-bit ones: exact products, sums in fp32, the
- * probabilities rounded once to the pages' type (bf16 for UD_MXFP4, twice that for half queries).  A NaN or infinity in
- * a key or value reaches only the rows that see it. */
+ * probabilities rounded once to the pages' type (bf16 for UD_MXFP4, twice that for half queries); a value past 2^90
+ * may pass fp32's range in the sums, which are divided at the end.  A NaN or infinity in a key or value reaches only the
+ * rows that see it: a NaN in a key makes them NaN, an infinity in a key may; a channel with an infinity among the values is
+ * that infinity, however small its probability (half outputs: 65504), with one of both signs or a NaN it is NaN. */
 UD_API size_t ud_gqa_window_workspace_bytes(int32_t n, int32_t n_queries, int32_t q_heads, int32_t kv_heads,
                                             int32_t head_dim, int32_t n_sinks, int32_t max_span);
 UD_API int ud_gqa_window_attention_paged(int32_t kv_format, int32_t dtype, const void* q_dev, const void* k_pages,

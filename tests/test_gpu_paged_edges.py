@@ -3,6 +3,7 @@ import numpy as np
 import pytest
 
 import paged_ref as ref
+from test_gpu_paged_window import P_STEP, PROMPT_STEP, Cache, causal, close, prefill, window
 
 pytestmark = pytest.mark.gpu
 
@@ -91,3 +92,64 @@ def test_fp4_keys_past_fp32_saturate(gpu, norm):
     assert np.abs(want[finite]).max() > 3.41e38
     np.testing.assert_array_equal(kb.download((rows, 1, d)), ref.held(want, "mxfp4"))
     np.testing.assert_array_equal(vb.download((rows, 1, d)), ref.held(x[:, 1:], "mxfp4"))
+
+
+def _infinite_values(ud, fmt, keys, d, low):
+    """A cache whose values are infinite in places: channel 1 +inf at key 5, 2 -inf at key 70, 3 both, 4 a NaN, 5 +inf at key 80, 6 +inf
+    near the end.  The scores of key 80 and of the first `low` keys, of queries along e, are so far below the rest's that their
+    probabilities, about exp(-300), are 0 in fp32."""
+    rng, hkv = np.random.default_rng([93, keys, d]), 2
+    e = rng.standard_normal(d)
+    e /= np.linalg.norm(e)
+    k, v = 0.3 * rng.standard_normal((keys, hkv, d)), rng.standard_normal((keys, hkv, d))
+    far = -300 * np.sqrt(d) / 8
+    k[:low] += far * e
+    k[80] = far * e
+    v[5, :, 1] = v[5, :, 3] = v[80, 0, 5] = v[keys - 25, 1, 6] = np.inf
+    v[70, :, 2] = v[70, :, 3] = -np.inf
+    v[70, 1, 4] = np.nan
+    return e, Cache(ud, rng, fmt, [keys], hkv, d, k=[ref.held(k, fmt)], v=[ref.held(v, fmt)])
+
+
+def _check_infinite(got, want, c, d, dtype, p_step):
+    """Outputs are infinite or NaN exactly where the formula's are (p > 0: an infinity however small p is), half ones saturated;
+    the others within their tolerance."""
+    out, mag, top, dot, count = want
+    got = got.reshape(out.shape).copy()
+    odd = ~np.isfinite(out)
+    assert np.isposinf(out).any() and np.isneginf(out).any() and np.isnan(out).any() and not odd[..., 7:].any()
+    np.testing.assert_array_equal(got[odd], np.clip(out[odd], -65504, 65504) if dtype == "f16" else out[odd])
+    got[odd] = 0
+    close(got, (np.where(odd, 0, out), np.where(odd, 0, mag), top, dot, count), c, d, dtype, p_step)
+
+
+@pytest.mark.filterwarnings("ignore:invalid value")
+@pytest.mark.parametrize("fmt,dtype", [("bf16", "bf16"), ("bf16", "f32"), ("f16", "f16"), ("f16", "f32")])
+@pytest.mark.parametrize("d,group,keys,low", [(128, 1, 160, 0), (64, 7, 160, 0), (128, 4, 6000, 2000), (64, 2, 6000, 2000)])
+def test_infinite_values_that_are_seen(gpu, fmt, dtype, d, group, keys, low):
+    """An infinity among a row's values makes its output that infinity, whether the other rows of the workgroup see its page whole
+    or in part."""
+    ud, hq, M = gpu, 2 * group, 3
+    e, c = _infinite_values(ud, fmt, keys, d, low)
+    q = ref.rounded(np.random.default_rng(94).standard_normal((1, M, hq, d)) * 0.3 + 8 * e, dtype)
+    for r in ([[0, keys]] * M, [[0, keys], [3, keys - 2], [37, keys - 31]], [[70, keys - 20], [71, keys], [9, 9]], [[0, keys], [0, 5], [5, 6]]):
+        ranges = np.array([r])
+        want = ref.attention(q[0], c.k, c.v, np.zeros(M, int), ranges[0], 4, 2, c.most * 16)
+        got = window(ud, c, q, ranges, 4, dtype, span=keys)
+        if r[0][0] == 70:                                # key 5 is not seen, nor key 70 by the second row
+            assert not np.isposinf(want[0][..., :4]).any()
+        _check_infinite(got, want, c, d, dtype, P_STEP[fmt, dtype])
+
+
+@pytest.mark.filterwarnings("ignore:invalid value")
+@pytest.mark.parametrize("fmt", ["bf16", "f16"])
+@pytest.mark.parametrize("d,keys,low,win", [(128, 160, 0, 0), (64, 320, 0, 260), (128, 6000, 2000, 0), (64, 6000, 2000, 5950)])
+def test_infinite_values_that_prompts_see(gpu, fmt, d, keys, low, win):
+    ud, hq, rows = gpu, 4, 70
+    e, c = _infinite_values(ud, fmt, keys, d, low)
+    q = ref.rounded(np.random.default_rng(95).standard_normal((rows, hq, d)) * 0.3 + 8 * e, fmt)
+    whole = np.tile([0, keys // 16 * 16], (rows, 1))
+    for ranges in (whole, causal([rows], [keys - rows], win)):
+        want = ref.attention(q, c.k, c.v, np.zeros(rows, int), ranges, 2, 2, c.most * 16)
+        got = prefill(ud, c, q, [0, rows], ranges, 2, fmt, span=keys)
+        _check_infinite(got, want, c, d, fmt, PROMPT_STEP[fmt])

@@ -53,10 +53,24 @@ template <bool H, int T> __device__ __forceinline__ void split8(const float (&x)
     }
 }
 
+// Channels ch .. ch + 3 of row `key` of a head's page of values, those that are no numbers added to sum.
+template <int FMT, int D> __device__ __forceinline__ void odd_values(const char* v, int key, int ch, float (&sum)[4]) {
+    float x[4];
+    if constexpr (FMT == FMT_FP4) {
+        const uint8_t e = *reinterpret_cast<const uint8_t*>(v + Page<FMT, D>::CODES + key * (D / FP4_BLOCK) + ch / FP4_BLOCK);
+        x[0] = x[1] = x[2] = x[3] = e == 255 ? NAN : 0.0f;
+    } else {
+        typedef typename std::conditional<FMT == FMT_BF16, ElBf, ElH>::type E;
+        load4<E>(reinterpret_cast<const uint16_t*>(v) + key * D + ch, x);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) sum[i] += __builtin_isfinite(x[i]) ? 0.0f : x[i];
+}
+
 // The splits of one (query row, head) joined, 16 a wave (one round trip to memory however many there are; at most 16
 // splits: four rows a workgroup): with split s's maximum m_s (of scores times log2(e)), sum l_s
 // and unnormalised output x_s,  out = sum_s 2^(m_s - m) x_s / sum_s 2^(m_s - m) l_s.  A split without a key has m = -inf,
-// l = 0 and its x is not looked at.
+// l = 0 and its x is not looked at.  An x that is no number stays what it is, also where its weight is 0 in fp32.
 // Bound: memory; of few rows the round trip.  57,600 rows of 3 splits at D = 128 (90 MB of partials) 23 us, 32 rows of 64
 // splits 4 us.
 // The rows: `count` of them, or (start) those of each sequence y, tokens start[y] .. start[y + 1] - 1 of `tokens`, at most
@@ -119,13 +133,27 @@ __global__ __launch_bounds__(1024) void join_splits_kernel(const float* part, co
     }
     sum = wave_sum(sum);
     float acc[DL];
+    bool odd = false;
 #pragma unroll
     for (int e = 0; e < DL; e++) acc[e] = 0.0f;
+    auto weight = [&](int s) { return first + s < splits ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), (first & 63) + s)) : -1.0f; };
 #pragma unroll
     for (int s = 0; s < DEEP; s++) {
-        const float w = first + s < splits ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(mine), (first & 63) + s)) : -1.0f;
+        const float w = weight(s);
 #pragma unroll
         for (int e = 0; e < DL; e++) acc[e] += w < 0.0f ? 0.0f : w * x[s][e];
+    }
+#pragma unroll
+    for (int e = 0; e < DL; e++) odd |= !__builtin_isfinite(acc[e]);
+    if (__builtin_expect(__any(odd), 0)) {                       // (selected in the sum above: 15.1 -> 16.0 us a call of one sequence)
+#pragma unroll
+        for (int e = 0; e < DL; e++) acc[e] = 0.0f;
+#pragma unroll
+        for (int s = 0; s < DEEP; s++) {
+            const float w = weight(s);
+#pragma unroll
+            for (int e = 0; e < DL; e++) acc[e] += w < 0.0f ? 0.0f : __builtin_isfinite(x[s][e]) ? w * x[s][e] : x[s][e];
+        }
     }
     if (each > 1) {
 #pragma unroll

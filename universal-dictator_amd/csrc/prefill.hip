@@ -391,34 +391,45 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
     }
     __syncthreads();
 
-    if (odd) {
-        // values that are no numbers, in pages that the workgroup's rows see in part: to the rows that see them
-        for (int u = 4 * t0; u < min(4 * t1, list.count); u++) {
-            const int blk = page_at(list, u), page = bt[blk];
-            if (!partial(blk) || page < 0 || page >= a.num_blocks) continue;
-            const char* v = a.vp + ((int64_t)page * a.Hkv + kvh) * HEAD;
-            for (int key = 0; key < KPAGE; key++) {
+    const float l = some_key ? xadd32(rsum) : 0.0f;
+    // Values that are no numbers, to the rows that see them: an infinity, or NaN for both signs or a NaN.  Those of pages that
+    // the workgroup's rows see in part were left out of the products, and those of whole pages may have become either there
+    // (0 x infinity, where a probability is 0 in 16 bits), so both are taken from the pages.  (A block of MXFP4 that is no
+    // number is NaN in every product.)
+    bool bad = odd;
+    if constexpr (FMT != FMT_FP4) {                // (one sum: a test for each of the 64 took 0.4 us of a short prompt)
+        f32x4_t t = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int c = 0; c < CT; c++)
+        for (int c = 0; c < CT; c++)
 #pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const int ch = 32 * c + 8 * (i >> 2) + 4 * h + (i & 3);
-                        float x;
-                        if constexpr (FMT == FMT_FP4) {
-                            const uint8_t e = *reinterpret_cast<const uint8_t*>(v + Page<FMT, D>::CODES + key * (D / FP4_BLOCK) + ch / FP4_BLOCK);
-                            x = e == 255 ? NAN : 0.0f;
-                        } else {
-                            const uint16_t w = *reinterpret_cast<const uint16_t*>(v + (key * D + ch) * 2);
-                            x = H ? h2f(w) : bf2f(w);
-                        }
-                        o[c][i] += sees(blk * KPAGE + key) && !__builtin_isfinite(x) ? x : 0.0f;
+            for (int i = 0; i < 16; i++) t[i & 3] += o[c][i];
+        bad |= !__builtin_isfinite((t[0] + t[1]) + (t[2] + t[3]));
+    }
+    bad = bad && some_key && l == l;
+    if (__builtin_expect(__any(bad), 0)) {
+#pragma unroll
+        for (int c = 0; c < CT; c++) {
+            float sum[4][4] = {};
+            for (int u = 4 * t0; u < min(4 * t1, list.count); u++) {
+                const int blk = page_at(list, u), page = bt[blk];
+                if (page < 0 || page >= a.num_blocks) continue;
+                bool open = false;                 // NaN is final
+#pragma unroll
+                for (int i = 0; i < 16; i++) open |= (odd || !__builtin_isfinite(o[c][i])) && sum[i >> 2][i & 3] == sum[i >> 2][i & 3];
+                if (!__any(bad && open)) break;
+                const char* v = a.vp + ((int64_t)page * a.Hkv + kvh) * HEAD;
+                for (int key = 0; key < KPAGE; key++)
+                    if (sees(blk * KPAGE + key)) {
+#pragma unroll
+                        for (int i = 0; i < 4; i++) odd_values<FMT, D>(v, key, 32 * c + 8 * i + 4 * h, sum[i]);
                     }
             }
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[c][i] = bad && sum[i >> 2][i & 3] != 0.0f ? sum[i >> 2][i & 3] : o[c][i];
         }
     }
 
     if (!real) return;
-    const float l = some_key ? xadd32(rsum) : 0.0f;
     // a row without a key: 0.  l is NaN where a score is (base may still be -inf then).
     const float inv = l == 0.0f ? 0.0f : a.splits > 1 ? 1.0f : 1.0f / l;
 #pragma unroll

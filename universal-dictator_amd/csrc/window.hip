@@ -443,30 +443,28 @@ __global__ __launch_bounds__(64 * NW, RT == 1 ? 2 : 1) void window_split_kernel(
         if (g == 0) { wmax[wave][16 * rt + col] = rmax[rt]; wsum[wave][16 * rt + col] = empty ? 0.0f : l; }
     }
     __syncthreads();
-    // To channels ch .. ch + 3 of row r: the values that are no numbers, of keys that it sees, in pages where they were left
-    // out.
-    auto give_odd = [&](int r, int ch, float (&y)[4]) {
+    // Channels ch .. ch + 3 of row r where it sees values that are no numbers: their sum, so an infinity, or NaN for both signs or
+    // a NaN.  Those of pages that rows see in part were left out of the products, and those of whole pages may have become
+    // either there (a probability that is 0 in fp32, or whose second term is), so both are taken from the pages.
+    auto give_odd = [&](int r, int ch, bool left_out, float (&y)[4]) {
         const int m = (r0 + r) / G, l = max(rg[2 * m], 0), e = min(rg[2 * m + 1], kmax), sk = l < e ? min(a.sinks, l) : 0;
+        float sum[4] = {0, 0, 0, 0};
+#pragma unroll 1
         for (int c = u0; c < u1; c++) {
             const int blk = page_at(list, c), page = bt[blk];
-            if (whole(blk) || page < 0 || page >= a.num_blocks) continue;
+            if (page < 0 || page >= a.num_blocks) continue;
+            bool open = false;                     // NaN is final
+            for (int i = 0; i < 4; i++) open |= (left_out || !__builtin_isfinite(y[i])) && sum[i] == sum[i];
+            if (!open) break;
             const char* v = a.vp + ((int64_t)page * a.Hkv + kvh) * HEAD;
+#pragma unroll 1
             for (int key = 0; key < KPAGE; key++) {
                 const int j = blk * KPAGE + key;
                 if (!((j >= l && j < e) || j < sk)) continue;
-                for (int i = 0; i < 4; i++) {
-                    float x;
-                    if constexpr (FMT == FMT_FP4) {
-                        const uint8_t b = *reinterpret_cast<const uint8_t*>(v + Page<FMT, D>::CODES + key * (D / FP4_BLOCK) + (ch + i) / FP4_BLOCK);
-                        x = b == 255 ? NAN : 0.0f;
-                    } else {
-                        const uint16_t w = *reinterpret_cast<const uint16_t*>(v + (key * D + ch + i) * 2);
-                        x = H ? h2f(w) : bf2f(w);
-                    }
-                    y[i] += __builtin_isfinite(x) ? 0.0f : x;
-                }
+                odd_values<FMT, D>(v, key, ch, sum);
             }
         }
+        for (int i = 0; i < 4; i++) y[i] = sum[i] != 0.0f ? sum[i] : y[i];
     };
     // a wave's share of a row with maximum m over the waves (1 where both are -inf: a sum of NaN scores stays NaN)
     auto share = [](float mine, float m) { return mine == m ? 1.0f : __builtin_amdgcn_exp2f(mine - m); };
@@ -501,7 +499,9 @@ __global__ __launch_bounds__(64 * NW, RT == 1 ? 2 : 1) void window_split_kernel(
                 l += wsum[w][r] * share(wmax[w][r], mm);
                 any_odd |= odd_of[w];
             }
-            if (any_odd) give_odd(r, 4 * piece, y);
+            // (a block of MXFP4 that is no number is NaN in every product)
+            const bool odd_here = any_odd || (FMT != FMT_FP4 && !__builtin_isfinite(y[0] + y[1] + y[2] + y[3]));
+            if (__builtin_expect(odd_here && l == l, 0)) give_odd(r, 4 * piece, any_odd, y);
             if (a.splits == 1) {
                 const float inv = l == 0.0f ? 0.0f : 1.0f / l;
 #pragma unroll
