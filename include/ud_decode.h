@@ -112,7 +112,8 @@ UD_API int ud_paged_kv_append(int32_t kv_dtype, const void* k_new, const void* v
  *   UD_MXFP4   per page and kv head block_size rows of head_dim / 2 bytes, channel 2b in the low nibble of byte b, then
  *              block_size rows of head_dim / 32 bytes: the exponent + 127 of each block of 32 channels.  A nibble is a
  *              sign bit and one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 (codes 0 .. 7), times 2^exponent: 4.25 bits a value.
- *              Exponent byte 255: the block held a NaN or an infinity and reads as NaN.
+ *              Exponent byte 255: the block held a NaN or an infinity and reads as NaN.  Else the byte is 27 .. 252, what
+ *              ud_qk_norm_rope_append writes: a page that a row sees has no other.
  * k_pages / v_pages are ud_kv_page_bytes(..) bytes a page, 16-byte aligned, num_blocks pages each.  A block-table entry
  * outside [0, num_blocks) is a page that is not held: nothing of it is read or written, and its keys are not there.
  * They have no counterpart in the reference beyond the ones named; limits: head_dim 64 or 128, block_size 16. */
@@ -189,8 +190,10 @@ UD_API int ud_gqa_window_attention_paged(int32_t kv_format, int32_t dtype, const
  *   max_span        upper bound of a sequence's keys from its lowest lo to its highest hi (a plan, as above; n and
  *                   max_rows count in it too)
  *   workspace       ud_gqa_prefill_workspace_bytes(..) bytes (0: may be null)
- * Precision: exact products, sums and softmax in fp32, probabilities rounded once to dtype, one rounding at the end.
- * UD_MXFP4 pages under half queries: cached values past half's range saturate. */
+ * Precision: exact products, sums and softmax in fp32, probabilities rounded once to dtype, one rounding at the end; NaN and
+ * infinities as above.  UD_MXFP4 pages under half queries: keys and values become halves.  Blocks of exponents -23 .. 13
+ * stay as they are; above, values past 65504 saturate to it, and below, values are rounded to a multiple of 2^-24, 2^-25 and
+ * less to 0 (ud_gqa_window_attention_paged takes all of them as they are). */
 UD_API size_t ud_gqa_prefill_workspace_bytes(int32_t n, int32_t rows, int32_t max_rows, int32_t q_heads, int32_t kv_heads,
                                              int32_t head_dim, int32_t n_sinks, int32_t max_span);
 UD_API int ud_gqa_prefill_paged(int32_t kv_format, int32_t dtype, const void* q_dev, const void* k_pages,

@@ -153,3 +153,39 @@ def test_infinite_values_that_prompts_see(gpu, fmt, d, keys, low, win):
         want = ref.attention(q, c.k, c.v, np.zeros(rows, int), ranges, 2, 2, c.most * 16)
         got = prefill(ud, c, q, [0, rows], ranges, 2, fmt, span=keys)
         _check_infinite(got, want, c, d, fmt, PROMPT_STEP[fmt])
+
+
+def test_half_queries_over_small_fp4_values(gpu):
+    """Blocks below half's normal range: the prompt's values are the nearest multiples of 2^-24, the windowed call's the cached
+    ones."""
+    ud, d = gpu, 128
+    v = np.zeros((1, 1, d))
+    for b, e in enumerate((-22, -23, -24, -25)):
+        v[0, 0, 32 * b:32 * b + 14] = np.concatenate([ref.LEVELS[1:], -ref.LEVELS[1:]]) * 2.0 ** e
+    c = Cache(ud, np.random.default_rng(96), "mxfp4", [1], 1, d, k=[np.zeros((1, 1, d))], v=[v])
+    got = prefill(ud, c, np.ones((1, 1, d)), [0, 1], np.array([[0, 1]]), 0, "f16")[0, 0]
+    np.testing.assert_array_equal(got, v[0, 0].astype(np.float16).astype(np.float64))
+    np.testing.assert_array_equal(got[:64], v[0, 0, :64])    # exponents -22 and -23 stay as they are
+    assert (got[64:] != v[0, 0, 64:]).any()
+    got = window(ud, c, np.ones((1, 1, 1, d)), np.array([[[0, 1]]]), 0, "f32")[0, 0, 0]
+    np.testing.assert_array_equal(got, v[0, 0])
+
+
+def test_half_queries_over_small_fp4_keys(gpu):
+    """Keys of 2^-25 under queries near half's end: the prompt's scores are those of the keys rounded to half (all 0), the
+    windowed call's those of the cached keys."""
+    ud, rng, d, keys = gpu, np.random.default_rng(97), 64, 32
+    sign = rng.choice([-1.0, 1.0], (keys, 1, 1))
+    k = np.tile(sign * 2.0 ** -25, (1, 1, d))
+    v = sign * rng.choice([1.0, 1.5, 2.0], (keys, 1, d))
+    c = Cache(ud, rng, "mxfp4", [keys], 1, d, k=[k], v=[v])
+    assert np.array_equal(ref.held(k, "mxfp4"), k) and np.array_equal(ref.held(v, "mxfp4"), v)
+    q = ref.rounded(rng.uniform(30_000, 60_000, (2, 4, d)), "f16")
+    ranges, seq = np.array([[0, keys], [3, keys]]), np.zeros(2, int)
+    exact = ref.attention(q, c.k, c.v, seq, ranges, 0, 1, keys)
+    half = ref.attention(q, [k.astype(np.float16).astype(np.float64)], c.v, seq, ranges, 0, 1, keys)
+    assert np.abs(exact[0] - half[0]).min() > 2 * ref.attention_tolerance(*exact, d, "f16", PROMPT_STEP["f16"]).max()
+    got = window(ud, c, q[None], ranges[None], 0, "f16")
+    close(got, exact, c, d, "f16", P_STEP["mxfp4", "f16"])
+    got = prefill(ud, c, q, [0, 2], ranges, 0, "f16")
+    close(got, half, c, d, "f16", PROMPT_STEP["f16"])

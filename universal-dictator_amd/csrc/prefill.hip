@@ -41,7 +41,9 @@ template <bool H> __device__ __forceinline__ f32x16_t mfma32(uint4 a, uint4 b, f
     else return __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
 }
 
-// Eight codes of a block as pairs of the products' type.  As halves, a block whose scale is past 2^13 saturates.
+// Eight codes of a block as pairs of the products' type.  As halves, a block whose scale is past 2^13 saturates and one below
+// 2^-23 is rounded: bf16 products of two terms of q and of the probabilities would be exact, but twice as many, and q's second
+// term does not fit the registers of two waves a SIMD.
 template <bool H> __device__ __forceinline__ uint4 fp4_to_16(uint32_t w, uint32_t byte) {
     const float scale = fp4_scale(byte);
     if constexpr (!H) {
