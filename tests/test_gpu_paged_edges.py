@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 import paged_ref as ref
-from test_gpu_paged_window import P_STEP, PROMPT_STEP, Cache, causal, close, prefill, window
+from test_gpu_paged_window import P_STEP, PROMPT_STEP, PROMPTS, TYPES, Cache, causal, close, prefill, window
 
 pytestmark = pytest.mark.gpu
 
@@ -189,3 +189,72 @@ def test_half_queries_over_small_fp4_keys(gpu):
     close(got, exact, c, d, "f16", P_STEP["mxfp4", "f16"])
     got = prefill(ud, c, q, [0, 2], ranges, 0, "f16")
     close(got, half, c, d, "f16", PROMPT_STEP["f16"])
+
+
+def _huge(ud, fmt, dtype, d, q_log, k_log):
+    """Keys and queries along one direction: scores of about 2^(q_log + k_log + 10.6) in binary digits that rise, fall and repeat
+    over the keys, and whose largest is ahead of the next by 1 in 128 or more (or by nothing: equal keys)."""
+    rng, keys, hkv, rows, hq = np.random.default_rng([98, q_log, k_log, d]), 330, 2, 6, 4
+    e = rng.choice([-1.0, 1.0], d)
+    a = 64 + np.concatenate([np.arange(60), 40 - np.arange(40), rng.integers(0, 63, keys - 100)])
+    a[[100, 217, 320]] = 127
+    a[[150, 151]] = 63
+    k = ref.held((a * 2.0 ** k_log)[:, None, None] * e * np.ones((1, hkv, 1)), fmt)
+    c = Cache(ud, rng, fmt, [keys], hkv, d, k=[k])
+    sign = rng.choice([-1.0, 1.0], (rows, hq, 1)) * np.array([1, 1.5, 1.25, 1.0, 1.75, 1.0])[:, None, None]
+    return c, ref.rounded(sign * 2.0 ** q_log * e, dtype)
+
+
+def _check_huge(got, want, dtype, p_step):
+    """The mean of the values of the equal keys whose score is the largest: every other's probability is 0."""
+    out, mag, top, dot, count = want
+    assert np.all(np.abs(got.reshape(out.shape) - out) <= (p_step + 2.0 ** -20) * mag + ref.HALF_STEP[dtype] * np.abs(out) * 1.01 + 2.0 ** -25)
+
+
+HUGE = {"f16": [(5, 0), (10, 1), (12, 4), (14, 8)], "bf16": [(5, 0), (9, 0), (12, 4), (20, 10), (40, 30), (55, 50)]}
+
+
+@pytest.mark.parametrize("fmt,dtype", TYPES)
+@pytest.mark.parametrize("d", [64, 128])
+def test_huge_scores(gpu, fmt, dtype, d):
+    """Scores up to 2^115, where one step of fp32 is far more than the exponents that a probability has room for."""
+    ud = gpu
+    for q_log, k_log in HUGE["f16" if "f16" in (fmt, dtype) else "bf16"]:
+        c, q = _huge(ud, fmt, dtype, d, q_log, k_log)
+        ranges = np.array([[0, 330], [0, 330], [3, 217], [150, 320], [50, 160], [99, 152]])
+        want = ref.attention(q, c.k, c.v, np.zeros(6, int), ranges, 0, 2, c.most * 16)
+        _check_huge(window(ud, c, q[None], ranges[None], 0, dtype), want, dtype, P_STEP[fmt, dtype])
+        split = window(ud, c, q[None], ranges[None], 0, dtype, span=100_000)      # (many splits, most of them empty)
+        _check_huge(split, want, dtype, P_STEP[fmt, dtype])
+
+
+@pytest.mark.parametrize("fmt,dtype", PROMPTS)
+@pytest.mark.parametrize("d", [64, 128])
+def test_huge_scores_of_prompts(gpu, fmt, dtype, d):
+    ud = gpu
+    for q_log, k_log in HUGE["f16" if "f16" in (fmt, dtype) else "bf16"]:
+        c, q = _huge(ud, fmt, dtype, d, q_log, k_log)
+        q = np.tile(q, (50, 1, 1))
+        ranges = causal([300], [30], 0)
+        want = ref.attention(q, c.k, c.v, np.zeros(300, int), ranges, 0, 2, c.most * 16)
+        for span in (330, 20_000):
+            _check_huge(prefill(ud, c, q, [0, 300], ranges, 0, dtype, span=span), want, dtype, PROMPT_STEP[dtype])
+
+
+@pytest.mark.parametrize("fmt,dtype", [("f16", "f16"), ("f16", "f32"), ("bf16", "bf16"), ("mxfp4", "bf16")])
+def test_huge_scores_in_all_directions(gpu, fmt, dtype):
+    """Random keys and queries up to half's end: outputs are mixtures of the values that a row sees, none infinite or NaN, none 0 for
+    want of a probability."""
+    ud, rng, d, keys = gpu, np.random.default_rng(99), 64, 700
+    for size in (600, 2_500, 9_000):
+        k = [ref.held(np.clip(rng.standard_normal((keys, 1, d)) * size, -60_000, 60_000), fmt)]
+        v = [ref.held(1 + rng.random((keys, 1, d)), fmt)]
+        c = Cache(ud, rng, fmt, [keys], 1, d, k=k, v=v)
+        q = ref.rounded(np.clip(rng.standard_normal((70, 8, d)) * size, -60_000, 60_000), dtype)
+        ends = keys - 69 + np.arange(70)
+        ranges = np.stack([0 * ends, ends], -1)
+        got = [window(ud, c, q[None, 62:], ranges[None, 62:], 0, dtype), window(ud, c, q[None, :5], ranges[None, :5], 0, dtype, span=50_000)]
+        if dtype != "f32":
+            got += [prefill(ud, c, q, [0, 70], ranges, 0, dtype, span=s) for s in (keys, 20_000)]
+        for x in got:
+            assert np.all((x >= v[0].min() * (1 - 2.0 ** -7)) & (x <= v[0].max() * (1 + 2.0 ** -7)))

@@ -53,6 +53,16 @@ template <bool H, int T> __device__ __forceinline__ void split8(const float (&x)
     }
 }
 
+// A probability is 2^(x scale - off) by one fused operation, which takes the product x scale as it is, while the base in off is
+// a rounded one.  From bases of STEEP on the two differ by more than 2^-4, and further up by more than a 16-bit probability has
+// room for, so that the largest would become infinite or 0.  There the product is rounded as the base was: this x gives
+// that by the same operation, the base left out of off.
+constexpr float STEEP = 0x1p20f;
+__device__ __forceinline__ float steep_score(float x, float scale, float base) {
+#pragma clang fp contract(off)
+    return (x * scale - base) * (1.0f / scale);
+}
+
 // Channels ch .. ch + 3 of row `key` of a head's page of values, those that are no numbers added to sum.
 template <int FMT, int D> __device__ __forceinline__ void odd_values(const char* v, int key, int ch, float (&sum)[4]) {
     float x[4];

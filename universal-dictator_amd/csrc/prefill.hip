@@ -300,9 +300,17 @@ __global__ __launch_bounds__(256, 2) void prefill_kernel(PrefillArgs a) {
             constexpr bool MORE = decltype(more)::value;
             // ---- the next tile's scores, two products at a time, and between them this tile's probabilities: packed pairs,
             // eight of a lane's scores being the B operand of 16 keys.  The order is kept by the scheduling barriers.
-            const f32x16_t x[2] = {p[0], p[1]};
+            f32x16_t x[2] = {p[0], p[1]};
             // halves: 2^7 times the probabilities, up to 2^15, so that small ones keep their bits (the sum has it too)
-            const float off = (base == -INFINITY ? 0.0f : base) - (H ? 7.0f : 0.0f);
+            float off = (base == -INFINITY ? 0.0f : base) - (H ? 7.0f : 0.0f);
+            const bool steep = fabsf(off) >= STEEP;
+            if (__builtin_expect(__any(steep), 0)) {
+#pragma unroll
+                for (int c = 0; c < 2; c++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) x[c][i] = steep ? steep_score(x[c][i], a.scale, base) : x[c][i];
+                off = steep ? (H ? -7.0f : 0.0f) : off;
+            }
             uint32_t pw[16];
             const char* kb = kt[(tile + 1 - t0) & 1] + k_lane;
             const char* vb = vt[(tile - t0) & 1] + v_lane;

@@ -393,7 +393,15 @@ __global__ __launch_bounds__(64 * NW, RT == 1 ? 2 : 1) void window_split_kernel(
                 rmax[rt] = to;
             }
             // halves: 2^7 times the probabilities, up to 2^15, so that small ones keep their bits (the sum has it too)
-            const float off = (rmax[rt] == -INFINITY ? 0.0f : rmax[rt]) - (H ? 7.0f : 0.0f);
+            float off = (rmax[rt] == -INFINITY ? 0.0f : rmax[rt]) - (H ? 7.0f : 0.0f);
+            const bool steep = fabsf(off) >= STEEP;
+            if (__builtin_expect(__any(steep), 0)) {
+#pragma unroll
+                for (int t = 0; t < CP; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) p[rt][t][i] = steep ? steep_score(p[rt][t][i], qscale[rt], rmax[rt]) : p[rt][t][i];
+                off = steep ? (H ? -7.0f : 0.0f) : off;
+            }
             float sum = 0.0f;
 #pragma unroll
             for (int t = 0; t < CP; t++)
