@@ -194,7 +194,7 @@ def test_half_queries_over_small_fp4_keys(gpu):
 def _huge(ud, fmt, dtype, d, q_log, k_log):
     """Keys and queries along one direction: scores of about 2^(q_log + k_log + 10.6) in binary digits that rise, fall and repeat
     over the keys, and whose largest is ahead of the next by 1 in 128 or more (or by nothing: equal keys)."""
-    rng, keys, hkv, rows, hq = np.random.default_rng([98, q_log, k_log, d]), 330, 2, 6, 4
+    rng, keys, hkv, rows, hq = np.random.default_rng([98, q_log, abs(k_log), d]), 330, 2, 6, 4
     e = rng.choice([-1.0, 1.0], d)
     a = 64 + np.concatenate([np.arange(60), 40 - np.arange(40), rng.integers(0, 63, keys - 100)])
     a[[100, 217, 320]] = 127
@@ -258,3 +258,21 @@ def test_huge_scores_in_all_directions(gpu, fmt, dtype):
             got += [prefill(ud, c, q, [0, 70], ranges, 0, dtype, span=s) for s in (keys, 20_000)]
         for x in got:
             assert np.all((x >= v[0].min() * (1 - 2.0 ** -7)) & (x <= v[0].max() * (1 + 2.0 ** -7)))
+
+
+@pytest.mark.parametrize("fmt", ["bf16", "f16", "mxfp4"])
+def test_fp32_queries_at_the_ends_of_their_range(gpu, fmt):
+    """fp32 queries from fp32's smallest values to 2^126, over keys that keep the scores finite."""
+    ud, d = gpu, 64
+    for q_log, k_log in ((100, 0), (111, -10), (118, -14), (125, -20)):
+        c, q = _huge(ud, fmt, "f32", d, q_log, k_log)
+        ranges = np.array([[0, 330], [0, 330], [3, 217], [150, 320], [50, 160], [99, 152]])
+        want = ref.attention(q, c.k, c.v, np.zeros(6, int), ranges, 0, 2, c.most * 16)
+        _check_huge(window(ud, c, q[None], ranges[None], 0, "f32"), want, "f32", P_STEP[fmt, "f32"])
+    rng = np.random.default_rng(100)
+    c = Cache(ud, rng, fmt, [500], 2, d)
+    for q_log in (-4, -30, -100, -120, -140):
+        q = ref.rounded(rng.standard_normal((2, 4, d)) * 2.0 ** q_log, "f32")
+        ranges = np.array([[0, 500], [20, 431]])
+        want = ref.attention(q, c.k, c.v, np.zeros(2, int), ranges, 0, 2, c.most * 16)
+        close(window(ud, c, q[None], ranges[None], 0, "f32"), want, c, d, "f32", P_STEP[fmt, "f32"])

@@ -172,7 +172,7 @@ __global__ __launch_bounds__(64 * NW, RT == 1 ? 2 : 1) void window_split_kernel(
             }
             if constexpr (H) {                     // the row's largest value to 2^10 .. 2^11
                 most = xmax32(xmax16(most));
-                const int ex = most > 0.0f && most < INFINITY ? 10 - min(max(ilogbf(most), -110), 110) : 0;
+                const int ex = most > 0.0f && most < INFINITY ? 10 - max(ilogbf(most), -110) : 0;
                 const float up = ldexpf(1.0f, ex);
                 qscale[rt] = a.scale * ldexpf(1.0f, -ex);
 #pragma unroll
