@@ -276,3 +276,78 @@ def test_fp32_queries_at_the_ends_of_their_range(gpu, fmt):
         ranges = np.array([[0, 500], [20, 431]])
         want = ref.attention(q, c.k, c.v, np.zeros(2, int), ranges, 0, 2, c.most * 16)
         close(window(ud, c, q[None], ranges[None], 0, "f32"), want, c, d, "f32", P_STEP[fmt, "f32"])
+
+
+def test_the_most_sequences(gpu):
+    """65,535 sequences of one key each, in both attentions and the append: every row is its own key's value."""
+    ud, rng, n, d = gpu, np.random.default_rng(101), 65_535, 64
+    table = rng.permutation(n)[:, None].astype(np.int32)
+    k, v, q = (ref.to_bits(rng.standard_normal((n, d)), "bf16") for _ in range(3))
+    kp, vp, out = ud.DeviceBuffer(n * 16 * d * 2), ud.DeviceBuffer(n * 16 * d * 2), ud.DeviceBuffer(n * d * 2)
+    bt, pos, qd = _dev(ud, table), _dev(ud, np.full(n, 5, np.int32)), _dev(ud, q)
+    ud.qk_norm_rope_append(None, _dev(ud, k), _dev(ud, v), None, kp, vp, n, bt, n, 1, pos, n, 0, 1, d)
+    ranges, start = _dev(ud, np.tile(np.array([5, 6], np.int32), (n, 1))), _dev(ud, np.arange(n + 1, dtype=np.int32))
+    assert ud.gqa_window_workspace_bytes(n, 1, 1, 1, d, 0, 1) == ud.gqa_prefill_workspace_bytes(n, n, 1, 1, 1, d, 0, 1) == 0
+    ud.gqa_window_attention_paged(qd, kp, vp, n, bt, 1, ranges, 0, out, n, 1, 1, 1, d, 1, None, dtype="bf16")
+    ud.synchronize()
+    np.testing.assert_array_equal(out.download((n, d), np.uint16), v)
+    out = _dev(ud, np.zeros((n, d), np.uint16))
+    ud.gqa_prefill_paged(qd, kp, vp, n, bt, 1, start, ranges, 0, out, n, n, 1, 1, 1, d, 1, None)
+    ud.synchronize()
+    np.testing.assert_array_equal(out.download((n, d), np.uint16), v)
+
+
+def _prompt_calls(ud, fmt, dtype, span):
+    """A ragged batch of prompts, and the call over given buffers."""
+    rng, hq, hkv, d, new, past = np.random.default_rng(102), 8, 2, 128, [90, 1, 37], [700, 300, 0]
+    rows, start = sum(new), np.concatenate([[0], np.cumsum(new)]).astype(np.int32)
+    c = Cache(ud, rng, fmt, [a + b for a, b in zip(new, past)], hkv, d)
+    ranges = causal(new, past, 200)
+    qs, rd, need = _dev(ud, start), _dev(ud, ranges.astype(np.int32)), ud.gqa_prefill_workspace_bytes(3, rows, 90, hq, hkv, d, 4, span)
+
+    def call(q, out, ws, stream):
+        ud.gqa_prefill_paged(q, c.kp, c.vp, c.num, c.bt, c.most, qs, rd, 4, out, 3, rows, 90, hq, hkv, d, span, ws, dtype=dtype, kv_format=fmt,
+                             hip_stream=stream)
+
+    def fresh():
+        q = ref.rounded(rng.standard_normal((rows, hq, d)), dtype)
+        return q, ref.to_bits(q, dtype).reshape(rows, -1)
+    expect = lambda q: prefill(ud, c, q, start, ranges, 4, dtype, span=span)  # noqa: E731
+    read = lambda out: ref.from_bits(out.download((rows, hq, d), np.uint16), dtype)  # noqa: E731
+    return call, fresh, expect, read, need, rows * hq * d * 2
+
+
+@pytest.mark.parametrize("fmt,dtype,span", [("bf16", "bf16", 300), ("mxfp4", "f16", 20_000), ("f16", "f16", 20_000)])
+def test_prompts_in_a_graph(gpu, fmt, dtype, span):
+    """Captured once and replayed over new queries, eager calls between: the same bits every time."""
+    ud, stream = gpu, gpu.HipStream()
+    call, fresh, expect, read, need, size = _prompt_calls(ud, fmt, dtype, span)
+    assert (need > 0) == (span > 1000)
+    qd, out, ws = ud.DeviceBuffer(size), ud.DeviceBuffer(size), ud.DeviceBuffer(need) if need else None
+    graph = None
+    for _ in range(4):
+        q, bits = fresh()
+        want = expect(q)
+        qd.upload(bits)
+        ud.synchronize()
+        if graph is None:
+            with ud.Graph.capture(stream) as graph:
+                call(qd, out, ws, stream)
+        graph.launch(stream)
+        stream.synchronize()
+        np.testing.assert_array_equal(read(out), want)
+
+
+def test_prompts_on_two_streams(gpu):
+    ud, streams = gpu, [gpu.HipStream() for _ in range(2)]
+    call, fresh, expect, read, need, size = _prompt_calls(ud, "mxfp4", "bf16", 20_000)
+    q = [fresh() for _ in streams]
+    want = [expect(x) for x, _ in q]
+    buf = [(_dev(ud, bits), ud.DeviceBuffer(size), ud.DeviceBuffer(need)) for _, bits in q]
+    ud.synchronize()
+    for _ in range(20):
+        for s, (qd, out, ws) in zip(streams, buf):
+            call(qd, out, ws, s)
+    ud.synchronize()
+    for (_, out, _), w in zip(buf, want):
+        np.testing.assert_array_equal(read(out), w)
