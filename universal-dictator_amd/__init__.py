@@ -687,7 +687,7 @@ def qk_norm_rope_append(q, k, v, q_out, k_pages, v_pages, num_blocks, block_tabl
     """The heads of projected rows in one pass: RMS norm per head of q and k (where a weight is given), rotation (where
     inv_freq is given), q to q_out, k and v into the paged cache (kv_format bf16, f16 or mxfp4).  Row t is position
     positions[t] of sequence seqs[t] (None: t); padding rows (see ud_decode.h) leave everything as it was.  *_ld: elements
-    between rows (None: contiguous)."""
+    between rows (None: contiguous).  q_out may be q, with q_out_ld as q_ld; other overlaps with q, k and v are refused."""
     ptr = lambda b: b.ptr if b is not None else None  # noqa: E731
     qw, kw = q_heads * head_dim, kv_heads * head_dim
     _check(lib().ud_qk_norm_rope_append(_DTYPES[dtype], _PAGES[kv_format], ptr(q), qw if q_ld is None else q_ld, k.ptr,

@@ -4,7 +4,8 @@
 //   y = x / sqrt(mean_c x_c^2 + eps) * w            per head, where a weight is given
 //   (y_i, y_{i+d/2}) -> (y_i cos a - y_{i+d/2} sin a, y_{i+d/2} cos a + y_i sin a),   a = position * inv_freq_i
 //
-// Bound: memory.  A row's heads are read once and written once (q to q_out, k and v to their pages).
+// Bound: memory, with the vector units not far behind (below).  A row's heads are read once and written once (q to q_out, k
+// and v to their pages).
 // Layout: one workgroup per row.  A lane holds channels 4i .. 4i + 3 of a head and the four they rotate with,
 // half a head on, so that the rotation stays in the lane and the norm's sum is one butterfly over the head's
 // D / 8 lanes.  The D / 2 angles of a row are the same for all heads: computed once, by one lane each, into LDS.
@@ -13,8 +14,8 @@
 // Keys for MXFP4 pages are normalised and rotated in 64 bits: a key next to a border between two codes would
 // otherwise move by a whole step of its block with the order of a sum, and so would every key of a block whose
 // largest value is next to a power of two's border.  That is 8 of 48 heads at 32/8.
-// Measured, 32/8 heads of 128: 8,200 rows of bf16 to MXFP4 pages 46 us (177 MB, 3.8 TB/s; a large copy on the same card
-// 4.7 .. 5.0; vector units busy 68 % of the time), 64 rows 5.7 us, one row of fp32 to half pages 3.2 us:
+// Measured, 32/8 heads of 128: 8,200 rows of bf16 to MXFP4 pages 45 .. 46 us (177 MB, 3.8 .. 3.9 TB/s, three quarters to four
+// fifths of a large copy's 4.7 .. 5.0; vector units busy 68 % of the time), 64 rows 5.7 us, one row of fp32 to half pages 3.2 us:
 // little more than an empty launch.  Read back: 17.6 (76 MB, 4.3 TB/s), 3.6 and 1.9 us.
 #include <type_traits>
 

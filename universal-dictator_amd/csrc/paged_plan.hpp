@@ -125,9 +125,10 @@ UD_HD int rank_of_layer(int z, int layer, int n) { return z < layer ? z : n - 1 
 // - At most 256 workgroups (one per CU; two fit): split until there are 512, down to 8 tiles of 64 keys each.
 // - Above: split up to 2,048, so that the unequal workgroups of unequal sequences fill each other's gaps, but not below 64
 //   tiles, since every split of a row costs its fp32 partial, written and read (520 bytes at D = 128).
-// us, 32/8 heads of 128, bf16, one split -> this rule: 16 rows behind 16,000 keys 322 -> 28 (64 splits), 512 rows 335 -> 181
-// (4); 512 behind 2,000 61 -> 45; 6 x 37-563 rows behind 4,000-12,000 (MXFP4) 400 -> 326 (3); 8 x 64-500 behind 2,700-8,000
-// 302 -> 291 (2).  Where it keeps one split, two lose: a causal prompt of 2,000 rows 58 -> 85, of 4,000 169 -> 232.
+// us, 32/8 heads of 128, bf16, one split -> this rule: 16 rows behind 16,000 keys 310 -> 26 (31 splits), 512 rows 322 -> 162
+// (4); 512 behind 2,000 58 -> 42 (4); 6 x 37-563 rows behind 4,000-12,000 368 -> 320, MXFP4 377 -> 309 (3); 8 x 64-500 behind
+// 2,700-8,000 283 -> 263, MXFP4 285 -> 253 (2).  Where it keeps one split, two lose: a causal prompt of 2,000 rows 58 -> 85,
+// of 4,000 169 -> 232.
 inline int64_t prefill_blocks(int64_t max_rows, int64_t group) { return (max_rows * group + 127) / 128; }
 inline int prefill_splits(int64_t n, int64_t kv_heads, int64_t blocks, int64_t n_sinks, int64_t max_span) {
     const int64_t units = n * kv_heads * blocks, tiles = (max_pages(max_span, n_sinks) + 3) / 4;

@@ -9,10 +9,10 @@
 //  - S^T = K . Q^T and O^T = V^T . P^T on v_mfma_f32_32x32x16, a wave's 32 rows in the lanes: a lane has 32 scores of its
 //    row (the other half of the wave has the row's other 32), so that the running maximum and sum are in-lane but for one
 //    swap of the halves, and its probabilities are the B operand of the second product as they stand.
-// Measured, 32/8 heads of 128, causal: 8,192 rows of bf16 439 .. 490 us a call, 0.84 .. 0.94 PFLOP/s (the library's 8192^3
-// product on the same card: 1.21); 6 x 37 .. 563 rows behind 4,000 .. 12,000 MXFP4 keys 327 us, 0.76 PFLOP/s with its join.  The chip holds
-// 1.9 GHz there; matrix cores and vector units are busy 48 % and 47 % of the time, one after the other within a wave, side by
-// side between the two of a SIMD.  Without bank conflicts.  One row group more per wave (64 rows) is slower, 515 us for 482:
+// Measured, 32/8 heads of 128, causal: 8,192 rows of bf16 429 .. 490 us a call, 0.84 .. 0.96 PFLOP/s (the library's 8192^3
+// product on the same card: 1.21); 6 x 37 .. 563 rows behind 4,000 .. 12,000 MXFP4 keys 300 .. 311 us, 0.80 .. 0.83 PFLOP/s with its
+// join (half queries 329).  The chip holds 1.9 GHz there; matrix cores and vector units are busy 48 % and 47 % of the time, one
+// after the other within a wave, side by side between the two of a SIMD.  Without bank conflicts.  One row group more per wave (64 rows) is slower, 515 us for 482:
 // its registers leave one wave per SIMD.
 //  - K and V rows lie in LDS at padded distances against bank conflicts; V^T is read by ds_read_b64_tr_b16.
 

@@ -22,7 +22,7 @@
 // Measured, 32/8 heads of 128: 64 contexts of 500 .. 20,000 keys with a window of 4,096, bf16 pages (982 MB) 168 us, 5.8 TB/s;
 // 64 x 4,096 keys 182 us, of which the loads alone take all but 2.  MXFP4 pages, 64 x 4,096 keys 55.5 us, the loads alone 52;
 // 64 x 512 .. 8,192 keys (304 MB) 66 us, 4.6 TB/s: conversions, products and softmax in turn in each wave.  One sequence of 8,192 half
-// keys is latency: 12.5 us in 32 splits, and 4 for the join.
+// keys is latency: 13 us in 32 splits, and 4 for the join.
 #include <type_traits>
 
 #include "paged_attention.hpp"
