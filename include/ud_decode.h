@@ -171,7 +171,8 @@ UD_API int ud_paged_kv_read(int32_t kv_format, int32_t dtype, const void* k_page
  * probabilities rounded once to the pages' type (bf16 for UD_MXFP4, twice that for half queries); a value past 2^90
  * may pass fp32's range in the sums, which are divided at the end.  A NaN or infinity in a key or value reaches only the
  * rows that see it: a NaN in a key makes them NaN, an infinity in a key may; a channel with an infinity among the values is
- * that infinity, however small its probability (half outputs: 65504), with one of both signs or a NaN it is NaN.
+ * that infinity, however small its probability (half outputs: 65504), with one of both signs or a NaN it is NaN; a
+ * call that meets one takes up to twelve times as long.
  * For fp32 queries over bf16 or half pages, without sinks and with 1, 2, 4 or 8 query heads to a kv head,
  * ud_gqa_attention_paged(_mq) computes the same.  Take this call where accuracy counts on bf16 pages (the other rounds
  * queries and probabilities to bf16), for batches and from some 2,000 keys on, the other for one short sequence and, a little,
