@@ -121,6 +121,12 @@ def _sig(lib):
         "ud_gqa_prefill_workspace_bytes": (ctypes.c_size_t, [_i32] * 8),
         "ud_gqa_prefill_paged": (i, [_i32, _i32, p, p, p, _i32, p, _i32, p, p, _i32, p, _i32, _i32, _i32, _i32, _i32, _i32, _i32,
                                      _i32, p, ctypes.c_size_t, p]),
+        "ud_rms_norm": (i, [_i32, p, _i32, _i32, p, p, _i32, p, ctypes.c_float, _i32, p, _i32, p, _i32, _i32, p]),
+        "ud_i8_quantize": (i, [_i32, p, p, _i32, p, _i32, p, _i32, _i32, p]),
+        "ud_i8_linear": (i, [_i32, p, _i32, p, p, _i32, p, p, p, _i32, p, _i32, _i32, _i32, _i32, p]),
+        "ud_logits_workspace_bytes": (ctypes.c_size_t, [_i32, _i32]),
+        "ud_logits_process": (i, [_i32, p, _i32, p, _i32, p, _i32, _i32, p, _i32, p, p, p, p, _i32, p, p, _i32, _i32, p, p,
+                                  ctypes.c_size_t, p]),
         "ud_encoder_get_config": (i, [p, ctypes.POINTER(_Config)]),
         "ud_safetensors_open": (i, [ctypes.c_char_p, ctypes.POINTER(_vp)]),
         "ud_safetensors_close": (v, [p]),
@@ -739,6 +745,57 @@ def gqa_prefill_paged(q, k_pages, v_pages, num_blocks, block_table, max_blocks, 
                                       workspace.ptr if workspace is not None else None,
                                       workspace.nbytes if workspace is not None else 0,
                                       hip_stream.ptr if hip_stream else None))
+
+
+# ---------------------------------------------------------------- a decoder's layer in 8 bits (ud_layer.h)
+
+UD_I8 = 32
+
+
+def _ptr(b):
+    return b.ptr if b is not None else None
+
+
+def rms_norm(x, out, rows, dim, weight=None, eps=1e-6, residual=None, sum_out=None, scales=None, dtype="bf16", sum_dtype=None,
+             out_dtype=None, x_ld=None, sum_ld=None, out_ld=None, hip_stream=None):
+    """out = RMS norm of s = x + residual (None: x) with weight fp32 [dim]; s is stored to sum_out (may be residual) in sum_dtype
+    (dtype or f32).  out_dtype None: dtype; "i8": int8 codes with fp32 scales [rows].  *_ld: elements between rows (None: dim)."""
+    od = UD_I8 if out_dtype == "i8" else _DTYPES[out_dtype or dtype]
+    _check(lib().ud_rms_norm(_DTYPES[dtype], _ptr(x), dim if x_ld is None else x_ld, _DTYPES[sum_dtype or dtype], _ptr(residual),
+                             _ptr(sum_out), dim if sum_ld is None else sum_ld, _ptr(weight), eps, od, _ptr(out),
+                             dim if out_ld is None else out_ld, _ptr(scales), rows, dim, hip_stream.ptr if hip_stream else None))
+
+
+def i8_quantize(x, codes, scales, rows, dim, gate=None, dtype="bf16", ld=None, codes_ld=None, hip_stream=None):
+    """Rows of dtype to int8 codes with a scale each, value = code * scale: x, or x * silu(gate) where a gate is given.
+    ld: elements between rows of x and of gate (None: dim).  Weights [out, in] take the same call: a scale per channel."""
+    _check(lib().ud_i8_quantize(_DTYPES[dtype], _ptr(x), _ptr(gate), dim if ld is None else ld, _ptr(codes),
+                                dim if codes_ld is None else codes_ld, _ptr(scales), rows, dim, hip_stream.ptr if hip_stream else None))
+
+
+def i8_linear(codes, scales, w, w_scales, out, M, N, K, bias=None, residual=None, dtype="bf16", codes_ld=None, w_ld=None,
+              res_ld=None, out_ld=None, hip_stream=None):
+    """out [M, N] of dtype = (codes [M, K] . w [N, K]^T) * scales[m] * w_scales[n] + bias + residual (may be out)."""
+    _check(lib().ud_i8_linear(_DTYPES[dtype], _ptr(codes), K if codes_ld is None else codes_ld, _ptr(scales), _ptr(w),
+                              K if w_ld is None else w_ld, _ptr(w_scales), _ptr(bias), _ptr(residual), N if res_ld is None else res_ld,
+                              _ptr(out), N if out_ld is None else out_ld, M, N, K, hip_stream.ptr if hip_stream else None))
+
+
+def logits_workspace_bytes(n, vocab):
+    return int(load_library().ud_logits_workspace_bytes(n, vocab))
+
+
+def logits_process(logits, out, n, vocab, token=None, tokens=None, n_tokens=0, ranges=None, penalties=None, bias_ids=None,
+                   bias_values=None, n_biases=0, bias_ranges=None, mask=None, n_masks=0, mask_rows=None, workspace=None, dtype="f32",
+                   ld=None, out_ld=None, mask_ld=None, hip_stream=None):
+    """out fp32 [n, vocab] = logits under penalties for the tokens of each row's history, biases and grammar masks; token int32 [n]:
+    the greedy choice (-1: nothing is left).  See ud_layer.h for the arrays.  workspace: logits_workspace_bytes(n, vocab) bytes where
+    token is given.  *_ld: elements (words of the mask) between rows (None: contiguous)."""
+    _check(lib().ud_logits_process(_DTYPES[dtype], _ptr(logits), vocab if ld is None else ld, _ptr(out), vocab if out_ld is None else out_ld,
+                                   _ptr(token), n, vocab, _ptr(tokens), n_tokens, _ptr(ranges), _ptr(penalties), _ptr(bias_ids),
+                                   _ptr(bias_values), n_biases, _ptr(bias_ranges), _ptr(mask), (vocab + 31) // 32 if mask_ld is None else mask_ld,
+                                   n_masks, _ptr(mask_rows), _ptr(workspace), workspace.nbytes if workspace is not None else 0,
+                                   hip_stream.ptr if hip_stream else None))
 
 
 # ---------------------------------------------------------------- synthetic weights
