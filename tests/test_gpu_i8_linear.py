@@ -100,10 +100,18 @@ def test_channels(gpu, M, N):
     check(gpu, rng, M, N, 256, "f16", residual=True, pad=(0, 16, 1, 2))
 
 
-@pytest.mark.parametrize("M", [1, 64, 200])
+@pytest.mark.parametrize("M,N,K", [(2049, 5500, 144), (1030, 12301, 80), (8200, 1500, 256), (700, 9000, 400), (130, 30001, 64)])
+def test_many_tiles(gpu, M, N, K):
+    """Grids of many tiles, none of them whole at the edges."""
+    rng = np.random.default_rng([M, N])
+    check(gpu, rng, M, N, K, "bf16", bias=True)
+    check(gpu, rng, M, N, K, "f32", residual=True, full=True, pad=(0, 16, 3, 1))
+
+
+@pytest.mark.parametrize("M", [1, 64, 200, 2100])
 def test_largest_sums(gpu, M):
     """All codes -128: 128 * 128 * 131056 is the largest sum, 2^31 less 2^18."""
-    K, N = 131056, 40
+    K, N = 131056, 40 if M < 2000 else 6000
     codes, w = np.full((M, K), -128, np.int8), np.full((N, K), -128, np.int8)
     w[1::2] = 127
     got = run(gpu, codes, np.ones(M), w, np.ones(N), "f32")

@@ -6,6 +6,7 @@
 namespace ud {
 
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
+typedef int i32x16_t __attribute__((ext_vector_type(16)));
 
 struct LinearArgs {
     const int8_t* a; const float* sa; const int8_t* w; const float* sw; const float* bias;
@@ -102,9 +103,159 @@ template <typename T, int MT, int NT, int WK, int U> static void launch_few(cons
     hipLaunchKernelGGL((i8_few_kernel<T, MT, NT, WK, U>), grid, dim3(64 * WK), 0, st, a);
 }
 
+// ---------------------------------------------------------------- many rows
+
+// Buffer resource of `bytes` bytes at p: loads past them give zeros.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t panel_buffer(const void* p, uint32_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000);
+}
+// 16 bytes per lane from byte voff + soff of the buffer into LDS at dst + 16 * lane.
+__device__ __forceinline__ void panel_load(__amdgpu_buffer_rsrc_t r, uint32_t voff, uint32_t soff, int8_t* dst) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, dst, 16, voff, soff, 0, 0);
+}
+
+constexpr int KB = 128;                            // bytes of k per LDS tile
+constexpr uint32_t kNowhere = 1u << 31;             // an offset that is past every buffer (256 rows, 2^22 apart)
+
+template <int FN, int FM> __device__ __forceinline__ void pin_sums(i32x16_t (&acc)[FN][FM]) {
+#pragma unroll
+    for (int i = 0; i < FN; i++)
+#pragma unroll
+        for (int j = 0; j < FM; j++) asm volatile("" : "+a"(acc[i][j]));
+}
+
+// A workgroup of four waves takes 64 FM rows and 64 FN channels, a wave 32 FM and 32 FN of them, through two LDS tiles of 128 of
+// k each.
+//  - The tiles are loaded straight into LDS, 8 rows of 128 bytes to an instruction.  The 16-byte pieces of row r lie in the order
+//    piece ^ (r / 2 % 8), so that the 16 rows that LDS serves at a time lie in different banks.
+//  - The products are inline assembly with the sums pinned to the accumulator registers: from the builtin the compiler moved them
+//    between the register files and spilled 137 registers (256 x 256).  The wait states between compiled code and the products are
+//    explicit at the loop's two ends; within it a sum is used again 4 or 16 products later.
+//  - The last quarter of a tile's products runs behind the barrier: its operands are in registers by then, so the tile is free
+//    for the loads after next, and the next tile's first operands arrive under its products.
+template <typename T, int FM, int FN>
+__global__ __launch_bounds__(256, FM * FN > 8 ? 1 : 2) void i8_panel_kernel(LinearArgs a) {
+    constexpr int TM = 64 * FM, TN = 64 * FN;
+    constexpr int LA = TM / 32, LW = TN / 32;      // loads per wave and tile
+    __shared__ __attribute__((aligned(16))) int8_t a0[TM * KB];
+    __shared__ __attribute__((aligned(16))) int8_t w0[TN * KB];
+    __shared__ __attribute__((aligned(16))) int8_t a1[TM * KB];
+    __shared__ __attribute__((aligned(16))) int8_t w1[TN * KB];
+    const int tid = threadIdx.x, lane = tid % 64;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    // An XCD's workgroups are neighbours, in blocks of four row panels: what they read is shared in its L2.
+    const int nM = (a.M + TM - 1) / TM, nN = (a.N + TN - 1) / TN, total = nM * nN;
+    const int xcd = blockIdx.x % 8, each = total / 8, more = total % 8;
+    const int t = xcd * each + min(xcd, more) + blockIdx.x / 8;
+    const int grp = t / (4 * nN), rem = t - grp * 4 * nN, gm = min(4, nM - grp * 4);
+    const int m0 = (grp * 4 + rem % gm) * TM, n0 = rem / gm * TN;
+
+    const int rows_a = min(TM, a.M - m0), rows_w = min(TN, a.N - n0);
+    const __amdgpu_buffer_rsrc_t ra = panel_buffer(a.a + m0 * a.a_ld, (uint32_t)((rows_a - 1) * a.a_ld + a.K));
+    const __amdgpu_buffer_rsrc_t rw = panel_buffer(a.w + n0 * a.w_ld, (uint32_t)((rows_w - 1) * a.w_ld + a.K));
+    uint32_t va[LA], vw[LW], last_a[LA], last_w[LW];
+    const int blocks = (a.K + KB - 1) / KB, tail = a.K - (blocks - 1) * KB;
+    // Rows behind the last are the last one again (computed, not stored); pieces behind K are zeros.
+#pragma unroll
+    for (int i = 0; i < LA; i++) {
+        const int r = (wave * LA + i) * 8 + lane / 8, piece = (lane % 8) ^ (r / 2 % 8);
+        va[i] = (uint32_t)(min(r, rows_a - 1) * a.a_ld) + 16 * piece;
+        last_a[i] = 16 * piece < tail ? va[i] : kNowhere;
+    }
+#pragma unroll
+    for (int i = 0; i < LW; i++) {
+        const int r = (wave * LW + i) * 8 + lane / 8, piece = (lane % 8) ^ (r / 2 % 8);
+        vw[i] = (uint32_t)(min(r, rows_w - 1) * a.w_ld) + 16 * piece;
+        last_w[i] = 16 * piece < tail ? vw[i] : kNowhere;
+    }
+    auto load_tile = [&](int b, int8_t* at, int8_t* wt) __attribute__((always_inline)) {
+        const bool last = b == blocks - 1;
+#pragma unroll
+        for (int i = 0; i < LA; i++) panel_load(ra, last ? last_a[i] : va[i], b * KB, at + (wave * LA + i) * 1024);
+#pragma unroll
+        for (int i = 0; i < LW; i++) panel_load(rw, last ? last_w[i] : vw[i], b * KB, wt + (wave * LW + i) * 1024);
+    };
+    // Fragments of k step q (32 of k): lane l holds row l % 32, pieces 2 q + l / 32.
+    const int wm = wave % 2 * (32 * FM), wn = wave / 2 * (32 * FN), r32 = lane % 32, half = lane / 32;
+    i32x4_t fa[2][FM], fw[2][FN];
+    auto read_frags = [&](int q, const int8_t* at, const int8_t* wt, i32x4_t (&da)[FM], i32x4_t (&dw)[FN]) __attribute__((always_inline)) {
+        const int off = r32 * KB + 16 * ((2 * q + half) ^ (r32 / 2 % 8));
+#pragma unroll
+        for (int i = 0; i < FN; i++) dw[i] = *reinterpret_cast<const i32x4_t*>(wt + (wn + 32 * i) * KB + off);
+#pragma unroll
+        for (int i = 0; i < FM; i++) da[i] = *reinterpret_cast<const i32x4_t*>(at + (wm + 32 * i) * KB + off);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    i32x16_t acc[FN][FM];
+#pragma unroll
+    for (int i = 0; i < FN; i++)
+#pragma unroll
+        for (int j = 0; j < FM; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[i][j][e] = 0;
+    auto products = [&](const i32x4_t (&da)[FM], const i32x4_t (&dw)[FN]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < FN; i++)
+#pragma unroll
+            for (int j = 0; j < FM; j++)
+                asm volatile("v_mfma_i32_32x32x32_i8 %0, %1, %2, %0" : "+a"(acc[i][j]) : "v"(dw[i]), "v"(da[j]));
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // Tile b lies in (at, wt) with its first fragments in fa[0], fw[0]; tile b + 1 is on its way to (an, wnx).
+    auto tile = [&](int b, int8_t* at, int8_t* wt, int8_t* an, int8_t* wnx) __attribute__((always_inline)) {
+        read_frags(1, at, wt, fa[1], fw[1]);
+        products(fa[0], fw[0]);
+        read_frags(2, at, wt, fa[0], fw[0]);
+        products(fa[1], fw[1]);
+        read_frags(3, at, wt, fa[1], fw[1]);
+        products(fa[0], fw[0]);
+        // this wave's loads of tile b + 1 have arrived, and its reads of tile b
+        __builtin_amdgcn_s_waitcnt(0);
+        __builtin_amdgcn_s_barrier();
+        __asm__ volatile("" ::: "memory");
+        if (b + 1 < blocks) read_frags(0, an, wnx, fa[0], fw[0]);
+        if (b + 2 < blocks) load_tile(b + 2, at, wt);
+        products(fa[1], fw[1]);
+    };
+    load_tile(0, a0, w0);
+    __builtin_amdgcn_s_waitcnt(0);
+    __builtin_amdgcn_s_barrier();
+    __asm__ volatile("" ::: "memory");
+    read_frags(0, a0, w0, fa[0], fw[0]);
+    if (blocks > 1) load_tile(1, a1, w1);
+    pin_sums<FN, FM>(acc);
+    asm volatile("s_nop 7");                       // zeros -> the first product
+    for (int b = 0; b < blocks; b += 2) {
+        tile(b, a0, w0, a1, w1);
+        if (b + 1 < blocks) tile(b + 1, a1, w1, a0, w0);
+    }
+    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7\n\ts_nop 7");   // the last product -> its reads below
+    pin_sums<FN, FM>(acc);
+    // A lane holds channels 8 q + 4 half + (0 .. 3) of one row; with the other half's it has eight in a row.
+#pragma unroll
+    for (int j = 0; j < FM; j++) {
+        const int m = m0 + wm + 32 * j + r32;
+#pragma unroll
+        for (int i = 0; i < FN; i++)
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+                finish4<T>(a, m, n0 + wn + 32 * i + 8 * q + 4 * half, i32x4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]});
+    }
+}
+
+template <typename T, int FM, int FN> static void launch_panel(const LinearArgs& a, hipStream_t st) {
+    const int64_t tiles = (int64_t)((a.M + 64 * FM - 1) / (64 * FM)) * ((a.N + 64 * FN - 1) / (64 * FN));
+    hipLaunchKernelGGL((i8_panel_kernel<T, FM, FN>), dim3((unsigned)tiles), dim3(256), 0, st, a);
+}
+
 template <typename T> static void launch_linear(const LinearArgs& a, hipStream_t st) {
+    auto tiles = [&](int fm, int fn) { return (int64_t)((a.M + 64 * fm - 1) / (64 * fm)) * ((a.N + 64 * fn - 1) / (64 * fn)); };
+    // 32-bit offsets within a tile's rows
+    const bool near = a.a_ld <= (1 << 22) && a.w_ld <= (1 << 22);
     if (a.M <= 16) launch_few<T, 1, 1, 8, 4>(a, st);
-    else launch_few<T, 4, 2, 4, 2>(a, st);
+    else if (a.M <= 64 || !near) launch_few<T, 4, 2, 4, 2>(a, st);
+    else if (tiles(4, 4) >= 192) launch_panel<T, 4, 4>(a, st);
+    else launch_panel<T, 2, 2>(a, st);
 }
 
 }  // namespace ud
