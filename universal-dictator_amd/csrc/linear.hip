@@ -46,6 +46,34 @@ template <typename T> __device__ __forceinline__ void finish4(const LinearArgs& 
     }
 }
 
+// Eight channels n .. n + 7 of row m, `left` of them there, their scales and biases (0 for none) in hand.
+template <typename T>
+__device__ __forceinline__ void finish8(const LinearArgs& a, int m, int n, int left, const i32x4_t& lo, const i32x4_t& hi,
+                                        const float (&sw)[8], const float (&bias)[8]) {
+    const float s = a.sa[m];
+    T* o = static_cast<T*>(a.out) + m * a.out_ld + n;
+    const T* r = a.res ? static_cast<const T*>(a.res) + m * a.res_ld + n : nullptr;
+    float v[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) v[e] = (float)(e < 4 ? lo[e % 4] : hi[e % 4]) * s * sw[e] + bias[e];
+    if (left >= 8) {
+        if (r) {
+            Raw8<T> x;
+            float f[8];
+            __builtin_memcpy(&x, r, sizeof x);
+            widen8<T>(x, f);
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] += f[e];
+        }
+        const Raw8<T> y = narrow8<T>(v);
+        __builtin_memcpy(o, &y, sizeof y);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (e < left) o[e] = from_f<T>(r ? v[e] + to_f<T>(r[e]) : v[e]);
+    }
+}
+
 // Few rows: the time is that of the weights' way from memory.  A workgroup takes 16 NT channels and 16 MT rows; its WK waves
 // take every WK-th block of 64 U of k, straight from memory into the matrix instruction's operands, and are summed in LDS.
 template <typename T, int MT, int NT, int WK, int U>
@@ -168,23 +196,21 @@ __global__ __launch_bounds__(256, FM * FN > 8 ? 1 : 2) void i8_panel_kernel(Line
         vw[i] = (uint32_t)(min(r, rows_w - 1) * a.w_ld) + 16 * piece;
         last_w[i] = 16 * piece < tail ? vw[i] : kNowhere;
     }
-    auto load_tile = [&](int b, int8_t* at, int8_t* wt) __attribute__((always_inline)) {
-        const bool last = b == blocks - 1;
+    auto load_part = [&](int i, int b, int8_t* at, int8_t* wt, bool last) __attribute__((always_inline)) {
+        if (i < LA) panel_load(ra, last ? last_a[i] : va[i], b * KB, at + (wave * LA + i) * 1024);
+        else panel_load(rw, last ? last_w[i - LA] : vw[i - LA], b * KB, wt + (wave * LW + i - LA) * 1024);
+    };
+    auto load_tile = [&](int b, int8_t* at, int8_t* wt, bool last) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < LA; i++) panel_load(ra, last ? last_a[i] : va[i], b * KB, at + (wave * LA + i) * 1024);
-#pragma unroll
-        for (int i = 0; i < LW; i++) panel_load(rw, last ? last_w[i] : vw[i], b * KB, wt + (wave * LW + i) * 1024);
+        for (int i = 0; i < LA + LW; i++) load_part(i, b, at, wt, last);
     };
     // Fragments of k step q (32 of k): lane l holds row l % 32, pieces 2 q + l / 32.
     const int wm = wave % 2 * (32 * FM), wn = wave / 2 * (32 * FN), r32 = lane % 32, half = lane / 32;
     i32x4_t fa[2][FM], fw[2][FN];
-    auto read_frags = [&](int q, const int8_t* at, const int8_t* wt, i32x4_t (&da)[FM], i32x4_t (&dw)[FN]) __attribute__((always_inline)) {
+    auto read_frag = [&](int i, int q, const int8_t* at, const int8_t* wt, i32x4_t (&da)[FM], i32x4_t (&dw)[FN]) __attribute__((always_inline)) {
         const int off = r32 * KB + 16 * ((2 * q + half) ^ (r32 / 2 % 8));
-#pragma unroll
-        for (int i = 0; i < FN; i++) dw[i] = *reinterpret_cast<const i32x4_t*>(wt + (wn + 32 * i) * KB + off);
-#pragma unroll
-        for (int i = 0; i < FM; i++) da[i] = *reinterpret_cast<const i32x4_t*>(at + (wm + 32 * i) * KB + off);
-        __builtin_amdgcn_sched_barrier(0);
+        if (i < FN) dw[i] = *reinterpret_cast<const i32x4_t*>(wt + (wn + 32 * i) * KB + off);
+        else da[i - FN] = *reinterpret_cast<const i32x4_t*>(at + (wm + 32 * (i - FN)) * KB + off);
     };
     i32x16_t acc[FN][FM];
 #pragma unroll
@@ -193,53 +219,102 @@ __global__ __launch_bounds__(256, FM * FN > 8 ? 1 : 2) void i8_panel_kernel(Line
         for (int j = 0; j < FM; j++)
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[i][j][e] = 0;
-    auto products = [&](const i32x4_t (&da)[FM], const i32x4_t (&dw)[FN]) __attribute__((always_inline)) {
+    // The products of a k step, with what(0), what(1), .. between them: `work` pieces, evenly.
+    constexpr int STEPS = FN * FM;
+    auto products = [&](const i32x4_t (&da)[FM], const i32x4_t (&dw)[FN], int work, auto what) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < FN; i++)
 #pragma unroll
-            for (int j = 0; j < FM; j++)
+            for (int j = 0; j < FM; j++) {
+                const int n = i * FM + j;
                 asm volatile("v_mfma_i32_32x32x32_i8 %0, %1, %2, %0" : "+a"(acc[i][j]) : "v"(dw[i]), "v"(da[j]));
-        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int k = 0; k < work; k++)
+                    if (k * STEPS / work == n) what(k);
+                __builtin_amdgcn_sched_barrier(0);
+            }
     };
-    // Tile b lies in (at, wt) with its first fragments in fa[0], fw[0]; tile b + 1 is on its way to (an, wnx).
-    auto tile = [&](int b, int8_t* at, int8_t* wt, int8_t* an, int8_t* wnx) __attribute__((always_inline)) {
-        read_frags(1, at, wt, fa[1], fw[1]);
-        products(fa[0], fw[0]);
-        read_frags(2, at, wt, fa[0], fw[0]);
-        products(fa[1], fw[1]);
-        read_frags(3, at, wt, fa[1], fw[1]);
-        products(fa[0], fw[0]);
+    // Tile b lies in (at, wt) with its first fragments in fa[0], fw[0]; tile b + 1 is on its way to (an, wnx).  INNER: tile b + 2
+    // is there and not the last.
+    auto tile = [&](int b, int8_t* at, int8_t* wt, int8_t* an, int8_t* wnx, auto inner) __attribute__((always_inline)) {
+        constexpr bool INNER = decltype(inner)::value;
+        constexpr int R = FM + FN;
+        products(fa[0], fw[0], R, [&](int k) __attribute__((always_inline)) { read_frag(k, 1, at, wt, fa[1], fw[1]); });
+        products(fa[1], fw[1], R, [&](int k) __attribute__((always_inline)) { read_frag(k, 2, at, wt, fa[0], fw[0]); });
+        products(fa[0], fw[0], R, [&](int k) __attribute__((always_inline)) { read_frag(k, 3, at, wt, fa[1], fw[1]); });
         // this wave's loads of tile b + 1 have arrived, and its reads of tile b
         __builtin_amdgcn_s_waitcnt(0);
         __builtin_amdgcn_s_barrier();
         __asm__ volatile("" ::: "memory");
-        if (b + 1 < blocks) read_frags(0, an, wnx, fa[0], fw[0]);
-        if (b + 2 < blocks) load_tile(b + 2, at, wt);
-        products(fa[1], fw[1]);
+        if constexpr (INNER) {
+#pragma unroll
+            for (int k = 0; k < R; k++) read_frag(k, 0, an, wnx, fa[0], fw[0]);
+            __builtin_amdgcn_sched_barrier(0);
+            products(fa[1], fw[1], LA + LW, [&](int k) __attribute__((always_inline)) { load_part(k, b + 2, at, wt, false); });
+        } else {
+            if (b + 1 < blocks) {
+#pragma unroll
+                for (int k = 0; k < R; k++) read_frag(k, 0, an, wnx, fa[0], fw[0]);
+            }
+            if (b + 2 < blocks) load_tile(b + 2, at, wt, b + 2 == blocks - 1);
+            __builtin_amdgcn_sched_barrier(0);
+            products(fa[1], fw[1], 0, [](int) {});
+        }
     };
-    load_tile(0, a0, w0);
+    load_tile(0, a0, w0, blocks == 1);
     __builtin_amdgcn_s_waitcnt(0);
     __builtin_amdgcn_s_barrier();
     __asm__ volatile("" ::: "memory");
-    read_frags(0, a0, w0, fa[0], fw[0]);
-    if (blocks > 1) load_tile(1, a1, w1);
+#pragma unroll
+    for (int k = 0; k < FM + FN; k++) read_frag(k, 0, a0, w0, fa[0], fw[0]);
+    if (blocks > 1) load_tile(1, a1, w1, blocks == 2);
     pin_sums<FN, FM>(acc);
     asm volatile("s_nop 7");                       // zeros -> the first product
-    for (int b = 0; b < blocks; b += 2) {
-        tile(b, a0, w0, a1, w1);
-        if (b + 1 < blocks) tile(b + 1, a1, w1, a0, w0);
+    // (without branches in the body: where loads into LDS are on their way over a branch, the compiler waits for all of them before the
+    // next read of LDS)
+    int b = 0;
+    for (; b + 4 < blocks; b += 2) {
+        tile(b, a0, w0, a1, w1, std::true_type{});
+        tile(b + 1, a1, w1, a0, w0, std::true_type{});
+    }
+    for (; b < blocks; b += 2) {
+        tile(b, a0, w0, a1, w1, std::false_type{});
+        if (b + 1 < blocks) tile(b + 1, a1, w1, a0, w0, std::false_type{});
     }
     asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7\n\ts_nop 7");   // the last product -> its reads below
     pin_sums<FN, FM>(acc);
-    // A lane holds channels 8 q + 4 half + (0 .. 3) of one row; with the other half's it has eight in a row.
+    // A lane holds channels 8 q + 4 half + (0 .. 3) of one row.  32 rows at a time go through LDS (each wave an array of its own, rows 16
+    // bytes further apart than they are long, against bank conflicts), so that a lane finishes eight channels in a row and a wave writes
+    // whole lines.
+    constexpr int WC = 32 * FN, LPR = WC / 8, RPI = 64 / LPR, LD = WC + 4;
+    static_assert(32 * LD * 4 <= TM * KB && 32 * LD * 4 <= TN * KB, "a wave's rows fit each array");
+    __builtin_amdgcn_s_barrier();                  // every wave's reads of the last tile
+    __asm__ volatile("" ::: "memory");
+    int* mine = reinterpret_cast<int*>(wave == 0 ? a0 : wave == 1 ? w0 : wave == 2 ? a1 : w1);
+    const int n = n0 + wn + lane % LPR * 8, left = a.N - n;
+    float sw[8], bias[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        sw[e] = e < left ? a.sw[n + e] : 0.0f;
+        bias[e] = a.bias && e < left ? a.bias[n + e] : 0.0f;
+    }
 #pragma unroll
     for (int j = 0; j < FM; j++) {
-        const int m = m0 + wm + 32 * j + r32;
 #pragma unroll
         for (int i = 0; i < FN; i++)
 #pragma unroll
             for (int q = 0; q < 4; q++)
-                finish4<T>(a, m, n0 + wn + 32 * i + 8 * q + 4 * half, i32x4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]});
+                *reinterpret_cast<i32x4_t*>(mine + r32 * LD + 32 * i + 8 * q + 4 * half) =
+                    i32x4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int k = 0; k < 32 / RPI; k++) {
+            const int r = k * RPI + lane / LPR, m = m0 + wm + 32 * j + r;
+            const int* from = mine + r * LD + lane % LPR * 8;
+            const i32x4_t lo = *reinterpret_cast<const i32x4_t*>(from), hi = *reinterpret_cast<const i32x4_t*>(from + 4);
+            if (m < a.M && left > 0) finish8<T>(a, m, n, left, lo, hi, sw, bias);
+        }
+        __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     }
 }
 
