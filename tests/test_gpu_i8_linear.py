@@ -100,12 +100,18 @@ def test_channels(gpu, M, N):
     check(gpu, rng, M, N, 256, "f16", residual=True, pad=(0, 16, 1, 2))
 
 
-@pytest.mark.parametrize("M,N,K", [(2049, 5500, 144), (1030, 12301, 80), (8200, 1500, 256), (700, 9000, 400), (130, 30001, 64)])
+# every kernel of csrc/linear_plan.hpp, over grids of several tiles, none whole at the edges
+TILES = [(3, 5001, 2064), (16, 1000, 8208), (2, 20003, 528), (30, 3001, 1040), (64, 4099, 656), (60, 9003, 272), (120, 6002, 400), (500, 6007, 784),
+         (1000, 9001, 272), (2049, 5500, 144), (2500, 4001, 400), (4050, 4030, 272), (8200, 1500, 256), (130, 30001, 64), (700, 9000, 400),
+         (60, 17003, 272), (130, 8003, 400)]
+
+
+@pytest.mark.parametrize("M,N,K", TILES)
 def test_many_tiles(gpu, M, N, K):
-    """Grids of many tiles, none of them whole at the edges."""
     rng = np.random.default_rng([M, N])
     check(gpu, rng, M, N, K, "bf16", bias=True)
     check(gpu, rng, M, N, K, "f32", residual=True, full=True, pad=(0, 16, 3, 1))
+    check(gpu, rng, M, N, K, "f16", bias=True, residual=True, in_place=True, off=3, pad=(32, 0, 0, 0))
 
 
 @pytest.mark.parametrize("M", [1, 64, 200, 2100])

@@ -72,7 +72,7 @@ def linear(ud, **kw):
 
 
 @pytest.mark.parametrize("kw", [
-    dict(dtype=I8), dict(M=-1), dict(M=(1 << 22) + 1), dict(N=0), dict(N=(1 << 24) + 1, out_ld=1 << 25), dict(K=0), dict(K=8), dict(K=72, codes_ld=80, w_ld=80),
+    dict(dtype=I8), dict(M=-1), dict(M=(1 << 22) + 1), dict(N=0), dict(N=(1 << 24) + 1, out_ld=1 << 25), dict(M=1 << 20, N=(1 << 18) + 1, out_ld=1 << 19), dict(codes_ld=(1 << 22) + 16), dict(w_ld=1 << 23), dict(K=0), dict(K=8), dict(K=72, codes_ld=80, w_ld=80),
     dict(K=131072, codes_ld=131072, w_ld=131072), dict(codes_ld=48), dict(codes_ld=72), dict(w_ld=56), dict(w_ld=68), dict(out_ld=39),
     dict(res=6 * P, res_ld=39), dict(codes=None), dict(scales=None), dict(w=None), dict(w_scales=None), dict(out=None), dict(codes=P + 8),
     dict(w=3 * P + 4), dict(scales=2 * P + 2), dict(w_scales=4 * P + 1), dict(bias=6 * P + 2), dict(out=5 * P + 1), dict(res=6 * P + 1),

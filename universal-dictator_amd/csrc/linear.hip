@@ -2,6 +2,7 @@
 //   out[m, n] = (sum_k codes[m, k] w[n, k]) * scales[m] * w_scales[n] + bias[n] + residual[m, n]
 // The sums are exact in 32 bits, so neither the order of k nor its split over waves changes a bit.
 #include "layer.hpp"
+#include "linear_plan.hpp"
 
 namespace ud {
 
@@ -15,59 +16,72 @@ struct LinearArgs {
     int M, N, K;
 };
 
-// Four channels n .. n + 3 of row m: scales, bias, residual, rounding.
-template <typename T> __device__ __forceinline__ void finish4(const LinearArgs& a, int m, int n, const i32x4_t& acc) {
-    if (m >= a.M || n >= a.N) return;
-    const float s = a.sa[m];
-    T* o = static_cast<T*>(a.out) + m * a.out_ld + n;
-    const T* r = a.res ? static_cast<const T*>(a.res) + m * a.res_ld + n : nullptr;
-    if (n + 4 <= a.N) {
-        // as the elements lie: their addresses need not be those of whole pieces
-        struct V4 { T v[4]; } x, y;
-        float sw[4], b[4];
-        __builtin_memcpy(sw, a.sw + n, 16);
-        if (a.bias) __builtin_memcpy(b, a.bias + n, 16);
-        if (r) __builtin_memcpy(&x, r, sizeof x);
+// What finishes four channels n .. n + 3 of row m, read ahead of the sums.
+template <typename T> struct Finish4 {
+    float s, sw[4], bias[4];
+    T res[4];
+    bool there;
+
+    __device__ __forceinline__ void read(const LinearArgs& a, int m, int n) {
+        there = m < a.M && n < a.N;
+        if (!there) return;
+        s = a.sa[m];
+        const T* r = a.res ? static_cast<const T*>(a.res) + m * a.res_ld + n : nullptr;
+        if (n + 4 <= a.N) {                        // as they lie: the addresses need not be those of whole pieces
+            __builtin_memcpy(sw, a.sw + n, 16);
+            if (a.bias) __builtin_memcpy(bias, a.bias + n, 16);
+            if (r) __builtin_memcpy(res, r, sizeof res);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 3; i++) {
+                if (n + i >= a.N) continue;
+                sw[i] = a.sw[n + i];
+                if (a.bias) bias[i] = a.bias[n + i];
+                if (r) res[i] = r[i];
+            }
+        }
+    }
+    __device__ __forceinline__ void write(const LinearArgs& a, int m, int n, const i32x4_t& acc) const {
+        if (!there) return;
+        T* o = static_cast<T*>(a.out) + m * a.out_ld + n;
+        T y[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             float v = (float)acc[i] * s * sw[i];
-            if (a.bias) v += b[i];
-            if (r) v += to_f<T>(x.v[i]);
-            y.v[i] = from_f<T>(v);
+            if (a.bias) v += bias[i];
+            if (a.res) v += to_f<T>(res[i]);
+            y[i] = from_f<T>(v);
         }
-        __builtin_memcpy(o, &y, sizeof y);
-    } else {
-        for (int i = 0; i < a.N - n; i++) {
-            float v = (float)acc[i] * s * a.sw[n + i];
-            if (a.bias) v += a.bias[n + i];
-            if (r) v += to_f<T>(r[i]);
-            o[i] = from_f<T>(v);
+        if (n + 4 <= a.N) {
+            __builtin_memcpy(o, y, sizeof y);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 3; i++)
+                if (n + i < a.N) o[i] = y[i];
         }
     }
-}
+};
 
-// Eight channels n .. n + 7 of row m, `left` of them there, their scales and biases (0 for none) in hand.
+// Eight channels n .. n + 7 of row m, `left` of them there; their scales, biases (0 for none) and residual (read already where all eight
+// are there) in hand.
 template <typename T>
-__device__ __forceinline__ void finish8(const LinearArgs& a, int m, int n, int left, const i32x4_t& lo, const i32x4_t& hi,
-                                        const float (&sw)[8], const float (&bias)[8]) {
-    const float s = a.sa[m];
+__device__ __forceinline__ void finish8(const LinearArgs& a, int m, int n, int left, const i32x4_t& lo, const i32x4_t& hi, float s,
+                                        const float (&sw)[8], const float (&bias)[8], const Raw8<T>& res) {
     T* o = static_cast<T*>(a.out) + m * a.out_ld + n;
-    const T* r = a.res ? static_cast<const T*>(a.res) + m * a.res_ld + n : nullptr;
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; e++) v[e] = (float)(e < 4 ? lo[e % 4] : hi[e % 4]) * s * sw[e] + bias[e];
     if (left >= 8) {
-        if (r) {
-            Raw8<T> x;
+        if (a.res) {
             float f[8];
-            __builtin_memcpy(&x, r, sizeof x);
-            widen8<T>(x, f);
+            widen8<T>(res, f);
 #pragma unroll
             for (int e = 0; e < 8; e++) v[e] += f[e];
         }
         const Raw8<T> y = narrow8<T>(v);
         __builtin_memcpy(o, &y, sizeof y);
     } else {
+        const T* r = a.res ? static_cast<const T*>(a.res) + m * a.res_ld + n : nullptr;
 #pragma unroll
         for (int e = 0; e < 8; e++)
             if (e < left) o[e] = from_f<T>(r ? v[e] + to_f<T>(r[e]) : v[e]);
@@ -78,9 +92,14 @@ __device__ __forceinline__ void finish8(const LinearArgs& a, int m, int n, int l
 // take every WK-th block of 64 U of k, straight from memory into the matrix instruction's operands, and are summed in LDS.
 template <typename T, int MT, int NT, int WK, int U>
 __global__ __launch_bounds__(64 * WK) void i8_few_kernel(LinearArgs a) {
+    static_assert(MT * NT <= WK, "a fragment of the sums to a wave");
     __shared__ i32x4_t part[WK][MT * NT][64];
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
     const int n0 = blockIdx.x * (16 * NT), m0 = blockIdx.y * (16 * MT);
+    // a wave finishes one fragment, whose lanes hold four channels of one row
+    const int m = m0 + 16 * (wave % MT) + r, n = n0 + 16 * (wave / MT) + 4 * g;
+    Finish4<T> fin;
+    if (wave < MT * NT) fin.read(a, m, n);
     // rows behind the last are the last one again: read, never stored
     const int8_t* wp[NT];
     const int8_t* ap[MT];
@@ -116,13 +135,11 @@ __global__ __launch_bounds__(64 * WK) void i8_few_kernel(LinearArgs a) {
 #pragma unroll
         for (int j = 0; j < MT; j++) part[wave][i * MT + j][lane] = acc[i][j];
     __syncthreads();
-    // a fragment's lane holds four channels of one row
-    for (int e = threadIdx.x; e < MT * NT * 64; e += 64 * WK) {
-        const int f = e / 64, l = e % 64;
-        i32x4_t s = part[0][f][l];
+    if (wave < MT * NT) {
+        i32x4_t s = part[0][wave][lane];
 #pragma unroll
-        for (int i = 1; i < WK; i++) s += part[i][f][l];
-        finish4<T>(a, m0 + 16 * (f % MT) + l % 16, n0 + 16 * (f / MT) + 4 * (l / 16), s);
+        for (int i = 1; i < WK; i++) s += part[i][wave][lane];
+        fin.write(a, m, n, s);
     }
 }
 
@@ -161,14 +178,20 @@ template <int FN, int FM> __device__ __forceinline__ void pin_sums(i32x16_t (&ac
 //    explicit at the loop's two ends; within it a sum is used again 4 or 16 products later.
 //  - The last quarter of a tile's products runs behind the barrier: its operands are in registers by then, so the tile is free
 //    for the loads after next, and the next tile's first operands arrive under its products.
-template <typename T, int FM, int FN>
-__global__ __launch_bounds__(256, FM * FN > 8 ? 1 : 2) void i8_panel_kernel(LinearArgs a) {
+template <typename T, int FM, int FN, int NS>
+__global__ __launch_bounds__(256, FM * FN > 8 || (FM + FN) * NS * 8 > 80 ? 1 : 2) void i8_panel_kernel(LinearArgs a) {
+    static_assert(NS == 2 || NS == 4, "the loop's body is written out for two and four");
     constexpr int TM = 64 * FM, TN = 64 * FN;
     constexpr int LA = TM / 32, LW = TN / 32;      // loads per wave and tile
+    // arrays of their own, so that the compiler can tell a tile that is read from one that is loaded
     __shared__ __attribute__((aligned(16))) int8_t a0[TM * KB];
     __shared__ __attribute__((aligned(16))) int8_t w0[TN * KB];
     __shared__ __attribute__((aligned(16))) int8_t a1[TM * KB];
     __shared__ __attribute__((aligned(16))) int8_t w1[TN * KB];
+    __shared__ __attribute__((aligned(16))) int8_t a2[NS > 2 ? TM * KB : 16];
+    __shared__ __attribute__((aligned(16))) int8_t w2[NS > 2 ? TN * KB : 16];
+    __shared__ __attribute__((aligned(16))) int8_t a3[NS > 2 ? TM * KB : 16];
+    __shared__ __attribute__((aligned(16))) int8_t w3[NS > 2 ? TN * KB : 16];
     const int tid = threadIdx.x, lane = tid % 64;
     const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
     // An XCD's workgroups are neighbours, in blocks of four row panels: what they read is shared in its L2.
@@ -196,13 +219,16 @@ __global__ __launch_bounds__(256, FM * FN > 8 ? 1 : 2) void i8_panel_kernel(Line
         vw[i] = (uint32_t)(min(r, rows_w - 1) * a.w_ld) + 16 * piece;
         last_w[i] = 16 * piece < tail ? vw[i] : kNowhere;
     }
-    auto load_part = [&](int i, int b, int8_t* at, int8_t* wt, bool last) __attribute__((always_inline)) {
-        if (i < LA) panel_load(ra, last ? last_a[i] : va[i], b * KB, at + (wave * LA + i) * 1024);
-        else panel_load(rw, last ? last_w[i - LA] : vw[i - LA], b * KB, wt + (wave * LW + i - LA) * 1024);
+    // Part i of tile b; behind the last tile zeros, which nothing reads (so that each tile counts the same loads).
+    auto load_part = [&](int i, int b, int8_t* at, int8_t* wt) __attribute__((always_inline)) {
+        const bool inner = b + 1 < blocks, there = b < blocks;
+        const uint32_t v = i < LA ? (inner ? va[i] : last_a[i]) : inner ? vw[i - LA] : last_w[i - LA];
+        if (i < LA) panel_load(ra, there ? v : kNowhere, there ? b * KB : 0, at + (wave * LA + i) * 1024);
+        else panel_load(rw, there ? v : kNowhere, there ? b * KB : 0, wt + (wave * LW + i - LA) * 1024);
     };
-    auto load_tile = [&](int b, int8_t* at, int8_t* wt, bool last) __attribute__((always_inline)) {
+    auto load_tile = [&](int b, int8_t* at, int8_t* wt) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < LA + LW; i++) load_part(i, b, at, wt, last);
+        for (int i = 0; i < LA + LW; i++) load_part(i, b, at, wt);
     };
     // Fragments of k step q (32 of k): lane l holds row l % 32, pieces 2 q + l / 32.
     const int wm = wave % 2 * (32 * FM), wn = wave / 2 * (32 * FN), r32 = lane % 32, half = lane / 32;
@@ -234,103 +260,134 @@ __global__ __launch_bounds__(256, FM * FN > 8 ? 1 : 2) void i8_panel_kernel(Line
                 __builtin_amdgcn_sched_barrier(0);
             }
     };
-    // Tile b lies in (at, wt) with its first fragments in fa[0], fw[0]; tile b + 1 is on its way to (an, wnx).  INNER: tile b + 2
-    // is there and not the last.
-    auto tile = [&](int b, int8_t* at, int8_t* wt, int8_t* an, int8_t* wnx, auto inner) __attribute__((always_inline)) {
-        constexpr bool INNER = decltype(inner)::value;
-        constexpr int R = FM + FN;
+    // Tile b lies in (at, wt) with its first fragments in fa[0], fw[0]; the next NS - 1 tiles are on their way, the first of them to
+    // (an, wnx).
+    constexpr int R = FM + FN;
+    auto tile = [&](int b, int8_t* at, int8_t* wt, int8_t* an, int8_t* wnx) __attribute__((always_inline)) {
         products(fa[0], fw[0], R, [&](int k) __attribute__((always_inline)) { read_frag(k, 1, at, wt, fa[1], fw[1]); });
         products(fa[1], fw[1], R, [&](int k) __attribute__((always_inline)) { read_frag(k, 2, at, wt, fa[0], fw[0]); });
         products(fa[0], fw[0], R, [&](int k) __attribute__((always_inline)) { read_frag(k, 3, at, wt, fa[1], fw[1]); });
         // this wave's loads of tile b + 1 have arrived, and its reads of tile b
-        __builtin_amdgcn_s_waitcnt(0);
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm((NS - 2) * (LA + LW)) & 0xF0FF);
         __builtin_amdgcn_s_barrier();
         __asm__ volatile("" ::: "memory");
-        if constexpr (INNER) {
 #pragma unroll
-            for (int k = 0; k < R; k++) read_frag(k, 0, an, wnx, fa[0], fw[0]);
-            __builtin_amdgcn_sched_barrier(0);
-            products(fa[1], fw[1], LA + LW, [&](int k) __attribute__((always_inline)) { load_part(k, b + 2, at, wt, false); });
-        } else {
-            if (b + 1 < blocks) {
-#pragma unroll
-                for (int k = 0; k < R; k++) read_frag(k, 0, an, wnx, fa[0], fw[0]);
-            }
-            if (b + 2 < blocks) load_tile(b + 2, at, wt, b + 2 == blocks - 1);
-            __builtin_amdgcn_sched_barrier(0);
-            products(fa[1], fw[1], 0, [](int) {});
-        }
+        for (int k = 0; k < R; k++) read_frag(k, 0, an, wnx, fa[0], fw[0]);
+        __builtin_amdgcn_sched_barrier(0);
+        products(fa[1], fw[1], LA + LW, [&](int k) __attribute__((always_inline)) { load_part(k, b + NS, at, wt); });
     };
-    load_tile(0, a0, w0, blocks == 1);
-    __builtin_amdgcn_s_waitcnt(0);
+    load_tile(0, a0, w0);
+    load_tile(1, a1, w1);
+    if constexpr (NS == 4) {
+        load_tile(2, a2, w2);
+        load_tile(3, a3, w3);
+    }
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm((NS - 1) * (LA + LW)));
     __builtin_amdgcn_s_barrier();
     __asm__ volatile("" ::: "memory");
 #pragma unroll
-    for (int k = 0; k < FM + FN; k++) read_frag(k, 0, a0, w0, fa[0], fw[0]);
-    if (blocks > 1) load_tile(1, a1, w1, blocks == 2);
+    for (int k = 0; k < R; k++) read_frag(k, 0, a0, w0, fa[0], fw[0]);
     pin_sums<FN, FM>(acc);
     asm volatile("s_nop 7");                       // zeros -> the first product
-    // (without branches in the body: where loads into LDS are on their way over a branch, the compiler waits for all of them before the
-    // next read of LDS)
+    // (no branch in the body: where loads into LDS are on their way over one, the compiler waits for all of them before the next read of
+    // LDS, which costs the last tiles little)
     int b = 0;
-    for (; b + 4 < blocks; b += 2) {
-        tile(b, a0, w0, a1, w1, std::true_type{});
-        tile(b + 1, a1, w1, a0, w0, std::true_type{});
+    for (; b + NS <= blocks; b += NS) {
+        if constexpr (NS == 2) {
+            tile(b, a0, w0, a1, w1);
+            tile(b + 1, a1, w1, a0, w0);
+        } else {
+            tile(b, a0, w0, a1, w1);
+            tile(b + 1, a1, w1, a2, w2);
+            tile(b + 2, a2, w2, a3, w3);
+            tile(b + 3, a3, w3, a0, w0);
+        }
     }
-    for (; b < blocks; b += 2) {
-        tile(b, a0, w0, a1, w1, std::false_type{});
-        if (b + 1 < blocks) tile(b + 1, a1, w1, a0, w0, std::false_type{});
+    if (b < blocks) tile(b, a0, w0, a1, w1);
+    if constexpr (NS == 4) {
+        if (b + 1 < blocks) tile(b + 1, a1, w1, a2, w2);
+        if (b + 2 < blocks) tile(b + 2, a2, w2, a3, w3);
     }
+    __builtin_amdgcn_s_waitcnt(0);                 // the zeros behind the last tile, before LDS is used again
     asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7\n\ts_nop 7");   // the last product -> its reads below
     pin_sums<FN, FM>(acc);
-    // A lane holds channels 8 q + 4 half + (0 .. 3) of one row.  32 rows at a time go through LDS (each wave an array of its own, rows 16
-    // bytes further apart than they are long, against bank conflicts), so that a lane finishes eight channels in a row and a wave writes
-    // whole lines.
-    constexpr int WC = 32 * FN, LPR = WC / 8, RPI = 64 / LPR, LD = WC + 4;
-    static_assert(32 * LD * 4 <= TM * KB && 32 * LD * 4 <= TN * KB, "a wave's rows fit each array");
+    // A lane holds channels 8 q + 4 half + (0 .. 3) of one row.  32 rows of CW channels at a time go through LDS (each wave in an array of
+    // its own; four channels' piece p of row r lies at p ^ r, against bank conflicts), so that a lane finishes eight channels in a row
+    // and a wave writes whole lines.
+    constexpr int CW = FN % 2 ? 32 : 64, CF = CW / 32, LPR = CW / 8, RPI = 64 / LPR, IT = 32 / RPI;
+    static_assert(32 * CW * 4 <= TM * KB && 32 * CW * 4 <= TN * KB, "a wave's rows fit each array");
+    auto place = [&](int r, int p) __attribute__((always_inline)) {
+        const int x = CW == 64 ? r % 16 : r / 2 % 8;
+        return r * CW + 4 * (p ^ x);
+    };
     __builtin_amdgcn_s_barrier();                  // every wave's reads of the last tile
     __asm__ volatile("" ::: "memory");
     int* mine = reinterpret_cast<int*>(wave == 0 ? a0 : wave == 1 ? w0 : wave == 2 ? a1 : w1);
-    const int n = n0 + wn + lane % LPR * 8, left = a.N - n;
-    float sw[8], bias[8];
+    const int n = n0 + wn + lane % LPR * 8, mw = m0 + wm + lane / LPR;
+    float sw[FN / CF][8], bias[FN / CF][8], sa[FM][IT];
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-        sw[e] = e < left ? a.sw[n + e] : 0.0f;
-        bias[e] = a.bias && e < left ? a.bias[n + e] : 0.0f;
-    }
+    for (int c = 0; c < FN / CF; c++)
 #pragma unroll
-    for (int j = 0; j < FM; j++) {
-#pragma unroll
-        for (int i = 0; i < FN; i++)
-#pragma unroll
-            for (int q = 0; q < 4; q++)
-                *reinterpret_cast<i32x4_t*>(mine + r32 * LD + 32 * i + 8 * q + 4 * half) =
-                    i32x4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-        __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll
-        for (int k = 0; k < 32 / RPI; k++) {
-            const int r = k * RPI + lane / LPR, m = m0 + wm + 32 * j + r;
-            const int* from = mine + r * LD + lane % LPR * 8;
-            const i32x4_t lo = *reinterpret_cast<const i32x4_t*>(from), hi = *reinterpret_cast<const i32x4_t*>(from + 4);
-            if (m < a.M && left > 0) finish8<T>(a, m, n, left, lo, hi, sw, bias);
+        for (int e = 0; e < 8; e++) {
+            const int at = n + c * CW + e;
+            sw[c][e] = at < a.N ? a.sw[at] : 0.0f;
+            bias[c][e] = a.bias && at < a.N ? a.bias[at] : 0.0f;
         }
-        __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-    }
+#pragma unroll
+    for (int j = 0; j < FM; j++)
+#pragma unroll
+        for (int k = 0; k < IT; k++) sa[j][k] = a.sa[min(mw + 32 * j + k * RPI, a.M - 1)];
+#pragma unroll
+    for (int j = 0; j < FM; j++)
+#pragma unroll
+        for (int c = 0; c < FN / CF; c++) {
+            const int nc = n + c * CW, left = a.N - nc, mj = mw + 32 * j;
+            Raw8<T> res[IT];
+            if (a.res && left >= 8) {
+#pragma unroll
+                for (int k = 0; k < IT; k++)
+                    if (mj + k * RPI < a.M) __builtin_memcpy(&res[k], static_cast<const T*>(a.res) + (mj + k * RPI) * a.res_ld + nc, sizeof res[k]);
+            }
+#pragma unroll
+            for (int i = 0; i < CF; i++)
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const i32x16_t& x = acc[c * CF + i][j];
+                    *reinterpret_cast<i32x4_t*>(mine + place(r32, 8 * i + 2 * q + half)) =
+                        i32x4_t{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+                }
+            i32x4_t v[IT][2];
+#pragma unroll
+            for (int k = 0; k < IT; k++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    v[k][h] = *reinterpret_cast<const i32x4_t*>(mine + place(k * RPI + lane / LPR, lane % LPR * 2 + h));
+#pragma unroll
+            for (int k = 0; k < IT; k++)
+                if (mj + k * RPI < a.M && left > 0)
+                    finish8<T>(a, mj + k * RPI, nc, left, v[k][0], v[k][1], sa[j][k], sw[c], bias[c], res[k]);
+        }
 }
 
-template <typename T, int FM, int FN> static void launch_panel(const LinearArgs& a, hipStream_t st) {
+template <typename T, int FM, int FN, int NS> static void launch_panel(const LinearArgs& a, hipStream_t st) {
     const int64_t tiles = (int64_t)((a.M + 64 * FM - 1) / (64 * FM)) * ((a.N + 64 * FN - 1) / (64 * FN));
-    hipLaunchKernelGGL((i8_panel_kernel<T, FM, FN>), dim3((unsigned)tiles), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((i8_panel_kernel<T, FM, FN, NS>), dim3((unsigned)tiles), dim3(256), 0, st, a);
 }
 
 template <typename T> static void launch_linear(const LinearArgs& a, hipStream_t st) {
-    auto tiles = [&](int fm, int fn) { return (int64_t)((a.M + 64 * fm - 1) / (64 * fm)) * ((a.N + 64 * fn - 1) / (64 * fn)); };
-    // 32-bit offsets within a tile's rows
-    const bool near = a.a_ld <= (1 << 22) && a.w_ld <= (1 << 22);
-    if (a.M <= 16) launch_few<T, 1, 1, 8, 4>(a, st);
-    else if (a.M <= 64 || !near) launch_few<T, 4, 2, 4, 2>(a, st);
-    else if (tiles(4, 4) >= 192) launch_panel<T, 4, 4>(a, st);
-    else launch_panel<T, 2, 2>(a, st);
+    switch (linear_kernel(a.M, a.N, a.K)) {
+        case FEW_16x16: return launch_few<T, 1, 1, 4, 16>(a, st);
+        case FEW_16x16_DEEP: return launch_few<T, 1, 1, 8, 16>(a, st);
+        case FEW_16x16_WIDE: return launch_few<T, 1, 1, 4, 8>(a, st);
+        case FEW_16x32: return launch_few<T, 1, 2, 4, 8>(a, st);
+        case PANEL_64x64: return launch_panel<T, 1, 1, 4>(a, st);
+        case PANEL_64x128: return launch_panel<T, 1, 2, 4>(a, st);
+        case PANEL_128x64: return launch_panel<T, 2, 1, 4>(a, st);
+        case PANEL_128x128: return launch_panel<T, 2, 2, 4>(a, st);
+        case PANEL_128x128_TWO: return launch_panel<T, 2, 2, 2>(a, st);
+        case PANEL_256x192: return launch_panel<T, 4, 3, 2>(a, st);
+        default: return launch_panel<T, 4, 4, 2>(a, st);
+    }
 }
 
 }  // namespace ud
@@ -344,11 +401,12 @@ extern "C" UD_API int ud_i8_linear(int32_t dtype, const int8_t* codes_dev, int32
     static const char* who = "ud_i8_linear";
     const int64_t size = type_bytes(dtype);
     if (!size) return layer_fail(UD_ERR_INVALID, "%s: dtype %d", who, dtype);
-    if (M < 0 || M > (1 << 22) || N < 1 || N > (1 << 24) || K < 16 || K > 131056 || K % 16)
-        return layer_fail(UD_ERR_SHAPE, "%s: M %d (0 .. 2^22), N %d (1 .. 2^24), K %d (a multiple of 16, 16 .. 131056)", who, M, N, K);
-    if (codes_ld < K || w_ld < K || ((codes_ld | w_ld) & 15) || out_ld < N || (residual_dev && res_ld < N))
-        return layer_fail(UD_ERR_SHAPE, "%s: rows %d/%d/%d/%d elements apart for K %d (multiples of 16), N %d", who, codes_ld, w_ld, res_ld,
-                          out_ld, K, N);
+    // (a launch holds fewer than 2^32 threads, a tile's rows lie within 32-bit offsets)
+    if (M < 0 || M > (1 << 22) || N < 1 || N > (1 << 24) || (int64_t)M * N > (int64_t)1 << 38 || K < 16 || K > 131056 || K % 16)
+        return layer_fail(UD_ERR_SHAPE, "%s: M %d (0 .. 2^22), N %d (1 .. 2^24, M N at most 2^38), K %d (a multiple of 16, 16 .. 131056)", who, M, N, K);
+    if (codes_ld < K || w_ld < K || ((codes_ld | w_ld) & 15) || codes_ld > (1 << 22) || w_ld > (1 << 22) || out_ld < N || (residual_dev && res_ld < N))
+        return layer_fail(UD_ERR_SHAPE, "%s: rows %d/%d/%d/%d elements apart for K %d (multiples of 16, at most 2^22), N %d", who, codes_ld, w_ld,
+                          res_ld, out_ld, K, N);
     if (M == 0) return UD_OK;
     if (!codes_dev || !scales_dev || !w_dev || !w_scales_dev || !out_dev) return layer_fail(UD_ERR_INVALID, "%s: null pointer", who);
     if ((((uintptr_t)codes_dev | (uintptr_t)w_dev) & 15) || (((uintptr_t)scales_dev | (uintptr_t)w_scales_dev | (uintptr_t)bias_dev) & 3) ||
