@@ -75,7 +75,8 @@ def compare(out, want, mag):
     far = ~np.isfinite(want) & ~np.isnan(want)
     np.testing.assert_array_equal(out[far], want[far])
     fine = np.isfinite(want)
-    # the repetition, the count's product, presence, the difference, the bias: five roundings of what is at most mag
+    # the repetition's reciprocal and product, the count's product with presence, the difference, the bias: five roundings of what is
+    # at most mag
     assert np.all(np.abs(out - want)[fine] <= 5.05 * ref.STEP32 * mag[fine])
 
 
@@ -179,6 +180,34 @@ def test_long_histories(gpu):
     want, mag = ref.logits_out(x, tokens, ranges, pen, None, None)
     compare(out, want, mag)
     np.testing.assert_array_equal(token, ref.chosen(out))
+
+
+@pytest.mark.parametrize("history,biases", [(65535, 32767), (65536, 10), (70000, 0), (10, 32768), (0, 40000), (70000, 40000)])
+def test_lists_of_any_length(gpu, history, biases):
+    """Lists that fit one word a token, just do not, and far from it."""
+    rng = np.random.default_rng([history, biases])
+    check(gpu, rng, 2, 9001, "f32", history=history, biases=biases)
+    check(gpu, rng, 1, 300, "bf16", history=history, biases=biases, masks=None)
+
+
+@pytest.mark.parametrize("n,V", [(2, 100001), (9, 60000), (20, 120001), (130, 32769), (260, 30000)])
+def test_segments(gpu, n, V):
+    """Each size of segment."""
+    check(gpu, np.random.default_rng([n, V]), n, V, "f16", history=400)
+
+
+def test_far_penalties(gpu):
+    """Quotients past fp32's range, infinities and NaN under penalties and biases."""
+    x = np.array([[3e38, -3e38, np.inf, -np.inf, np.nan, 0.0, -0.0, 1e-38, 5.0]]).astype(np.float32).astype(np.float64)
+    tokens = np.arange(9, dtype=np.int32)
+    out, token = process(gpu, x, "f32", tokens, np.array([[0, 9, 9]], np.int32), np.array([[0.5, 9, 9]], np.float32))
+    with np.errstate(over="ignore"):
+        want = np.where(x > 0, x / 0.5, x * 0.5).astype(np.float32)
+    np.testing.assert_array_equal(out, want)
+    assert token[0] == 0                                   # the first of two infinities
+    out, token = process(gpu, x, "f32", tokens, np.array([[0, 0, 9]], np.int32), np.array([[1, 1, 1]], np.float32),
+                         (np.array([2, 3, 8], np.int32), np.array([-np.inf, np.inf, 1], np.float32), np.array([[0, 3]], np.int32)))
+    assert np.all(np.isnan(out[0, 2:5])) and out[0, 8] == 4 and token[0] == 0
 
 
 def test_no_rows(gpu):

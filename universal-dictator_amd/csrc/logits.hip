@@ -9,7 +9,7 @@
 namespace ud {
 
 struct LogitArgs {
-    const void* logits; float* out; uint64_t* best;
+    const void* logits; float* out; uint64_t* best; int32_t* token;
     int64_t ld, out_ld;
     const int32_t* tokens; const int32_t* ranges; const float* penalties;
     const int32_t* bias_ids; const float* bias_values; const int32_t* bias_ranges;
@@ -17,7 +17,9 @@ struct LogitArgs {
     int vocab, n_tokens, n_biases, n_masks;
 };
 
-constexpr uint32_t kInPrompt = 1u << 31;           // a token's word: in the prompt, and how often it was generated
+// A token's word: whether it is in the prompt, and how often it was generated; of a row whose lists are not longer than that, the place of
+// its last bias + 1 in the bits between.
+constexpr uint32_t kInPrompt = 1u << 31, kCounts = 0xffff, kSlots = 0x7fff;
 
 // Larger for a larger logit, and for the lower token of equal ones; 0 for one that may not be chosen.
 __device__ __forceinline__ uint64_t choice_key(float l, int t) {
@@ -25,6 +27,7 @@ __device__ __forceinline__ uint64_t choice_key(float l, int t) {
     const uint32_t u = __float_as_uint(l + 0.0f);  // -0 as 0
     return (uint64_t)(u & kInPrompt ? ~u : u | kInPrompt) << 32 | (uint32_t)~t;
 }
+__device__ __forceinline__ int32_t chosen(uint64_t key) { return key ? (int32_t)~(uint32_t)key : -1; }
 __device__ __forceinline__ uint64_t wave_max_key(uint64_t v) {
 #pragma unroll
     for (int d = 32; d; d /= 2) v = max(v, (uint64_t)__shfl_xor((unsigned long long)v, d));
@@ -32,139 +35,225 @@ __device__ __forceinline__ uint64_t wave_max_key(uint64_t v) {
 }
 
 // Eight logits from p, `left` of them there (the others -inf); p need not be aligned to more than an element.
-template <typename T> __device__ __forceinline__ void load_logits(const T* p, int left, float (&f)[8]) {
+template <typename T> __device__ __forceinline__ Raw8<T> load_logits(const T* p, int left) {
+    Raw8<T> r;
     if (left >= 8) {
-        Raw8<T> r;
         __builtin_memcpy(&r, p, sizeof r);
-        widen8<T>(r, f);
     } else {
+        float f[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) f[e] = e < left ? to_f<T>(p[e]) : -__builtin_inff();
+        r = exact8<T>(f);
     }
+    return r;
 }
 
-// 256 threads; a thread's E pieces of eight tokens are 2,048 apart.
-template <typename T, int E> __global__ __launch_bounds__(256) void logits_kernel(LogitArgs a) {
-    constexpr int SEG = 2048 * E;
-    __shared__ __attribute__((aligned(16))) uint32_t word[SEG];
-    __shared__ uint64_t top[4];
-    const int tid = threadIdx.x, row = blockIdx.y, t0 = blockIdx.x * SEG, len = min(SEG, a.vocab - t0);
-    const T* in = static_cast<const T*>(a.logits) + row * a.ld + t0;
-    float l[E][8];
+// Entries at .. of a list of ids that ends at `hi`, D loads of four of them a thread, 4 THREADS apart; -1 behind the end.
+template <int THREADS, int D> __device__ __forceinline__ void load_ids(const int32_t* ids, int64_t at, int hi, int32_t (&v)[D][4]) {
 #pragma unroll
-    for (int i = 0; i < E; i++) load_logits<T>(in + (i * 256 + tid) * 8, len - (i * 256 + tid) * 8, l[i]);
-    auto clear = [&]() {
-#pragma unroll
-        for (int i = 0; i < SEG / 1024; i++) *reinterpret_cast<uint4*>(&word[(i * 256 + tid) * 4]) = make_uint4(0, 0, 0, 0);
-        __syncthreads();
-    };
-    // what(token's place in the segment, index) for entries lo .. hi - 1 of `ids`
-    auto scan = [&](const int32_t* ids, int lo, int hi, auto what) {
-        for (int64_t i = lo + 4 * tid; i < hi; i += 1024) {
-            int32_t v[4];
-            if (i + 4 <= hi) {
-                __builtin_memcpy(v, ids + i, 16);
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; e++) v[e] = i + e < hi ? ids[i + e] : -1;
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (v[e] >= t0 && v[e] - t0 < len) what(v[e] - t0, (int)i + e);
-        }
-        __syncthreads();
-    };
-    if (a.tokens) {
-        const int lo = max(a.ranges[3 * row], 0), hi = min(a.ranges[3 * row + 2], a.n_tokens), fresh = a.ranges[3 * row + 1];
-        if (lo < hi) {
-            clear();
-            scan(a.tokens, lo, hi, [&](int at, int i) {
-                if (i < fresh) atomicOr(&word[at], kInPrompt);
-                else atomicAdd(&word[at], 1u);
-            });
-            const float rep = a.penalties[3 * row], pres = a.penalties[3 * row + 1], freq = a.penalties[3 * row + 2];
-#pragma unroll
-            for (int i = 0; i < E; i++)
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const uint32_t w = word[(i * 256 + tid) * 8 + e];
-                    if (!w) continue;
-                    float x = l[i][e];
-                    x = x > 0.0f ? x / rep : x * rep;
-                    const uint32_t c = w & ~kInPrompt;
-                    l[i][e] = c ? x - (freq * (float)c + pres) : x;
-                }
-        }
-    }
-    if (a.bias_ids) {
-        const int lo = max(a.bias_ranges[2 * row], 0), hi = min(a.bias_ranges[2 * row + 1], a.n_biases);
-        if (lo < hi) {
-            __syncthreads();
-            clear();
-            scan(a.bias_ids, lo, hi, [&](int at, int i) { atomicMax(&word[at], (uint32_t)(i - lo) + 1); });
-#pragma unroll
-            for (int i = 0; i < E; i++)
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const uint32_t w = word[(i * 256 + tid) * 8 + e];
-                    if (w) l[i][e] += a.bias_values[lo + (int64_t)w - 1];
-                }
-        }
-    }
-    const int m = a.mask ? (a.mask_rows ? a.mask_rows[row] : row) : -1;
-    const bool masked = m >= 0 && m < a.n_masks;
-    const uint8_t* mask = masked ? reinterpret_cast<const uint8_t*>(a.mask + m * a.mask_ld) + t0 / 8 : nullptr;
-    uint64_t best = 0;
-#pragma unroll
-    for (int i = 0; i < E; i++) {
-        const int c = (i * 256 + tid) * 8, left = len - c;
-        if (left <= 0) continue;
-        if (masked) {
-            const uint32_t bits = mask[c / 8];
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (!(bits >> e & 1)) l[i][e] = -__builtin_inff();
-        }
-        float* o = a.out + row * a.out_ld + t0 + c;
-        if (left >= 8) {
-            __builtin_memcpy(o, l[i], 32);
+    for (int d = 0; d < D; d++) {
+        const int64_t i = at + 4 * (d * THREADS + (int)threadIdx.x);
+        if (i + 4 <= hi) {
+            __builtin_memcpy(v[d], ids + i, 16);
         } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (e < left) o[e] = l[i][e];
+            for (int e = 0; e < 4; e++) v[d][e] = i + e < hi ? ids[i + e] : -1;
         }
-        if (a.best)
+    }
+}
+
+// 16 waves, SEG tokens: a thread's E pieces of eight are 8,192 apart (a small segment leaves threads that only read the lists: one row of
+// 131,072 with a history of 100,000 38 -> 19 us).  What the row's lists say is asked for at once, at the start: one after
+// the other their latencies would be most of a short call.
+template <typename T, int SEG> __global__ __launch_bounds__(1024) void logits_kernel(LogitArgs a) {
+    constexpr int W = 16, THREADS = 64 * W, E = (SEG + 8 * THREADS - 1) / (8 * THREADS);
+    __shared__ __attribute__((aligned(16))) uint32_t word[SEG];
+    __shared__ float top[W];
+    __shared__ int first;
+    const int tid = threadIdx.x, row = blockIdx.y, t0 = blockIdx.x * SEG, len = min(SEG, a.vocab - t0);
+    int lo = 0, fresh = 0, hi = 0, blo = 0, bhi = 0, m = -1;
+    float rep = 1.0f, pres = 0.0f, freq = 0.0f;
+    if (a.tokens) {
+        lo = max(a.ranges[3 * row], 0), fresh = a.ranges[3 * row + 1], hi = min(a.ranges[3 * row + 2], a.n_tokens);
+        rep = a.penalties[3 * row], pres = a.penalties[3 * row + 1], freq = a.penalties[3 * row + 2];
+    }
+    if (a.bias_ids) blo = max(a.bias_ranges[2 * row], 0), bhi = min(a.bias_ranges[2 * row + 1], a.n_biases);
+    if (a.mask) m = a.mask_rows ? a.mask_rows[row] : row;
+    const bool masked = m >= 0 && m < a.n_masks;
+    const T* in = static_cast<const T*>(a.logits) + row * a.ld + t0;
+    Raw8<T> raw[E];
+    uint8_t bits[E];
+    int32_t ids[4][4], bias_ids[1][4];             // the first of each list
+#pragma unroll
+    for (int i = 0; i < E; i++) {
+        const int c = (i * THREADS + tid) * 8;
+        raw[i] = load_logits<T>(in + c, len - c);
+    }
+    if (lo < hi) load_ids<THREADS>(a.tokens, lo, hi, ids);
+    if (blo < bhi) load_ids<THREADS>(a.bias_ids, blo, bhi, bias_ids);
+    if (masked) {
+        const uint8_t* mask = reinterpret_cast<const uint8_t*>(a.mask + m * a.mask_ld) + t0 / 8;
+#pragma unroll
+        for (int i = 0; i < E; i++) bits[i] = (i * THREADS + tid) * 8 < len ? mask[i * THREADS + tid] : 0;
+    }
+    auto clear = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 2 * E; i++)
+            if (SEG >= 8 * THREADS || (i * THREADS + tid) * 4 < SEG) *reinterpret_cast<uint4*>(&word[(i * THREADS + tid) * 4]) = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+    };
+    auto words = [&](int i, uint32_t (&w)[8]) __attribute__((always_inline)) {
+        const int at = SEG >= 8 * THREADS ? i * THREADS + tid : min(tid, SEG / 8 - 1);
+        const uint4 u = ld16(&word[at * 4]), v = ld16(&word[SEG / 2 + at * 4]);
+        w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+        w[4] = v.x; w[5] = v.y; w[6] = v.z; w[7] = v.w;
+    };
+    // what(token's word, index) for entries from .. to - 1 of a list, the first of which are in v
+    auto scan = [&](const int32_t* list, int from, int to, auto& v, auto what) __attribute__((always_inline)) {
+        constexpr int D = sizeof(v) / 16;
+        auto place = [](uint32_t p) { return (p / 8 * 4 + p % 4) + (p & 4) * (SEG / 8); };   // a piece's two halves apart: fewer bank conflicts
+        for (int64_t at = from; at < to; at += 4 * THREADS * D) {
+            if (at != from) load_ids<THREADS>(list, at, to, v);
+#pragma unroll
+            for (int d = 0; d < D; d++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const uint32_t p = (uint32_t)v[d][e] - (uint32_t)t0;   // (an id below t0 is past len, too)
+                    if (p < (uint32_t)len) what(word[place(p)], (int)at + 4 * (d * THREADS + tid) + e);
+                }
+        }
+        __syncthreads();
+    };
+    auto count = [&](uint32_t& w, int i) __attribute__((always_inline)) {
+        if (i < fresh) atomicOr(&w, kInPrompt);
+        else atomicAdd(&w, 1u);
+    };
+    float l[E][8];
+#pragma unroll
+    for (int i = 0; i < E; i++) widen8<T>(raw[i], l[i]);
+    const float r = 1.0f / rep;
+    // A token in the prompt, generated c times.
+    auto penalize = [&](float x, bool seen, uint32_t c) __attribute__((always_inline)) {
+        const float y = x * (x > 0.0f ? r : rep);
+        const float z = c ? y - fmaf(freq, (float)c, pres) : y;
+        return seen ? z : x;
+    };
+    if (hi - (int64_t)lo <= kCounts && bhi - (int64_t)blo <= kSlots) {
+        // Both lists in one pass over the words: the last bias of a token and the number of times it was generated, side by side.
+        if (lo < hi || blo < bhi) {
+            clear();
+            if (blo < bhi)
+                scan(a.bias_ids, blo, bhi, bias_ids,
+                     [&](uint32_t& w, int i) __attribute__((always_inline)) { atomicMax(&w, (uint32_t)(i - blo + 1) << 16); });
+            if (lo < hi) scan(a.tokens, lo, hi, ids, count);
+#pragma unroll
+            for (int i = 0; i < E; i++) {
+                uint32_t w[8], any = 0;
+                words(i, w);
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    any |= w[e];
+                    l[i][e] = penalize(l[i][e], w[e] & (kInPrompt | kCounts), w[e] & kCounts);
+                }
+                if (any & kSlots << 16)
+#pragma unroll
+                    for (int e = 0; e < 8; e++)
+                        if (const uint32_t s = w[e] >> 16 & kSlots) l[i][e] += a.bias_values[blo + (int64_t)s - 1];
+            }
+        }
+    } else {
+        clear();
+        scan(a.tokens, lo, hi, ids, count);
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+            uint32_t w[8];
+            words(i, w);
+#pragma unroll
+            for (int e = 0; e < 8; e++) l[i][e] = penalize(l[i][e], w[e], w[e] & ~kInPrompt);
+        }
+        __syncthreads();
+        clear();
+        scan(a.bias_ids, blo, bhi, bias_ids, [&](uint32_t& w, int i) __attribute__((always_inline)) { atomicMax(&w, (uint32_t)(i - blo) + 1); });
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+            uint32_t w[8];
+            words(i, w);
 #pragma unroll
             for (int e = 0; e < 8; e++)
-                if (e < left) best = max(best, choice_key(l[i][e], t0 + c + e));
+                if (w[e]) l[i][e] += a.bias_values[blo + (int64_t)w[e] - 1];
+        }
     }
-    if (!a.best) return;
-    best = wave_max_key(best);
-    if (tid % 64 == 0) top[tid / 64] = best;
+    float most = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < E; i++) {
+        const int c = (i * THREADS + tid) * 8, left = len - c;
+        if (left <= 0) continue;
+        if (masked)
+#pragma unroll
+            for (int e = 0; e < 8; e++) l[i][e] = bits[i] >> e & 1 ? l[i][e] : -__builtin_inff();
+        float* o = a.out + row * a.out_ld + t0 + c;
+        if (left >= 8) {
+            // (past the caches: 64 rows of 131,072 29.5 -> 25.1 us, much of it the next kernel's wait for what the caches write back)
+            typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+            __builtin_nontemporal_store(f4{l[i][0], l[i][1], l[i][2], l[i][3]}, reinterpret_cast<f4*>(o));
+            __builtin_nontemporal_store(f4{l[i][4], l[i][5], l[i][6], l[i][7]}, reinterpret_cast<f4*>(o + 4));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                if (e < left) o[e] = l[i][e];
+                else l[i][e] = -__builtin_inff();
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; e++) most = fmaxf(most, l[i][e]);     // (a NaN is passed over)
+    }
+    if (!a.best && !a.token) return;
+    // The segment's largest, and the first of the places that hold it.
+    most = wave_max(most);
+    if (tid % 64 == 0) top[tid / 64] = most;
+    if (tid == 0) first = INT32_MAX;
     __syncthreads();
-    if (tid == 0) a.best[(int64_t)row * gridDim.x + blockIdx.x] = max(max(top[0], top[1]), max(top[2], top[3]));
+    const float largest = wave_max(top[tid % W]);
+    if (most == largest && largest > -__builtin_inff()) {            // the wave's
+        int at = INT32_MAX;
+#pragma unroll
+        for (int i = E - 1; i >= 0; i--)
+#pragma unroll
+            for (int e = 7; e >= 0; e--)
+                if (l[i][e] == largest && (i * THREADS + tid) * 8 + e < len) at = (i * THREADS + tid) * 8 + e;
+        if (at != INT32_MAX) atomicMin(&first, at);
+    }
+    __syncthreads();
+    if (tid) return;
+    const uint64_t best = choice_key(largest, t0 + first);
+    if (a.best) a.best[(int64_t)row * gridDim.x + blockIdx.x] = best;
+    else a.token[row] = chosen(best);
 }
 
-// The largest of a row's segments.
-__global__ __launch_bounds__(64) void choose_kernel(const uint64_t* best, int segments, int32_t* token) {
+// The largest of a row's segments: a wave a row.
+__global__ __launch_bounds__(256) void choose_kernel(const uint64_t* best, int segments, int32_t* token, int n) {
+    const int row = blockIdx.x * 4 + threadIdx.x / 64, lane = threadIdx.x % 64;
+    if (row >= n) return;
     uint64_t v = 0;
-    for (int i = threadIdx.x; i < segments; i += 64) v = max(v, best[(int64_t)blockIdx.x * segments + i]);
+    for (int i = lane; i < segments; i += 64) v = max(v, best[(int64_t)row * segments + i]);
     v = wave_max_key(v);
-    if (threadIdx.x == 0) token[blockIdx.x] = v ? (int32_t)~(uint32_t)v : -1;
+    if (lane == 0) token[row] = chosen(v);
 }
 
-// Pieces of eight tokens per thread: as many as leave the chip two workgroups per CU, since each reads the row's history.
-static int logit_pieces(int64_t n, int64_t vocab) {
-    for (int e = 4; e > 1; e /= 2)
-        if (n * ((vocab + 2048 * e - 1) / (2048 * e)) >= 512) return e;
-    return 1;
+// Tokens of a workgroup, 2,048 to 32,768: as many as leave the chip a workgroup per CU, since each reads the row's history.
+static int logit_segment(int64_t n, int64_t vocab) {
+    for (int s = 32768; s > 2048; s /= 2)
+        if (n * ((vocab + s - 1) / s) >= 256) return s;
+    return 2048;
 }
 
-template <typename T> static void launch_logits(const LogitArgs& a, int n, int e, int segments, hipStream_t st) {
-    const dim3 grid(segments, n);
-    if (e == 4) hipLaunchKernelGGL((logits_kernel<T, 4>), grid, dim3(256), 0, st, a);
-    else if (e == 2) hipLaunchKernelGGL((logits_kernel<T, 2>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((logits_kernel<T, 1>), grid, dim3(256), 0, st, a);
+template <typename T> static void launch_logits(const LogitArgs& a, int n, int seg, hipStream_t st) {
+    const dim3 grid((a.vocab + seg - 1) / seg, n);
+    if (seg == 32768) hipLaunchKernelGGL((logits_kernel<T, 32768>), grid, dim3(1024), 0, st, a);
+    else if (seg == 16384) hipLaunchKernelGGL((logits_kernel<T, 16384>), grid, dim3(1024), 0, st, a);
+    else if (seg == 8192) hipLaunchKernelGGL((logits_kernel<T, 8192>), grid, dim3(1024), 0, st, a);
+    else if (seg == 4096) hipLaunchKernelGGL((logits_kernel<T, 4096>), grid, dim3(1024), 0, st, a);
+    else hipLaunchKernelGGL((logits_kernel<T, 2048>), grid, dim3(1024), 0, st, a);
 }
 
 }  // namespace ud
@@ -173,7 +262,7 @@ using namespace ud;
 
 extern "C" UD_API size_t ud_logits_workspace_bytes(int32_t n, int32_t vocab) {
     if (n < 1 || n > 65535 || vocab < 1 || vocab > (1 << 24)) return 0;
-    const int seg = 2048 * logit_pieces(n, vocab);
+    const int seg = logit_segment(n, vocab);
     return (size_t)n * ((vocab + seg - 1) / seg) * sizeof(uint64_t);
 }
 
@@ -214,17 +303,20 @@ extern "C" UD_API int ud_logits_process(int32_t dtype, const void* logits_dev, i
     for (const Block& b : inputs) clash = clash || (b.width && (blocks_meet(out, b) || blocks_meet(token, b) || blocks_meet(ws, b)));
     if (clash) return layer_fail(UD_ERR_INVALID, "%s: an output overlaps an input or another output (out may be fp32 logits, at the same ld)", who);
     LogitArgs a{};
-    a.logits = logits_dev; a.out = out_dev; a.best = token_dev ? static_cast<uint64_t*>(workspace) : nullptr;
+    a.logits = logits_dev; a.out = out_dev;
     a.ld = ld; a.out_ld = out_ld;
     if (tokens_dev && penalties_dev && n_tokens) { a.tokens = tokens_dev; a.ranges = ranges_dev; a.penalties = penalties_dev; }
     if (bias_ids_dev && n_biases) { a.bias_ids = bias_ids_dev; a.bias_values = bias_values_dev; a.bias_ranges = bias_ranges_dev; }
     if (mask_dev) { a.mask = mask_dev; a.mask_rows = mask_rows_dev; a.mask_ld = mask_ld; }
     a.vocab = vocab; a.n_tokens = n_tokens; a.n_biases = n_biases; a.n_masks = n_masks;
     hipStream_t st = static_cast<hipStream_t>(hip_stream);
-    const int e = logit_pieces(n, vocab), segments = (vocab + 2048 * e - 1) / (2048 * e);
-    if (dtype == UD_F32) launch_logits<float>(a, n, e, segments, st);
-    else if (dtype == UD_BF16) launch_logits<bf16>(a, n, e, segments, st);
-    else launch_logits<f16>(a, n, e, segments, st);
-    if (token_dev) hipLaunchKernelGGL(choose_kernel, dim3(n), dim3(64), 0, st, a.best, segments, token_dev);
+    const int seg = logit_segment(n, vocab), segments = (vocab + seg - 1) / seg;
+    // one segment a row: the token is written at once
+    if (token_dev && segments > 1) a.best = static_cast<uint64_t*>(workspace);
+    else a.token = token_dev;
+    if (dtype == UD_F32) launch_logits<float>(a, n, seg, st);
+    else if (dtype == UD_BF16) launch_logits<bf16>(a, n, seg, st);
+    else launch_logits<f16>(a, n, seg, st);
+    if (a.best) hipLaunchKernelGGL(choose_kernel, dim3((n + 3) / 4), dim3(256), 0, st, a.best, segments, token_dev, n);
     return layer_launched(who);
 }
