@@ -178,11 +178,11 @@ template <int FN, int FM> __device__ __forceinline__ void pin_sums(i32x16_t (&ac
 //    explicit at the loop's two ends; within it a sum is used again 4 or 16 products later.
 //  - The last quarter of a tile's products runs behind the barrier: its operands are in registers by then, so the tile is free
 //    for the loads after next, and the next tile's first operands arrive under its products.
-template <typename T, int FM, int FN, int NS>
-__global__ __launch_bounds__(256, FM * FN > 8 || (FM + FN) * NS * 8 > 80 ? 1 : 2) void i8_panel_kernel(LinearArgs a) {
+template <typename T, int FM, int FN, int NS, int NW>
+__global__ __launch_bounds__(64 * NW, NW == 8 || FM * FN > 8 || (FM + FN) * NS * 8 > 80 ? 1 : 2) void i8_panel_kernel(LinearArgs a) {
     static_assert(NS == 2 || NS == 4, "the loop's body is written out for two and four");
-    constexpr int TM = 64 * FM, TN = 64 * FN;
-    constexpr int LA = TM / 32, LW = TN / 32;      // loads per wave and tile
+    constexpr int TM = 64 * FM, TN = 16 * NW * FN;
+    constexpr int LA = TM / (8 * NW), LW = TN / (8 * NW);          // loads per wave and tile
     // arrays of their own, so that the compiler can tell a tile that is read from one that is loaded
     __shared__ __attribute__((aligned(16))) int8_t a0[TM * KB];
     __shared__ __attribute__((aligned(16))) int8_t w0[TN * KB];
@@ -232,7 +232,11 @@ __global__ __launch_bounds__(256, FM * FN > 8 || (FM + FN) * NS * 8 > 80 ? 1 : 2
     };
     // Fragments of k step q (32 of k): lane l holds row l % 32, pieces 2 q + l / 32.
     const int wm = wave % 2 * (32 * FM), wn = wave / 2 * (32 * FN), r32 = lane % 32, half = lane / 32;
-    i32x4_t fa[2][FM], fw[2][FN];
+    // Fragments in registers: of two whole tiles where there is room (a tile is read under the products of the one before), else of two
+    // k steps.
+    constexpr int R = FM + FN;
+    constexpr bool WHOLE = R <= 4 && NW == 4;
+    i32x4_t fa[WHOLE ? 8 : 2][FM], fw[WHOLE ? 8 : 2][FN];
     auto read_frag = [&](int i, int q, const int8_t* at, const int8_t* wt, i32x4_t (&da)[FM], i32x4_t (&dw)[FN]) __attribute__((always_inline)) {
         const int off = r32 * KB + 16 * ((2 * q + half) ^ (r32 / 2 % 8));
         if (i < FN) dw[i] = *reinterpret_cast<const i32x4_t*>(wt + (wn + 32 * i) * KB + off);
@@ -260,22 +264,40 @@ __global__ __launch_bounds__(256, FM * FN > 8 || (FM + FN) * NS * 8 > 80 ? 1 : 2
                 __builtin_amdgcn_sched_barrier(0);
             }
     };
-    // Tile b lies in (at, wt) with its first fragments in fa[0], fw[0]; the next NS - 1 tiles are on their way, the first of them to
-    // (an, wnx).
-    constexpr int R = FM + FN;
-    auto tile = [&](int b, int8_t* at, int8_t* wt, int8_t* an, int8_t* wnx) __attribute__((always_inline)) {
-        products(fa[0], fw[0], R, [&](int k) __attribute__((always_inline)) { read_frag(k, 1, at, wt, fa[1], fw[1]); });
-        products(fa[1], fw[1], R, [&](int k) __attribute__((always_inline)) { read_frag(k, 2, at, wt, fa[0], fw[0]); });
-        products(fa[0], fw[0], R, [&](int k) __attribute__((always_inline)) { read_frag(k, 3, at, wt, fa[1], fw[1]); });
-        // this wave's loads of tile b + 1 have arrived, and its reads of tile b
-        __builtin_amdgcn_s_waitcnt(vmcnt_imm((NS - 2) * (LA + LW)) & 0xF0FF);
-        __builtin_amdgcn_s_barrier();
-        __asm__ volatile("" ::: "memory");
+    // Tile b lies in (at, wt) with its first fragments in fa[0], fw[0] (WHOLE: with all of them, in the half `which`); the next NS - 1 tiles
+    // are on their way, the first of them to (an, wnx).
+    auto tile = [&](int b, int8_t* at, int8_t* wt, int8_t* an, int8_t* wnx, auto which) __attribute__((always_inline)) {
+        constexpr int L = LA + LW;
+        if constexpr (WHOLE) {
+            constexpr int H = decltype(which)::value * 4;
+            // this wave's loads of tile b + 1 have arrived, and its reads of tile b
+            __builtin_amdgcn_s_waitcnt(vmcnt_imm((NS - 2) * L) & 0xF0FF);
+            __builtin_amdgcn_s_barrier();
+            __asm__ volatile("" ::: "memory");
 #pragma unroll
-        for (int k = 0; k < R; k++) read_frag(k, 0, an, wnx, fa[0], fw[0]);
-        __builtin_amdgcn_sched_barrier(0);
-        products(fa[1], fw[1], LA + LW, [&](int k) __attribute__((always_inline)) { load_part(k, b + NS, at, wt); });
+            for (int q = 0; q < 4; q++) {
+                const int first = q * L / 4;
+                products(fa[H + q], fw[H + q], R + (q + 1) * L / 4 - first, [&](int k) __attribute__((always_inline)) {
+                    if (k < R) read_frag(k, q, an, wnx, fa[4 - H + q], fw[4 - H + q]);
+                    else load_part(first + k - R, b + NS, at, wt);
+                });
+            }
+        } else {
+            products(fa[0], fw[0], R, [&](int k) __attribute__((always_inline)) { read_frag(k, 1, at, wt, fa[1], fw[1]); });
+            products(fa[1], fw[1], R, [&](int k) __attribute__((always_inline)) { read_frag(k, 2, at, wt, fa[0], fw[0]); });
+            products(fa[0], fw[0], R, [&](int k) __attribute__((always_inline)) { read_frag(k, 3, at, wt, fa[1], fw[1]); });
+            // this wave's loads of tile b + 1 have arrived, and its reads of tile b
+            __builtin_amdgcn_s_waitcnt(vmcnt_imm((NS - 2) * L) & 0xF0FF);
+            __builtin_amdgcn_s_barrier();
+            __asm__ volatile("" ::: "memory");
+#pragma unroll
+            for (int k = 0; k < R; k++) read_frag(k, 0, an, wnx, fa[0], fw[0]);
+            __builtin_amdgcn_sched_barrier(0);
+            products(fa[1], fw[1], L, [&](int k) __attribute__((always_inline)) { load_part(k, b + NS, at, wt); });
+        }
     };
+    const std::integral_constant<int, 0> even{};
+    const std::integral_constant<int, 1> odd{};
     load_tile(0, a0, w0);
     load_tile(1, a1, w1);
     if constexpr (NS == 4) {
@@ -286,7 +308,9 @@ __global__ __launch_bounds__(256, FM * FN > 8 || (FM + FN) * NS * 8 > 80 ? 1 : 2
     __builtin_amdgcn_s_barrier();
     __asm__ volatile("" ::: "memory");
 #pragma unroll
-    for (int k = 0; k < R; k++) read_frag(k, 0, a0, w0, fa[0], fw[0]);
+    for (int q = 0; q < (WHOLE ? 4 : 1); q++)
+#pragma unroll
+        for (int k = 0; k < R; k++) read_frag(k, q, a0, w0, fa[q], fw[q]);
     pin_sums<FN, FM>(acc);
     asm volatile("s_nop 7");                       // zeros -> the first product
     // (no branch in the body: where loads into LDS are on their way over one, the compiler waits for all of them before the next read of
@@ -294,19 +318,19 @@ __global__ __launch_bounds__(256, FM * FN > 8 || (FM + FN) * NS * 8 > 80 ? 1 : 2
     int b = 0;
     for (; b + NS <= blocks; b += NS) {
         if constexpr (NS == 2) {
-            tile(b, a0, w0, a1, w1);
-            tile(b + 1, a1, w1, a0, w0);
+            tile(b, a0, w0, a1, w1, even);
+            tile(b + 1, a1, w1, a0, w0, odd);
         } else {
-            tile(b, a0, w0, a1, w1);
-            tile(b + 1, a1, w1, a2, w2);
-            tile(b + 2, a2, w2, a3, w3);
-            tile(b + 3, a3, w3, a0, w0);
+            tile(b, a0, w0, a1, w1, even);
+            tile(b + 1, a1, w1, a2, w2, odd);
+            tile(b + 2, a2, w2, a3, w3, even);
+            tile(b + 3, a3, w3, a0, w0, odd);
         }
     }
-    if (b < blocks) tile(b, a0, w0, a1, w1);
+    if (b < blocks) tile(b, a0, w0, a1, w1, even);
     if constexpr (NS == 4) {
-        if (b + 1 < blocks) tile(b + 1, a1, w1, a2, w2);
-        if (b + 2 < blocks) tile(b + 2, a2, w2, a3, w3);
+        if (b + 1 < blocks) tile(b + 1, a1, w1, a2, w2, odd);
+        if (b + 2 < blocks) tile(b + 2, a2, w2, a3, w3, even);
     }
     __builtin_amdgcn_s_waitcnt(0);                 // the zeros behind the last tile, before LDS is used again
     asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7\n\ts_nop 7");   // the last product -> its reads below
@@ -315,14 +339,15 @@ __global__ __launch_bounds__(256, FM * FN > 8 || (FM + FN) * NS * 8 > 80 ? 1 : 2
     // its own; four channels' piece p of row r lies at p ^ r, against bank conflicts), so that a lane finishes eight channels in a row
     // and a wave writes whole lines.
     constexpr int CW = FN % 2 ? 32 : 64, CF = CW / 32, LPR = CW / 8, RPI = 64 / LPR, IT = 32 / RPI;
-    static_assert(32 * CW * 4 <= TM * KB && 32 * CW * 4 <= TN * KB, "a wave's rows fit each array");
+    static_assert(NW / 4 * 32 * CW * 4 <= TM * KB && NW / 4 * 32 * CW * 4 <= TN * KB, "a wave's rows fit each array");
     auto place = [&](int r, int p) __attribute__((always_inline)) {
         const int x = CW == 64 ? r % 16 : r / 2 % 8;
         return r * CW + 4 * (p ^ x);
     };
     __builtin_amdgcn_s_barrier();                  // every wave's reads of the last tile
     __asm__ volatile("" ::: "memory");
-    int* mine = reinterpret_cast<int*>(wave == 0 ? a0 : wave == 1 ? w0 : wave == 2 ? a1 : w1);
+    const int part = wave % 4;
+    int* mine = reinterpret_cast<int*>(part == 0 ? a0 : part == 1 ? w0 : part == 2 ? a1 : w1) + wave / 4 * (32 * CW);
     const int n = n0 + wn + lane % LPR * 8, mw = m0 + wm + lane / LPR;
     float sw[FN / CF][8], bias[FN / CF][8], sa[FM][IT];
 #pragma unroll
@@ -369,9 +394,9 @@ __global__ __launch_bounds__(256, FM * FN > 8 || (FM + FN) * NS * 8 > 80 ? 1 : 2
         }
 }
 
-template <typename T, int FM, int FN, int NS> static void launch_panel(const LinearArgs& a, hipStream_t st) {
-    const int64_t tiles = (int64_t)((a.M + 64 * FM - 1) / (64 * FM)) * ((a.N + 64 * FN - 1) / (64 * FN));
-    hipLaunchKernelGGL((i8_panel_kernel<T, FM, FN, NS>), dim3((unsigned)tiles), dim3(256), 0, st, a);
+template <typename T, int FM, int FN, int NS, int NW = 4> static void launch_panel(const LinearArgs& a, hipStream_t st) {
+    const int64_t tiles = tiles_of(a.M, a.N, 64 * FM, 16 * NW * FN);
+    hipLaunchKernelGGL((i8_panel_kernel<T, FM, FN, NS, NW>), dim3((unsigned)tiles), dim3(64 * NW), 0, st, a);
 }
 
 template <typename T> static void launch_linear(const LinearArgs& a, hipStream_t st) {
@@ -386,7 +411,7 @@ template <typename T> static void launch_linear(const LinearArgs& a, hipStream_t
         case PANEL_128x128: return launch_panel<T, 2, 2, 4>(a, st);
         case PANEL_128x128_TWO: return launch_panel<T, 2, 2, 2>(a, st);
         case PANEL_256x192: return launch_panel<T, 4, 3, 2>(a, st);
-        default: return launch_panel<T, 4, 4, 2>(a, st);
+        default: return launch_panel<T, 4, 2, 2, 8>(a, st);
     }
 }
 

@@ -5,7 +5,7 @@
 namespace ud {
 
 // Kernels for few rows: workgroups of 16 rows and 16 (or 32) channels whose waves share out k, 4 or 8 of them, with blocks of 64 u of k.
-// Kernels for many: tiles of 64 fm rows and 64 fn channels through ns LDS tiles.
+// Kernels for many: tiles of rows and channels through two or four LDS tiles, by four waves (eight where it says so).
 enum LinearKernel {
     FEW_16x16,          // 4 waves, blocks of 1,024 of k
     FEW_16x16_DEEP,     // 8 waves
@@ -17,7 +17,7 @@ enum LinearKernel {
     PANEL_128x128,      // 4: one workgroup a CU
     PANEL_128x128_TWO,  // 2: two workgroups a CU
     PANEL_256x192,      // 2
-    PANEL_256x256,      // 2
+    PANEL_256x256,      // 2, eight waves
     LINEAR_KERNELS
 };
 
@@ -38,7 +38,7 @@ inline LinearKernel linear_kernel(int64_t M, int64_t N, int64_t K) {
     if (tiles_of(M, N, 16, 32) <= 256) return FEW_16x32;
     struct Shape { LinearKernel kernel; int tm, tn; double step, once; };
     const Shape shapes[] = {{PANEL_64x64, 64, 64, 0.23, 1.5},   {PANEL_64x128, 64, 128, 0.31, 2},  {PANEL_128x64, 128, 64, 0.29, 2},
-                            {PANEL_128x128, 128, 128, 0.54, 3}, {PANEL_256x192, 256, 192, 1.42, 6}, {PANEL_256x256, 256, 256, 1.75, 8}};
+                            {PANEL_128x128, 128, 128, 0.54, 3}, {PANEL_256x192, 256, 192, 1.42, 6}, {PANEL_256x256, 256, 256, 1.70, 6}};
     const int64_t steps = (K + 127) / 128;
     LinearKernel best = PANEL_256x256;
     double least = 1e300;
