@@ -10,7 +10,7 @@ import pytest
 import test_gpu_i8_linear as gpu_tests
 from conftest import ROOT
 
-NAMES = ["few 16x16", "few 16x16 deep", "few 16x16 wide", "few 16x32", "64x64", "64x128", "128x64", "128x128", "128x128 two", "256x192", "256x256"]
+NAMES = ["few 16x16", "few 16x16 deep", "few 16x16 short", "few 16x32", "64x64", "64x128", "128x64", "128x128", "128x128 two", "256x192", "256x256"]
 TILE = [(16, 16), (16, 16), (16, 16), (16, 32), (64, 64), (64, 128), (128, 64), (128, 128), (128, 128), (256, 192), (256, 256)]
 THREADS = [256, 512] + 8 * [256] + [512]
 

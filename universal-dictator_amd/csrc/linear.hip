@@ -96,10 +96,6 @@ __global__ __launch_bounds__(64 * WK) void i8_few_kernel(LinearArgs a) {
     __shared__ i32x4_t part[WK][MT * NT][64];
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
     const int n0 = blockIdx.x * (16 * NT), m0 = blockIdx.y * (16 * MT);
-    // a wave finishes one fragment, whose lanes hold four channels of one row
-    const int m = m0 + 16 * (wave % MT) + r, n = n0 + 16 * (wave / MT) + 4 * g;
-    Finish4<T> fin;
-    if (wave < MT * NT) fin.read(a, m, n);
     // rows behind the last are the last one again: read, never stored
     const int8_t* wp[NT];
     const int8_t* ap[MT];
@@ -113,7 +109,7 @@ __global__ __launch_bounds__(64 * WK) void i8_few_kernel(LinearArgs a) {
 #pragma unroll
         for (int j = 0; j < MT; j++) acc[i][j] = i32x4_t{0, 0, 0, 0};
     i32x4_t wf[U][NT], af[U][MT];
-    for (int k = wave * (64 * U); k < a.K; k += WK * 64 * U) {
+    auto load = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < U; u++) {
             const int at = k + 64 * u;
@@ -123,12 +119,23 @@ __global__ __launch_bounds__(64 * WK) void i8_few_kernel(LinearArgs a) {
 #pragma unroll
             for (int j = 0; j < MT; j++) af[u][j] = in ? *reinterpret_cast<const i32x4_t*>(ap[j] + at) : i32x4_t{0, 0, 0, 0};
         }
+    };
+    int k = wave * (64 * U);
+    load(k);
+    // a wave finishes one fragment, whose lanes hold four channels of one row
+    const int m = m0 + 16 * (wave % MT) + r, n = n0 + 16 * (wave / MT) + 4 * g;
+    Finish4<T> fin;
+    if (wave < MT * NT) fin.read(a, m, n);
+    for (;;) {
 #pragma unroll
         for (int u = 0; u < U; u++)
 #pragma unroll
             for (int i = 0; i < NT; i++)
 #pragma unroll
                 for (int j = 0; j < MT; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u][i], af[u][j], acc[i][j], 0, 0, 0);
+        k += WK * 64 * U;
+        if (k >= a.K) break;
+        load(k);
     }
 #pragma unroll
     for (int i = 0; i < NT; i++)
@@ -169,18 +176,22 @@ template <int FN, int FM> __device__ __forceinline__ void pin_sums(i32x16_t (&ac
         for (int j = 0; j < FM; j++) asm volatile("" : "+a"(acc[i][j]));
 }
 
-// A workgroup of four waves takes 64 FM rows and 64 FN channels, a wave 32 FM and 32 FN of them, through two LDS tiles of 128 of
-// k each.
+// A workgroup of NW waves takes 64 FM rows and 16 NW FN channels, a wave 32 FM and 32 FN of them, through NS LDS tiles of 128 of k
+// each.  8,192 rows of 4,096 -> 6,144 take 181 us (2.3 POP/s; 64-row operand panels shared in an XCD's L2), 8,192^3 2.4 POP/s, where the
+// library's product of the same sizes reaches 1.9 and 2.1 and the instructions alone 3.2 at the clock the card keeps under them.
 //  - The tiles are loaded straight into LDS, 8 rows of 128 bytes to an instruction.  The 16-byte pieces of row r lie in the order
-//    piece ^ (r / 2 % 8), so that the 16 rows that LDS serves at a time lie in different banks.
+//    piece ^ (r / 2 % 8), so that the 16 rows that LDS serves at a time lie in different banks.  (Tiles of 64 of k, four of them: 190 -> 198.)
 //  - The products are inline assembly with the sums pinned to the accumulator registers: from the builtin the compiler moved them
 //    between the register files and spilled 137 registers (256 x 256).  The wait states between compiled code and the products are
-//    explicit at the loop's two ends; within it a sum is used again 4 or 16 products later.
-//  - The last quarter of a tile's products runs behind the barrier: its operands are in registers by then, so the tile is free
-//    for the loads after next, and the next tile's first operands arrive under its products.
+//    explicit at the loop's two ends; within it a sum goes from product to product in its own registers, which needs none.
+//  - Reads of LDS and loads of later tiles lie between the products.  With large fragments the last quarter of a tile's products runs behind
+//    the barrier: its operands are in registers by then, so the tile is free for loads, and the next tile's first operands arrive
+//    under its products.  Small ones are read a whole tile ahead (1,024 rows of 4,096 -> 4,096 22.4 -> 20.4 us).
+//  - Four LDS tiles where a CU holds one small workgroup: its loads are three tiles ahead (64 rows of 4,096 -> 6,144 17 -> 10 us).  Eight waves for
+//    256 x 256: two per SIMD cover each other's waits (190 -> 181).
 template <typename T, int FM, int FN, int NS, int NW>
 __global__ __launch_bounds__(64 * NW, NW == 8 || FM * FN > 8 || (FM + FN) * NS * 8 > 80 ? 1 : 2) void i8_panel_kernel(LinearArgs a) {
-    static_assert(NS == 2 || NS == 4, "the loop's body is written out for two and four");
+    static_assert(NS == 2 || NS == 4, "the loop's body is written out for two and four LDS tiles");
     constexpr int TM = 64 * FM, TN = 16 * NW * FN;
     constexpr int LA = TM / (8 * NW), LW = TN / (8 * NW);          // loads per wave and tile
     // arrays of their own, so that the compiler can tell a tile that is read from one that is loaded
@@ -403,7 +414,7 @@ template <typename T> static void launch_linear(const LinearArgs& a, hipStream_t
     switch (linear_kernel(a.M, a.N, a.K)) {
         case FEW_16x16: return launch_few<T, 1, 1, 4, 16>(a, st);
         case FEW_16x16_DEEP: return launch_few<T, 1, 1, 8, 16>(a, st);
-        case FEW_16x16_WIDE: return launch_few<T, 1, 1, 4, 8>(a, st);
+        case FEW_16x16_SHORT: return launch_few<T, 1, 1, 4, 8>(a, st);
         case FEW_16x32: return launch_few<T, 1, 2, 4, 8>(a, st);
         case PANEL_64x64: return launch_panel<T, 1, 1, 4>(a, st);
         case PANEL_64x128: return launch_panel<T, 1, 2, 4>(a, st);

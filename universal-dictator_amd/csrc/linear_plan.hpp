@@ -9,7 +9,7 @@ namespace ud {
 enum LinearKernel {
     FEW_16x16,          // 4 waves, blocks of 1,024 of k
     FEW_16x16_DEEP,     // 8 waves
-    FEW_16x16_WIDE,     // 4 waves, blocks of 512
+    FEW_16x16_SHORT,     // 4 waves, blocks of 512
     FEW_16x32,          // 4 waves, blocks of 512
     PANEL_64x64,        // 4 LDS tiles
     PANEL_64x128,       // 4
@@ -23,18 +23,19 @@ enum LinearKernel {
 
 constexpr int64_t tiles_of(int64_t M, int64_t N, int64_t tm, int64_t tn) { return ((M + tm - 1) / tm) * ((N + tn - 1) / tn); }
 
-// Few rows while their workgroups are one round of the chip: the weights' way from memory is the time then, and small tiles spread
-// it over all CUs.  us, 16 x 16 / 16 x 32 / 64 x 64 (weights from HBM): 16 rows of 4,096 -> 4,096 6.1 / 7.9 / 9.6, 24 rows 8.9 / 7.8 / 9.8,
-// 48 rows 13 / 12 / 9.8; 1 row of 4,096 -> 6,144 7.9 / 8.4 / 11.4, of 2,048 -> 32,001 (blocks of 512) 13.1 / 13.7 / 14.5 but 13 rows 18.2 /
-// 17.0 / 15.0 (64 x 128: 14.2); 1 row of 12,288 -> 4,096 with 8 waves 10.8, with 4 11.8.
+// Few rows while their workgroups are one round of the chip, or the rows so few that reading them again for every 16 channels costs
+// nothing: the weights' way from memory is the time then, and small tiles spread it over all CUs.  us, 16 x 16 / 16 x 32 / 64 x 64 (weights
+// from HBM): 16 rows of 4,096 -> 4,096 6.1 / 7.9 / 9.6, 24 rows 8.9 / 7.8 / 9.8, 48 rows 13 / 12 / 9.8; one row of 4,096 -> 6,144 7.6 / 8.4 / 11.4;
+// 13 rows of 2,048 -> 32,001 18.2 / 17.0 / 15.0 (64 x 128: 14.1).  All of k at one time where it fits: one row of 4,096 -> 32,000 in blocks of
+// 1,024 24.0, of 512 31.8, but of 2,048 -> 32,001 14.1 and 12.9, with 8 waves of 12,288 -> 4,096 10.9, with 4 11.8.
 //
 // Otherwise the tile whose rounds over the 256 CUs cost least, from what one tile took per 128 of k and beside them (us, all CUs at
-// work).  us predicted and measured: 563 rows of 4,096 -> 6,144 128 x 128 23 and 22.4, 64 x 64 33 and 30.4, 256 x 256 64 and 50; 2,469 of
-// 12,288 -> 4,096 256 x 192 144 and 124, 128 x 128 159 and 164, 256 x 256 176 and 142; 8,192 of 4,096 -> 6,144 256 x 256 176 and 185,
-// 256 x 192 190 and 200.
+// work).  us predicted and measured: 563 rows of 4,096 -> 6,144 128 x 128 20 and 21.3, 64 x 64 36 and 30.4, 256 x 256 60 and 49; 2,469 of
+// 12,288 -> 4,096 256 x 192 142 and 129, 128 x 128 165 and 164, 256 x 256 169 and 145; 8,192 of 4,096 -> 6,144 256 x 256 181 and 181,
+// 256 x 192 206 and 200.
 inline LinearKernel linear_kernel(int64_t M, int64_t N, int64_t K) {
     const int64_t few = tiles_of(M, N, 16, 16);
-    if (M <= 4 || few <= 256) return K >= 8192 ? FEW_16x16_DEEP : few > 512 ? FEW_16x16_WIDE : FEW_16x16;
+    if (M <= 4 || few <= 256) return K >= 8192 ? FEW_16x16_DEEP : K > 2048 ? FEW_16x16 : FEW_16x16_SHORT;
     if (tiles_of(M, N, 16, 32) <= 256) return FEW_16x32;
     struct Shape { LinearKernel kernel; int tm, tn; double step, once; };
     const Shape shapes[] = {{PANEL_64x64, 64, 64, 0.23, 1.5},   {PANEL_64x128, 64, 128, 0.31, 2},  {PANEL_128x64, 128, 64, 0.29, 2},

@@ -145,18 +145,17 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void i8_rows_kernel(RowArgs 
     store_codes<W, P>(y, t, a.dim, at_top, static_cast<int8_t*>(a.out) + row * a.out_ld, a.scales + row);
 }
 
-// A kernel's waves per row and pieces per lane.
+// A row's waves and each lane's pieces, by its length: two pieces a lane where a row is long enough, so that few enough waves meet at
+// the barriers and enough loads are on their way.  us, bf16 with its residual to 8 bits, W x P: 8,200 rows of 1,024 1 x 2 13.2, 4 x 1
+// 16.0; of 4,096 4 x 2 39.7, 8 x 1 46.0, 16 x 1 53; of 8,192 8 x 2 85, 16 x 1 101, 4 x 4 90; 563 of 4,096 4 x 2 6.3, 16 x 1 7.7, but 256 4.8
+// and 4.5, and one row (its latency, in the trace) 3.8 and 3.2.
 template <template <int, int> class L> static void launch_rows(const RowArgs& a, hipStream_t st) {
-    const bool few = a.rows < 1024;
-    const int d = a.dim;
-    if (d <= 512) L<1, 1>::go(a, st);
-    else if (few && d <= 2048) L<4, 1>::go(a, st);
-    else if (few && d <= 8192) L<16, 1>::go(a, st);
-    else if (d <= 1024) L<1, 2>::go(a, st);
-    else if (d <= 2048) L<1, 4>::go(a, st);
-    else if (d <= 4096) L<4, 2>::go(a, st);
-    else if (d <= 8192) L<4, 4>::go(a, st);
-    else if (d <= 16384) L<16, 2>::go(a, st);
+    if (a.dim <= 1024) L<1, 2>::go(a, st);
+    else if (a.dim <= 2048) L<4, 1>::go(a, st);
+    else if (a.rows <= 256 && a.dim <= 8192) L<16, 1>::go(a, st);
+    else if (a.dim <= 4096) L<4, 2>::go(a, st);
+    else if (a.dim <= 8192) L<8, 2>::go(a, st);
+    else if (a.dim <= 16384) L<16, 2>::go(a, st);
     else L<16, 4>::go(a, st);
 }
 static dim3 row_grid(int rows, int w) { return dim3((unsigned)(w == 1 ? (rows + 3) / 4 : rows)); }
