@@ -16,7 +16,8 @@ struct LinearArgs {
     int M, N, K;
 };
 
-// What finishes four channels n .. n + 3 of row m, read ahead of the sums.
+// What finishes four channels n .. n + 3 of row m, read ahead of the sums.  (The operations are those of finish8, so that a row's result does
+// not follow the kernel.)
 template <typename T> struct Finish4 {
     float s, sw[4], bias[4];
     T res[4];
@@ -24,6 +25,8 @@ template <typename T> struct Finish4 {
 
     __device__ __forceinline__ void read(const LinearArgs& a, int m, int n) {
         there = m < a.M && n < a.N;
+#pragma unroll
+        for (int i = 0; i < 4; i++) bias[i] = 0.0f;
         if (!there) return;
         s = a.sa[m];
         const T* r = a.res ? static_cast<const T*>(a.res) + m * a.res_ld + n : nullptr;
@@ -47,8 +50,7 @@ template <typename T> struct Finish4 {
         T y[4];
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            float v = (float)acc[i] * s * sw[i];
-            if (a.bias) v += bias[i];
+            float v = fmaf((float)acc[i] * s, sw[i], bias[i]);
             if (a.res) v += to_f<T>(res[i]);
             y[i] = from_f<T>(v);
         }
@@ -70,7 +72,7 @@ __device__ __forceinline__ void finish8(const LinearArgs& a, int m, int n, int l
     T* o = static_cast<T*>(a.out) + m * a.out_ld + n;
     float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; e++) v[e] = (float)(e < 4 ? lo[e % 4] : hi[e % 4]) * s * sw[e] + bias[e];
+    for (int e = 0; e < 8; e++) v[e] = fmaf((float)(e < 4 ? lo[e % 4] : hi[e % 4]) * s, sw[e], bias[e]);
     if (left >= 8) {
         if (a.res) {
             float f[8];
