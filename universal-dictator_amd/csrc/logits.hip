@@ -71,14 +71,19 @@ template <typename T, int SEG> __global__ __launch_bounds__(1024) void logits_ke
     __shared__ float top[W];
     __shared__ int first;
     const int tid = threadIdx.x, row = blockIdx.y, t0 = blockIdx.x * SEG, len = min(SEG, a.vocab - t0);
-    int lo = 0, fresh = 0, hi = 0, blo = 0, bhi = 0, m = -1;
+    // (used behind the last of these branches only, so that all of a row's numbers are on their way together)
+    int from = 0, fresh = 0, to = 0, bias_from = 0, bias_to = 0, mask_row = row;
     float rep = 1.0f, pres = 0.0f, freq = 0.0f;
     if (a.tokens) {
-        lo = max(a.ranges[3 * row], 0), fresh = a.ranges[3 * row + 1], hi = min(a.ranges[3 * row + 2], a.n_tokens);
-        rep = a.penalties[3 * row], pres = a.penalties[3 * row + 1], freq = a.penalties[3 * row + 2];
+        const int32_t* range = a.ranges + 3 * row;
+        const float* pen = a.penalties + 3 * row;
+        from = range[0], fresh = range[1], to = range[2];
+        rep = pen[0], pres = pen[1], freq = pen[2];
     }
-    if (a.bias_ids) blo = max(a.bias_ranges[2 * row], 0), bhi = min(a.bias_ranges[2 * row + 1], a.n_biases);
-    if (a.mask) m = a.mask_rows ? a.mask_rows[row] : row;
+    if (a.bias_ids) bias_from = a.bias_ranges[2 * row], bias_to = a.bias_ranges[2 * row + 1];
+    if (a.mask_rows) mask_row = a.mask_rows[row];
+    const int lo = max(from, 0), hi = min(to, a.n_tokens), blo = max(bias_from, 0), bhi = min(bias_to, a.n_biases);
+    const int m = a.mask ? mask_row : -1;
     const bool masked = m >= 0 && m < a.n_masks;
     const T* in = static_cast<const T*>(a.logits) + row * a.ld + t0;
     Raw8<T> raw[E];
@@ -138,55 +143,55 @@ template <typename T, int SEG> __global__ __launch_bounds__(1024) void logits_ke
         const float z = c ? y - fmaf(freq, (float)c, pres) : y;
         return seen ? z : x;
     };
-    if (hi - (int64_t)lo <= kCounts && bhi - (int64_t)blo <= kSlots) {
-        // Both lists in one pass over the words: the last bias of a token and the number of times it was generated, side by side.
-        if (lo < hi || blo < bhi) {
-            clear();
+    // Lists that are short enough: both in one pass over the words, the last bias of a token and the number of times it was generated
+    // side by side.
+    const bool lists = lo < hi || blo < bhi, packed = hi - (int64_t)lo <= kCounts && bhi - (int64_t)blo <= kSlots;
+    if (lists) {
+        clear();
+        if (packed) {
             if (blo < bhi)
                 scan(a.bias_ids, blo, bhi, bias_ids,
                      [&](uint32_t& w, int i) __attribute__((always_inline)) { atomicMax(&w, (uint32_t)(i - blo + 1) << 16); });
             if (lo < hi) scan(a.tokens, lo, hi, ids, count);
+        } else {
+            scan(a.tokens, lo, hi, ids, count);
 #pragma unroll
             for (int i = 0; i < E; i++) {
-                uint32_t w[8], any = 0;
+                uint32_t w[8];
                 words(i, w);
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    any |= w[e];
-                    l[i][e] = penalize(l[i][e], w[e] & (kInPrompt | kCounts), w[e] & kCounts);
-                }
-                if (any & kSlots << 16)
-#pragma unroll
-                    for (int e = 0; e < 8; e++)
-                        if (const uint32_t s = w[e] >> 16 & kSlots) l[i][e] += a.bias_values[blo + (int64_t)s - 1];
+                for (int e = 0; e < 8; e++) l[i][e] = penalize(l[i][e], w[e], w[e] & ~kInPrompt);
             }
-        }
-    } else {
-        clear();
-        scan(a.tokens, lo, hi, ids, count);
+            __syncthreads();
+            clear();
+            scan(a.bias_ids, blo, bhi, bias_ids, [&](uint32_t& w, int i) __attribute__((always_inline)) { atomicMax(&w, (uint32_t)(i - blo) + 1); });
 #pragma unroll
-        for (int i = 0; i < E; i++) {
-            uint32_t w[8];
-            words(i, w);
+            for (int i = 0; i < E; i++) {
+                uint32_t w[8];
+                words(i, w);
 #pragma unroll
-            for (int e = 0; e < 8; e++) l[i][e] = penalize(l[i][e], w[e], w[e] & ~kInPrompt);
-        }
-        __syncthreads();
-        clear();
-        scan(a.bias_ids, blo, bhi, bias_ids, [&](uint32_t& w, int i) __attribute__((always_inline)) { atomicMax(&w, (uint32_t)(i - blo) + 1); });
-#pragma unroll
-        for (int i = 0; i < E; i++) {
-            uint32_t w[8];
-            words(i, w);
-#pragma unroll
-            for (int e = 0; e < 8; e++)
-                if (w[e]) l[i][e] += a.bias_values[blo + (int64_t)w[e] - 1];
+                for (int e = 0; e < 8; e++)
+                    if (w[e]) l[i][e] += a.bias_values[blo + (int64_t)w[e] - 1];
+            }
         }
     }
     float most = -__builtin_inff();
 #pragma unroll
     for (int i = 0; i < E; i++) {
         const int c = (i * THREADS + tid) * 8, left = len - c;
+        if (lists && packed) {
+            uint32_t w[8], any = 0;
+            words(i, w);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                any |= w[e];
+                l[i][e] = penalize(l[i][e], w[e] & (kInPrompt | kCounts), w[e] & kCounts);
+            }
+            if (any & kSlots << 16)
+#pragma unroll
+                for (int e = 0; e < 8; e++)
+                    if (const uint32_t s = w[e] >> 16 & kSlots) l[i][e] += a.bias_values[blo + (int64_t)s - 1];
+        }
         if (left <= 0) continue;
         if (masked)
 #pragma unroll
