@@ -16,7 +16,7 @@
  * Rows in 8 bits: codes int8 [rows, dim] and one fp32 scale per row (a token of activations, an output channel of weights),
  * value = code * scale.  Of a row y: scale = max(max|y| / 127, 2^-126), code = y / scale rounded to the nearest whole number
  * (even one of two), so -127 .. 127; a row with an infinity or a NaN has the scale NaN and codes 0.  fp32 arithmetic: a y within
- * 2^-16 of the border between two codes may get either.
+ * 2^-12 scale of the border between two codes may get either.
  */
 #ifndef UD_LAYER_H
 #define UD_LAYER_H
@@ -40,7 +40,7 @@ extern "C" {
  *   residual     sum_dtype (dtype, or UD_F32), rows sum_ld apart; sum_out: the same, may be residual itself
  *   weight       fp32 [dim] or null (1)
  *   out          out_dtype: dtype, or UD_I8 with scales fp32 [rows] (otherwise null)
- * dim a multiple of 8, 8 .. 32768; lds multiples of 8, pointers 16-byte aligned (codes 8, scales 4).  eps >= 1e-30.
+ * dim a multiple of 8, 8 .. 32768; rows below 2^22; lds multiples of 8, pointers 16-byte aligned (codes 8, scales 4).  eps 1e-30 .. 1e30.
  * The norm is that of the sums as they are stored.  An output may be an input of the same type and ld (in place); any
  * other overlap is refused.  Precision: squares summed in 64 bits, the rest in fp32, one rounding at the end. */
 UD_API int ud_rms_norm(int32_t dtype, const void* x_dev, int32_t x_ld, int32_t sum_dtype, const void* residual_dev,
@@ -52,8 +52,8 @@ UD_API int ud_rms_norm(int32_t dtype, const void* x_dev, int32_t x_ld, int32_t s
  *   y = x, or x * gate / (1 + exp(-gate)) where gate_dev is given
  *   x, gate      dtype, rows ld apart both (two pieces of one fused row, or buffers of their own)
  *   codes        int8, rows codes_ld apart;  scales fp32 [rows]
- * dim a multiple of 8, 8 .. 32768; lds multiples of 8, x and gate 16-byte aligned, codes 8.  An output that overlaps an input is
- * refused. */
+ * dim a multiple of 8, 8 .. 32768; rows below 2^22; lds multiples of 8, x and gate 16-byte aligned, codes 8.  An output that overlaps
+ * an input is refused.  exp(-gate) past fp32's range (gates below -88) makes y 0. */
 UD_API int ud_i8_quantize(int32_t dtype, const void* x_dev, const void* gate_dev, int32_t ld, int8_t* codes_dev, int32_t codes_ld,
                           float* scales_dev, int32_t rows, int32_t dim, void* hip_stream);
 
@@ -66,7 +66,7 @@ UD_API int ud_i8_quantize(int32_t dtype, const void* x_dev, const void* gate_dev
  *   residual     dtype [M, N], rows res_ld apart, or null; may be out itself where res_ld is out_ld
  *   out          dtype [M, N], rows out_ld apart
  * K a multiple of 16, 16 .. 131056 (the sum stays in 32 bits); codes and w 16-byte aligned, their lds multiples of 16, at most
- * 2^22; N 1 .. 2^24, M 0 .. 2^22, M N at most 2^38.  out and residual need the alignment of their elements only.  Other overlaps
+ * 2^22; N 1 .. 2^24, M below 2^22, M N at most 2^38.  out and residual need the alignment of their elements only.  Other overlaps
  * of out are refused.  Precision: the sum exact, then fp32 in the order written (the second scale and the bias in one
  * operation), one rounding at the end: a row's result is the same in a batch of any size. */
 UD_API int ud_i8_linear(int32_t dtype, const int8_t* codes_dev, int32_t codes_ld, const float* scales_dev, const int8_t* w_dev,

@@ -36,7 +36,7 @@ def test_gpu_tests_reach_every_kernel(kernel):
 
 def test_launches_stay_small(kernel):
     rng = np.random.default_rng(1)
-    sizes = [(1 << 22, 1 << 16, 16), (1 << 14, 1 << 24, 131056), (4, 1 << 24, 8192), (5, 1 << 24, 64), (1 << 22, 1, 16), (1 << 22, 65536, 131056), (64, 1 << 24, 64),
+    sizes = [((1 << 22) - 1, 1 << 16, 16), (1 << 14, 1 << 24, 131056), (4, 1 << 24, 8192), (5, 1 << 24, 64), ((1 << 22) - 1, 1, 16), ((1 << 22) - 1, 65536, 131056), (64, 1 << 24, 64),
              (65, 1 << 24, 64), (300, 1 << 24, 64)]
     sizes += [tuple(int(x) for x in np.exp(rng.uniform(0, [15.2, 16.6, 11.7]))) for _ in range(20000)]
     for M, N, K in sizes:

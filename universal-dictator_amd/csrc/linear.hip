@@ -248,7 +248,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || FM * FN > 8 || (FM + FN) * NS *
     // Fragments in registers: of two whole tiles where there is room (a tile is read under the products of the one before), else of two
     // k steps.
     constexpr int R = FM + FN;
-    constexpr bool WHOLE = R <= 4 && NW == 4;
+    constexpr bool WHOLE = R <= 4 && NS == 4 && NW == 4;
     i32x4_t fa[WHOLE ? 8 : 2][FM], fw[WHOLE ? 8 : 2][FN];
     auto read_frag = [&](int i, int q, const int8_t* at, const int8_t* wt, i32x4_t (&da)[FM], i32x4_t (&dw)[FN]) __attribute__((always_inline)) {
         const int off = r32 * KB + 16 * ((2 * q + half) ^ (r32 / 2 % 8));
@@ -440,8 +440,8 @@ extern "C" UD_API int ud_i8_linear(int32_t dtype, const int8_t* codes_dev, int32
     const int64_t size = type_bytes(dtype);
     if (!size) return layer_fail(UD_ERR_INVALID, "%s: dtype %d", who, dtype);
     // (a launch holds fewer than 2^32 threads, a tile's rows lie within 32-bit offsets)
-    if (M < 0 || M > (1 << 22) || N < 1 || N > (1 << 24) || (int64_t)M * N > (int64_t)1 << 38 || K < 16 || K > 131056 || K % 16)
-        return layer_fail(UD_ERR_SHAPE, "%s: M %d (0 .. 2^22), N %d (1 .. 2^24, M N at most 2^38), K %d (a multiple of 16, 16 .. 131056)", who, M, N, K);
+    if (M < 0 || M >= (1 << 22) || N < 1 || N > (1 << 24) || (int64_t)M * N > (int64_t)1 << 38 || K < 16 || K > 131056 || K % 16)
+        return layer_fail(UD_ERR_SHAPE, "%s: M %d (0 .. 2^22 - 1), N %d (1 .. 2^24, M N at most 2^38), K %d (a multiple of 16, 16 .. 131056)", who, M, N, K);
     if (codes_ld < K || w_ld < K || ((codes_ld | w_ld) & 15) || codes_ld > (1 << 22) || w_ld > (1 << 22) || out_ld < N || (residual_dev && res_ld < N))
         return layer_fail(UD_ERR_SHAPE, "%s: rows %d/%d/%d/%d elements apart for K %d (multiples of 16, at most 2^22), N %d", who, codes_ld, w_ld,
                           res_ld, out_ld, K, N);

@@ -302,7 +302,7 @@ extern "C" UD_API int ud_logits_process(int32_t dtype, const void* logits_dev, i
     const Block token = flat(token_dev, n), ws{token_dev ? workspace : nullptr, 0, (int64_t)need, 1};
     const Block inputs[] = {flat(tokens_dev, n_tokens), flat(ranges_dev, tokens_dev ? 3 * (int64_t)n : 0), flat(penalties_dev, 3 * (int64_t)n),
                             flat(bias_ids_dev, n_biases), flat(bias_values_dev, n_biases), flat(bias_ranges_dev, bias_ids_dev ? 2 * (int64_t)n : 0),
-                            flat(mask_dev, (int64_t)n_masks * mask_ld), flat(mask_rows_dev, n)};
+                            Block{mask_dev, 4 * (int64_t)mask_ld, (vocab + 31) / 32 * (int64_t)4, n_masks}, flat(mask_rows_dev, n)};
     bool clash = (blocks_meet(out, in) && !(size == 4 && blocks_same(out, in))) || blocks_meet(token, in) || blocks_meet(ws, in) ||
                  blocks_meet(out, token) || blocks_meet(out, ws) || blocks_meet(token, ws);
     for (const Block& b : inputs) clash = clash || (b.width && (blocks_meet(out, b) || blocks_meet(token, b) || blocks_meet(ws, b)));

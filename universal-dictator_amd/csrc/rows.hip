@@ -186,7 +186,8 @@ template <typename T> static void launch_eight(const RowArgs& a, hipStream_t st)
 // The checks that both calls make.
 static int rows_check(const char* who, int32_t dtype, int32_t rows, int32_t dim) {
     if (!type_bytes(dtype)) return layer_fail(UD_ERR_INVALID, "%s: dtype %d", who, dtype);
-    if (rows < 0 || rows > (1 << 22)) return layer_fail(UD_ERR_SHAPE, "%s: rows %d (0 .. 2^22)", who, rows);
+    // (a launch holds fewer than 2^32 threads)
+    if (rows < 0 || rows >= (1 << 22)) return layer_fail(UD_ERR_SHAPE, "%s: rows %d (0 .. 2^22 - 1)", who, rows);
     if (dim < 8 || dim > 32768 || dim % 8) return layer_fail(UD_ERR_SHAPE, "%s: dim %d (a multiple of 8, 8 .. 32768)", who, dim);
     return UD_OK;
 }
