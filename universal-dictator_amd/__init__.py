@@ -752,33 +752,30 @@ def gqa_prefill_paged(q, k_pages, v_pages, num_blocks, block_table, max_blocks, 
 UD_I8 = 32
 
 
-def _ptr(b):
-    return b.ptr if b is not None else None
-
-
 def rms_norm(x, out, rows, dim, weight=None, eps=1e-6, residual=None, sum_out=None, scales=None, dtype="bf16", sum_dtype=None,
              out_dtype=None, x_ld=None, sum_ld=None, out_ld=None, hip_stream=None):
     """out = RMS norm of s = x + residual (None: x) with weight fp32 [dim]; s is stored to sum_out (may be residual) in sum_dtype
     (dtype or f32).  out_dtype None: dtype; "i8": int8 codes with fp32 scales [rows].  *_ld: elements between rows (None: dim)."""
     od = UD_I8 if out_dtype == "i8" else _DTYPES[out_dtype or dtype]
-    _check(lib().ud_rms_norm(_DTYPES[dtype], _ptr(x), dim if x_ld is None else x_ld, _DTYPES[sum_dtype or dtype], _ptr(residual),
-                             _ptr(sum_out), dim if sum_ld is None else sum_ld, _ptr(weight), eps, od, _ptr(out),
-                             dim if out_ld is None else out_ld, _ptr(scales), rows, dim, hip_stream.ptr if hip_stream else None))
+    _check(lib().ud_rms_norm(_DTYPES[dtype], x.ptr, dim if x_ld is None else x_ld, _DTYPES[sum_dtype or dtype], residual and residual.ptr,
+                             sum_out and sum_out.ptr, dim if sum_ld is None else sum_ld, weight and weight.ptr, eps, od, out.ptr,
+                             dim if out_ld is None else out_ld, scales and scales.ptr, rows, dim, hip_stream and hip_stream.ptr))
 
 
 def i8_quantize(x, codes, scales, rows, dim, gate=None, dtype="bf16", ld=None, codes_ld=None, hip_stream=None):
     """Rows of dtype to int8 codes with a scale each, value = code * scale: x, or x * silu(gate) where a gate is given.
     ld: elements between rows of x and of gate (None: dim).  Weights [out, in] take the same call: a scale per channel."""
-    _check(lib().ud_i8_quantize(_DTYPES[dtype], _ptr(x), _ptr(gate), dim if ld is None else ld, _ptr(codes),
-                                dim if codes_ld is None else codes_ld, _ptr(scales), rows, dim, hip_stream.ptr if hip_stream else None))
+    _check(lib().ud_i8_quantize(_DTYPES[dtype], x.ptr, gate and gate.ptr, dim if ld is None else ld, codes.ptr,
+                                dim if codes_ld is None else codes_ld, scales.ptr, rows, dim, hip_stream and hip_stream.ptr))
 
 
 def i8_linear(codes, scales, w, w_scales, out, M, N, K, bias=None, residual=None, dtype="bf16", codes_ld=None, w_ld=None,
               res_ld=None, out_ld=None, hip_stream=None):
     """out [M, N] of dtype = (codes [M, K] . w [N, K]^T) * scales[m] * w_scales[n] + bias + residual (may be out)."""
-    _check(lib().ud_i8_linear(_DTYPES[dtype], _ptr(codes), K if codes_ld is None else codes_ld, _ptr(scales), _ptr(w),
-                              K if w_ld is None else w_ld, _ptr(w_scales), _ptr(bias), _ptr(residual), N if res_ld is None else res_ld,
-                              _ptr(out), N if out_ld is None else out_ld, M, N, K, hip_stream.ptr if hip_stream else None))
+    _check(lib().ud_i8_linear(_DTYPES[dtype], codes.ptr, K if codes_ld is None else codes_ld, scales.ptr, w.ptr,
+                              K if w_ld is None else w_ld, w_scales.ptr, bias and bias.ptr, residual and residual.ptr,
+                              N if res_ld is None else res_ld, out.ptr, N if out_ld is None else out_ld, M, N, K,
+                              hip_stream and hip_stream.ptr))
 
 
 def logits_workspace_bytes(n, vocab):
@@ -791,11 +788,12 @@ def logits_process(logits, out, n, vocab, token=None, tokens=None, n_tokens=0, r
     """out fp32 [n, vocab] = logits under penalties for the tokens of each row's history, biases and grammar masks; token int32 [n]:
     the greedy choice (-1: nothing is left).  See ud_layer.h for the arrays.  workspace: logits_workspace_bytes(n, vocab) bytes where
     token is given.  *_ld: elements (words of the mask) between rows (None: contiguous)."""
-    _check(lib().ud_logits_process(_DTYPES[dtype], _ptr(logits), vocab if ld is None else ld, _ptr(out), vocab if out_ld is None else out_ld,
-                                   _ptr(token), n, vocab, _ptr(tokens), n_tokens, _ptr(ranges), _ptr(penalties), _ptr(bias_ids),
-                                   _ptr(bias_values), n_biases, _ptr(bias_ranges), _ptr(mask), (vocab + 31) // 32 if mask_ld is None else mask_ld,
-                                   n_masks, _ptr(mask_rows), _ptr(workspace), workspace.nbytes if workspace is not None else 0,
-                                   hip_stream.ptr if hip_stream else None))
+    _check(lib().ud_logits_process(_DTYPES[dtype], logits.ptr, vocab if ld is None else ld, out.ptr, vocab if out_ld is None else out_ld,
+                                   token and token.ptr, n, vocab, tokens and tokens.ptr, n_tokens, ranges and ranges.ptr,
+                                   penalties and penalties.ptr, bias_ids and bias_ids.ptr, bias_values and bias_values.ptr, n_biases,
+                                   bias_ranges and bias_ranges.ptr, mask and mask.ptr, (vocab + 31) // 32 if mask_ld is None else mask_ld,
+                                   n_masks, mask_rows and mask_rows.ptr, workspace and workspace.ptr, workspace.nbytes if workspace else 0,
+                                   hip_stream and hip_stream.ptr))
 
 
 # ---------------------------------------------------------------- synthetic weights
