@@ -28,18 +28,6 @@ template <typename T> __device__ __forceinline__ void widen8(const Raw8<T>& r, f
 #pragma unroll
     for (int i = 0; i < (int)(sizeof(T) / 2); i++) unpack16<T>(r.v[i], f + i * Vec16<T>::N);
 }
-// Floats that T holds (infinities among them).
-template <typename T> __device__ __forceinline__ Raw8<T> exact8(const float (&f)[8]) {
-    T v[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-        if constexpr (std::is_same<T, bf16>::value) v[e] = (bf16)(__float_as_uint(f[e]) >> 16);
-        else v[e] = (T)f[e];
-    }
-    Raw8<T> r;
-    __builtin_memcpy(&r, v, sizeof r);
-    return r;
-}
 // Rounded to nearest even; half saturates.
 template <typename T> __device__ __forceinline__ Raw8<T> narrow8(const float (&f)[8]) {
     Raw8<T> r;

@@ -34,16 +34,21 @@ __device__ __forceinline__ uint64_t wave_max_key(uint64_t v) {
     return v;
 }
 
-// Eight logits from p, `left` of them there (the others -inf); p need not be aligned to more than an element.
-template <typename T> __device__ __forceinline__ Raw8<T> load_logits(const T* p, int left) {
-    Raw8<T> r;
-    if (left >= 8) {
+// Four logits as they lie in memory, and as floats.
+template <typename T> struct Raw4 { T v[4]; };
+// From p, `left` of them there (the others -inf); p need not be aligned to more than an element.
+template <typename T> __device__ __forceinline__ Raw4<T> load_logits(const T* p, int left) {
+    Raw4<T> r;
+    if (left >= 4) {
         __builtin_memcpy(&r, p, sizeof r);
     } else {
-        float f[8];
+        const float none = -__builtin_inff();
 #pragma unroll
-        for (int e = 0; e < 8; e++) f[e] = e < left ? to_f<T>(p[e]) : -__builtin_inff();
-        r = exact8<T>(f);
+        for (int e = 0; e < 4; e++) {
+            if (e < left) r.v[e] = p[e];
+            else if constexpr (std::is_same<T, bf16>::value) r.v[e] = (bf16)(__float_as_uint(none) >> 16);
+            else r.v[e] = (T)none;
+        }
     }
     return r;
 }
@@ -62,11 +67,11 @@ template <int THREADS, int D> __device__ __forceinline__ void load_ids(const int
     }
 }
 
-// 16 waves, SEG tokens: a thread's E pieces of eight are 8,192 apart (a small segment leaves threads that only read the lists: one row of
-// 131,072 with a history of 100,000 38 -> 19 us).  What the row's lists say is asked for at once, at the start: one after
+// 16 waves, SEG tokens: a thread's E pieces of four are 4,096 apart, so that a wave reads and writes whole lines (pieces of eight: 22.9 -> 21.0 us
+// at 64 rows).  A small segment leaves threads that only read the lists (one row of 131,072 with a history of 100,000 38 -> 15 us).  What the row's lists say is asked for at once, at the start: one after
 // the other their latencies would be most of a short call.
 template <typename T, int SEG> __global__ __launch_bounds__(1024) void logits_kernel(LogitArgs a) {
-    constexpr int W = 16, THREADS = 64 * W, E = (SEG + 8 * THREADS - 1) / (8 * THREADS);
+    constexpr int W = 16, THREADS = 64 * W, E = (SEG + 4 * THREADS - 1) / (4 * THREADS);
     __shared__ __attribute__((aligned(16))) uint32_t word[SEG];
     __shared__ float top[W];
     __shared__ int first;
@@ -86,12 +91,12 @@ template <typename T, int SEG> __global__ __launch_bounds__(1024) void logits_ke
     const int m = a.mask ? mask_row : -1;
     const bool masked = m >= 0 && m < a.n_masks;
     const T* in = static_cast<const T*>(a.logits) + row * a.ld + t0;
-    Raw8<T> raw[E];
-    uint8_t bits[E];
+    Raw4<T> raw[E];
+    uint32_t allowed = 0;                          // four bits of the mask a piece
     int32_t ids[4][4], bias_ids[1][4];             // the first of each list
 #pragma unroll
     for (int i = 0; i < E; i++) {
-        const int c = (i * THREADS + tid) * 8;
+        const int c = (i * THREADS + tid) * 4;
         raw[i] = load_logits<T>(in + c, len - c);
     }
     if (lo < hi) load_ids<THREADS>(a.tokens, lo, hi, ids);
@@ -99,24 +104,22 @@ template <typename T, int SEG> __global__ __launch_bounds__(1024) void logits_ke
     if (masked) {
         const uint8_t* mask = reinterpret_cast<const uint8_t*>(a.mask + m * a.mask_ld) + t0 / 8;
 #pragma unroll
-        for (int i = 0; i < E; i++) bits[i] = (i * THREADS + tid) * 8 < len ? mask[i * THREADS + tid] : 0;
+        for (int i = 0; i < E; i++)
+            if ((i * THREADS + tid) * 4 < len) allowed |= (uint32_t)(mask[(i * THREADS + tid) / 2] >> (tid % 2 * 4) & 15) << (4 * i);
     }
     auto clear = [&]() __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < 2 * E; i++)
-            if (SEG >= 8 * THREADS || (i * THREADS + tid) * 4 < SEG) *reinterpret_cast<uint4*>(&word[(i * THREADS + tid) * 4]) = make_uint4(0, 0, 0, 0);
+        for (int i = 0; i < E; i++)
+            if (SEG >= 4 * THREADS || tid * 4 < SEG) *reinterpret_cast<uint4*>(&word[(i * THREADS + tid) * 4]) = make_uint4(0, 0, 0, 0);
         __syncthreads();
     };
-    auto words = [&](int i, uint32_t (&w)[8]) __attribute__((always_inline)) {
-        const int at = SEG >= 8 * THREADS ? i * THREADS + tid : min(tid, SEG / 8 - 1);
-        const uint4 u = ld16(&word[at * 4]), v = ld16(&word[SEG / 2 + at * 4]);
+    auto words = [&](int i, uint32_t (&w)[4]) __attribute__((always_inline)) {
+        const uint4 u = ld16(&word[SEG >= 4 * THREADS ? (i * THREADS + tid) * 4 : min(tid * 4, SEG - 4)]);
         w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
-        w[4] = v.x; w[5] = v.y; w[6] = v.z; w[7] = v.w;
     };
     // what(token's word, index) for entries from .. to - 1 of a list, the first of which are in v
     auto scan = [&](const int32_t* list, int from, int to, auto& v, auto what) __attribute__((always_inline)) {
         constexpr int D = sizeof(v) / 16;
-        auto place = [](uint32_t p) { return (p / 8 * 4 + p % 4) + (p & 4) * (SEG / 8); };   // a piece's two halves apart: fewer bank conflicts
         for (int64_t at = from; at < to; at += 4 * THREADS * D) {
             if (at != from) load_ids<THREADS>(list, at, to, v);
 #pragma unroll
@@ -124,7 +127,7 @@ template <typename T, int SEG> __global__ __launch_bounds__(1024) void logits_ke
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     const uint32_t p = (uint32_t)v[d][e] - (uint32_t)t0;   // (an id below t0 is past len, too)
-                    if (p < (uint32_t)len) what(word[place(p)], (int)at + 4 * (d * THREADS + tid) + e);
+                    if (p < (uint32_t)len) what(word[p], (int)at + 4 * (d * THREADS + tid) + e);
                 }
         }
         __syncthreads();
@@ -133,9 +136,6 @@ template <typename T, int SEG> __global__ __launch_bounds__(1024) void logits_ke
         if (i < fresh) atomicOr(&w, kInPrompt);
         else atomicAdd(&w, 1u);
     };
-    float l[E][8];
-#pragma unroll
-    for (int i = 0; i < E; i++) widen8<T>(raw[i], l[i]);
     const float r = 1.0f / rep;
     // A token in the prompt, generated c times.
     auto penalize = [&](float x, bool seen, uint32_t c) __attribute__((always_inline)) {
@@ -143,91 +143,100 @@ template <typename T, int SEG> __global__ __launch_bounds__(1024) void logits_ke
         const float z = c ? y - fmaf(freq, (float)c, pres) : y;
         return seen ? z : x;
     };
+    float most = -__builtin_inff();
+    int at = 0;                                    // the first place that holds it
+    auto widen = [&](int i, float (&x)[4]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = to_f<T>(raw[i].v[e]);
+    };
+    // A piece whose lists are done with: masked, written, its largest kept (a NaN is passed over).
+    auto finish = [&](int i, float (&x)[4]) __attribute__((always_inline)) {
+        const int c = (i * THREADS + tid) * 4, left = len - c;
+        if (left <= 0) return;
+        if (masked)
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[e] = allowed >> (4 * i + e) & 1 ? x[e] : -__builtin_inff();
+        float* o = a.out + row * a.out_ld + t0 + c;
+        if (left >= 4) {
+            // (past the caches: 64 rows of 131,072 29.5 -> 25.1 us, much of it the next kernel's wait for what the caches write back)
+            typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
+            __builtin_nontemporal_store(f4{x[0], x[1], x[2], x[3]}, reinterpret_cast<f4*>(o));
+        } else {
+#pragma unroll
+            for (int e = 0; e < 3; e++)
+                if (e < left) o[e] = x[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (x[e] > most && e < left) {
+                most = x[e];
+                at = c + e;
+            }
+    };
     // Lists that are short enough: both in one pass over the words, the last bias of a token and the number of times it was generated
     // side by side.
-    const bool lists = lo < hi || blo < bhi, packed = hi - (int64_t)lo <= kCounts && bhi - (int64_t)blo <= kSlots;
-    if (lists) {
-        clear();
-        if (packed) {
+    const bool lists = lo < hi || blo < bhi;
+    if (!lists || (hi - (int64_t)lo <= kCounts && bhi - (int64_t)blo <= kSlots)) {
+        if (lists) {
+            clear();
             if (blo < bhi)
                 scan(a.bias_ids, blo, bhi, bias_ids,
                      [&](uint32_t& w, int i) __attribute__((always_inline)) { atomicMax(&w, (uint32_t)(i - blo + 1) << 16); });
             if (lo < hi) scan(a.tokens, lo, hi, ids, count);
-        } else {
-            scan(a.tokens, lo, hi, ids, count);
-#pragma unroll
-            for (int i = 0; i < E; i++) {
-                uint32_t w[8];
-                words(i, w);
-#pragma unroll
-                for (int e = 0; e < 8; e++) l[i][e] = penalize(l[i][e], w[e], w[e] & ~kInPrompt);
-            }
-            __syncthreads();
-            clear();
-            scan(a.bias_ids, blo, bhi, bias_ids, [&](uint32_t& w, int i) __attribute__((always_inline)) { atomicMax(&w, (uint32_t)(i - blo) + 1); });
-#pragma unroll
-            for (int i = 0; i < E; i++) {
-                uint32_t w[8];
-                words(i, w);
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (w[e]) l[i][e] += a.bias_values[blo + (int64_t)w[e] - 1];
-            }
         }
-    }
-    float most = -__builtin_inff();
 #pragma unroll
-    for (int i = 0; i < E; i++) {
-        const int c = (i * THREADS + tid) * 8, left = len - c;
-        if (lists && packed) {
-            uint32_t w[8], any = 0;
+        for (int i = 0; i < E; i++) {
+            float x[4];
+            widen(i, x);
+            if (lists) {
+                uint32_t w[4], any = 0;
+                words(i, w);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    any |= w[e];
+                    x[e] = penalize(x[e], w[e] & (kInPrompt | kCounts), w[e] & kCounts);
+                }
+                if (any & kSlots << 16)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (const uint32_t s = w[e] >> 16 & kSlots) x[e] += a.bias_values[blo + (int64_t)s - 1];
+            }
+            finish(i, x);
+            __builtin_amdgcn_sched_barrier(0);     // piece by piece: all at once they would not fit the registers
+        }
+    } else {
+        float l[E][4];
+        clear();
+        scan(a.tokens, lo, hi, ids, count);
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+            uint32_t w[4];
+            words(i, w);
+            widen(i, l[i]);
+#pragma unroll
+            for (int e = 0; e < 4; e++) l[i][e] = penalize(l[i][e], w[e], w[e] & ~kInPrompt);
+        }
+        __syncthreads();
+        clear();
+        scan(a.bias_ids, blo, bhi, bias_ids, [&](uint32_t& w, int i) __attribute__((always_inline)) { atomicMax(&w, (uint32_t)(i - blo) + 1); });
+#pragma unroll
+        for (int i = 0; i < E; i++) {
+            uint32_t w[4];
             words(i, w);
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                any |= w[e];
-                l[i][e] = penalize(l[i][e], w[e] & (kInPrompt | kCounts), w[e] & kCounts);
-            }
-            if (any & kSlots << 16)
-#pragma unroll
-                for (int e = 0; e < 8; e++)
-                    if (const uint32_t s = w[e] >> 16 & kSlots) l[i][e] += a.bias_values[blo + (int64_t)s - 1];
+            for (int e = 0; e < 4; e++)
+                if (w[e]) l[i][e] += a.bias_values[blo + (int64_t)w[e] - 1];
+            finish(i, l[i]);
         }
-        if (left <= 0) continue;
-        if (masked)
-#pragma unroll
-            for (int e = 0; e < 8; e++) l[i][e] = bits[i] >> e & 1 ? l[i][e] : -__builtin_inff();
-        float* o = a.out + row * a.out_ld + t0 + c;
-        if (left >= 8) {
-            // (past the caches: 64 rows of 131,072 29.5 -> 25.1 us, much of it the next kernel's wait for what the caches write back)
-            typedef float f4 __attribute__((ext_vector_type(4), aligned(4)));
-            __builtin_nontemporal_store(f4{l[i][0], l[i][1], l[i][2], l[i][3]}, reinterpret_cast<f4*>(o));
-            __builtin_nontemporal_store(f4{l[i][4], l[i][5], l[i][6], l[i][7]}, reinterpret_cast<f4*>(o + 4));
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-                if (e < left) o[e] = l[i][e];
-                else l[i][e] = -__builtin_inff();
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < 8; e++) most = fmaxf(most, l[i][e]);     // (a NaN is passed over)
     }
     if (!a.best && !a.token) return;
     // The segment's largest, and the first of the places that hold it.
-    most = wave_max(most);
-    if (tid % 64 == 0) top[tid / 64] = most;
+    const float wave_most = wave_max(most);
+    if (tid % 64 == 0) top[tid / 64] = wave_most;
     if (tid == 0) first = INT32_MAX;
     __syncthreads();
     const float largest = wave_max(top[tid % W]);
-    if (most == largest && largest > -__builtin_inff()) {            // the wave's
-        int at = INT32_MAX;
-#pragma unroll
-        for (int i = E - 1; i >= 0; i--)
-#pragma unroll
-            for (int e = 7; e >= 0; e--)
-                if (l[i][e] == largest && (i * THREADS + tid) * 8 + e < len) at = (i * THREADS + tid) * 8 + e;
-        if (at != INT32_MAX) atomicMin(&first, at);
-    }
+    if (most == largest && largest > -__builtin_inff()) atomicMin(&first, at);
     __syncthreads();
     if (tid) return;
     const uint64_t best = choice_key(largest, t0 + first);
@@ -245,10 +254,10 @@ __global__ __launch_bounds__(256) void choose_kernel(const uint64_t* best, int s
     if (lane == 0) token[row] = chosen(v);
 }
 
-// Tokens of a workgroup, 2,048 to 32,768: as many as leave the chip a workgroup per CU, since each reads the row's history.
+// Tokens of a workgroup, 2,048 to 32,768: as many as the row has and leave the chip a workgroup per CU, since each reads the row's history.
 static int logit_segment(int64_t n, int64_t vocab) {
     for (int s = 32768; s > 2048; s /= 2)
-        if (n * ((vocab + s - 1) / s) >= 256) return s;
+        if (s / 2 < vocab && n * ((vocab + s - 1) / s) >= 256) return s;
     return 2048;
 }
 
