@@ -10,9 +10,9 @@ import pytest
 import test_gpu_i8_linear as gpu_tests
 from conftest import ROOT
 
-NAMES = ["few 16x16", "few 16x16 deep", "few 16x16 short", "few 16x32", "64x64", "64x128", "128x64", "128x128", "128x128 two", "256x192", "256x256"]
-TILE = [(16, 16), (16, 16), (16, 16), (16, 32), (64, 64), (64, 128), (128, 64), (128, 128), (128, 128), (256, 192), (256, 256)]
-THREADS = [256, 512] + 8 * [256] + [512]
+NAMES = ["few 16x16", "few 16x16 deep", "few 16x16 short", "split 16x16", "split 16x32", "split 32x32", "split 64x32", "64x64", "64x128", "128x64", "128x128", "128x128 two", "256x192", "256x256"]
+TILE = [(16, 16), (16, 16), (16, 16), (16, 16), (16, 32), (32, 32), (64, 32), (64, 64), (64, 128), (128, 64), (128, 128), (128, 128), (256, 192), (256, 256)]
+THREADS = [256, 512, 256, 512] + 9 * [256] + [512]
 
 
 @pytest.fixture(scope="module")
@@ -45,5 +45,5 @@ def test_launches_stay_small(kernel):
         tm, tn = TILE[k]
         gm, gn = -(-M // tm), -(-N // tn)
         assert gm * gn * THREADS[k] < 1 << 32, (M, N, K, NAMES[k])
-        if k < 4:                                  # a grid of two dimensions
+        if k < 3:                                  # a grid of two dimensions
             assert gm <= 65535

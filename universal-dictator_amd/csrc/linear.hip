@@ -157,8 +157,6 @@ template <typename T, int MT, int NT, int WK, int U> static void launch_few(cons
     hipLaunchKernelGGL((i8_few_kernel<T, MT, NT, WK, U>), grid, dim3(64 * WK), 0, st, a);
 }
 
-// ---------------------------------------------------------------- many rows
-
 // Buffer resource of `bytes` bytes at p: loads past them give zeros.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t panel_buffer(const void* p, uint32_t bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, bytes, 0x00020000);
@@ -171,6 +169,134 @@ __device__ __forceinline__ void panel_load(__amdgpu_buffer_rsrc_t r, uint32_t vo
 constexpr int KB = 128;                            // bytes of k per LDS tile
 constexpr uint32_t kNowhere = 1u << 31;             // an offset that is past every buffer (256 rows, 2^22 apart)
 
+// ---------------------------------------------------------------- some rows
+
+// Some rows: a workgroup takes S FM rows and S FN channels, each of its waves all of them for every NW-th block of 128 of k, through two LDS
+// tiles of the wave's own: nothing is shared before the end, so a wave waits for its own loads alone.  A CU gets some 58 bytes a ns into LDS
+// (in pieces of 128 bytes a row; straight to registers, 64 bytes a row, half of it), whichever memory they come from, so the smallest
+// tiles that are one round of the chip are the fastest, though they read more: 64 rows of 14,336 -> 4,096 take 19.5 us with tiles of 32 x 32,
+// 26.5 with 64 x 32, 35.2 with 64 x 64 shared by four waves; 16 rows of 4,096 -> 6,144 7.2 with 16 x 32, 10.2 from memory to registers.
+// (Four LDS tiles a wave: 7.2 -> 7.5.)
+template <typename T, int S, int FM, int FN, int NW>
+__global__ __launch_bounds__(64 * NW) void i8_split_kernel(LinearArgs a) {
+    constexpr int TM = S * FM, TN = S * FN, R = FM + FN, L = S * R / 8, TILE = S * R * KB;   // L loads per wave and tile
+    constexpr int G = 64 / S, Q = KB / (16 * G), E = S * S / 64;       // pieces per row and product, products per tile, sums per lane
+    __shared__ __attribute__((aligned(16))) int8_t t0[NW * TILE];
+    __shared__ __attribute__((aligned(16))) int8_t t1[NW * TILE];
+    const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    // An XCD's workgroups are neighbours: the rows of a channel panel read its weights from one L2.
+    const int nM = (a.M + TM - 1) / TM, nN = (a.N + TN - 1) / TN, total = nM * nN;
+    const int xcd = blockIdx.x % 8, each = total / 8, more = total % 8;
+    const int t = xcd * each + min(xcd, more) + blockIdx.x / 8;
+    const int m0 = t % nM * TM, n0 = t / nM * TN;
+
+    const int rows_a = min(TM, a.M - m0), rows_w = min(TN, a.N - n0);
+    const __amdgpu_buffer_rsrc_t ra = panel_buffer(a.a + m0 * a.a_ld, (uint32_t)((rows_a - 1) * a.a_ld + a.K));
+    const __amdgpu_buffer_rsrc_t rw = panel_buffer(a.w + n0 * a.w_ld, (uint32_t)((rows_w - 1) * a.w_ld + a.K));
+    // Rows behind the last are the last one again (computed, not stored); pieces behind K are zeros.  The pieces of a row lie in the order
+    // piece ^ (r / 2 % 8), against bank conflicts.
+    uint32_t v[L];
+    int room[L];                                   // the k before which a block holds this lane's piece
+#pragma unroll
+    for (int i = 0; i < L; i++) {
+        const int r = i * 8 + lane / 8, piece = (lane % 8) ^ (r / 2 % 8);
+        v[i] = (uint32_t)(r < TM ? min(r, rows_a - 1) * a.a_ld : min(r - TM, rows_w - 1) * a.w_ld) + 16 * piece;
+        room[i] = a.K - 16 * piece;
+    }
+    auto load_tile = [&](int step, int8_t* at) __attribute__((always_inline)) {
+        const int k = (step * NW + wave) * KB;
+#pragma unroll
+        for (int i = 0; i < L; i++)
+            panel_load(i < TM / 8 ? ra : rw, k < room[i] ? v[i] : kNowhere, k < a.K ? k : 0, at + (wave * TILE + i * 1024));
+    };
+    load_tile(0, t0);
+    load_tile(1, t1);
+    // Four channels of a row to a thread at the end; what they need is read under the first tiles' way (before it 0.1 - 0.4 us more, behind the
+    // products 0.1 - 0.3).
+    constexpr int PR = TN / 4, PIECES = TM * PR, PER = (PIECES + 64 * NW - 1) / (64 * NW);
+    Finish4<T> fin[PER];
+#pragma unroll
+    for (int f = 0; f < PER; f++) {
+        const int p = tid + f * 64 * NW;
+        fin[f].read(a, p < PIECES ? m0 + p / PR : a.M, n0 + p % PR * 4);
+    }
+    typedef int Sums __attribute__((ext_vector_type(E)));
+    Sums acc[FN][FM];
+#pragma unroll
+    for (int i = 0; i < FN; i++)
+#pragma unroll
+        for (int j = 0; j < FM; j++)
+#pragma unroll
+            for (int e = 0; e < E; e++) acc[i][j][e] = 0;
+    const int r = lane % S, g = lane / S;
+    auto tile = [&](int step, int8_t* at) __attribute__((always_inline)) {
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm(L));  // this wave's loads of the tile have arrived (the next one's may not)
+        __asm__ volatile("" ::: "memory");
+        i32x4_t f[Q][R];
+#pragma unroll
+        for (int q = 0; q < Q; q++)
+#pragma unroll
+            for (int i = 0; i < R; i++)
+                f[q][i] = *reinterpret_cast<const i32x4_t*>(at + wave * TILE + (S * i + r) * KB + 16 * ((G * q + g) ^ (r / 2 % 8)));
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_waitcnt(0xC07F);        // and are read (lgkmcnt 0), before the next loads overwrite them
+        __asm__ volatile("" ::: "memory");
+        load_tile(step + 2, at);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int q = 0; q < Q; q++)
+#pragma unroll
+            for (int i = 0; i < FN; i++)
+#pragma unroll
+                for (int j = 0; j < FM; j++) {
+                    if constexpr (S == 32) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(f[q][FM + i], f[q][j], acc[i][j], 0, 0, 0);
+                    else acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(f[q][FM + i], f[q][j], acc[i][j], 0, 0, 0);
+                }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    const int steps = ((a.K + KB - 1) / KB + NW - 1) / NW;
+    int b = 0;
+    for (; b + 2 <= steps; b += 2) {
+        tile(b, t0);
+        tile(b + 1, t1);
+    }
+    if (b < steps) tile(b, t0);
+    __builtin_amdgcn_s_waitcnt(0);                 // the zeros behind the last tile, before LDS is used again
+    __asm__ volatile("" ::: "memory");
+    // A lane holds channels S / 4 i' + 4 g + (0 .. 3) of one row; a wave's sums go to its own tile, row by row (against bank conflicts four
+    // channels' piece p at p ^ (row % X)).
+    static_assert(TM * TN * 4 <= TILE, "a wave's sums fit its tile");
+    constexpr int X = PR < 8 ? PR : 8;
+    int* mine = reinterpret_cast<int*>(t0 + wave * TILE);
+#pragma unroll
+    for (int i = 0; i < FN; i++)
+#pragma unroll
+        for (int j = 0; j < FM; j++)
+#pragma unroll
+            for (int q = 0; q < E / 4; q++) {
+                const int row = S * j + r, p = S / 4 * i + G * q + g;
+                *reinterpret_cast<i32x4_t*>(mine + row * TN + 4 * (p ^ (row % X))) =
+                    i32x4_t{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+            }
+    __syncthreads();
+#pragma unroll
+    for (int f = 0; f < PER; f++) {
+        const int p = tid + f * 64 * NW, row = p / PR;
+        if (p >= PIECES) continue;
+        const int8_t* at = t0 + (row * TN + 4 * (p % PR ^ (row % X))) * 4;
+        i32x4_t s = *reinterpret_cast<const i32x4_t*>(at);
+#pragma unroll
+        for (int w = 1; w < NW; w++) s += *reinterpret_cast<const i32x4_t*>(at + w * TILE);
+        fin[f].write(a, m0 + row, n0 + p % PR * 4, s);
+    }
+}
+
+template <typename T, int S, int FM, int FN, int NW> static void launch_split(const LinearArgs& a, hipStream_t st) {
+    const int64_t tiles = tiles_of(a.M, a.N, S * FM, S * FN);
+    hipLaunchKernelGGL((i8_split_kernel<T, S, FM, FN, NW>), dim3((unsigned)tiles), dim3(64 * NW), 0, st, a);
+}
+
+// ---------------------------------------------------------------- many rows
 template <int FN, int FM> __device__ __forceinline__ void pin_sums(i32x16_t (&acc)[FN][FM]) {
 #pragma unroll
     for (int i = 0; i < FN; i++)
@@ -417,7 +543,10 @@ template <typename T> static void launch_linear(const LinearArgs& a, hipStream_t
         case FEW_16x16: return launch_few<T, 1, 1, 4, 16>(a, st);
         case FEW_16x16_DEEP: return launch_few<T, 1, 1, 8, 16>(a, st);
         case FEW_16x16_SHORT: return launch_few<T, 1, 1, 4, 8>(a, st);
-        case FEW_16x32: return launch_few<T, 1, 2, 4, 8>(a, st);
+        case SPLIT_16x16: return launch_split<T, 16, 1, 1, 8>(a, st);
+        case SPLIT_16x32: return launch_split<T, 16, 1, 2, 4>(a, st);
+        case SPLIT_32x32: return launch_split<T, 32, 1, 1, 4>(a, st);
+        case SPLIT_64x32: return launch_split<T, 32, 2, 1, 4>(a, st);
         case PANEL_64x64: return launch_panel<T, 1, 1, 4>(a, st);
         case PANEL_64x128: return launch_panel<T, 1, 2, 4>(a, st);
         case PANEL_128x64: return launch_panel<T, 2, 1, 4>(a, st);
