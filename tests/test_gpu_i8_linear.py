@@ -104,7 +104,7 @@ def test_channels(gpu, M, N):
 TILES = [(3, 5001, 2064), (16, 1000, 8208), (2, 20003, 528), (30, 3001, 1040), (64, 4099, 656), (60, 9003, 272), (120, 6002, 400), (500, 6007, 784),
          (1000, 9001, 272), (2049, 5500, 144), (2500, 4001, 400), (4050, 4030, 272), (8200, 1500, 256), (130, 30001, 64), (700, 9000, 400),
          (60, 17003, 272), (130, 8003, 400), (300, 9001, 16), (2060, 5400, 48), (520, 3001, 112), (4, 700, 8208), (3, 9001, 2064), (16, 9001, 400),
-         (63, 4001, 656), (29, 9001, 2064), (33, 4090, 16), (127, 4001, 2064), (9, 4095, 144), (17, 2003, 12304)]
+         (63, 4001, 656), (29, 9001, 2064), (33, 4090, 16), (127, 4001, 2064), (9, 4095, 144), (17, 2003, 12304), (445, 4140, 960)]
 
 
 @pytest.mark.parametrize("M,N,K", TILES)

@@ -37,10 +37,12 @@ constexpr int64_t tiles_of(int64_t M, int64_t N, int64_t tm, int64_t tn) { retur
 // one or two tiles of rows, more rounds cost less than larger tiles: 16 rows of 4,096 -> 32,000 16 x 32 26.9, 32 rows 32 x 32 30.2,
 // 64 x 128 by four waves 31.8 and 33.2; of 2,048 -> 32,001, whose tiles are short, 14.6, 16.8 and 14.5, 15.0.
 //
-// Otherwise the tile whose rounds over the 256 CUs cost least, from what one tile took per 128 of k and beside them (us, all CUs at
-// work).  us predicted and measured: 563 rows of 4,096 -> 6,144 128 x 128 20 and 21.3, 64 x 64 36 and 30.4, 256 x 256 60 and 49; 2,469 of
-// 12,288 -> 4,096 256 x 192 142 and 129, 128 x 128 165 and 164, 256 x 256 169 and 145; 8,192 of 4,096 -> 6,144 256 x 256 181 and 181,
-// 256 x 192 206 and 200.
+// Otherwise the tile with the least time on the CU that has the most of them: for each 128 of k of each tile, and beside that for each time
+// that the CU is filled with as many as its LDS holds of them (us, fitted to 425 sizes with 33 to 8,192 rows: with 2 us between launches
+// they lie within 7 to 15 % of the measured times at the median; the choice costs 0.4 % over the best tile on average, 2 % at the 95th
+// percentile, 28 % at most).  us predicted and measured: 563 rows of 4,096 -> 6,144 128 x 128 21 and 24, two a CU 24 and 33, 64 x 64 41 and 33;
+// 1,695 of 5,072 -> 2,914 two a CU 44 and 47, one 48 and 58, 64 x 64 62 and 66; 2,469 of 12,288 -> 4,096 256 x 192 117 and 128, 256 x 256 133 and
+// 145; 8,192 of 4,096 -> 6,144 256 x 256 151 and 185.
 inline LinearKernel linear_kernel(int64_t M, int64_t N, int64_t K) {
     const int64_t small = tiles_of(M, N, 16, 16), wide = tiles_of(M, N, 16, 32);
     if (M <= 4 && (small <= 256 || wide > 256)) return K >= 8192 ? FEW_16x16_DEEP : K > 2048 ? FEW_16x16 : FEW_16x16_SHORT;
@@ -48,16 +50,18 @@ inline LinearKernel linear_kernel(int64_t M, int64_t N, int64_t K) {
     if (wide <= 256 || M <= 16) return SPLIT_16x32;
     if (tiles_of(M, N, 32, 32) <= 256 || (M <= 32 && K > 2048)) return SPLIT_32x32;
     if (tiles_of(M, N, 64, 32) <= 256) return SPLIT_64x32;
-    struct Shape { LinearKernel kernel; int tm, tn; double step, once; };
-    const Shape shapes[] = {{PANEL_64x64, 64, 64, 0.23, 1.5},   {PANEL_64x128, 64, 128, 0.31, 2},  {PANEL_128x64, 128, 64, 0.29, 2},
-                            {PANEL_128x128, 128, 128, 0.54, 3}, {PANEL_256x192, 256, 192, 1.42, 6}, {PANEL_256x256, 256, 256, 1.70, 6}};
+    struct Shape { LinearKernel kernel; int tm, tn, held; double step, once; };
+    const Shape shapes[] = {{PANEL_64x64, 64, 64, 2, 0.27, 2.03},       {PANEL_64x128, 64, 128, 1, 0.44, 2.55},
+                            {PANEL_128x64, 128, 64, 1, 0.37, 2.65},     {PANEL_128x128, 128, 128, 1, 0.42, 6.02},
+                            {PANEL_128x128_TWO, 128, 128, 2, 0.42, 8.25},{PANEL_256x192, 256, 192, 1, 1.10, 8.90},
+                            {PANEL_256x256, 256, 256, 1, 1.27, 9.14}};
     const int64_t steps = (K + 127) / 128;
     LinearKernel best = PANEL_256x256;
     double least = 1e300;
     for (const Shape& s : shapes) {
-        const int64_t tiles = tiles_of(M, N, s.tm, s.tn);
-        const double cost = (double)((tiles + 255) / 256) * ((double)steps * s.step + s.once);
-        if (cost < least) { least = cost; best = s.kernel == PANEL_128x128 && tiles > 256 ? PANEL_128x128_TWO : s.kernel; }
+        const int64_t tiles = (tiles_of(M, N, s.tm, s.tn) + 255) / 256;    // on one CU
+        const double cost = (double)((tiles + s.held - 1) / s.held) * s.once + (double)(tiles * steps) * s.step;
+        if (cost < least) { least = cost; best = s.kernel; }
     }
     return best;
 }
