@@ -53,7 +53,7 @@ UD_API int ud_rms_norm(int32_t dtype, const void* x_dev, int32_t x_ld, int32_t s
  *   x, gate      dtype, rows ld apart both (two pieces of one fused row, or buffers of their own)
  *   codes        int8, rows codes_ld apart;  scales fp32 [rows]
  * dim a multiple of 8, 8 .. 32768; rows below 2^22; lds multiples of 8, x and gate 16-byte aligned, codes 8.  An output that overlaps
- * an input is refused.  exp(-gate) past fp32's range (gates below -88) makes y 0. */
+ * an input is refused.  exp(-gate) near fp32's largest or past it (gates below -87) makes y 0. */
 UD_API int ud_i8_quantize(int32_t dtype, const void* x_dev, const void* gate_dev, int32_t ld, int8_t* codes_dev, int32_t codes_ld,
                           float* scales_dev, int32_t rows, int32_t dim, void* hip_stream);
 
@@ -67,8 +67,8 @@ UD_API int ud_i8_quantize(int32_t dtype, const void* x_dev, const void* gate_dev
  *   out          dtype [M, N], rows out_ld apart
  * K a multiple of 16, 16 .. 131056 (the sum stays in 32 bits); codes and w 16-byte aligned, their lds multiples of 16, at most
  * 2^22; N 1 .. 2^24, M below 2^22, M N at most 2^38.  out and residual need the alignment of their elements only.  Other overlaps
- * of out are refused.  Rows of codes and w that start at multiples of 64 bytes are read fastest (others cost up to half the time
- * again: pad the lds).  Precision: the sum exact, then fp32 in the order written (the second scale and the bias in one
+ * of out are refused.  Rows of codes and w that start at multiples of 128 bytes are read fastest (others cost up to half the
+ * time again: pad the lds).  Precision: the sum exact, then fp32 in the order written (the second scale and the bias in one
  * operation), one rounding at the end: a row's result is the same in a batch of any size. */
 UD_API int ud_i8_linear(int32_t dtype, const int8_t* codes_dev, int32_t codes_ld, const float* scales_dev, const int8_t* w_dev,
                         int32_t w_ld, const float* w_scales_dev, const float* bias_dev, const void* residual_dev, int32_t res_ld,
