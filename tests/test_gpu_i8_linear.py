@@ -92,6 +92,13 @@ def test_depths(gpu, M, K):
     check(gpu, rng, M, 77, K, "bf16", bias=True, pad=(16, 0, 0, 1))
 
 
+@pytest.mark.parametrize("K", [16, 112, 128, 144, 496, 512, 528, 1008, 1024, 1040, 1152, 2064])
+@pytest.mark.parametrize("M,N", [(16, 500), (30, 3001), (60, 4001), (125, 4001)])
+def test_depths_shared_by_waves(gpu, M, N, K):
+    """Blocks of 128 of k that do not come out even over the waves, or fewer than these; ends within a block."""
+    check(gpu, np.random.default_rng([M, K]), M, N, K, "f32", bias=True, full=True, pad=(16, 0, 0, 0))
+
+
 @pytest.mark.parametrize("N", [3, 15, 17, 31, 33, 64, 127, 129, 255, 257, 1025, 6144])
 @pytest.mark.parametrize("M", [1, 20, 64, 140, 270])
 def test_channels(gpu, M, N):
