@@ -52,7 +52,7 @@ def test_norm_rows_far_apart(gpu, eight):
         assert np.all(np.abs(got - y) <= (2.0 ** -8 * 1.01 + NORM_REL) * np.abs(y))
 
 
-@pytest.mark.parametrize("M,N,K", [(3, 1100, 64), (1100, 130, 80), (1030, 1100, 144)])
+@pytest.mark.parametrize("M,N,K", [(3, 1100, 64), (1100, 130, 80), (1030, 1100, 144), (40, 1100, 400), (24, 2100, 272)])
 def test_products_of_rows_far_apart(gpu, M, N, K):
     """Rows 2^22 bytes apart, the largest distance: over a thousand of them pass 4 GiB."""
     ud, rng, ld = gpu, np.random.default_rng([M, N]), 1 << 22
