@@ -31,7 +31,9 @@ template <int W, typename V, typename F> __device__ __forceinline__ V row_join(V
 }
 
 // Pieces y of a row as 8-bit codes, and the row's scale.  The largest magnitude is taken as an unsigned number, so that a NaN
-// is larger than all.
+// is larger than all.  A code is the quotient y / scale as a division rounds it, to the nearest whole number: the product with the
+// reciprocal, corrected by what it leaves of y (the product alone gives the other code to one in twelve of the values next to a border).  1.5 * 2^23 + code: the sum is
+// rounded to whole numbers, and the code is its lowest byte.
 template <int W, int P>
 __device__ __forceinline__ void store_codes(const float (&y)[P][8], int t, int dim, uint32_t* at, int8_t* codes, float* scale_out) {
     uint32_t top = 0;
@@ -50,7 +52,11 @@ __device__ __forceinline__ void store_codes(const float (&y)[P][8], int t, int d
         if (c >= dim) continue;
         uint32_t w[2] = {0, 0};
 #pragma unroll
-        for (int e = 0; e < 8; e++) w[e / 4] |= ((uint32_t)(bad ? 0 : (int)rintf(y[p][e] * inv)) & 255u) << (8 * (e % 4));
+        for (int e = 0; e < 8; e++) {
+            const float q = y[p][e] * inv;
+            const uint32_t code = __float_as_uint(fmaf(fmaf(-q, scale, y[p][e]), inv, q) + 0x1.8p23f) & 255u;
+            w[e / 4] |= (bad ? 0u : code) << (8 * (e % 4));
+        }
         *reinterpret_cast<uint2*>(codes + c) = make_uint2(w[0], w[1]);
     }
     if (t == 0) *scale_out = scale;
