@@ -137,9 +137,9 @@ template <typename T, int SEG> __global__ __launch_bounds__(1024) void logits_ke
         else atomicAdd(&w, 1u);
     };
     const float r = 1.0f / rep;
-    // A token in the prompt, generated c times.
-    auto penalize = [&](float x, bool seen, uint32_t c) __attribute__((always_inline)) {
-        const float y = x * (x > 0.0f ? r : rep);
+    auto repeated = [&](float x) __attribute__((always_inline)) { return x * (x > 0.0f ? r : rep); };
+    // A token in the prompt, generated c times; y: its logit under the repetition's penalty.
+    auto penalize = [&](float x, float y, bool seen, uint32_t c) __attribute__((always_inline)) {
         const float z = c ? y - fmaf(freq, (float)c, pres) : y;
         return seen ? z : x;
     };
@@ -174,9 +174,10 @@ template <typename T, int SEG> __global__ __launch_bounds__(1024) void logits_ke
             }
     };
     // Lists that are short enough: both in one pass over the words, the last bias of a token and the number of times it was generated
-    // side by side.
-    const bool lists = lo < hi || blo < bhi;
-    if (!lists || (hi - (int64_t)lo <= kCounts && bhi - (int64_t)blo <= kSlots)) {
+    // side by side.  A repetition whose reciprocal would be infinite or short of bits goes the other way, where it divides (a division for all
+    // rows: 64 rows of 131,072 21.4 -> 23.6 us).
+    const bool lists = lo < hi || blo < bhi, far = !(rep >= 0x1p-100f && rep <= 0x1p100f);
+    if (!lists || (hi - (int64_t)lo <= kCounts && bhi - (int64_t)blo <= kSlots && !far)) {
         if (lists) {
             clear();
             if (blo < bhi)
@@ -194,7 +195,7 @@ template <typename T, int SEG> __global__ __launch_bounds__(1024) void logits_ke
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
                     any |= w[e];
-                    x[e] = penalize(x[e], w[e] & (kInPrompt | kCounts), w[e] & kCounts);
+                    x[e] = penalize(x[e], repeated(x[e]), w[e] & (kInPrompt | kCounts), w[e] & kCounts);
                 }
                 if (any & kSlots << 16)
 #pragma unroll
@@ -214,7 +215,10 @@ template <typename T, int SEG> __global__ __launch_bounds__(1024) void logits_ke
             words(i, w);
             widen(i, l[i]);
 #pragma unroll
-            for (int e = 0; e < 4; e++) l[i][e] = penalize(l[i][e], w[e], w[e] & ~kInPrompt);
+            for (int e = 0; e < 4; e++) {
+                const float x = l[i][e];
+                l[i][e] = penalize(x, far && x > 0.0f ? x / rep : repeated(x), w[e], w[e] & ~kInPrompt);
+            }
         }
         __syncthreads();
         clear();
