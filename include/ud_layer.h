@@ -93,7 +93,8 @@ UD_API int ud_i8_linear(int32_t dtype, const int8_t* codes_dev, int32_t codes_ld
  *   mask         uint32 [n_masks, mask_ld], bit t % 32 of word t / 32: token t is allowed;  mask_rows int32 [n]: row i's mask,
  *                outside [0, n_masks): none (everything is allowed); null: mask i (n_masks >= n).  mask null: none
  *   workspace    ud_logits_workspace_bytes(n, vocab) bytes, 8-byte aligned, where token is given (else may be null); its contents
- *                need not be kept, and calls that may run at the same time need one each
+ *                need not be kept, and calls that may run at the same time need one each.  More rows or a larger vocabulary never
+ *                need less: one for the largest batch serves the smaller ones
  * vocab 1 .. 2^24, n 0 .. 65535.  Pointers need the alignment of their elements only.  An out that overlaps an input in any other
  * way is refused.  fp32 arithmetic. */
 UD_API size_t ud_logits_workspace_bytes(int32_t n, int32_t vocab);

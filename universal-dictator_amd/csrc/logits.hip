@@ -280,8 +280,10 @@ using namespace ud;
 
 extern "C" UD_API size_t ud_logits_workspace_bytes(int32_t n, int32_t vocab) {
     if (n < 1 || n > 65535 || vocab < 1 || vocab > (1 << 24)) return 0;
-    const int seg = logit_segment(n, vocab);
-    return (size_t)n * ((vocab + seg - 1) / seg) * sizeof(uint64_t);
+    // A key for each of the row's segments at least, and never less for more rows or more tokens.  (Segments between the smallest and the
+    // largest are taken where twice as large ones would be fewer than 256, or a row is one: there are fewer than 512 of them, or as many as rows.)
+    const size_t most = (size_t)n * ((vocab + 2047) / 2048), least = (size_t)n * ((vocab + 32767) / 32768);
+    return sizeof(uint64_t) * (most < 512 ? most : least < 512 ? 512 : least);
 }
 
 extern "C" UD_API int ud_logits_process(int32_t dtype, const void* logits_dev, int32_t ld, float* out_dev, int32_t out_ld,
