@@ -8,6 +8,7 @@ import subprocess
 import numpy as np
 import pytest
 
+import test_gpu_long_lists as long_lists
 from conftest import ROOT
 
 
@@ -40,3 +41,10 @@ def test_a_workspace_holds_every_segment(ud, segment):
     for n, v in sizes:
         need = 8 * n * -(-v // segment(n, v))
         assert need <= ud.logits_workspace_bytes(n, v) <= max(need, 8 * 512) or segment(n, v) == 2048, (n, v)
+
+
+def test_long_lists_reach_every_segment(segment):
+    """The GPU tests of long lists take the segments that they say, each size of them."""
+    for n, v, tokens in long_lists.SIZES:
+        assert segment(n, v) == tokens, (n, v)
+    assert {s for _, _, s in long_lists.SIZES} == {2048, 4096, 8192, 16384, 32768}
