@@ -782,17 +782,21 @@ def logits_workspace_bytes(n, vocab):
     return int(load_library().ud_logits_workspace_bytes(n, vocab))
 
 
-def logits_process(logits, out, n, vocab, token=None, tokens=None, n_tokens=0, ranges=None, penalties=None, bias_ids=None,
-                   bias_values=None, n_biases=0, bias_ranges=None, mask=None, n_masks=0, mask_rows=None, workspace=None, dtype="f32",
-                   ld=None, out_ld=None, mask_ld=None, hip_stream=None):
+def logits_process(logits, out, n, vocab, token=None, tokens=None, n_tokens=None, ranges=None, penalties=None, bias_ids=None,
+                   bias_values=None, n_biases=None, bias_ranges=None, mask=None, n_masks=None, mask_rows=None, workspace=None,
+                   dtype="f32", ld=None, out_ld=None, mask_ld=None, hip_stream=None):
     """out fp32 [n, vocab] = logits under penalties for the tokens of each row's history, biases and grammar masks; token int32 [n]:
-    the greedy choice (-1: nothing is left).  See ud_layer.h for the arrays.  workspace: logits_workspace_bytes(n, vocab) bytes where
-    token is given.  *_ld: elements (words of the mask) between rows (None: contiguous)."""
+    the greedy choice (-1: nothing is left).  See ud_layer.h for the arrays; tokens, bias_ids and mask go with their n_tokens,
+    n_biases and n_masks (0: none).  workspace: logits_workspace_bytes(n, vocab) bytes, or those of a larger batch, where token is
+    given.  *_ld: elements (words of the mask) between rows (None: contiguous)."""
+    for name, array, count in (("n_tokens", tokens, n_tokens), ("n_biases", bias_ids, n_biases), ("n_masks", mask, n_masks)):
+        if array is not None and count is None:
+            raise EngineError(-1, "logits_process: %s is missing" % name)
     _check(lib().ud_logits_process(_DTYPES[dtype], logits.ptr, vocab if ld is None else ld, out.ptr, vocab if out_ld is None else out_ld,
-                                   token and token.ptr, n, vocab, tokens and tokens.ptr, n_tokens, ranges and ranges.ptr,
-                                   penalties and penalties.ptr, bias_ids and bias_ids.ptr, bias_values and bias_values.ptr, n_biases,
+                                   token and token.ptr, n, vocab, tokens and tokens.ptr, n_tokens or 0, ranges and ranges.ptr,
+                                   penalties and penalties.ptr, bias_ids and bias_ids.ptr, bias_values and bias_values.ptr, n_biases or 0,
                                    bias_ranges and bias_ranges.ptr, mask and mask.ptr, (vocab + 31) // 32 if mask_ld is None else mask_ld,
-                                   n_masks, mask_rows and mask_rows.ptr, workspace and workspace.ptr, workspace.nbytes if workspace else 0,
+                                   n_masks or 0, mask_rows and mask_rows.ptr, workspace and workspace.ptr, workspace.nbytes if workspace else 0,
                                    hip_stream and hip_stream.ptr))
 
 
