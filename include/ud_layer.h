@@ -84,9 +84,10 @@ UD_API int ud_i8_linear(int32_t dtype, const int8_t* codes_dev, int32_t codes_ld
  *   logits       dtype [n, vocab], rows ld apart;  out fp32 [n, vocab], rows out_ld apart, may be logits itself (UD_F32, ld ==
  *                out_ld)
  *   token        int32 [n] or null
- *   tokens       int32 [n_tokens]: the rows' histories;  ranges int32 [n, 3]: row i's prompt is tokens[a .. b), what it has
- *                generated tokens[b .. c), of (a, b, c) = ranges[i];  cut to [0, n_tokens).  An id outside [0, vocab) is padding.
- *                Rows may share tokens.  null: no histories
+ *   tokens       int32 [n_tokens]: the rows' histories;  ranges int32 [n, 3], (a, b, c) = ranges[i]: row i's history is
+ *                tokens[a .. c), cut to [0, n_tokens); what of it lies in front of place b is its prompt, the rest it has
+ *                generated (where b <= a all of it, where b >= c nothing).  An id outside [0, vocab) is padding.  Rows may share tokens.
+ *                null: no histories
  *   penalties    fp32 [n, 3]: repetition (> 0), presence, frequency; null: 1, 0, 0
  *   bias_ids, bias_values   int32 / fp32 [n_biases];  bias_ranges int32 [n, 2]: row i's are [lo, hi), cut to [0, n_biases); rows may
  *                share them.  An id outside [0, vocab) is padding.  null: none
