@@ -90,16 +90,16 @@ __device__ __forceinline__ void finish8(const LinearArgs& a, int m, int n, int l
     }
 }
 
-// A few rows: the time is that of the weights' way from memory.  A workgroup takes 16 channels and 16 rows; its WK waves take every WK-th block
+// Up to 16 rows: the time is that of the weights' way from memory.  A workgroup takes 16 channels; its WK waves take every WK-th block
 // of 64 U of k, straight from memory into the matrix instruction's operands, up to 32 loads of 1 KB a wave at once, and are summed in LDS.  One row
 // of 12,288 -> 4,096 takes 10.4 us, where reading the weights alone, in the same pieces, takes 9.5 - 10.2.
 template <typename T, int WK, int U> __global__ __launch_bounds__(64 * WK) void i8_few_kernel(LinearArgs a) {
     __shared__ i32x4_t part[WK][64];
     const int wave = threadIdx.x / 64, lane = threadIdx.x % 64, r = lane % 16, g = lane / 16;
-    const int n0 = blockIdx.x * 16, m0 = blockIdx.y * 16;
+    const int n0 = blockIdx.x * 16;
     // rows behind the last are the last one again: read, never stored
     const int8_t* wp = a.w + min(n0 + r, a.N - 1) * a.w_ld + 16 * g;
-    const int8_t* ap = a.a + min(m0 + r, a.M - 1) * a.a_ld + 16 * g;
+    const int8_t* ap = a.a + min(r, a.M - 1) * a.a_ld + 16 * g;
     i32x4_t acc{0, 0, 0, 0}, wf[U], af[U];
     auto load = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
@@ -114,7 +114,7 @@ template <typename T, int WK, int U> __global__ __launch_bounds__(64 * WK) void 
     load(k);
     // the first wave finishes; its lanes hold four channels of one row
     Finish4<T> fin;
-    if (wave == 0) fin.read(a, m0 + r, n0 + 4 * g);
+    if (wave == 0) fin.read(a, r, n0 + 4 * g);
     for (;;) {
 #pragma unroll
         for (int u = 0; u < U; u++) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(wf[u], af[u], acc, 0, 0, 0);
@@ -128,13 +128,12 @@ template <typename T, int WK, int U> __global__ __launch_bounds__(64 * WK) void 
         i32x4_t s = part[0][lane];
 #pragma unroll
         for (int i = 1; i < WK; i++) s += part[i][lane];
-        fin.write(a, m0 + r, n0 + 4 * g, s);
+        fin.write(a, r, n0 + 4 * g, s);
     }
 }
 
 template <typename T, int WK, int U> static void launch_few(const LinearArgs& a, hipStream_t st) {
-    const dim3 grid((a.N + 15) / 16, (a.M + 15) / 16);
-    hipLaunchKernelGGL((i8_few_kernel<T, WK, U>), grid, dim3(64 * WK), 0, st, a);
+    hipLaunchKernelGGL((i8_few_kernel<T, WK, U>), dim3((a.N + 15) / 16), dim3(64 * WK), 0, st, a);
 }
 
 // Buffer resource of `bytes` bytes at p: loads past them give zeros.
