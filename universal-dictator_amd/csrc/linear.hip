@@ -351,10 +351,11 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || FM * FN > 8 || (FM + FN) * NS *
     };
     // Fragments of k step q (32 of k): lane l holds row l % 32, pieces 2 q + l / 32.
     const int wm = wave % 2 * (32 * FM), wn = wave / 2 * (32 * FN), r32 = lane % 32, half = lane / 32;
-    // Fragments in registers: of two whole tiles where there is room (a tile is read under the products of the one before), else of two
-    // k steps.
+    // Fragments in registers: of two whole tiles with four LDS tiles, which the small ones have (a tile is read under the products of the
+    // one before), else of two k steps.
     constexpr int R = FM + FN;
-    constexpr bool WHOLE = R <= 4 && NS == 4 && NW == 4;
+    constexpr bool WHOLE = NS == 4;
+    static_assert(!WHOLE || (R <= 4 && NW == 4), "two whole tiles fit the registers");
     i32x4_t fa[WHOLE ? 8 : 2][FM], fw[WHOLE ? 8 : 2][FN];
     auto read_frag = [&](int i, int q, const int8_t* at, const int8_t* wt, i32x4_t (&da)[FM], i32x4_t (&dw)[FN]) __attribute__((always_inline)) {
         const int off = r32 * KB + 16 * ((2 * q + half) ^ (r32 / 2 % 8));
@@ -390,7 +391,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || FM * FN > 8 || (FM + FN) * NS *
         if constexpr (WHOLE) {
             constexpr int H = decltype(which)::value * 4;
             // this wave's loads of tile b + 1 have arrived, and its reads of tile b
-            __builtin_amdgcn_s_waitcnt(vmcnt_imm((NS - 2) * L) & 0xF0FF);
+            __builtin_amdgcn_s_waitcnt(vmcnt_imm(2 * L) & 0xF0FF);
             __builtin_amdgcn_s_barrier();
             __asm__ volatile("" ::: "memory");
 #pragma unroll
@@ -398,7 +399,7 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || FM * FN > 8 || (FM + FN) * NS *
                 const int first = q * L / 4;
                 products(fa[H + q], fw[H + q], R + (q + 1) * L / 4 - first, [&](int k) __attribute__((always_inline)) {
                     if (k < R) read_frag(k, q, an, wnx, fa[4 - H + q], fw[4 - H + q]);
-                    else load_part(first + k - R, b + NS, at, wt);
+                    else load_part(first + k - R, b + 4, at, wt);
                 });
             }
         } else {
@@ -406,13 +407,13 @@ __global__ __launch_bounds__(64 * NW, NW == 8 || FM * FN > 8 || (FM + FN) * NS *
             products(fa[1], fw[1], R, [&](int k) __attribute__((always_inline)) { read_frag(k, 2, at, wt, fa[0], fw[0]); });
             products(fa[0], fw[0], R, [&](int k) __attribute__((always_inline)) { read_frag(k, 3, at, wt, fa[1], fw[1]); });
             // this wave's loads of tile b + 1 have arrived, and its reads of tile b
-            __builtin_amdgcn_s_waitcnt(vmcnt_imm((NS - 2) * L) & 0xF0FF);
+            __builtin_amdgcn_s_waitcnt(vmcnt_imm(0) & 0xF0FF);
             __builtin_amdgcn_s_barrier();
             __asm__ volatile("" ::: "memory");
 #pragma unroll
             for (int k = 0; k < R; k++) read_frag(k, 0, an, wnx, fa[0], fw[0]);
             __builtin_amdgcn_sched_barrier(0);
-            products(fa[1], fw[1], L, [&](int k) __attribute__((always_inline)) { load_part(k, b + NS, at, wt); });
+            products(fa[1], fw[1], L, [&](int k) __attribute__((always_inline)) { load_part(k, b + 2, at, wt); });
         }
     };
     const std::integral_constant<int, 0> even{};
