@@ -285,12 +285,13 @@ template <int FN, int FM> __device__ __forceinline__ void pin_sums(i32x16_t (&ac
 }
 
 // A workgroup of NW waves takes 64 FM rows and 16 NW FN channels, a wave 32 FM and 32 FN of them, through NS LDS tiles of 128 of k
-// each.  8,192 rows of 4,096 -> 6,144 take 181 us (2.3 POP/s; 64-row operand panels shared in an XCD's L2), 8,192^3 2.4 POP/s, where the
-// library's product of the same sizes reaches 1.9 and 2.1 and the instructions alone 3.2 at the clock the card keeps under them.
+// each.  8,192 rows of 4,096 -> 6,144 take 184 us in a loop of their own (2.2 POP/s; traced between other calls 197), 8,192^3 2.4 POP/s, where
+// the library's product of the same sizes reaches 1.9 and 2.1 and the instructions alone 3.2 at the clock the card keeps under them.
 //  - The tiles are loaded straight into LDS, 8 rows of 128 bytes to an instruction.  The 16-byte pieces of row r lie in the order
 //    piece ^ (r / 2 % 8), so that the 16 rows that LDS serves at a time lie in different banks.  (Tiles of 64 of k, four of them: 190 -> 198.)
 //  - The products are inline assembly with the sums pinned to the accumulator registers: from the builtin the compiler moved them
-//    between the register files and spilled 137 registers (256 x 256).  The wait states between compiled code and the products are
+//    between the register files and spilled 137 registers (256 x 256).  (Finishing fp32 rows of 256 x 256 still spills 84, behind the
+//    products: 209 us, of bf16 184.)  The wait states between compiled code and the products are
 //    explicit at the loop's two ends; within it a sum goes from product to product in its own registers, which needs none.
 //  - Reads of LDS and loads of later tiles lie between the products.  With large fragments the last quarter of a tile's products runs behind
 //    the barrier: its operands are in registers by then, so the tile is free for loads, and the next tile's first operands arrive

@@ -4,7 +4,7 @@
 
 namespace ud {
 
-// Kernels for a few rows: workgroups of 16 rows and 16 channels whose waves share out k, 4 or 8 of them, with blocks of 64 u of k.
+// Kernels for a few rows, 16 at most: workgroups of 16 channels whose waves share out k, 4 or 8 of them, with blocks of 64 u of k.
 // For some rows: the waves share out k too, through LDS tiles of their own.
 // For many: tiles of rows and channels through two or four LDS tiles, by four waves (eight where it says so).
 enum LinearKernel {
@@ -39,8 +39,9 @@ constexpr int64_t tiles_of(int64_t M, int64_t N, int64_t tm, int64_t tn) { retur
 //
 // Otherwise the tile with the least time on the CU that has the most of them: for each 128 of k of each tile, and beside that for each time
 // that the CU is filled with as many as its LDS holds of them (us, fitted to 425 sizes with 33 to 8,192 rows: with 2 us between launches
-// they lie within 7 to 15 % of the measured times at the median; the choice costs 0.4 % over the best tile on average, 2 % at the 95th
-// percentile, 28 % at most).  us predicted and measured: 563 rows of 4,096 -> 6,144 128 x 128 21 and 24, two a CU 24 and 33, 64 x 64 41 and 33;
+// they lie within 7 to 15 % of the measured times at the median; the choice costs 0.4 % over the best tile on average, 3 % at the 95th
+// percentile, 28 % at most, for 2,048 rows of 1,024 -> 2,048: 128 x 128 14.4, two a CU 11.3; after it 16 %, for 1,466 of 944 -> 11,826).
+// us predicted and measured: 563 rows of 4,096 -> 6,144 128 x 128 21 and 24, two a CU 24 and 33, 64 x 64 41 and 33;
 // 1,695 of 5,072 -> 2,914 two a CU 44 and 47, one 48 and 58, 64 x 64 62 and 66; 2,469 of 12,288 -> 4,096 256 x 192 117 and 128, 256 x 256 133 and
 // 145; 8,192 of 4,096 -> 6,144 256 x 256 151 and 185.
 inline LinearKernel linear_kernel(int64_t M, int64_t N, int64_t K) {

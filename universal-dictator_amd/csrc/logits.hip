@@ -203,7 +203,7 @@ template <typename T, int SEG> __global__ __launch_bounds__(1024) void logits_ke
                         if (const uint32_t s = w[e] >> 16 & kSlots) x[e] += a.bias_values[blo + (int64_t)s - 1];
             }
             finish(i, x);
-            __builtin_amdgcn_sched_barrier(0);     // piece by piece: all at once they would not fit the registers
+            __builtin_amdgcn_sched_barrier(0);     // piece by piece: all at once they would not fit the registers (nor do they all below)
         }
     } else {
         float l[E][4];
