@@ -69,7 +69,8 @@ UD_API int ud_i8_quantize(int32_t dtype, const void* x_dev, const void* gate_dev
  * 2^22; N 1 .. 2^24, M below 2^22, M N at most 2^38.  out and residual need the alignment of their elements only.  Other overlaps
  * of out are refused.  Rows of codes and w that start at multiples of 128 bytes are read fastest (others cost up to half the
  * time again: pad the lds).  Precision: the sum exact, then fp32 in the order written (the second scale and the bias in one
- * operation), one rounding at the end: a row's result is the same in a batch of any size. */
+ * operation), one rounding at the end: a row's result is the same in a batch of any size (of a NaN,
+ * that it is one: its sign and its other bits may differ). */
 UD_API int ud_i8_linear(int32_t dtype, const int8_t* codes_dev, int32_t codes_ld, const float* scales_dev, const int8_t* w_dev,
                         int32_t w_ld, const float* w_scales_dev, const float* bias_dev, const void* residual_dev, int32_t res_ld,
                         void* out_dev, int32_t out_ld, int32_t M, int32_t N, int32_t K, void* hip_stream);
